@@ -55,7 +55,8 @@ typedef enum {
     ACL_UINT64 = 10,
     ACL_DOUBLE = 11,
     ACL_BOOL = 12,
-    ACL_BF16 = 27
+    ACL_BF16 = 27,
+    ACL_FLOAT8_E4M3FN = 36
 } aclDataType;
 
 typedef enum {

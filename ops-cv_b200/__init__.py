@@ -1,6 +1,8 @@
-"""opscv_b200: Python caller of libopscv_b200.so, the B200 implementation of the ops-cv resampling aclnn API.
+"""opscv_b200: Python caller of libopscv_b200.so, the B200 implementation of the ops-cv resampling aclnn API and of
+operators on sequences of tokens in the same manner.
 
-The product is the shared library (C ABI declared in include/aclnn_resample.h and include/opscv_acl.h). This
+The product is the shared library (C ABI declared in include/aclnn_resample.h, include/aclnn_sequence.h and
+include/opscv_acl.h). This
 package is the thin Python caller used by the tests and the benchmark, playing the part that the reference's
 ATK `pyaclnn` backend plays for the original library: it builds aclTensor handles over torch CUDA tensors
 (device memory and streams only), runs the two-phase calls and raises on any non-zero status. The operators go through
@@ -21,6 +23,7 @@ NATIVE_PATH = os.path.join(_HERE, "lib", "_opscv_torch.so")
 CSRC_DIR = os.path.join(_HERE, "csrc")
 
 # aclDataType / aclFormat values (include/opscv_acl.h)
+ACL_FLOAT8_E4M3FN = 36
 ACL_FLOAT, ACL_FLOAT16, ACL_INT8, ACL_INT32, ACL_UINT8, ACL_INT64, ACL_DOUBLE, ACL_BOOL, ACL_BF16 = 0, 1, 2, 3, 4, 9, 11, 12, 27
 ACL_FORMAT_NCHW, ACL_FORMAT_NHWC, ACL_FORMAT_ND, ACL_FORMAT_NCL = 0, 1, 2, 47
 ACL_FORMAT_NDHWC, ACL_FORMAT_NCDHW = 27, 30
@@ -118,6 +121,22 @@ SYMBOLS = {
     "aclnnGridSampler2DBackward": _PHASE2,
 }
 
+# and those of include/aclnn_sequence.h
+SEQUENCE_SYMBOLS = {
+    "aclnnResidualRmsNormGetWorkspaceSize": (_I32, [_P, _P, _P, _D, _P, _P, _P, _PU64, _PP]),
+    "aclnnResidualRmsNorm": _PHASE2,
+    "aclnnResidualRmsNormBackwardGetWorkspaceSize": (_I32, [_P, _P, _P, _P, _P, _P, _P, _PU64, _PP]),
+    "aclnnResidualRmsNormBackward": _PHASE2,
+    "aclnnResidualRmsNormQuantGetWorkspaceSize": (_I32, [_P, _P, _P, _D, _I64, _P, _P, _P, _PU64, _PP]),
+    "aclnnResidualRmsNormQuant": _PHASE2,
+    "aclnnRotaryEmbeddingGetWorkspaceSize": (_I32, [_P, _P, _P, _P, _P, _B, _D, _P, _P, _PU64, _PP]),
+    "aclnnRotaryEmbedding": _PHASE2,
+    "aclnnRotaryEmbeddingBackwardGetWorkspaceSize": (_I32, [_P, _P, _P, _P, _P, _B, _D, _P, _P, _PU64, _PP]),
+    "aclnnRotaryEmbeddingBackward": _PHASE2,
+    "aclnnRotaryFrequenciesGetWorkspaceSize": (_I32, [_D, _I64, _D, _D, _D, _D, _P, _PU64, _PP]),
+    "aclnnRotaryFrequencies": _PHASE2,
+}
+
 _lib = None
 
 
@@ -128,7 +147,7 @@ def lib():
         if not os.path.exists(LIB_PATH):
             raise OSError(f"{LIB_PATH} not found: build it with __graft_entry__.build() or `make -C {CSRC_DIR}`")
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (restype, argtypes) in SYMBOLS.items():
+        for name, (restype, argtypes) in (*SYMBOLS.items(), *SEQUENCE_SYMBOLS.items()):
             fn = getattr(handle, name)
             fn.restype = restype
             fn.argtypes = argtypes
@@ -150,3 +169,4 @@ def native_module():
 
 
 from .aclnn import *  # noqa: E402,F401,F403
+from .sequence import *  # noqa: E402,F401,F403

@@ -195,6 +195,7 @@ const char* DtypeName(aclDataType d)
         case ACL_INT64: return "INT64";
         case ACL_UINT8: return "UINT8";
         case ACL_BOOL: return "BOOL";
+        case ACL_FLOAT8_E4M3FN: return "FLOAT8_E4M3FN";
         default: return "UNKNOWN";
     }
 }

@@ -4,6 +4,7 @@
 // a call, several times the GPU time of a small one; this costs about 3 us.
 //
 // The functions take positional arguments in the order of the wrappers in aclnn.py, which document them.
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -14,6 +15,7 @@
 
 #include <string>
 
+#include "../../include/aclnn_sequence.h"
 #include "host_common.h"
 
 namespace {
@@ -611,6 +613,215 @@ PyObject* GridSamplerBackward(Args a)
     return pair;
 }
 
+// ---- operators on sequences of tokens ----------------------------------------------------------------------------------------
+bool Given(PyObject* o) { return o != Py_None; }
+
+// The tensors of one call: all on the first one's device, which is the current one while the call lasts.
+class Call {
+public:
+    explicit Call(const at::Tensor& first) : device_(first.device())
+    {
+        if (device_.is_cuda()) {
+            guard_.set_index(device_.index());
+        }
+    }
+    const at::Device& Device() const { return device_; }
+    const at::Tensor& Of(PyObject* o) const
+    {
+        const at::Tensor& t = TensorOf(o);
+        if (t.device() != device_) {
+            Raise(PyExc_ValueError, "expected all tensors on one device");
+        }
+        return t;
+    }
+    // The acl object of a tensor argument that may be None: `Ptr` is null then.
+    struct Acl {
+        aclTensor t;
+        bool given = false;
+        aclTensor* Ptr() { return given ? &t : nullptr; }
+    };
+    Acl Maybe(PyObject* o) const
+    {
+        Acl a;
+        if (Given(o)) {
+            a.t = AclOf(Of(o), ACL_FORMAT_ND);
+            a.given = true;
+        }
+        return a;
+    }
+    at::Tensor OutOr(PyObject* o, at::IntArrayRef shape, const at::TensorOptions& options) const
+    {
+        return Given(o) ? Of(o) : at::empty(shape, options);
+    }
+
+private:
+    at::Device device_;
+    c10::cuda::OptionalCUDAGuard guard_;
+};
+
+PyObject* GiveAll(std::initializer_list<const at::Tensor*> ts)
+{
+    PyObject* tuple = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
+    if (tuple == nullptr) {
+        throw Raised{};
+    }
+    Py_ssize_t i = 0;
+    for (const at::Tensor* t : ts) {
+        if (t->defined()) {
+            PyTuple_SET_ITEM(tuple, i++, Give(*t));
+        } else {
+            Py_INCREF(Py_None);
+            PyTuple_SET_ITEM(tuple, i++, Py_None);
+        }
+    }
+    return tuple;
+}
+
+at::IntArrayRef LeadOf(const at::Tensor& t)
+{
+    if (t.dim() < 1) {
+        Raise(PyExc_ValueError, "expected at least one dimension");
+    }
+    return t.sizes().slice(0, t.dim() - 1);
+}
+
+// (x, residual, weight, eps, y, sum, rstd, workspace)
+PyObject* ResidualRmsNorm(Args a)
+{
+    const at::Tensor& x = TensorOf(a[0]);
+    const Call call(x);
+    Call::Acl tr = call.Maybe(a[1]), tw = call.Maybe(a[2]);
+    const double eps = DoubleOf(a[3]);
+    const at::Tensor y = call.OutOr(a[4], x.sizes(), x.options());
+    const at::Tensor sum = Given(a[1]) || Given(a[5]) ? call.OutOr(a[5], x.sizes(), x.options()) : x;
+    const at::Tensor rstd = call.OutOr(a[6], LeadOf(x), x.options().dtype(at::kFloat));
+    const aclTensor tx = AclOf(x, ACL_FORMAT_ND);
+    aclTensor ty = AclOf(y, ACL_FORMAT_ND), ts = AclOf(sum, ACL_FORMAT_ND), tv = AclOf(rstd, ACL_FORMAT_ND);
+    aclTensor* sumOut = Given(a[1]) || Given(a[5]) ? &ts : nullptr;
+    TwoPhase("aclnnResidualRmsNorm", [&](uint64_t* n, aclOpExecutor** e) {
+        return aclnnResidualRmsNormGetWorkspaceSize(&tx, tr.Ptr(), tw.Ptr(), eps, &ty, sumOut, &tv, n, e);
+    }, aclnnResidualRmsNorm, call.Device(), a[7]);
+    return GiveAll({&y, &sum, &rstd});
+}
+
+// (grad_y, sum, rstd, weight, grad_sum, grad_x, grad_weight, workspace)
+PyObject* ResidualRmsNormBackward(Args a)
+{
+    const at::Tensor& g = TensorOf(a[0]);
+    const Call call(g);
+    const aclTensor tg = AclOf(g, ACL_FORMAT_ND), tz = AclOf(call.Of(a[1]), ACL_FORMAT_ND), tv = AclOf(call.Of(a[2]), ACL_FORMAT_ND);
+    Call::Acl tw = call.Maybe(a[3]), ta = call.Maybe(a[4]);
+    const at::Tensor gx = call.OutOr(a[5], g.sizes(), g.options());
+    at::Tensor gw;
+    if (Given(a[6])) {
+        gw = call.Of(a[6]);
+    } else if (tw.given) {
+        gw = at::empty(TensorOf(a[3]).sizes(), TensorOf(a[3]).options());
+    }
+    aclTensor tx = AclOf(gx, ACL_FORMAT_ND), tgw;
+    if (gw.defined()) {
+        tgw = AclOf(gw, ACL_FORMAT_ND);
+    }
+    TwoPhase("aclnnResidualRmsNormBackward", [&](uint64_t* n, aclOpExecutor** e) {
+        return aclnnResidualRmsNormBackwardGetWorkspaceSize(&tg, &tz, &tv, tw.Ptr(), ta.Ptr(), &tx, gw.defined() ? &tgw : nullptr, n,
+                                                            e);
+    }, aclnnResidualRmsNormBackward, call.Device(), a[7]);
+    return GiveAll({&gx, &gw});
+}
+
+// (x, residual, weight, eps, int8, group, out, scales, sum, workspace)
+PyObject* ResidualRmsNormQuant(Args a)
+{
+    const at::Tensor& x = TensorOf(a[0]);
+    const Call call(x);
+    Call::Acl tr = call.Maybe(a[1]), tw = call.Maybe(a[2]);
+    const double eps = DoubleOf(a[3]);
+    const bool int8 = BoolOf(a[4]);
+    const int64_t group = IntOf(a[5]);
+    const at::Tensor q = call.OutOr(a[6], x.sizes(), x.options().dtype(int8 ? at::kChar : at::kFloat8_e4m3fn));
+    if (q.scalar_type() != (int8 ? at::kChar : at::kFloat8_e4m3fn)) {
+        Raise(PyExc_ValueError, "out does not have the type that is asked for");
+    }
+    std::vector<int64_t> shape = LeadOf(x).vec();
+    shape.push_back(group > 0 ? (x.size(-1) + group - 1) / group : 1);
+    const at::Tensor scales = call.OutOr(a[7], shape, x.options().dtype(at::kFloat));
+    const at::Tensor sum = Given(a[1]) || Given(a[8]) ? call.OutOr(a[8], x.sizes(), x.options()) : x;
+    const aclTensor tx = AclOf(x, ACL_FORMAT_ND);
+    aclTensor tq;
+    if (q.dim() > 8) {
+        RaiseStatus("aclCreateTensor", -1);
+    }
+    tq.dims.assign(q.sizes().begin(), q.sizes().end());
+    tq.strides.assign(q.strides().begin(), q.strides().end());
+    tq.dtype = int8 ? ACL_INT8 : ACL_FLOAT8_E4M3FN;
+    tq.data = q.data_ptr();
+    aclTensor tc = AclOf(scales, ACL_FORMAT_ND), ts = AclOf(sum, ACL_FORMAT_ND);
+    aclTensor* sumOut = Given(a[1]) || Given(a[8]) ? &ts : nullptr;
+    TwoPhase("aclnnResidualRmsNormQuant", [&](uint64_t* n, aclOpExecutor** e) {
+        return aclnnResidualRmsNormQuantGetWorkspaceSize(&tx, tr.Ptr(), tw.Ptr(), eps, group, &tq, &tc, sumOut, n, e);
+    }, aclnnResidualRmsNormQuant, call.Device(), a[9]);
+    return GiveAll({&q, &scales, &sum});
+}
+
+// (q, k, positions, frequencies, interleaved, sections, scale, q_out, k_out, workspace, backward)
+PyObject* Rotary(Args a)
+{
+    const at::Tensor& q = TensorOf(a[0]);
+    const Call call(q);
+    Call::Acl tk = call.Maybe(a[1]);
+    at::Tensor positions = call.Of(a[2]);
+    const aclTensor tf = AclOf(call.Of(a[3]), ACL_FORMAT_ND);
+    const bool interleaved = BoolOf(a[4]);
+    aclIntArray sections;
+    if (Given(a[5])) {
+        sections = IntArrayOf(a[5]);
+    } else if (q.dim() >= 2) {
+        positions = positions.expand(q.sizes().slice(0, q.dim() - 2)); // one position for several tokens
+    }
+    const double scale = DoubleOf(a[6]);
+    const at::Tensor qo = call.OutOr(a[7], q.sizes(), q.options());
+    at::Tensor ko;
+    if (tk.given) {
+        ko = call.OutOr(a[8], TensorOf(a[1]).sizes(), TensorOf(a[1]).options());
+    } else if (Given(a[8])) {
+        Raise(PyExc_ValueError, "an output for k without k");
+    }
+    const bool backward = BoolOf(a[10]);
+    const aclTensor tq = AclOf(q, ACL_FORMAT_ND), tp = AclOf(positions, ACL_FORMAT_ND);
+    aclTensor tqo = AclOf(qo, ACL_FORMAT_ND), tko;
+    if (tk.given) {
+        tko = AclOf(ko, ACL_FORMAT_ND);
+    }
+    const aclIntArray* parts = Given(a[5]) ? &sections : nullptr;
+    if (backward) {
+        TwoPhase("aclnnRotaryEmbeddingBackward", [&](uint64_t* n, aclOpExecutor** e) {
+            return aclnnRotaryEmbeddingBackwardGetWorkspaceSize(&tq, tk.Ptr(), &tp, &tf, parts, interleaved, scale, &tqo,
+                                                                tk.given ? &tko : nullptr, n, e);
+        }, aclnnRotaryEmbeddingBackward, call.Device(), a[9]);
+    } else {
+        TwoPhase("aclnnRotaryEmbedding", [&](uint64_t* n, aclOpExecutor** e) {
+            return aclnnRotaryEmbeddingGetWorkspaceSize(&tq, tk.Ptr(), &tp, &tf, parts, interleaved, scale, &tqo,
+                                                        tk.given ? &tko : nullptr, n, e);
+        }, aclnnRotaryEmbedding, call.Device(), a[9]);
+    }
+    return GiveAll({&qo, &ko});
+}
+
+// (out, base, scaling, factor, original_length, low, high)
+PyObject* RotaryFrequenciesOf(Args a)
+{
+    const at::Tensor& out = TensorOf(a[0]);
+    const Call call(out);
+    const double base = DoubleOf(a[1]);
+    const int64_t scaling = IntOf(a[2]);
+    const double factor = DoubleOf(a[3]), length = DoubleOf(a[4]), low = DoubleOf(a[5]), high = DoubleOf(a[6]);
+    aclTensor t = AclOf(out, ACL_FORMAT_ND);
+    TwoPhase("aclnnRotaryFrequencies", [&](uint64_t* n, aclOpExecutor** e) {
+        return aclnnRotaryFrequenciesGetWorkspaceSize(base, scaling, factor, length, low, high, &t, n, e);
+    }, aclnnRotaryFrequencies, call.Device(), Py_None);
+    return Give(out);
+}
+
 // Argument count, C++ exceptions.
 template <PyObject* (*F)(Args), int N>
 PyObject* Entry(PyObject*, PyObject* const* args, Py_ssize_t n)
@@ -668,6 +879,11 @@ PyMethodDef kMethods[] = {
     OPSCV_METHOD("upsample_trilinear3d_backward", Trilinear3dBackward, 8),
     OPSCV_METHOD("grid_sampler", GridSampler, 8),
     OPSCV_METHOD("grid_sampler_backward", GridSamplerBackward, 11),
+    OPSCV_METHOD("residual_rms_norm", ResidualRmsNorm, 8),
+    OPSCV_METHOD("residual_rms_norm_backward", ResidualRmsNormBackward, 8),
+    OPSCV_METHOD("residual_rms_norm_quant", ResidualRmsNormQuant, 10),
+    OPSCV_METHOD("rotary_embedding", Rotary, 11),
+    OPSCV_METHOD("rotary_frequencies", RotaryFrequenciesOf, 7),
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -1,0 +1,882 @@
+// Root-mean-square norm of a residual sum, with its gradient and with 8-bit outputs.
+//
+// z = T(x + residual) is rounded to the storage type first and everything else is a function of that stored value, so that the
+// backward, which reads z and not its two terms, is the gradient of exactly what the forward computed. Squares, their mean, the
+// dot product of the backward and the sums of the weight's gradient are fp32.
+//
+// Bound by HBM: the forward moves two rows in and two out, the backward three in and one out. A row stays in registers between
+// the reduction and the output (each thread owns the same columns in every pass over the row), so each value moves once.
+#include <cuda_fp8.h>
+
+#include "launch_util.cuh"
+#include "sequence_kernels.h"
+
+namespace opscv {
+
+namespace {
+
+constexpr int kMaxThreads = 1024;
+
+__device__ __forceinline__ int64_t RowAt(int64_t row, int64_t inner, RowStride s)
+{
+    return row < inner ? row * s.s1 : row / inner * s.s0 + row % inner * s.s1;
+}
+
+// V values of T as fp32; loads of up to 16 bytes.
+template <typename T, int V>
+__device__ __forceinline__ void LoadF(const T* p, float (&v)[V])
+{
+    if constexpr (V == 1) {
+        v[0] = DType<T>::ToF(*p);
+    } else {
+        LoadPack<T, V>(p, v);
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void StoreF(T* p, const float (&v)[V])
+{
+    if constexpr (V == 1) {
+        *p = DType<T>::FromF(v[0]);
+    } else {
+        StorePack<T, V>(p, v);
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void LoadWeight(const void* w, bool w32, int32_t col, float (&v)[V])
+{
+    if (w == nullptr) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] = 1.0f;
+        }
+    } else if (w32) {
+        const float* p = static_cast<const float*>(w) + col;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] = __ldg(p + i);
+        }
+    } else {
+        LoadF<T, V>(static_cast<const T*>(w) + col, v);
+    }
+}
+
+// The sum of v over the blockDim.x threads of a row, for all of them. Rows of one warp need no shared memory. The order of the
+// additions is fixed, so equal inputs give equal bits.
+__device__ __forceinline__ float RowSum(float v, float* part)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    if (blockDim.x == 32) {
+        return v;
+    }
+    // one row a block: rows of several warps have blockDim.y == 1
+    const int warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) {
+        part[threadIdx.x >> 5] = v;
+    }
+    __syncthreads();
+    v = static_cast<int>(threadIdx.x & 31) < warps ? part[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    return v;
+}
+
+struct FwdArgs {
+    const void *x, *residual, *weight;
+    void *y, *sum;
+    float* rstd;
+    RowStride xs, rs, ys, ss;
+    int64_t rows, inner;
+    int32_t width;
+    float eps;
+    bool weight32;
+    // 8-bit outputs
+    float* scales;
+    int32_t group, groups;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void LoadSum(const T* x, const T* r, int32_t col, float (&z)[V])
+{
+    LoadF<T, V>(x + col, z);
+    if (r != nullptr) {
+        float b[V];
+        LoadF<T, V>(r + col, b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            z[i] = DType<T>::ToF(DType<T>::FromF(z[i] + b[i]));
+        }
+    }
+}
+
+// NV > 0: the row is held in NV * V values a thread. NV == 0: rows too wide for that are read again for the second pass (from L2
+// mostly), from `sum` where there is one, since it may lie over one of the terms.
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(kMaxThreads) RmsNormFwdKernel(FwdArgs a)
+{
+    // the weight is read before the reduction's wait, whose time covers the load's, where the registers hold both
+    constexpr bool kEarlyWeight = NV > 0 && NV * V <= 16;
+    __shared__ float part[32];
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (row >= a.rows) { // rows of several warps have one row a block, so that no barrier is left out
+        return;
+    }
+    const T* x = static_cast<const T*>(a.x) + RowAt(row, a.inner, a.xs);
+    const T* r = a.residual != nullptr ? static_cast<const T*>(a.residual) + RowAt(row, a.inner, a.rs) : nullptr;
+    T* y = static_cast<T*>(a.y) + RowAt(row, a.inner, a.ys);
+    T* sum = a.sum != nullptr ? static_cast<T*>(a.sum) + RowAt(row, a.inner, a.ss) : nullptr;
+    const int32_t step = blockDim.x * V;
+    const int32_t first = threadIdx.x * V;
+    constexpr int N = NV > 0 ? NV : 1;
+    float z[N][V];
+    float w[kEarlyWeight ? N : 1][V];
+    float sq = 0.0f;
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int32_t col = first + k * step;
+            if (col < a.width) {
+                LoadSum<T, V>(x, r, col, z[k]);
+                if constexpr (kEarlyWeight) {
+                    LoadWeight<T, V>(a.weight, a.weight32, col, w[k]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    z[k][i] = 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                sq = fmaf(z[k][i], z[k][i], sq);
+            }
+            const int32_t col = first + k * step;
+            if (sum != nullptr && col < a.width) {
+                StoreF<T, V>(sum + col, z[k]);
+            }
+        }
+    } else {
+        for (int32_t col = first; col < a.width; col += step) {
+            LoadSum<T, V>(x, r, col, z[0]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                sq = fmaf(z[0][i], z[0][i], sq);
+            }
+            if (sum != nullptr) {
+                StoreF<T, V>(sum + col, z[0]);
+            }
+        }
+    }
+    const float mean = RowSum(sq, part) / static_cast<float>(a.width);
+    const float rstd = 1.0f / sqrtf(mean + a.eps);
+    if (a.rstd != nullptr && threadIdx.x == 0) {
+        a.rstd[row] = rstd;
+    }
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int32_t col = first + k * step;
+            if (col < a.width) {
+                float(&wk)[V] = w[kEarlyWeight ? k : 0];
+                if constexpr (!kEarlyWeight) {
+                    LoadWeight<T, V>(a.weight, a.weight32, col, wk);
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    z[k][i] *= rstd * wk[i];
+                }
+                StoreF<T, V>(y + col, z[k]);
+            }
+        }
+    } else {
+        for (int32_t col = first; col < a.width; col += step) {
+            if (sum != nullptr) {
+                LoadF<T, V>(sum + col, z[0]);
+            } else {
+                LoadSum<T, V>(x, r, col, z[0]);
+            }
+            LoadWeight<T, V>(a.weight, a.weight32, col, w[0]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                z[0][i] *= rstd * w[0][i];
+            }
+            StoreF<T, V>(y + col, z[0]);
+        }
+    }
+}
+
+// ---- 8-bit outputs ---------------------------------------------------------------------------------------------------------
+// The largest magnitude of non-negative floats as unsigned integers, which order alike; a NaN is above all others, so a row or
+// group with one gets a NaN as its scale.
+__device__ __forceinline__ uint32_t Magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+template <Q8 Q>
+struct Q8Type;
+template <>
+struct Q8Type<Q8::E4M3> {
+    static constexpr float kMost = 448.0f;
+    template <int V>
+    static __device__ __forceinline__ void Store(uint8_t* p, const float (&v)[V])
+    {
+        if constexpr (V == 1) {
+            *p = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
+        } else {
+            Pack<uint16_t, V / 2> b;
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                b.v[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+            }
+            *reinterpret_cast<Pack<uint16_t, V / 2>*>(p) = b;
+        }
+    }
+};
+template <>
+struct Q8Type<Q8::INT8> {
+    static constexpr float kMost = 127.0f;
+    template <int V>
+    static __device__ __forceinline__ void Store(uint8_t* p, const float (&v)[V])
+    {
+        Pack<uint8_t, V> b;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            b.v[i] = static_cast<uint8_t>(max(-127, min(127, __float2int_rn(v[i]))));
+        }
+        *reinterpret_cast<Pack<uint8_t, V>*>(p) = b;
+    }
+};
+
+// Value times this is the quantised value. A group of zeros (or one whose scale underflows) has scale 0 and zeros.
+__device__ __forceinline__ float Inverse(uint32_t most, float range) { return most == 0 ? 0.0f : range / __uint_as_float(most); }
+
+// LG: lanes of a group where a group lies within a warp (a power of two), 0 where groups go through shared memory, one word each.
+template <typename T, int V, int NV, Q8 Q, int LG>
+__global__ void __launch_bounds__(kMaxThreads) RmsNormQuantKernel(FwdArgs a)
+{
+    extern __shared__ uint32_t most[]; // [groups] (LG == 0)
+    __shared__ float part[32];
+    constexpr bool kEarlyWeight = NV > 0 && NV * V <= 16;
+    using QT = Q8Type<Q>;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (row >= a.rows) {
+        return;
+    }
+    const T* x = static_cast<const T*>(a.x) + RowAt(row, a.inner, a.xs);
+    const T* r = a.residual != nullptr ? static_cast<const T*>(a.residual) + RowAt(row, a.inner, a.rs) : nullptr;
+    uint8_t* q = static_cast<uint8_t*>(a.y) + row * a.width;
+    T* sum = a.sum != nullptr ? static_cast<T*>(a.sum) + RowAt(row, a.inner, a.ss) : nullptr;
+    float* scales = a.scales + row * a.groups;
+    const int32_t step = blockDim.x * V;
+    const int32_t first = threadIdx.x * V;
+    constexpr int N = NV > 0 ? NV : 1;
+    float z[N][V], w[kEarlyWeight ? N : 1][V];
+    float sq = 0.0f;
+    if constexpr (LG == 0) { // one row a block (the launcher sees to it)
+        for (int32_t g = threadIdx.x; g < a.groups; g += blockDim.x) {
+            most[g] = 0;
+        }
+        __syncthreads();
+    }
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int32_t col = first + k * step;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                z[k][i] = w[kEarlyWeight ? k : 0][i] = 0.0f;
+            }
+            if (col < a.width) {
+                LoadSum<T, V>(x, r, col, z[k]);
+                if constexpr (kEarlyWeight) {
+                    LoadWeight<T, V>(a.weight, a.weight32, col, w[k]);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                sq = fmaf(z[k][i], z[k][i], sq);
+            }
+            const int32_t col = first + k * step;
+            if (sum != nullptr && col < a.width) {
+                StoreF<T, V>(sum + col, z[k]);
+            }
+        }
+    } else {
+        for (int32_t col = first; col < a.width; col += step) {
+            LoadSum<T, V>(x, r, col, z[0]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                sq = fmaf(z[0][i], z[0][i], sq);
+            }
+            if (sum != nullptr) {
+                StoreF<T, V>(sum + col, z[0]);
+            }
+        }
+    }
+    const float rstd = 1.0f / sqrtf(RowSum(sq, part) / static_cast<float>(a.width) + a.eps);
+    if constexpr (NV > 0) {
+        uint32_t top[N]; // of this thread's values of chunk k
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            top[k] = 0;
+            const int32_t col = first + k * step;
+            float(&wk)[V] = w[kEarlyWeight ? k : 0];
+            if constexpr (!kEarlyWeight) {
+                if (col < a.width) {
+                    LoadWeight<T, V>(a.weight, a.weight32, col, wk);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                z[k][i] *= rstd * wk[i];
+                top[k] = max(top[k], Magnitude(z[k][i]));
+            }
+            if constexpr (LG > 0) {
+#pragma unroll
+                for (int o = LG / 2; o > 0; o >>= 1) {
+                    top[k] = max(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+                }
+                if (col < a.width) {
+                    const float inv = Inverse(top[k], QT::kMost);
+                    if ((threadIdx.x & (LG - 1)) == 0) {
+                        scales[col / a.group] = __uint_as_float(top[k]) / QT::kMost;
+                    }
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        z[k][i] *= inv;
+                    }
+                    QT::template Store<V>(q + col, z[k]);
+                }
+            } else if (a.groups > 1 && col < a.width) {
+                atomicMax(&most[col / a.group], top[k]);
+            }
+        }
+        if constexpr (LG == 0) {
+            if (a.groups == 1) {
+                uint32_t t = 0;
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    t = max(t, top[k]);
+                }
+                t = __reduce_max_sync(0xffffffffu, t);
+                if ((threadIdx.x & 31) == 0) {
+                    atomicMax(&most[0], t);
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int32_t col = first + k * step;
+                if (col < a.width) {
+                    const float inv = Inverse(most[a.groups > 1 ? col / a.group : 0], QT::kMost);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        z[k][i] *= inv;
+                    }
+                    QT::template Store<V>(q + col, z[k]);
+                }
+            }
+        }
+    } else {
+        static_assert(LG == 0, "wide rows use shared memory");
+        for (int pass = 0; pass < 2; ++pass) {
+            for (int32_t col = first; col < a.width; col += step) {
+                if (sum != nullptr) {
+                    LoadF<T, V>(sum + col, z[0]);
+                } else {
+                    LoadSum<T, V>(x, r, col, z[0]);
+                }
+                LoadWeight<T, V>(a.weight, a.weight32, col, w[0]);
+                const int32_t g = a.groups > 1 ? col / a.group : 0;
+                const float inv = pass == 0 ? 0.0f : Inverse(most[g], QT::kMost);
+                uint32_t t = 0;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    z[0][i] *= rstd * w[0][i];
+                    t = max(t, Magnitude(z[0][i]));
+                    z[0][i] *= inv;
+                }
+                if (pass == 0) {
+                    atomicMax(&most[g], t);
+                } else {
+                    QT::template Store<V>(q + col, z[0]);
+                }
+            }
+            __syncthreads();
+        }
+    }
+    if constexpr (LG == 0) {
+        for (int32_t g = threadIdx.x; g < a.groups; g += blockDim.x) {
+            scales[g] = __uint_as_float(most[g]) / QT::kMost;
+        }
+    }
+}
+
+// ---- backward --------------------------------------------------------------------------------------------------------------
+struct BwdArgs {
+    const void *gradY, *sum, *weight, *gradSum;
+    const float* rstd;
+    void* gradX;
+    float* scratch; // [gridDim.x][width] sums of the weight's gradient, null without a weight
+    RowStride gs, ss, as, xs;
+    int64_t rows, inner;
+    int32_t width;
+    bool weight32;
+};
+
+// A block walks rows blockIdx.x, + gridDim.x, ...; each thread keeps its columns' weight and the sum of the weight's gradient in
+// registers over all of them, so the weight's gradient costs no second pass over gradY and z. The rows' loads of one step are
+// issued before the reduction of the step before is waited for.
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(NV * V == 16 ? 512 : 1024) RmsNormBwdKernel(BwdArgs a)
+{
+    __shared__ float part[2][32];
+    const int32_t step = blockDim.x * V;
+    const int32_t first = threadIdx.x * V;
+    const float inverse = 1.0f / static_cast<float>(a.width);
+    float w[NV][V], gw[NV][V];
+    Pack<T, V> nextG[NV], nextZ[NV], nextA[NV];
+    float nextRstd = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int32_t col = first + k * step;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            w[k][i] = gw[k][i] = 0.0f;
+            nextG[k].v[i] = nextZ[k].v[i] = nextA[k].v[i] = DType<T>::FromF(0.0f);
+        }
+        if (col < a.width) {
+            LoadWeight<T, V>(a.weight, a.weight32, col, w[k]);
+        }
+    }
+    auto fetch = [&](int64_t row) {
+        const T* g = static_cast<const T*>(a.gradY) + RowAt(row, a.inner, a.gs);
+        const T* z = static_cast<const T*>(a.sum) + RowAt(row, a.inner, a.ss);
+        const T* s = a.gradSum != nullptr ? static_cast<const T*>(a.gradSum) + RowAt(row, a.inner, a.as) : nullptr;
+        nextRstd = a.rstd[row];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int32_t col = first + k * step;
+            if (col < a.width) {
+                nextG[k] = *reinterpret_cast<const Pack<T, V>*>(g + col);
+                nextZ[k] = *reinterpret_cast<const Pack<T, V>*>(z + col);
+                if (s != nullptr) {
+                    nextA[k] = *reinterpret_cast<const Pack<T, V>*>(s + col);
+                }
+            }
+        }
+    };
+    int64_t row = blockIdx.x;
+    if (row < a.rows) {
+        fetch(row);
+    }
+    int turn = 0;
+    for (; row < a.rows; row += gridDim.x, turn ^= 1) {
+        float g[NV][V], u[NV][V];
+        Pack<T, V> add[NV];
+        const float rstd = nextRstd;
+        float dot = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            UnpackToF<T, V>(nextG[k], g[k]);
+            UnpackToF<T, V>(nextZ[k], u[k]);
+            add[k] = nextA[k];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                u[k][i] *= rstd;
+                gw[k][i] = fmaf(g[k][i], u[k][i], gw[k][i]);
+                g[k][i] *= w[k][i];
+                dot = fmaf(g[k][i], u[k][i], dot);
+            }
+        }
+        if (row + gridDim.x < a.rows) {
+            fetch(row + gridDim.x);
+        }
+        // two sets of partial sums in turn: the next row's are written while a slow warp still reads this row's
+        const float c = RowSum(dot, part[turn]) * inverse;
+        T* out = static_cast<T*>(a.gradX) + RowAt(row, a.inner, a.xs);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int32_t col = first + k * step;
+            if (col < a.width) {
+                float v[V];
+                UnpackToF<T, V>(add[k], v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    v[i] = fmaf(rstd, g[k][i] - u[k][i] * c, v[i]);
+                }
+                StoreF<T, V>(out + col, v);
+            }
+        }
+    }
+    if (a.scratch != nullptr) {
+        float* s = a.scratch + static_cast<int64_t>(blockIdx.x) * a.width;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int32_t col = first + k * step;
+            if (col < a.width) {
+                StoreF<float, V>(s + col, gw[k]);
+            }
+        }
+    }
+}
+
+// Rows too wide for the registers of a block: gradX with two passes over the row.
+template <typename T, int V>
+__global__ void __launch_bounds__(kMaxThreads) RmsNormBwdWideKernel(BwdArgs a)
+{
+    __shared__ float part[32];
+    const int64_t row = blockIdx.x;
+    const T* gy = static_cast<const T*>(a.gradY) + RowAt(row, a.inner, a.gs);
+    const T* z = static_cast<const T*>(a.sum) + RowAt(row, a.inner, a.ss);
+    const T* s = a.gradSum != nullptr ? static_cast<const T*>(a.gradSum) + RowAt(row, a.inner, a.as) : nullptr;
+    T* out = static_cast<T*>(a.gradX) + RowAt(row, a.inner, a.xs);
+    const float rstd = a.rstd[row];
+    float dot = 0.0f;
+    const int32_t step = blockDim.x * V;
+    for (int32_t col = threadIdx.x * V; col < a.width; col += step) {
+        float g[V], u[V], w[V];
+        LoadF<T, V>(gy + col, g);
+        LoadF<T, V>(z + col, u);
+        LoadWeight<T, V>(a.weight, a.weight32, col, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            dot = fmaf(g[i] * w[i], u[i] * rstd, dot);
+        }
+    }
+    const float c = RowSum(dot, part) / static_cast<float>(a.width);
+    for (int32_t col = threadIdx.x * V; col < a.width; col += step) {
+        float g[V], u[V], w[V], v[V];
+        LoadF<T, V>(gy + col, g);
+        LoadF<T, V>(z + col, u);
+        LoadWeight<T, V>(a.weight, a.weight32, col, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] = 0.0f;
+        }
+        if (s != nullptr) {
+            LoadF<T, V>(s + col, v);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] = fmaf(rstd, g[i] * w[i] - u[i] * rstd * c, v[i]);
+        }
+        StoreF<T, V>(out + col, v);
+    }
+}
+// and the sums of the weight's gradient: a thread per column, a block per (columns, share of the rows).
+template <typename T>
+__global__ void RmsNormWeightSumsKernel(BwdArgs a)
+{
+    const int32_t col = blockIdx.y * blockDim.x + threadIdx.x;
+    if (col >= a.width) {
+        return;
+    }
+    float acc = 0.0f;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float g = DType<T>::ToF(static_cast<const T*>(a.gradY)[RowAt(row, a.inner, a.gs) + col]);
+        const float z = DType<T>::ToF(static_cast<const T*>(a.sum)[RowAt(row, a.inner, a.ss) + col]);
+        acc = fmaf(g, z * a.rstd[row], acc);
+    }
+    a.scratch[static_cast<int64_t>(blockIdx.x) * a.width + col] = acc;
+}
+
+// The blocks' sums of one column, added in a fixed order: 8 warps take every eighth block, then add up.
+template <typename W>
+__global__ void __launch_bounds__(256) RmsNormWeightGradKernel(const float* scratch, int32_t blocks, int32_t width, W* out)
+{
+    __shared__ float part[8][33];
+    const int32_t col = blockIdx.x * 32 + threadIdx.x;
+    float acc = 0.0f;
+    if (col < width) {
+        for (int32_t b = threadIdx.y; b < blocks; b += 8) {
+            acc += scratch[static_cast<int64_t>(b) * width + col];
+        }
+    }
+    part[threadIdx.y][threadIdx.x] = acc;
+    __syncthreads();
+    if (threadIdx.y == 0 && col < width) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+            acc += part[i][threadIdx.x];
+        }
+        out[col] = DType<W>::FromF(acc);
+    }
+}
+
+// ---- launch shapes ---------------------------------------------------------------------------------------------------------
+// The widest vector that the row length, the row strides and the pointers allow.
+struct RowUse {
+    const void* p;
+    RowStride s;
+};
+int VecOfRows(int elem, const NormShape& n, std::initializer_list<RowUse> uses)
+{
+    int v = 16 / elem;
+    for (; v > 1; v >>= 1) {
+        bool ok = n.width % v == 0;
+        for (const RowUse& u : uses) {
+            ok = ok && (u.p == nullptr || (Aligned(u.p, static_cast<size_t>(v) * elem) && u.s.s0 % v == 0 && u.s.s1 % v == 0));
+        }
+        if (ok) {
+            break;
+        }
+    }
+    return v;
+}
+
+// Threads of a row and chunks of V values per thread. Rows of up to 4 chunks a lane take one warp each, 4 rows a block; wider
+// ones a block of their own with as few chunks per thread as 512 threads allow, and up to 1024 threads with the most chunks that
+// `values` a thread allow. nv 0: too wide for that.
+struct RowShape {
+    int nv, threads, rows;
+};
+RowShape ShapeOfRow(int32_t width, int v, int values, int mostThreads)
+{
+    const int32_t chunks = (width + v - 1) / v;
+    if (chunks <= 32 * 4) {
+        const int nv = chunks <= 32 ? 1 : (chunks <= 64 ? 2 : 4);
+        if (nv * v <= values) {
+            return {nv, 32, 4};
+        }
+    }
+    for (int nv = 1; nv <= 8 && nv * v <= values; nv *= 2) {
+        const bool last = nv == 8 || 2 * nv * v > values;
+        const int32_t threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
+        if (threads <= (last ? mostThreads : 512)) {
+            return {nv, threads, 1};
+        }
+    }
+    return {0, kMaxThreads, 1};
+}
+
+#define OPSCV_DISPATCH_NV(nv, NV, ...)                                 \
+    {                                                                  \
+        auto opscvNv_ = [&](auto opscvNvTag_) {                        \
+            constexpr int NV = decltype(opscvNvTag_)::value;           \
+            __VA_ARGS__;                                               \
+        };                                                             \
+        switch (nv) {                                                  \
+            case 8: opscvNv_(std::integral_constant<int, 8>{}); break; \
+            case 4: opscvNv_(std::integral_constant<int, 4>{}); break; \
+            case 2: opscvNv_(std::integral_constant<int, 2>{}); break; \
+            case 1: opscvNv_(std::integral_constant<int, 1>{}); break; \
+            default: opscvNv_(std::integral_constant<int, 0>{}); break; \
+        }                                                              \
+    }
+
+FwdArgs MakeFwd(const NormShape& n, const void* x, RowStride xs, const void* residual, RowStride rs, const void* weight,
+                void* sum, RowStride ss)
+{
+    FwdArgs a{};
+    a.x = x;
+    a.residual = residual;
+    a.weight = weight;
+    a.sum = sum;
+    a.xs = xs;
+    a.rs = rs;
+    a.ss = ss;
+    a.rows = n.rows;
+    a.inner = n.inner;
+    a.width = n.width;
+    a.eps = static_cast<float>(n.eps);
+    a.weight32 = n.weight32;
+    return a;
+}
+
+bool GridFits(int64_t blocks) { return blocks <= INT32_MAX; }
+
+} // namespace
+
+cudaError_t RmsNormFwd(Dt dt, const NormShape& n, const void* x, RowStride xs, const void* residual, RowStride rs,
+                       const void* weight, void* y, RowStride ys, void* sum, RowStride ss, float* rstd, cudaStream_t s)
+{
+    FwdArgs a = MakeFwd(n, x, xs, residual, rs, weight, sum, ss);
+    a.y = y;
+    a.ys = ys;
+    a.rstd = rstd;
+    const int v = VecOfRows(DtSize(dt), n,
+                            {{x, xs}, {residual, rs}, {y, ys}, {sum, ss}, {n.weight32 ? nullptr : weight, {}}});
+    const RowShape shape = ShapeOfRow(n.width, v, 32, kMaxThreads);
+    const int64_t blocks = CeilDiv(n.rows, shape.rows);
+    if (!GridFits(blocks)) {
+        return cudaErrorInvalidConfiguration;
+    }
+    const dim3 block(shape.threads, shape.rows);
+    OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
+        OPSCV_DISPATCH_NV(shape.nv, NV, if constexpr (NV * V <= 32) {
+            RmsNormFwdKernel<T, V, NV><<<static_cast<unsigned>(blocks), block, 0, s>>>(a);
+        });
+    }));
+    CountLaunch();
+    return cudaGetLastError();
+}
+
+cudaError_t RmsNormQuant(Dt dt, const NormShape& n, const void* x, RowStride xs, const void* residual, RowStride rs,
+                         const void* weight, Q8 type, int32_t group, void* q, float* scales, void* sum, RowStride ss,
+                         cudaStream_t s)
+{
+    FwdArgs a = MakeFwd(n, x, xs, residual, rs, weight, sum, ss);
+    a.y = q;
+    a.scales = scales;
+    a.group = group > 0 ? group : n.width;
+    a.groups = (n.width + a.group - 1) / a.group;
+    int v = VecOfRows(DtSize(dt), n, {{x, xs}, {residual, rs}, {sum, ss}, {n.weight32 ? nullptr : weight, {}}});
+    while (v > 1 && !(n.width % v == 0 && Aligned(q, v))) {
+        v >>= 1;
+    }
+    RowShape shape = ShapeOfRow(n.width, v, 32, kMaxThreads);
+    // Groups of 128 columns read with at least four to a lane lie within a warp (lanes hold consecutive chunks of a row, and a
+    // warp's first chunk starts a group); others go through shared memory, with one row a block.
+    const bool inWarp = a.groups > 1 && a.group == 128 && shape.nv > 0 && v >= 4;
+    if (!inWarp) {
+        shape.rows = 1;
+    }
+    const int64_t blocks = CeilDiv(n.rows, shape.rows);
+    const size_t shared = inWarp ? 0 : static_cast<size_t>(a.groups) * 4;
+    if (!GridFits(blocks) || shared > 40 * 1024) {
+        return cudaErrorInvalidConfiguration;
+    }
+    const dim3 block(shape.threads, shape.rows);
+    const unsigned grid = static_cast<unsigned>(blocks);
+    OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
+        OPSCV_DISPATCH_NV(shape.nv, NV, if constexpr (NV * V <= 32) {
+            constexpr int LG = NV > 0 && V >= 4 ? 128 / V : 0;
+            if (type == Q8::E4M3) {
+                if (inWarp) {
+                    RmsNormQuantKernel<T, V, NV, Q8::E4M3, LG><<<grid, block, shared, s>>>(a);
+                } else {
+                    RmsNormQuantKernel<T, V, NV, Q8::E4M3, 0><<<grid, block, shared, s>>>(a);
+                }
+            } else if (inWarp) {
+                RmsNormQuantKernel<T, V, NV, Q8::INT8, LG><<<grid, block, shared, s>>>(a);
+            } else {
+                RmsNormQuantKernel<T, V, NV, Q8::INT8, 0><<<grid, block, shared, s>>>(a);
+            }
+        });
+    }));
+    CountLaunch();
+    return cudaGetLastError();
+}
+
+namespace {
+
+// The backward's grid: the weight's gradient takes a row of fp32 sums per block, so the blocks walk the rows, as many of them as
+// the device holds at once (about 1024 threads an SM: two blocks of 512 or more of fewer threads).
+struct BwdPlan {
+    int v;
+    RowShape shape;
+    int64_t blocks;
+};
+BwdPlan PlanBwd(int v, const NormShape& n)
+{
+    BwdPlan p{};
+    p.v = v;
+    p.shape = ShapeOfRow(n.width, v, 16, v >= 4 ? 512 : kMaxThreads);
+    if (p.shape.nv > 0 && p.shape.threads == 32 && p.shape.rows > 1) {
+        // one row a block here too, of as many warps as give each lane one chunk
+        const int32_t chunks = (n.width + v - 1) / v;
+        p.shape.nv = 1;
+        p.shape.threads = (chunks + 31) / 32 * 32;
+        p.shape.rows = 1;
+    }
+    if (p.shape.nv > 0) {
+        const int perSm = p.shape.threads >= 512 ? (p.shape.threads > 512 ? 1 : 2) : 1024 / p.shape.threads;
+        p.blocks = static_cast<int64_t>(NumSMs()) * (perSm < 16 ? perSm : 16);
+    } else {
+        p.blocks = 64;
+    }
+    p.blocks = p.blocks < n.rows ? p.blocks : n.rows;
+    return p;
+}
+
+} // namespace
+
+int64_t RmsNormBwdScratch(Dt dt, const NormShape& n, bool weight)
+{
+    if (!weight) {
+        return 0;
+    }
+    int64_t most = 0; // the vector width is known only with the pointers
+    for (int v = 16 / DtSize(dt); v >= 1; v >>= 1) {
+        const int64_t b = PlanBwd(v, n).blocks;
+        most = b > most ? b : most;
+    }
+    return most * n.width;
+}
+
+cudaError_t RmsNormBwd(Dt dt, const NormShape& n, const void* gradY, RowStride gs, const void* sum, RowStride ss,
+                       const float* rstd, const void* weight, const void* gradSum, RowStride as, void* gradX,
+                       RowStride xs, void* gradWeight, float* scratch, int64_t scratchFloats, cudaStream_t s)
+{
+    if (n.rows == 0) { // no rows: the weight's gradient is zero
+        return gradWeight == nullptr ? cudaSuccess :
+                                       cudaMemsetAsync(gradWeight, 0, static_cast<size_t>(n.width) * (n.weight32 ? 4 : DtSize(dt)), s);
+    }
+    BwdArgs a{};
+    a.gradY = gradY;
+    a.sum = sum;
+    a.weight = weight;
+    a.gradSum = gradSum;
+    a.rstd = rstd;
+    a.gradX = gradX;
+    a.scratch = gradWeight != nullptr ? scratch : nullptr;
+    a.gs = gs;
+    a.ss = ss;
+    a.as = as;
+    a.xs = xs;
+    a.rows = n.rows;
+    a.inner = n.inner;
+    a.width = n.width;
+    a.weight32 = n.weight32;
+    const int v = VecOfRows(DtSize(dt), n,
+                            {{gradY, gs}, {sum, ss}, {gradSum, as}, {gradX, xs}, {n.weight32 ? nullptr : weight, {}}});
+    BwdPlan p = PlanBwd(v, n);
+    if (gradWeight != nullptr) { // the scratch was sized in the first phase
+        const int64_t room = scratchFloats / n.width;
+        p.blocks = p.blocks < room ? p.blocks : room;
+    }
+    if (p.shape.nv == 0) {
+        if (!GridFits(n.rows)) {
+            return cudaErrorInvalidConfiguration;
+        }
+        if (a.scratch != nullptr) { // before gradX, which may lie over gradY
+            const dim3 grid(static_cast<unsigned>(p.blocks), static_cast<unsigned>(CeilDiv(n.width, 256)));
+            OPSCV_DISPATCH_DT(dt, T, RmsNormWeightSumsKernel<T><<<grid, 256, 0, s>>>(a));
+            CountLaunch();
+        }
+        OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
+            RmsNormBwdWideKernel<T, V><<<static_cast<unsigned>(n.rows), kMaxThreads, 0, s>>>(a);
+        }));
+    } else {
+        OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
+            OPSCV_DISPATCH_NV(p.shape.nv, NV, if constexpr (NV > 0 && NV * V <= 16) {
+                RmsNormBwdKernel<T, V, NV><<<static_cast<unsigned>(p.blocks), p.shape.threads, 0, s>>>(a);
+            });
+        }));
+    }
+    CountLaunch();
+    if (gradWeight != nullptr) {
+        const unsigned grid = static_cast<unsigned>(CeilDiv(n.width, 32));
+        const dim3 block(32, 8);
+        if (n.weight32) {
+            RmsNormWeightGradKernel<float><<<grid, block, 0, s>>>(scratch, static_cast<int32_t>(p.blocks), n.width,
+                                                                  static_cast<float*>(gradWeight));
+        } else {
+            OPSCV_DISPATCH_DT(dt, T, RmsNormWeightGradKernel<T><<<grid, block, 0, s>>>(scratch, static_cast<int32_t>(p.blocks),
+                                                                                      n.width, static_cast<T*>(gradWeight)));
+        }
+        CountLaunch();
+    }
+    return cudaGetLastError();
+}
+
+} // namespace opscv

@@ -1,0 +1,155 @@
+"""First phases of the token-sequence operators (no GPU): exported symbols, what they accept and what they refuse, with which status.
+Tensors of these tests are on the CPU, so an accepted call ends before its second phase with the binding's ValueError."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+NULLPTR, INVALID = 161001, 161002
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def accepted(call):
+    with pytest.raises(ValueError, match="cuda device"):
+        call()
+
+
+def refused(ops, call, text="", status=INVALID):
+    with pytest.raises(ops.AclnnError) as e:
+        call()
+    assert e.value.status == status and text in str(e.value)
+
+
+def test_library_exports_the_declared_symbols(ops):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = open(os.path.join(root, "include", "aclnn_sequence.h")).read()
+    declared = set(re.findall(r"ACLNN_API\s+[\w\s\*]+?\b(\w+)\s*\(", text))
+    assert declared == set(ops.SEQUENCE_SYMBOLS)
+    handle = ctypes.CDLL(ops.LIB_PATH)
+    assert not [s for s in declared if not hasattr(handle, s)]
+
+
+def test_null_arguments(ops):
+    n, e = ctypes.c_uint64(7), ctypes.c_void_p(None)
+    L = ops.lib()
+    for name in sorted(s[:-len("GetWorkspaceSize")] for s in ops.SEQUENCE_SYMBOLS if s.endswith("GetWorkspaceSize")):
+        types = ops.SEQUENCE_SYMBOLS[name + "GetWorkspaceSize"][1]
+        zeros = [None if t is ctypes.c_void_p else t(0) for t in types[:-2]]
+        first = getattr(L, name + "GetWorkspaceSize")
+        assert first(*zeros, ctypes.byref(n), ctypes.byref(e)) == NULLPTR
+        assert first(*zeros, None, ctypes.byref(e)) == NULLPTR
+        assert first(*zeros, ctypes.byref(n), None) == NULLPTR
+        assert n.value == 7 and e.value is None
+        assert getattr(L, name)(None, 0, None, None) == NULLPTR
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+def test_norm_accepts(ops, t):
+    x = torch.zeros(2, 3, 8, dtype=t)
+    w = torch.ones(8, dtype=t)
+    accepted(lambda: ops.residual_rms_norm(x))
+    accepted(lambda: ops.residual_rms_norm(x, x, w, 0.0))
+    accepted(lambda: ops.residual_rms_norm(x, x, torch.ones(8)))
+    accepted(lambda: ops.residual_rms_norm(torch.zeros(8, dtype=t)))
+    accepted(lambda: ops.residual_rms_norm(torch.zeros(0, 8, dtype=t)))
+    accepted(lambda: ops.residual_rms_norm(x.expand(5, 2, 3, 8), None, w))
+    accepted(lambda: ops.residual_rms_norm(torch.zeros(2, 8, 3, dtype=t).transpose(1, 2), None, w))
+    accepted(lambda: ops.residual_rms_norm_backward(x, x, torch.zeros(2, 3), w, x))
+    accepted(lambda: ops.residual_rms_norm_backward(x, x, torch.zeros(2, 3)))
+    for group in (0, 32, 96, 128, 4096):
+        accepted(lambda: ops.residual_rms_norm_quant(x, x, w, group=group))
+        accepted(lambda: ops.residual_rms_norm_quant(x, x, w, dtype=torch.int8, group=group))
+
+
+def test_norm_refuses(ops):
+    x, w = torch.zeros(2, 3, 8), torch.ones(8)
+    norm, quant, back = ops.residual_rms_norm, ops.residual_rms_norm_quant, ops.residual_rms_norm_backward
+    refused(ops, lambda: norm(x.double(), out=x, rstd_out=x), "dtype DOUBLE")
+    refused(ops, lambda: norm(torch.zeros(3, 0)), "last extent")
+    refused(ops, lambda: norm(x, x.half()), "residual must have the type")
+    refused(ops, lambda: norm(x, x[:1]), "residual must have the shape")
+    refused(ops, lambda: norm(x, None, w[:7]), "weight must be [8]")
+    refused(ops, lambda: norm(x, None, w.half()), "weight must have")
+    refused(ops, lambda: norm(x, eps=-1e-6), "eps")
+    refused(ops, lambda: norm(x, eps=float("nan")), "eps")
+    refused(ops, lambda: norm(x, out=x[..., :7]), "y must have the shape")
+    refused(ops, lambda: norm(x, out=torch.zeros(1, 3, 8).expand(2, 3, 8)), "overlap")
+    refused(ops, lambda: norm(x, x, sum_out=torch.zeros(1, 1, 8).expand(2, 3, 8)), "overlap")
+    refused(ops, lambda: norm(x, rstd_out=torch.zeros(2, 3, dtype=F16)), "rstd must be FLOAT")
+    refused(ops, lambda: norm(x, rstd_out=torch.zeros(3, 2)), "rstd")
+    refused(ops, lambda: norm(x, rstd_out=torch.zeros(3, 2).t()), "rstd must be contiguous")
+    refused(ops, lambda: back(x, x, torch.zeros(2, 2), w), "rstd")
+    refused(ops, lambda: back(x, x, torch.zeros(2, 3), None, grad_weight=w), "without a weight")
+    refused(ops, lambda: back(x, x, torch.zeros(2, 3), w, grad_weight=w.half()), "gradWeight")
+    refused(ops, lambda: back(x, x, torch.zeros(2, 3), w, x.half()), "gradSum")
+    refused(ops, lambda: back(x, x, torch.zeros(2, 3), w, grad_x=torch.zeros(1, 1, 8).expand(2, 3, 8)), "overlap")
+    for group in (-32, 1, 31, 48):
+        refused(ops, lambda: quant(x, group=group), "group")
+    refused(ops, lambda: quant(x, scales_out=torch.zeros(2, 3)), "scales")
+    refused(ops, lambda: quant(x, out=torch.zeros(2, 3, 16, dtype=torch.float8_e4m3fn)[..., ::2]), "contiguous")
+    with pytest.raises(ValueError, match="dtype"):
+        quant(x, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="type"):
+        quant(x, out=torch.zeros(2, 3, 8, dtype=torch.int8))
+
+
+def test_rotary_accepts(ops):
+    q, k, f = torch.zeros(2, 5, 4, 16), torch.zeros(2, 5, 2, 16), torch.zeros(8)
+    p = torch.arange(5)
+    accepted(lambda: ops.rotary_embedding(q, k, p, f))
+    accepted(lambda: ops.rotary_embedding(q, None, p.int().expand(2, 5), f.double(), True, scale=1.3))
+    accepted(lambda: ops.rotary_embedding(q, k, p.expand(3, 2, 5), f, sections=(4, 0, 4)))
+    accepted(lambda: ops.rotary_embedding_backward(q, k, p, f[:3]))
+    accepted(lambda: ops.rotary_embedding(q.transpose(1, 2), None, p[:4], f))
+    accepted(lambda: ops.rotary_embedding(torch.zeros(0, 5, 4, 16), None, p, f))
+    accepted(lambda: ops.rotary_embedding(q[0, 0], None, p[0], f))
+
+
+def test_rotary_refuses(ops):
+    q, k, f, p = torch.zeros(2, 5, 4, 16), torch.zeros(2, 5, 2, 16), torch.zeros(8), torch.arange(5)
+    turn = ops.rotary_embedding
+    refused(ops, lambda: turn(q.double(), None, p, f), "dtype DOUBLE")
+    refused(ops, lambda: turn(q, k.half(), p, f), "one type")
+    refused(ops, lambda: turn(q, k[:1], p, f), "leading dimensions")
+    refused(ops, lambda: turn(q, k[..., :8], p, f), "dim")
+    refused(ops, lambda: turn(q, k, p.to(torch.float32), f), "positions must be")
+    refused(ops, lambda: turn(q, k, p, f.half()), "frequencies must be")
+    refused(ops, lambda: turn(q, k, p, torch.zeros(9)), "do not fit")
+    refused(ops, lambda: turn(q, k, p, torch.zeros(0)), "do not fit")
+    refused(ops, lambda: turn(q, k, p, torch.zeros(16)[::2]), "contiguous")
+    refused(ops, lambda: turn(q, k, p, f, scale=float("inf")), "scale")
+    refused(ops, lambda: turn(q, k, p.expand(2, 2, 5), f, sections=(4, 3)), "add up")
+    refused(ops, lambda: turn(q, k, p.expand(2, 2, 5), f, sections=(9, -1)), "section")
+    refused(ops, lambda: turn(q, k, p.expand(3, 2, 5), f, sections=(4, 4)), "positions must be")
+    refused(ops, lambda: turn(q, k, p.expand(5, 2, 5), f, sections=(2, 2, 2, 1, 1)), "sections")
+    refused(ops, lambda: turn(q, k, p, f, q_out=torch.zeros(1, 1, 1, 16).expand(2, 5, 4, 16)), "overlap")
+    refused(ops, lambda: turn(q, k, p, f, q_out=q[:1]), "q's shape")
+    with pytest.raises(RuntimeError, match="expand"):
+        turn(q, k, p[:4], f)
+    with pytest.raises(ValueError, match="without k"):
+        turn(q, None, p, f, k_out=k)
+    with pytest.raises(RuntimeError, match="positions|strided"):
+        turn(torch.zeros(2, 3, 4, 1, 8), None, torch.zeros(8, 8, 8, dtype=torch.int64)[:2, ::2, ::2][:, :3, :4], f[:4])
+
+
+def test_rotary_frequencies_refuses(ops):
+    make = ops.rotary_frequencies
+    for how in (dict(base=1.0), dict(base=float("nan")), dict(factor=0.5), dict(scaling="wavelength", factor=2.0),
+                dict(scaling="wavelength", original_length=100.0, low=4.0, high=4.0), dict(scaling="ramp", original_length=100.0, low=0.0)):
+        refused(ops, lambda: make(8, device="cpu", **how))
+    refused(ops, lambda: make(8, dtype=F16, device="cpu"), "out must be")
+    refused(ops, lambda: make(8, out=torch.zeros(8)[::2]), "contiguous")
+    with pytest.raises(ValueError, match="even"):
+        make(7)
+    with pytest.raises(ValueError, match="scaling"):
+        make(8, scaling="none")
+    accepted(lambda: make(8, device="cpu"))
+    accepted(lambda: make(8, scaling="ramp", factor=4.0, original_length=100.0, low=1.0, high=32.0, dtype=torch.float64, device="cpu"))
+
+
+def test_tensors_of_two_devices(ops):
+    x = torch.zeros(2, 8)
+    with pytest.raises(ValueError, match="one device"):
+        ops.residual_rms_norm(x, torch.zeros(2, 8, device="meta"))
