@@ -105,6 +105,39 @@ ACLNN_API aclnnStatus aclnnRotaryFrequenciesGetWorkspaceSize(double base, int64_
 ACLNN_API aclnnStatus aclnnRotaryFrequencies(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
                                              aclrtStream stream);
 
+/* ---- WindowAttention ---------------------------------------------------------------------------------------------------------
+ * Causal attention over a sliding window with a few first tokens ("sinks") that stay visible, for prompts, chunks of new tokens
+ * over a cache, single tokens and training.
+ * q, out: [batch, queries, heads, dim]; k, v: [batch, keys, kvHeads, dim]; heads a multiple of kvHeads (head h reads key head
+ * h / (heads / kvHeads)), 1 <= dim <= 256.
+ * kvLengths, qLengths: [batch], ACL_INT32 or ACL_INT64, contiguous, or null (all keys, all queries): how many keys and queries of
+ * each sequence count; values outside [0, keys] and [0, queries] are cut to it. Query i of a sequence sits at position
+ * p = kvLength - qLength + i, so that the last query sits at the last key; it sees the keys j <= p with j > p - window
+ * (window >= 1) or j < sinks (sinks >= 0; both are cut to 2^30). scale multiplies the scores.
+ * out = softmax(scale q.k over the keys seen) v; lse: [batch, heads, queries], ACL_FLOAT, contiguous, the natural logarithm of the
+ * softmax's sum, or null. A query behind its sequence's length, or that sees no key, has out 0 and lse -infinity.
+ * What lies in keys that a query does not see, NaN and infinities included, does not reach its result. */
+ACLNN_API aclnnStatus aclnnWindowAttentionGetWorkspaceSize(const aclTensor* q, const aclTensor* k, const aclTensor* v,
+                                                           const aclTensor* qLengths, const aclTensor* kvLengths,
+                                                           int64_t window, int64_t sinks, double scale, aclTensor* out,
+                                                           aclTensor* lse, uint64_t* workspaceSize,
+                                                           aclOpExecutor** executor);
+ACLNN_API aclnnStatus aclnnWindowAttention(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
+                                           aclrtStream stream);
+
+/* The gradients of q, k and v, each of its tensor's shape, from out's, with the out and lse that the forward returned for the
+ * same arguments. The gradients of queries behind their sequence's length and of keys that no query sees are 0. The sums are
+ * formed in a fixed order: equal inputs give equal bits. No output may lie over an input. */
+ACLNN_API aclnnStatus aclnnWindowAttentionBackwardGetWorkspaceSize(const aclTensor* gradOut, const aclTensor* q,
+                                                                   const aclTensor* k, const aclTensor* v,
+                                                                   const aclTensor* out, const aclTensor* lse,
+                                                                   const aclTensor* qLengths, const aclTensor* kvLengths,
+                                                                   int64_t window, int64_t sinks, double scale,
+                                                                   aclTensor* gradQ, aclTensor* gradK, aclTensor* gradV,
+                                                                   uint64_t* workspaceSize, aclOpExecutor** executor);
+ACLNN_API aclnnStatus aclnnWindowAttentionBackward(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
+                                                   aclrtStream stream);
+
 #ifdef __cplusplus
 }
 #endif

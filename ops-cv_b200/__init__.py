@@ -135,6 +135,10 @@ SEQUENCE_SYMBOLS = {
     "aclnnRotaryEmbeddingBackward": _PHASE2,
     "aclnnRotaryFrequenciesGetWorkspaceSize": (_I32, [_D, _I64, _D, _D, _D, _D, _P, _PU64, _PP]),
     "aclnnRotaryFrequencies": _PHASE2,
+    "aclnnWindowAttentionGetWorkspaceSize": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _D, _P, _P, _PU64, _PP]),
+    "aclnnWindowAttention": _PHASE2,
+    "aclnnWindowAttentionBackwardGetWorkspaceSize": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _D, _P, _P, _P, _PU64, _PP]),
+    "aclnnWindowAttentionBackward": _PHASE2,
 }
 
 _lib = None

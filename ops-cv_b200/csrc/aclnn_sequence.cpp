@@ -77,6 +77,9 @@ bool WritesApart(const aclTensor* t)
     return true;
 }
 
+// of a tensor that goes to the kernels as it is
+bool Dense(const aclTensor* t) { return IsEmpty(t) || IsContiguous(t); }
+
 bool LastContiguous(const aclTensor* t)
 {
     const size_t n = t->dims.size();
@@ -256,7 +259,7 @@ aclnnStatus CheckPerRow(const char* api, const aclTensor* x, const aclTensor* t,
     OPSCV_REQUIRE(t->dtype == ACL_FLOAT, "%s: %s must be FLOAT, got %s", api, name, DtypeName(t->dtype));
     OPSCV_REQUIRE(t->dims.size() == lead + (last > 0 ? 1 : 0) && LeadEqual(x, t, lead) && (last <= 0 || Last(t) == last),
                   "%s: %s does not have the rows' shape", api, name);
-    OPSCV_REQUIRE(IsContiguous(t), "%s: %s must be contiguous", api, name);
+    OPSCV_REQUIRE(Dense(t), "%s: %s must be contiguous", api, name);
     return ACLNN_SUCCESS;
 }
 
@@ -301,7 +304,7 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
                   api, DtypeName(positions->dtype));
     OPSCV_REQUIRE(frequencies->dtype == ACL_DOUBLE || frequencies->dtype == ACL_FLOAT,
                   "%s: frequencies must be DOUBLE or FLOAT, got %s", api, DtypeName(frequencies->dtype));
-    OPSCV_REQUIRE(frequencies->dims.size() == 1 && IsContiguous(frequencies), "%s: frequencies must be one contiguous dimension",
+    OPSCV_REQUIRE(frequencies->dims.size() == 1 && Dense(frequencies), "%s: frequencies must be one contiguous dimension",
                   api);
     const int64_t half = frequencies->dims[0];
     OPSCV_REQUIRE(half >= 1 && 2 * half <= Last(q) && half <= 2048, "%s: %ld frequencies do not fit a head of %ld values", api,
@@ -389,6 +392,70 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
     return ACLNN_SUCCESS;
 }
 
+// ---- attention ---------------------------------------------------------------------------------------------------------------
+aclnnStatus CheckAttention(const char* api, const aclTensor* q, const aclTensor* k, const aclTensor* v, const aclTensor* qLengths,
+                           const aclTensor* kvLengths, int64_t window, int64_t sinks, double scale, AttnShape& s)
+{
+    OPSCV_REQUIRE(DtypeSupported(q->dtype), "%s: dtype %s not supported (FLOAT, FLOAT16, BF16)", api, DtypeName(q->dtype));
+    OPSCV_REQUIRE(k->dtype == q->dtype && v->dtype == q->dtype, "%s: q, k and v must have one type", api);
+    OPSCV_REQUIRE(q->dims.size() == 4 && k->dims.size() == 4, "%s: q and k must be [batch, tokens, heads, dim]", api);
+    OPSCV_REQUIRE(v->dims == k->dims, "%s: v must have k's shape", api);
+    OPSCV_REQUIRE(k->dims[0] == q->dims[0] && k->dims[3] == q->dims[3], "%s: q and k must have one batch and one dim", api);
+    OPSCV_REQUIRE(k->dims[2] >= 1 && q->dims[2] % k->dims[2] == 0, "%s: %ld heads are not a multiple of %ld key heads", api,
+                  (long)q->dims[2], (long)k->dims[2]);
+    OPSCV_REQUIRE(q->dims[3] >= 1 && q->dims[3] <= kMaxAttnDim, "%s: dim must be in [1, %d], got %ld", api, kMaxAttnDim,
+                  (long)q->dims[3]);
+    constexpr int64_t most = 1 << 30;
+    OPSCV_REQUIRE(q->dims[1] <= most && k->dims[1] <= most && q->dims[0] <= most && q->dims[2] <= most &&
+                      q->dims[0] * q->dims[2] <= most,
+                  "%s: extents above 2^30 are not supported", api);
+    for (const aclTensor* n : {qLengths, kvLengths}) {
+        OPSCV_REQUIRE(n == nullptr || n->dtype == ACL_INT32 || n->dtype == ACL_INT64, "%s: lengths must be INT32 or INT64, got %s",
+                      api, DtypeName(n->dtype));
+        OPSCV_REQUIRE(n == nullptr || (n->dims.size() == 1 && n->dims[0] == q->dims[0] && Dense(n)),
+                      "%s: lengths must be [batch] and contiguous", api);
+    }
+    OPSCV_REQUIRE(window >= 1, "%s: window must be at least 1, got %ld", api, (long)window);
+    OPSCV_REQUIRE(sinks >= 0, "%s: sinks must not be negative, got %ld", api, (long)sinks);
+    OPSCV_REQUIRE(std::isfinite(scale), "%s: scale must be finite", api);
+    s.batch = static_cast<int32_t>(q->dims[0]);
+    s.lq = static_cast<int32_t>(q->dims[1]);
+    s.lk = static_cast<int32_t>(k->dims[1]);
+    s.heads = static_cast<int32_t>(q->dims[2]);
+    s.kvHeads = static_cast<int32_t>(k->dims[2]);
+    s.dim = static_cast<int32_t>(q->dims[3]);
+    s.window = static_cast<int32_t>(window < most ? window : most);
+    s.sinks = static_cast<int32_t>(sinks < most ? sinks : most);
+    s.scale = static_cast<float>(scale);
+    if (qLengths != nullptr) {
+        s.qLen64 = qLengths->dtype == ACL_INT64;
+        s.qLen = DataOf(qLengths, s.qLen64 ? 8 : 4);
+    }
+    if (kvLengths != nullptr) {
+        s.kvLen64 = kvLengths->dtype == ACL_INT64;
+        s.kvLen = DataOf(kvLengths, s.kvLen64 ? 8 : 4);
+    }
+    return ACLNN_SUCCESS;
+}
+
+aclnnStatus CheckLse(const char* api, const aclTensor* q, const aclTensor* lse)
+{
+    OPSCV_REQUIRE(lse->dtype == ACL_FLOAT && Dense(lse) && lse->dims.size() == 3 && lse->dims[0] == q->dims[0] &&
+                      lse->dims[1] == q->dims[2] && lse->dims[2] == q->dims[1],
+                  "%s: lse must be [batch, heads, queries], FLOAT and contiguous", api);
+    return ACLNN_SUCCESS;
+}
+
+AttnTensor AttnOf(const Operand& o, char* w)
+{
+    AttnTensor t;
+    t.p = o.buf.At(w);
+    t.b = o.view.strides[0];
+    t.l = o.view.strides[1];
+    t.h = o.view.strides[2];
+    return t;
+}
+
 } // namespace
 
 extern "C" {
@@ -469,7 +536,7 @@ aclnnStatus aclnnResidualRmsNormBackwardGetWorkspaceSize(const aclTensor* gradY,
         OPSCV_TRY(CheckPerRow(api, sum, rstd, 0, "rstd"));
         if (gradWeight != nullptr) {
             OPSCV_REQUIRE(weight != nullptr, "%s: gradWeight without a weight", api);
-            OPSCV_REQUIRE(gradWeight->dtype == weight->dtype && gradWeight->dims == weight->dims && IsContiguous(gradWeight),
+            OPSCV_REQUIRE(gradWeight->dtype == weight->dtype && gradWeight->dims == weight->dims && Dense(gradWeight),
                           "%s: gradWeight must be contiguous, of weight's type and shape", api);
         }
         OPSCV_REQUIRE(WritesApart(gradX), "%s: an output's elements overlap", api);
@@ -542,7 +609,7 @@ aclnnStatus aclnnResidualRmsNormQuantGetWorkspaceSize(const aclTensor* x, const 
                       (long)group);
         OPSCV_REQUIRE(out->dtype == ACL_FLOAT8_E4M3FN || out->dtype == ACL_INT8, "%s: out must be FLOAT8_E4M3FN or INT8, got %s",
                       api, DtypeName(out->dtype));
-        OPSCV_REQUIRE(out->dims == x->dims && IsContiguous(out), "%s: out must be contiguous and have x's shape", api);
+        OPSCV_REQUIRE(out->dims == x->dims && Dense(out), "%s: out must be contiguous and have x's shape", api);
         const int64_t width = Last(x);
         const int64_t groups = group == 0 ? 1 : (width + group - 1) / group;
         OPSCV_REQUIRE(groups <= 10240, "%s: more than 10240 groups a row are not supported", api);
@@ -648,7 +715,7 @@ aclnnStatus aclnnRotaryFrequenciesGetWorkspaceSize(double base, int64_t scaling,
         }
         OPSCV_REQUIRE(out->dtype == ACL_DOUBLE || out->dtype == ACL_FLOAT, "%s: out must be DOUBLE or FLOAT, got %s", api,
                       DtypeName(out->dtype));
-        OPSCV_REQUIRE(out->dims.size() == 1 && IsContiguous(out) && out->dims[0] <= (1 << 20),
+        OPSCV_REQUIRE(out->dims.size() == 1 && Dense(out) && out->dims[0] <= (1 << 20),
                       "%s: out must be one contiguous dimension", api);
         const int32_t half = static_cast<int32_t>(out->dims[0]);
         if (half == 0) {
@@ -666,6 +733,86 @@ aclnnStatus aclnnRotaryFrequenciesGetWorkspaceSize(double base, int64_t scaling,
 aclnnStatus aclnnRotaryFrequencies(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor, aclrtStream stream)
 {
     return RunExecutor("aclnnRotaryFrequencies", workspace, workspaceSize, executor, stream);
+}
+
+aclnnStatus aclnnWindowAttentionGetWorkspaceSize(const aclTensor* q, const aclTensor* k, const aclTensor* v,
+                                                 const aclTensor* qLengths, const aclTensor* kvLengths, int64_t window,
+                                                 int64_t sinks, double scale, aclTensor* out, aclTensor* lse,
+                                                 uint64_t* workspaceSize, aclOpExecutor** executor)
+{
+    static const char* api = "aclnnWindowAttention";
+    return Guarded(api, workspaceSize, executor, [&](aclOpExecutor& ex, WsPlan& ws) -> aclnnStatus {
+        OPSCV_NOT_NULL(q != nullptr && k != nullptr && v != nullptr && out != nullptr, api);
+        AttnShape shape;
+        OPSCV_TRY(CheckAttention(api, q, k, v, qLengths, kvLengths, window, sinks, scale, shape));
+        OPSCV_REQUIRE(out->dtype == q->dtype && out->dims == q->dims, "%s: out must have q's type and shape", api);
+        OPSCV_REQUIRE(WritesApart(out), "%s: an output's elements overlap", api);
+        if (lse != nullptr) {
+            OPSCV_TRY(CheckLse(api, q, lse));
+        }
+        if (Numel(q) == 0) {
+            return ACLNN_SUCCESS;
+        }
+        Operand oq = In(q), ok = In(k), ov = In(v), oo = Out(out);
+        OPSCV_TRY(Place(api, {&oq, &ok, &ov, &oo}, false, ex, ws));
+        const Dt dt = ToDt(q->dtype);
+        const uint64_t own = ws.Alloc(WindowAttentionFwdWorkspace(dt, shape));
+        float* lseAt = lse != nullptr ? reinterpret_cast<float*>(DataOf(lse, 4)) : nullptr;
+        ex.steps.push_back([=](char* w, cudaStream_t s) {
+            return WindowAttentionFwd(dt, shape, AttnOf(oq, w), AttnOf(ok, w), AttnOf(ov, w), AttnOf(oo, w), lseAt, w + own, s);
+        });
+        Finish({&oo}, ex);
+        return ACLNN_SUCCESS;
+    });
+}
+
+aclnnStatus aclnnWindowAttention(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor, aclrtStream stream)
+{
+    return RunExecutor("aclnnWindowAttention", workspace, workspaceSize, executor, stream);
+}
+
+aclnnStatus aclnnWindowAttentionBackwardGetWorkspaceSize(const aclTensor* gradOut, const aclTensor* q, const aclTensor* k,
+                                                         const aclTensor* v, const aclTensor* out, const aclTensor* lse,
+                                                         const aclTensor* qLengths, const aclTensor* kvLengths, int64_t window,
+                                                         int64_t sinks, double scale, aclTensor* gradQ, aclTensor* gradK,
+                                                         aclTensor* gradV, uint64_t* workspaceSize, aclOpExecutor** executor)
+{
+    static const char* api = "aclnnWindowAttentionBackward";
+    return Guarded(api, workspaceSize, executor, [&](aclOpExecutor& ex, WsPlan& ws) -> aclnnStatus {
+        OPSCV_NOT_NULL(gradOut != nullptr && q != nullptr && k != nullptr && v != nullptr && out != nullptr && lse != nullptr &&
+                           gradQ != nullptr && gradK != nullptr && gradV != nullptr,
+                       api);
+        AttnShape shape;
+        OPSCV_TRY(CheckAttention(api, q, k, v, qLengths, kvLengths, window, sinks, scale, shape));
+        for (const aclTensor* t : {gradOut, out, static_cast<const aclTensor*>(gradQ)}) {
+            OPSCV_REQUIRE(t->dtype == q->dtype && t->dims == q->dims, "%s: gradOut, out and gradQ must have q's type and shape", api);
+        }
+        for (const aclTensor* t : {gradK, gradV}) {
+            OPSCV_REQUIRE(t->dtype == q->dtype && t->dims == k->dims, "%s: gradK and gradV must have k's type and shape", api);
+        }
+        OPSCV_TRY(CheckLse(api, q, lse));
+        OPSCV_REQUIRE(WritesApart(gradQ) && WritesApart(gradK) && WritesApart(gradV), "%s: an output's elements overlap", api);
+        if (Numel(q) == 0 && Numel(k) == 0) {
+            return ACLNN_SUCCESS;
+        }
+        Operand og = In(gradOut), oq = In(q), ok = In(k), ov = In(v), oo = In(out);
+        Operand gq = Out(gradQ), gk = Out(gradK), gv = Out(gradV);
+        OPSCV_TRY(Place(api, {&og, &oq, &ok, &ov, &oo, &gq, &gk, &gv}, false, ex, ws));
+        const Dt dt = ToDt(q->dtype);
+        const uint64_t own = ws.Alloc(WindowAttentionBwdWorkspace(dt, shape));
+        const float* lseAt = reinterpret_cast<const float*>(DataOf(lse, 4));
+        ex.steps.push_back([=](char* w, cudaStream_t s) {
+            return WindowAttentionBwd(dt, shape, AttnOf(og, w), AttnOf(oq, w), AttnOf(ok, w), AttnOf(ov, w), AttnOf(oo, w), lseAt,
+                                      AttnOf(gq, w), AttnOf(gk, w), AttnOf(gv, w), w + own, s);
+        });
+        Finish({&gq, &gk, &gv}, ex);
+        return ACLNN_SUCCESS;
+    });
+}
+
+aclnnStatus aclnnWindowAttentionBackward(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor, aclrtStream stream)
+{
+    return RunExecutor("aclnnWindowAttentionBackward", workspace, workspaceSize, executor, stream);
 }
 
 } // extern "C"

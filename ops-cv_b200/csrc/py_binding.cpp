@@ -13,6 +13,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 
+#include <cmath>
 #include <string>
 
 #include "../../include/aclnn_sequence.h"
@@ -822,6 +823,52 @@ PyObject* RotaryFrequenciesOf(Args a)
     return Give(out);
 }
 
+// (q, k, v, q_lengths, kv_lengths, window, sinks, scale or None, out, lse, workspace)
+double AttentionScale(PyObject* scale, const at::Tensor& q)
+{
+    if (Given(scale)) {
+        return DoubleOf(scale);
+    }
+    return q.dim() > 0 && q.size(-1) > 0 ? 1.0 / std::sqrt(static_cast<double>(q.size(-1))) : 1.0;
+}
+PyObject* WindowAttention(Args a)
+{
+    const at::Tensor& q = TensorOf(a[0]);
+    const Call call(q);
+    const aclTensor tq = AclOf(q, ACL_FORMAT_ND), tk = AclOf(call.Of(a[1]), ACL_FORMAT_ND), tv = AclOf(call.Of(a[2]), ACL_FORMAT_ND);
+    Call::Acl nq = call.Maybe(a[3]), nk = call.Maybe(a[4]);
+    const int64_t window = IntOf(a[5]), sinks = IntOf(a[6]);
+    const double scale = AttentionScale(a[7], q);
+    const at::Tensor out = call.OutOr(a[8], q.sizes(), q.options());
+    const at::Tensor lse = call.OutOr(a[9], {DimOf(q, 0), DimOf(q, 2), DimOf(q, 1)}, q.options().dtype(at::kFloat));
+    aclTensor to = AclOf(out, ACL_FORMAT_ND), tl = AclOf(lse, ACL_FORMAT_ND);
+    TwoPhase("aclnnWindowAttention", [&](uint64_t* n, aclOpExecutor** e) {
+        return aclnnWindowAttentionGetWorkspaceSize(&tq, &tk, &tv, nq.Ptr(), nk.Ptr(), window, sinks, scale, &to, &tl, n, e);
+    }, aclnnWindowAttention, call.Device(), a[10]);
+    return GiveAll({&out, &lse});
+}
+
+// (grad_out, q, k, v, out, lse, q_lengths, kv_lengths, window, sinks, scale or None, grad_q, grad_k, grad_v, workspace)
+PyObject* WindowAttentionBackward(Args a)
+{
+    const at::Tensor& q = TensorOf(a[1]);
+    const Call call(q);
+    const at::Tensor &k = call.Of(a[2]), &v = call.Of(a[3]);
+    const aclTensor tg = AclOf(call.Of(a[0]), ACL_FORMAT_ND), tq = AclOf(q, ACL_FORMAT_ND), tk = AclOf(k, ACL_FORMAT_ND),
+                    tv = AclOf(v, ACL_FORMAT_ND), to = AclOf(call.Of(a[4]), ACL_FORMAT_ND), tl = AclOf(call.Of(a[5]), ACL_FORMAT_ND);
+    Call::Acl nq = call.Maybe(a[6]), nk = call.Maybe(a[7]);
+    const int64_t window = IntOf(a[8]), sinks = IntOf(a[9]);
+    const double scale = AttentionScale(a[10], q);
+    const at::Tensor gq = call.OutOr(a[11], q.sizes(), q.options()), gk = call.OutOr(a[12], k.sizes(), k.options()),
+                     gv = call.OutOr(a[13], v.sizes(), v.options());
+    aclTensor tgq = AclOf(gq, ACL_FORMAT_ND), tgk = AclOf(gk, ACL_FORMAT_ND), tgv = AclOf(gv, ACL_FORMAT_ND);
+    TwoPhase("aclnnWindowAttentionBackward", [&](uint64_t* n, aclOpExecutor** e) {
+        return aclnnWindowAttentionBackwardGetWorkspaceSize(&tg, &tq, &tk, &tv, &to, &tl, nq.Ptr(), nk.Ptr(), window, sinks, scale,
+                                                            &tgq, &tgk, &tgv, n, e);
+    }, aclnnWindowAttentionBackward, call.Device(), a[14]);
+    return GiveAll({&gq, &gk, &gv});
+}
+
 // Argument count, C++ exceptions.
 template <PyObject* (*F)(Args), int N>
 PyObject* Entry(PyObject*, PyObject* const* args, Py_ssize_t n)
@@ -884,6 +931,8 @@ PyMethodDef kMethods[] = {
     OPSCV_METHOD("residual_rms_norm_quant", ResidualRmsNormQuant, 10),
     OPSCV_METHOD("rotary_embedding", Rotary, 11),
     OPSCV_METHOD("rotary_frequencies", RotaryFrequenciesOf, 7),
+    OPSCV_METHOD("window_attention", WindowAttention, 11),
+    OPSCV_METHOD("window_attention_backward", WindowAttentionBackward, 15),
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -63,4 +63,27 @@ struct RotaryShape {
 cudaError_t RotaryTurn(Dt dt, const RotaryShape& r, const RotaryTensor& q, const RotaryTensor& k, const void* positions,
                        const void* frequencies, cudaStream_t s);
 
+// ---- attention over a sliding window with sinks ------------------------------------------------------------------------------
+struct AttnTensor { // [batch, token, head, dim], dim contiguous; strides in elements
+    const void* p = nullptr;
+    int64_t b = 0, l = 0, h = 0;
+};
+struct AttnShape {
+    int32_t batch = 0, lq = 0, lk = 0, heads = 0, kvHeads = 0, dim = 0;
+    int32_t window = 1, sinks = 0; // at most 2^30
+    float scale = 1.0f;
+    const void *qLen = nullptr, *kvLen = nullptr; // [batch], null: lq, lk
+    bool qLen64 = false, kvLen64 = false;
+};
+constexpr int kMaxAttnDim = 256;
+
+// out and lse ([batch, heads, lq] contiguous) of queries over keys and values.
+uint64_t WindowAttentionFwdWorkspace(Dt dt, const AttnShape& a);
+cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& a, AttnTensor q, AttnTensor k, AttnTensor v, AttnTensor out, float* lse,
+                               void* workspace, cudaStream_t s);
+uint64_t WindowAttentionBwdWorkspace(Dt dt, const AttnShape& a);
+cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& a, AttnTensor gradOut, AttnTensor q, AttnTensor k, AttnTensor v,
+                               AttnTensor out, const float* lse, AttnTensor gradQ, AttnTensor gradK, AttnTensor gradV,
+                               void* workspace, cudaStream_t s);
+
 } // namespace opscv

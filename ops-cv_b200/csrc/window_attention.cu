@@ -1,0 +1,132 @@
+// Attention over a sliding window with sinks: which kernel a call takes, and the kernels that take a warp per row.
+#include "window_attention.cuh"
+
+namespace opscv {
+
+namespace {
+
+constexpr int kRowWarps = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kRowWarps) AttnForwardRowsKernel(AttnArgs a)
+{
+    const int32_t i = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+    if (i < a.s.lq) {
+        for (int32_t bh = blockIdx.y; bh < a.s.batch * a.s.heads; bh += gridDim.y) {
+            AttnForwardRow<T>(a, bh / a.s.heads, bh % a.s.heads, i);
+        }
+    }
+}
+
+// delta = gradOut . out, a warp per row
+template <typename T>
+__global__ void __launch_bounds__(32 * kRowWarps) AttnDeltaKernel(AttnArgs a, float* delta)
+{
+    const int lane = threadIdx.x & 31;
+    const int32_t i = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+    if (i >= a.s.lq) {
+        return;
+    }
+    for (int32_t bh = blockIdx.y; bh < a.s.batch * a.s.heads; bh += gridDim.y) {
+        const int32_t b = bh / a.s.heads, h = bh % a.s.heads;
+        const T* g = RowOf<T>(a.gradOut, b, i, h);
+        const T* o = RowOf<T>(a.out, b, i, h);
+        float s = 0.0f;
+        for (int32_t d = lane; d < a.s.dim; d += 32) {
+            s = fmaf(DType<T>::ToF(g[d]), DType<T>::ToF(o[d]), s);
+        }
+        s = WarpSum(s);
+        if (lane == 0) {
+            delta[static_cast<int64_t>(bh) * a.s.lq + i] = s;
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kRowWarps) AttnGradQRowsKernel(AttnArgs a)
+{
+    const int32_t i = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+    if (i < a.s.lq) {
+        for (int32_t bh = blockIdx.y; bh < a.s.batch * a.s.heads; bh += gridDim.y) {
+            AttnGradQRow<T>(a, bh / a.s.heads, bh % a.s.heads, i);
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kRowWarps) AttnGradKvRowsKernel(AttnArgs a)
+{
+    const int32_t j = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+    if (j < a.s.lk) {
+        for (int32_t bu = blockIdx.y; bu < a.s.batch * a.s.kvHeads; bu += gridDim.y) {
+            AttnGradKvRow<T>(a, bu / a.s.kvHeads, bu % a.s.kvHeads, j);
+        }
+    }
+}
+
+dim3 RowGrid(int32_t rows, int64_t others)
+{
+    return dim3(static_cast<unsigned>(CeilDiv(rows, kRowWarps)), static_cast<unsigned>(others < 65535 ? others : 65535));
+}
+
+} // namespace
+
+uint64_t WindowAttentionFwdWorkspace(Dt, const AttnShape&) { return 0; }
+
+cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& s, AttnTensor q, AttnTensor k, AttnTensor v, AttnTensor out, float* lse, void*,
+                               cudaStream_t stream)
+{
+    AttnArgs a{};
+    a.s = s;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = out;
+    a.lse = lse;
+    a.group = s.heads / s.kvHeads;
+    const dim3 grid = RowGrid(s.lq, static_cast<int64_t>(s.batch) * s.heads);
+    OPSCV_DISPATCH_DT(dt, T, AttnForwardRowsKernel<T><<<grid, 32 * kRowWarps, 0, stream>>>(a));
+    CountLaunch();
+    return cudaGetLastError();
+}
+
+uint64_t WindowAttentionBwdWorkspace(Dt, const AttnShape& s)
+{
+    return static_cast<uint64_t>(s.batch) * s.heads * s.lq * 4;
+}
+
+cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& s, AttnTensor gradOut, AttnTensor q, AttnTensor k, AttnTensor v, AttnTensor out,
+                               const float* lse, AttnTensor gradQ, AttnTensor gradK, AttnTensor gradV, void* workspace,
+                               cudaStream_t stream)
+{
+    AttnArgs a{};
+    a.s = s;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = out;
+    a.gradOut = gradOut;
+    a.gradQ = gradQ;
+    a.gradK = gradK;
+    a.gradV = gradV;
+    a.lse = const_cast<float*>(lse);
+    float* delta = static_cast<float*>(workspace);
+    a.delta = delta;
+    a.group = s.heads / s.kvHeads;
+    const dim3 rows = RowGrid(s.lq, static_cast<int64_t>(s.batch) * s.heads);
+    const dim3 keys = RowGrid(s.lk, static_cast<int64_t>(s.batch) * s.kvHeads);
+    OPSCV_DISPATCH_DT(dt, T, {
+        if (s.lq > 0) {
+            AttnDeltaKernel<T><<<rows, 32 * kRowWarps, 0, stream>>>(a, delta);
+            AttnGradQRowsKernel<T><<<rows, 32 * kRowWarps, 0, stream>>>(a);
+            CountLaunch(2);
+        }
+        if (s.lk > 0) {
+            AttnGradKvRowsKernel<T><<<keys, 32 * kRowWarps, 0, stream>>>(a);
+            CountLaunch();
+        }
+    });
+    return cudaGetLastError();
+}
+
+} // namespace opscv

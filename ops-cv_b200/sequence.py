@@ -6,7 +6,7 @@ from .aclnn import native
 
 __all__ = [
     "residual_rms_norm", "residual_rms_norm_backward", "residual_rms_norm_quant", "rotary_embedding", "rotary_embedding_backward",
-    "rotary_frequencies",
+    "rotary_frequencies", "window_attention", "window_attention_backward",
 ]
 
 
@@ -60,3 +60,17 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
             raise ValueError(f"rotary_dim must be even, got {rotary_dim}")
         out = torch.empty(rotary_dim // 2, dtype=dtype, device=device)
     return native().rotary_frequencies(out, base, _SCALINGS[scaling], factor, original_length, low, high)
+
+
+def window_attention(q, k, v, window, sinks=0, scale=None, q_lengths=None, kv_lengths=None, out=None, lse=None, workspace=None):
+    """(out, lse) of causal attention over the last `window` keys and the first `sinks`: q [batch, queries, heads, dim] against k and
+    v [batch, keys, kv heads, dim]; scale is 1 / sqrt(dim) unless given. Sequence b has q_lengths[b] queries and kv_lengths[b] keys
+    (all of them unless given), its last query at its last key. lse [batch, heads, queries] is what the backward needs."""
+    return native().window_attention(q, k, v, q_lengths, kv_lengths, window, sinks, scale, out, lse, workspace)
+
+
+def window_attention_backward(grad_out, q, k, v, out, lse, window, sinks=0, scale=None, q_lengths=None, kv_lengths=None, grad_q=None,
+                              grad_k=None, grad_v=None, workspace=None):
+    """(grad_q, grad_k, grad_v) from the forward's out and lse; the other arguments are the forward's."""
+    return native().window_attention_backward(grad_out, q, k, v, out, lse, q_lengths, kv_lengths, window, sinks, scale, grad_q, grad_k,
+                                              grad_v, workspace)

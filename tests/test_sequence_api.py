@@ -149,6 +149,48 @@ def test_rotary_frequencies_refuses(ops):
     accepted(lambda: make(8, scaling="ramp", factor=4.0, original_length=100.0, low=1.0, high=32.0, dtype=torch.float64, device="cpu"))
 
 
+def test_attention_accepts(ops):
+    for t in (F32, F16, BF16):
+        q, k = torch.zeros(2, 5, 4, 16, dtype=t), torch.zeros(2, 9, 2, 16, dtype=t)
+        accepted(lambda: ops.window_attention(q, k, k, 3, 1))
+        accepted(lambda: ops.window_attention(q, k, k, 2 ** 40, 2 ** 40, scale=-1.0))
+        accepted(lambda: ops.window_attention(q, k[:, :0], k[:, :0], 3))
+        accepted(lambda: ops.window_attention(q[:, :0], k, k, 3))
+        n = torch.tensor([5, 9])
+        accepted(lambda: ops.window_attention(q, k, k, 3, kv_lengths=n, q_lengths=n.int()))
+        lse = torch.zeros(2, 4, 5)
+        accepted(lambda: ops.window_attention_backward(q, q, k, k, q, lse, 3, 1))
+        accepted(lambda: ops.window_attention_backward(q[:, :0], q[:, :0], k, k, q[:, :0], lse[..., :0].contiguous(), 3, 1))
+
+
+def test_attention_refuses(ops):
+    q, k, lse = torch.zeros(2, 5, 4, 16), torch.zeros(2, 9, 2, 16), torch.zeros(2, 4, 5)
+    att, back = ops.window_attention, ops.window_attention_backward
+    refused(ops, lambda: att(q.double(), k.double(), k.double(), 3, out=q, lse=lse), "dtype DOUBLE")
+    refused(ops, lambda: att(q, k.half(), k.half(), 3), "one type")
+    refused(ops, lambda: att(q, k, k[:, :8], 3), "k's shape")
+    refused(ops, lambda: att(q, k[:1], k[:1], 3), "one batch")
+    refused(ops, lambda: att(q, k[..., :8], k[..., :8], 3), "one dim")
+    refused(ops, lambda: att(q[:, :, :3], k, k, 3), "multiple")
+    refused(ops, lambda: att(q, k[:, :, :0], k[:, :, :0], 3), "multiple")
+    refused(ops, lambda: att(torch.zeros(1, 1, 1, 257), torch.zeros(1, 1, 1, 257), torch.zeros(1, 1, 1, 257), 3), "dim must be")
+    refused(ops, lambda: att(q, k, k, 0), "window")
+    refused(ops, lambda: att(q, k, k, 3, -1), "sinks")
+    refused(ops, lambda: att(q, k, k, 3, scale=float("nan")), "scale")
+    refused(ops, lambda: att(q, k, k, 3, kv_lengths=torch.zeros(2)), "lengths must be INT32")
+    refused(ops, lambda: att(q, k, k, 3, kv_lengths=torch.zeros(3, dtype=torch.int32)), "lengths must be [batch]")
+    refused(ops, lambda: att(q, k, k, 3, q_lengths=torch.zeros(4, dtype=torch.int32)[::2]), "lengths must be [batch]")
+    refused(ops, lambda: att(q, k, k, 3, out=q.half()), "out must have")
+    refused(ops, lambda: att(q, k, k, 3, out=torch.zeros(1, 5, 4, 16).expand(2, 5, 4, 16)), "overlap")
+    refused(ops, lambda: att(q, k, k, 3, lse=torch.zeros(2, 5, 4)), "lse must be")
+    refused(ops, lambda: back(q, q, k, k, q, lse.half(), 3), "lse must be")
+    refused(ops, lambda: back(q, q, k, k, q[:, :4], lse, 3), "gradOut, out and gradQ")
+    refused(ops, lambda: back(q, q, k, k, q, lse, 3, grad_k=q), "gradK and gradV")
+    refused(ops, lambda: back(q, q, k, k, q, lse, 3, grad_v=torch.zeros(1, 1, 1, 16).expand(2, 9, 2, 16)), "overlap")
+    with pytest.raises(IndexError):
+        att(q[0, 0], k, k, 3)
+
+
 def test_tensors_of_two_devices(ops):
     x = torch.zeros(2, 8)
     with pytest.raises(ValueError, match="one device"):
