@@ -459,6 +459,10 @@ int32_t opscvGetBackwardAlgo(void) { return g_backwardAlgo; }
 int32_t opscvVersion(void) { return 100; }
 uint64_t opscvGetLaunchCount(void) { return LaunchCount(); }
 void opscvResetLaunchCount(void) { ResetLaunchCount(); }
-uint32_t opscvGetAsyncCopyTimeouts(void) { return AsyncCopyTimeouts(); }
+uint32_t opscvGetAsyncCopyTimeouts(void)
+{
+    const uint32_t copies = AsyncCopyTimeouts(), attention = AttentionTimeouts();
+    return copies == 0xffffffffu || attention == 0xffffffffu ? 0xffffffffu : copies + attention;
+}
 
 } // extern "C"

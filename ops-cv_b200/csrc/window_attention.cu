@@ -69,6 +69,15 @@ dim3 RowGrid(int32_t rows, int64_t others)
     return dim3(static_cast<unsigned>(CeilDiv(rows, kRowWarps)), static_cast<unsigned>(others < 65535 ? others : 65535));
 }
 
+// Whether a call can take the tensor-core kernels: scores of a scale near 0 keep to the others, where 0 times an infinity is handled.
+bool MmaTakes(Dt dt, const AttnArgs& a)
+{
+    const AttnShape& s = a.s;
+    return dt != Dt::F32 && s.dim <= kMmaMostDim && fabsf(s.scale) > 1e-30f && s.lk > 0 &&
+           static_cast<int64_t>(s.batch) * s.heads * CeilDiv(s.lq, 128) <= INT32_MAX && AttnTmaReadable(a.q, s.lq, s.heads, s.batch) &&
+           AttnTmaReadable(a.k, s.lk, s.kvHeads, s.batch) && AttnTmaReadable(a.v, s.lk, s.kvHeads, s.batch);
+}
+
 } // namespace
 
 uint64_t WindowAttentionFwdWorkspace(Dt, const AttnShape&) { return 0; }
@@ -84,6 +93,9 @@ cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& s, AttnTensor q, AttnTens
     a.out = out;
     a.lse = lse;
     a.group = s.heads / s.kvHeads;
+    if (s.lq > 16 && MmaTakes(dt, a)) {
+        return AttnForwardMma(dt, a, stream);
+    }
     const dim3 grid = RowGrid(s.lq, static_cast<int64_t>(s.batch) * s.heads);
     OPSCV_DISPATCH_DT(dt, T, AttnForwardRowsKernel<T><<<grid, 32 * kRowWarps, 0, stream>>>(a));
     CountLaunch();

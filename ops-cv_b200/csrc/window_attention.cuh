@@ -247,4 +247,10 @@ __device__ __noinline__ void AttnGradKvRow(const AttnArgs& a, int32_t b, int32_t
     }
 }
 
+// ---- tensor-core kernels (window_attention_mma.cu) ---------------------------------------------------------------------------
+bool AttnTmaReadable(const AttnTensor& t, int32_t tokens, int32_t heads, int32_t batch);
+// 16-bit tensors that boxes can be loaded from, heads of at most 128 values, scale != 0
+cudaError_t AttnForwardMma(Dt dt, const AttnArgs& a, cudaStream_t stream);
+constexpr int kMmaMostDim = 128;
+
 } // namespace opscv
