@@ -44,6 +44,9 @@ __device__ __forceinline__ int32_t StepKey(const KeySteps& r, int32_t n)
     return n < r.sinkSteps ? n * kTile : r.first + (n - r.sinkSteps) * kTile;
 }
 
+// Bits 0 to n - 1 of a word, n cut to [0, 32].
+__device__ __forceinline__ uint32_t Below(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
 // ---- forward -----------------------------------------------------------------------------------------------------------------
 // A block has 128 queries of a head. Warp 4's first thread loads the tiles and issues the products; warps 0 to 3 have a query a
 // thread: S = Q K^T arrives in tensor memory, the thread forms the weights of its row, writes them over S as 16-bit values, and
@@ -177,24 +180,30 @@ __global__ void __launch_bounds__(160, 2)
             TmemLoadWait();
             const bool whole = it >= steps.sinkSteps && j0 + kTile - 1 <= wLow && j0 > wHigh - s.window && i0 + 32 * warp + 31 <= iLast;
             if (!whole) {
-                // visible columns of the step: those of the window, or those of the sinks
-                const int32_t from = it < steps.sinkSteps ? 0 : seen.first - j0;
-                const int32_t to = it < steps.sinkSteps ? steps.sinkEnd - j0 : p - j0 + 1;
-                const bool none = p < 0;
-                // a window step may hold sinks as well: those behind the block's first key, in front of the row's window
-                const int32_t sinkTo = it < steps.sinkSteps ? 0 : seen.sinkEnd - j0;
+                // visible columns of the step: those of the window, or those of the sinks. A window step may hold sinks as well:
+                // those behind the block's first key, in front of the row's window.
+                const bool sinkStep = it < steps.sinkSteps;
+                const int32_t from = sinkStep ? 0 : seen.first - j0;
+                const int32_t to = p < 0 ? 0 : sinkStep ? steps.sinkEnd - j0 : p - j0 + 1;
+                const int32_t sinkTo = sinkStep ? 0 : seen.sinkEnd - j0;
 #pragma unroll
-                for (int c = 0; c < kTile; ++c) {
-                    const bool live = !none && ((c >= from && c < to) || c < sinkTo);
-                    x[c] = live ? x[c] : 0xff800000u;
+                for (int c = 0; c < kTile; c += 32) {
+                    const uint32_t live = (Below(to - c) & ~Below(from - c)) | Below(sinkTo - c);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        x[c + e] = (live >> e & 1) != 0 ? x[c + e] : 0xff800000u;
+                    }
                 }
             }
-            float most = -INFINITY;
+            float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < kTile; ++c) {
-                most = fmaxf(most, __uint_as_float(x[c]));
+            for (int c = 0; c < kTile; c += 8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    part[e] = fmaxf(fmaxf(part[e], __uint_as_float(x[c + 2 * e])), __uint_as_float(x[c + 2 * e + 1]));
+                }
             }
-            most *= factor;
+            const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * factor;
             const float grown = fmaxf(top, most);
             const bool grow = grown > top + kGrowth; // always from -infinity to a number
             if (it == 0) {
@@ -203,37 +212,39 @@ __global__ void __launch_bounds__(160, 2)
                 const float fade = grow ? Exp2(top - grown) : 1.0f;
                 top = grow ? grown : top;
                 total *= fade;
-#pragma unroll
-                for (int c = 0; c < 2 * HALVES; ++c) {
-                    uint32_t o[32];
-                    TmemLoad32(tO + lanes + 32 * c, o);
+#pragma unroll 1
+                for (int c = 0; c < 8 * HALVES; ++c) {
+                    uint32_t o[8];
+                    TmemLoad8(tO + lanes + 8 * c, o);
                     TmemLoadWait();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
+                    for (int e = 0; e < 8; ++e) {
                         o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
                     }
-                    TmemStore32(tO + lanes + 32 * c, o);
+                    TmemStore8(tO + lanes + 8 * c, o);
                 }
             }
             const float off = top == -INFINITY ? 0.0f : -top;
             const F2 factor2 = MakeF2(factor, factor), off2 = MakeF2(off, off);
-            F2 sum2 = MakeF2(0.0f, 0.0f);
-            uint32_t w[kTile / 2];
+            F2 sum2[2] = {MakeF2(0.0f, 0.0f), MakeF2(0.0f, 0.0f)};
 #pragma unroll
-            for (int c = 0; c < kTile / 2; ++c) {
-                const F2 e = Fma2(MakeF2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), factor2, off2);
-                float e0, e1;
-                SplitF2(e, e0, e1);
-                e0 = Exp2(e0);
-                e1 = Exp2(e1);
-                sum2 = Add2(sum2, MakeF2(e0, e1));
-                w[c] = PackPair(e0, e1, static_cast<const T*>(nullptr));
+            for (int c = 0; c < kTile; c += 32) {
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const F2 z = Fma2(MakeF2(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])), factor2, off2);
+                    float e0, e1;
+                    SplitF2(z, e0, e1);
+                    e0 = Exp2(e0);
+                    e1 = Exp2(e1);
+                    sum2[e & 1] = Add2(sum2[e & 1], MakeF2(e0, e1));
+                    w[e] = PackPair(e0, e1, static_cast<const T*>(nullptr));
+                }
+                TmemStore16(tS + lanes + c / 2, w);
             }
             float a0, a1;
-            SplitF2(sum2, a0, a1);
+            SplitF2(Add2(sum2[0], sum2[1]), a0, a1);
             total += a0 + a1;
-            TmemStore32(tS + lanes, w);
-            TmemStore32(tS + lanes + 32, w + 32);
             TmemStoreWait();
             TcFenceBefore();
             BarArrive(&sh.pFull);
