@@ -66,9 +66,12 @@ __device__ __forceinline__ void TmaLoad4(void* dst, const CUtensorMap* map, uint
                  "l"(map), "r"(SharedAddr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                  : "memory");
 }
-__device__ __forceinline__ void TmaPrefetch(const CUtensorMap* map)
+// `bytes` in a row; both addresses and the size multiples of 16
+__device__ __forceinline__ void BulkLoad(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
 {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(SharedAddr(dst)), "l"(src),
+                 "r"(bytes), "r"(SharedAddr(bar))
+                 : "memory");
 }
 
 // ---- tensor memory -------------------------------------------------------------------------------------------------------------

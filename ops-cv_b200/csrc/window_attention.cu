@@ -102,9 +102,11 @@ cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& s, AttnTensor q, AttnTens
     return cudaGetLastError();
 }
 
-uint64_t WindowAttentionBwdWorkspace(Dt, const AttnShape& s)
+uint64_t WindowAttentionBwdWorkspace(Dt dt, const AttnShape& s)
 {
-    return static_cast<uint64_t>(s.batch) * s.heads * s.lq * 4;
+    const uint64_t rows = static_cast<uint64_t>(s.batch) * s.heads * s.lq * 4;
+    const uint64_t mma = dt != Dt::F32 && s.dim <= kMmaMostDim ? AttnBackwardMmaWorkspace(s) : 0;
+    return rows > mma ? rows : mma; // which kernels a call takes is known only with the pointers
 }
 
 cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& s, AttnTensor gradOut, AttnTensor q, AttnTensor k, AttnTensor v, AttnTensor out,
@@ -124,7 +126,11 @@ cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& s, AttnTensor gradOut, At
     a.lse = const_cast<float*>(lse);
     float* delta = static_cast<float*>(workspace);
     a.delta = delta;
+    a.deltaStride = s.lq;
     a.group = s.heads / s.kvHeads;
+    if (s.lq > 16 && MmaTakes(dt, a) && AttnTmaReadable(gradOut, s.lq, s.heads, s.batch)) {
+        return AttnBackwardMma(dt, a, workspace, stream);
+    }
     const dim3 rows = RowGrid(s.lq, static_cast<int64_t>(s.batch) * s.heads);
     const dim3 keys = RowGrid(s.lk, static_cast<int64_t>(s.batch) * s.kvHeads);
     OPSCV_DISPATCH_DT(dt, T, {

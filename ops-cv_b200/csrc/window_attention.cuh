@@ -16,7 +16,8 @@ struct AttnArgs {
     AttnShape s;
     AttnTensor q, k, v, out, gradOut, gradQ, gradK, gradV;
     float* lse;         // [batch, heads, lq], null where it is not wanted
-    const float* delta; // the same (backward)
+    const float* delta; // the same with rows of deltaStride (backward)
+    int64_t deltaStride;
     int32_t group;      // heads / kvHeads
 };
 
@@ -161,8 +162,8 @@ __device__ __noinline__ void AttnGradQRow(const AttnArgs& a, int32_t b, int32_t 
     const T* q = RowOf<T>(a.q, b, i, h);
     const T* g = RowOf<T>(a.gradOut, b, i, h);
     const int32_t u = h / a.group;
-    const int64_t row = (static_cast<int64_t>(b) * a.s.heads + h) * a.s.lq + i;
-    const float lse = a.lse[row], delta = a.delta[row];
+    const int64_t head = static_cast<int64_t>(b) * a.s.heads + h;
+    const float lse = a.lse[head * a.s.lq + i], delta = a.delta[head * a.deltaStride + i];
     float acc[kLaneDims] = {};
     for (int32_t at = 0; at < seen.count; at += 32) {
         const bool live = at + lane < seen.count;
@@ -211,13 +212,13 @@ __device__ __noinline__ void AttnGradKvRow(const AttnArgs& a, int32_t b, int32_t
     const T* v = RowOf<T>(a.v, b, j, u);
     float accK[kLaneDims] = {}, accV[kLaneDims] = {};
     for (int32_t h = u * a.group; h < (u + 1) * a.group; ++h) {
-        const int64_t rows = (static_cast<int64_t>(b) * a.s.heads + h) * a.s.lq;
+        const int64_t head = static_cast<int64_t>(b) * a.s.heads + h;
         for (int32_t at = first; at <= last; at += 32) {
             const int32_t i = at + lane - n.shift;
             float p = 0.0f, ds = 0.0f;
             if (at + lane <= last) {
-                p = expf(DotRows(RowOf<T>(a.q, b, i, h), k, a.s.dim) * a.s.scale - a.lse[rows + i]);
-                ds = p * (DotRows(RowOf<T>(a.gradOut, b, i, h), v, a.s.dim) - a.delta[rows + i]) * a.s.scale;
+                p = expf(DotRows(RowOf<T>(a.q, b, i, h), k, a.s.dim) * a.s.scale - a.lse[head * a.s.lq + i]);
+                ds = p * (DotRows(RowOf<T>(a.gradOut, b, i, h), v, a.s.dim) - a.delta[head * a.deltaStride + i]) * a.s.scale;
             }
             const int32_t m = last - at + 1 < 32 ? last - at + 1 : 32;
             for (int32_t r = 0; r < m; ++r) {
@@ -251,6 +252,9 @@ __device__ __noinline__ void AttnGradKvRow(const AttnArgs& a, int32_t b, int32_t
 bool AttnTmaReadable(const AttnTensor& t, int32_t tokens, int32_t heads, int32_t batch);
 // 16-bit tensors that boxes can be loaded from, heads of at most 128 values, scale != 0
 cudaError_t AttnForwardMma(Dt dt, const AttnArgs& a, cudaStream_t stream);
+// a.lse, a.out and a.gradOut too; the workspace holds delta and the statistics, and partial sums of the sinks' gradients
+uint64_t AttnBackwardMmaWorkspace(const AttnShape& s);
+cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStream_t stream);
 constexpr int kMmaMostDim = 128;
 
 } // namespace opscv

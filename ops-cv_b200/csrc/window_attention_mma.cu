@@ -53,7 +53,7 @@ __device__ __forceinline__ uint32_t Below(int32_t n) { return n <= 0 ? 0u : n >=
 // O += P V takes them from there, so that neither S nor P touches shared memory. Two blocks share an SM (256 columns of tensor memory
 // and 97 KB each): while one forms its weights, the other's products run.
 struct ForwardShared {
-    uint64_t qFull, kFull, vFull, sFull, pFull, oFull;
+    uint64_t qFull, kFull, vFull, sFull, pFull, oFull, drain;
     uint32_t tmem;
     uint32_t failed;
 };
@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(160, 2)
         BarInit(&sh.sFull, 1);
         BarInit(&sh.pFull, 128);
         BarInit(&sh.oFull, 1);
+        BarInit(&sh.drain, 1);
         BarInitDone();
     }
     if (warp == 4) {
@@ -154,6 +155,10 @@ __global__ void __launch_bounds__(160, 2)
                 if (it + 1 < steps.steps) {
                     load(sv, &mapV, &sh.vFull, StepKey(steps, it + 1), u);
                 }
+            }
+            if (*failed != 0) {
+                MmaCommit(&sh.drain);
+                BarDrain(&sh.drain, 0);
             }
         }
         __syncwarp();
@@ -324,6 +329,833 @@ __global__ void __launch_bounds__(160, 2)
     }
 }
 
+// ---- backward ----------------------------------------------------------------------------------------------------------------
+// Two kernels, each with the sums that it owns in tensor memory, so that no sum crosses blocks but for the sinks' (below) and all are
+// formed in a fixed order: gradQ by blocks of 128 queries that walk their keys, gradK and gradV by blocks of 128 keys that walk the
+// queries that see them. S and dP are formed twice for that (7 products where one kernel would do 5 and add gradQ up in memory, in an
+// order of chance). Both have one block an SM: warps 0 to 7 have a row each two threads (64 columns each), warp 8 loads, warp 9 issues
+// the products. The weights are scaled by 2^8 (folded into the statistics), which keeps small ones out of fp16's subnormal range.
+constexpr float kWeightShift = 8.0f;
+constexpr float kWeightScale = 0.00390625f; // 2^-8
+constexpr int kRowThreads = 256;
+
+struct BackwardArgs {
+    AttnArgs a;
+    int32_t qTiles, kTiles;
+    float* lse2;  // [batch, heads, stride]: lse in powers of two less kWeightShift; +infinity where a query sees nothing, so that its
+                  // weights are 0
+    float* delta; // [batch, heads, stride], 0 there
+    int64_t stride;
+    int32_t sinkTiles, farChunks; // see AttnGradKvMmaKernel
+    float* partial;
+    bool vecQ, vecK, vecV;
+};
+
+__device__ __forceinline__ void RowBarrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// delta and lse2 of a row by 16 lanes
+template <typename T>
+__global__ void __launch_bounds__(256) AttnStatisticsKernel(BackwardArgs m, bool vec)
+{
+    const AttnShape& s = m.a.s;
+    const int32_t lane = threadIdx.x & 15;
+    const int64_t total = static_cast<int64_t>(s.batch) * s.heads * m.stride;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+    const bool inside = row < total;
+    const int64_t bh = inside ? row / m.stride : 0;
+    const int32_t i = inside ? static_cast<int32_t>(row - bh * m.stride) : s.lq;
+    float sum = 0.0f;
+    float lse = INFINITY;
+    if (i < s.lq) {
+        const int32_t b = static_cast<int32_t>(bh / s.heads), h = static_cast<int32_t>(bh % s.heads);
+        const Lengths n = LengthsOf(s, b);
+        if (i < n.q && n.shift + i >= 0) {
+            const T* g = RowOf<T>(m.a.gradOut, b, i, h);
+            const T* o = RowOf<T>(m.a.out, b, i, h);
+            if (vec) {
+                const int32_t d = lane * 8;
+                if (d < s.dim) {
+                    float x[8], y[8];
+                    LoadPack<T, 8>(g + d, x);
+                    LoadPack<T, 8>(o + d, y);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        sum = fmaf(x[e], y[e], sum);
+                    }
+                }
+            } else {
+                for (int32_t d = lane; d < s.dim; d += 16) {
+                    sum = fmaf(DType<T>::ToF(g[d]), DType<T>::ToF(o[d]), sum);
+                }
+            }
+            lse = fmaf(m.a.lse[bh * s.lq + i], kLog2e, -kWeightShift);
+        }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    if (inside && lane == 0) {
+        m.lse2[row] = lse;
+        m.delta[row] = sum;
+    }
+}
+
+// fp16 alone: the rows of ds are scaled to its range by powers of two that follow the exponent (as it is stored, 0 to 255) of the
+// largest value so far. Returns the factor for what the accumulator holds already (1: as it is).
+struct RowScale {
+    float scale = 1.0f;
+    int32_t e = 0;
+    bool set = false;
+    __device__ __forceinline__ float Follow(uint32_t exponent)
+    {
+        const int32_t x = static_cast<int32_t>(exponent) - 127;
+        if (exponent == 0 || (set && x + e <= 13)) { // below 2^14 when scaled
+            return 1.0f;
+        }
+        const float before = scale;
+        const bool was = set;
+        e = 8 - x; // the largest becomes 2^8 to 2^9
+        e = e > 100 ? 100 : (e < -100 ? -100 : e);
+        scale = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+        set = true;
+        return was ? scale / before : 1.0f; // nothing but zeros before the first
+    }
+};
+__device__ __forceinline__ uint32_t ExponentOf(float positive) { return __float_as_uint(positive) >> 23; }
+
+// columns of an accumulator times a factor a row
+template <int N>
+__device__ __forceinline__ void TmemScale(uint32_t addr, float f)
+{
+#pragma unroll 1
+    for (int c = 0; c < N; c += 8) {
+        uint32_t o[8];
+        TmemLoad8(addr + c, o);
+        TmemLoadWait();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+        }
+        TmemStore8(addr + c, o);
+    }
+    TmemStoreWait();
+}
+
+// 32 values of a row of an output, of which `left` exist
+template <typename T>
+__device__ __forceinline__ void StoreRow32(T* out, const float (&v)[32], int32_t left, bool vec)
+{
+    if (vec) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+            if (e < left) {
+                float w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    w[k] = v[e + k];
+                }
+                StorePack<T, 8>(out + e, w);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            if (e < left) {
+                out[e] = DType<T>::FromF(v[e]);
+            }
+        }
+    }
+}
+
+// the weights of 64 columns, 0 in masked ones: exp2(factor s - lse2)
+__device__ __forceinline__ void MaskColumns(uint32_t (&x)[64], uint32_t live0, uint32_t live1)
+{
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        x[e] = (live0 >> e & 1) != 0 ? x[e] : 0xff800000u;
+        x[32 + e] = (live1 >> e & 1) != 0 ? x[32 + e] : 0xff800000u;
+    }
+}
+
+struct GradQShared {
+    uint64_t qFull, kFull[3], kEmpty[3], vFull[2], vEmpty[2], sFull[2], dpFull, dsReady, dqDone, allDone, exchanged, drain;
+    uint32_t tmem, failed, bad[4];
+    uint8_t most[2][2][kTile]; // fp16: exponents of a row's largest ds, of even and odd steps, of its two threads
+};
+
+// Tensor memory: S of even and odd steps at 0 and 128 (ds of a step goes over its S), dP at 256, gradQ at 384. The products of a step in
+// the order dP(n + 1), gradQ(n), S(n + 2): the row threads form the weights of step n + 1 from an S that is there already while the
+// first two run.
+template <typename T, int HALVES>
+__global__ void __launch_bounds__(320, 1)
+    AttnGradQMmaKernel(const __grid_constant__ BackwardArgs m, const __grid_constant__ CUtensorMap mapQ,
+                       const __grid_constant__ CUtensorMap mapG, const __grid_constant__ CUtensorMap mapK,
+                       const __grid_constant__ CUtensorMap mapV)
+{
+    extern __shared__ unsigned char raw[];
+    __shared__ GradQShared sh;
+    constexpr uint32_t kBytes = HALVES * kHalfBytes;
+    unsigned char* base = raw + (1024 - (SharedAddr(raw) & 1023)) % 1024;
+    unsigned char *sq = base, *sg = base + kBytes, *sk = base + 2 * kBytes, *sv = base + 5 * kBytes;
+    const AttnShape& s = m.a.s;
+    const int32_t tile = blockIdx.x % m.qTiles;
+    const int32_t bh = blockIdx.x / m.qTiles;
+    const int32_t b = bh / s.heads, h = bh % s.heads;
+    const Lengths n = LengthsOf(s, b);
+    const int32_t i0 = tile * kTile;
+    const int32_t iLast = min(i0 + kTile, n.q) - 1;
+    const int32_t low = n.shift + i0, high = iLast >= i0 ? n.shift + iLast : -1;
+    const KeySteps steps = StepsOf(s, low, high);
+    const int32_t count = steps.steps;
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        sh.failed = 0;
+        BarInit(&sh.qFull, 1);
+        for (int e = 0; e < 3; ++e) {
+            BarInit(&sh.kFull[e], 1);
+            BarInit(&sh.kEmpty[e], 1);
+        }
+        for (int e = 0; e < 2; ++e) {
+            BarInit(&sh.vFull[e], 1);
+            BarInit(&sh.vEmpty[e], 1);
+            BarInit(&sh.sFull[e], 1);
+        }
+        BarInit(&sh.dpFull, 1);
+        BarInit(&sh.dsReady, kRowThreads);
+        BarInit(&sh.dqDone, 1);
+        BarInit(&sh.allDone, 1);
+        BarInit(&sh.exchanged, kRowThreads);
+        BarInit(&sh.drain, 1);
+        BarInitDone();
+    }
+    if (threadIdx.x < 4) {
+        sh.bad[threadIdx.x] = 0;
+    }
+    if (warp == 9) {
+        TmemAlloc(&sh.tmem, 512);
+    }
+    TcFenceBefore();
+    __syncthreads();
+    TcFenceAfter();
+    const uint32_t tS = sh.tmem, tDp = tS + 256, tDq = tS + 384;
+    volatile uint32_t* failed = &sh.failed;
+
+    if (warp == 8) {
+        if ((threadIdx.x & 31) == 0 && count > 0) {
+            const int32_t u = h / m.a.group;
+            auto load = [&](unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int32_t row, int32_t head) {
+#pragma unroll
+                for (int c = 0; c < HALVES; ++c) {
+                    TmaLoad4(dst + c * kHalfBytes, map, bar, 64 * c, row, head, b);
+                }
+            };
+            BarExpect(&sh.qFull, 2 * kBytes);
+            load(sq, &mapQ, &sh.qFull, i0, h);
+            load(sg, &mapG, &sh.qFull, i0, h);
+            int32_t it = 0;
+            for (; it < count; ++it) {
+                const int32_t j0 = StepKey(steps, it), ks = it % 3, vs = it & 1;
+                if (it >= 3) {
+                    BarWait(&sh.kEmpty[ks], (it / 3 - 1) & 1, failed);
+                }
+                if (it >= 2) {
+                    BarWait(&sh.vEmpty[vs], (it / 2 - 1) & 1, failed);
+                }
+                if (*failed != 0) {
+                    break;
+                }
+                BarExpect(&sh.kFull[ks], kBytes);
+                load(sk + ks * kBytes, &mapK, &sh.kFull[ks], j0, u);
+                BarExpect(&sh.vFull[vs], kBytes);
+                load(sv + vs * kBytes, &mapV, &sh.vFull[vs], j0, u);
+            }
+            // own copies end before the block does, whatever became of the others
+            BarDrain(&sh.qFull, 0);
+            for (int32_t e = it > 3 ? it - 3 : 0; e < it; ++e) {
+                BarDrain(&sh.kFull[e % 3], (e / 3) & 1);
+            }
+            for (int32_t e = it > 2 ? it - 2 : 0; e < it; ++e) {
+                BarDrain(&sh.vFull[e & 1], (e / 2) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if ((threadIdx.x & 31) == 0 && count > 0) {
+            const int32_t kSteps = (s.dim + 15) / 16;
+            const uint32_t descS = ProductDesc<T>(kTile, false, s.scale < 0.0f), descDp = ProductDesc<T>(kTile, false, false);
+            const uint32_t descDq = ProductDesc<T>(kSteps * 16, true, false);
+            const uint32_t aq = SharedAddr(sq), ag = SharedAddr(sg), ak = SharedAddr(sk), av = SharedAddr(sv);
+            auto scores = [&](int32_t it) {
+                BarWait(&sh.kFull[it % 3], (it / 3) & 1, failed);
+                TcFenceAfter();
+                for (int32_t k = 0; k < kSteps; ++k) {
+                    const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
+                    MmaShared(tS + (it & 1) * 128, OperandDesc(aq + off, 16), OperandDesc(ak + (it % 3) * kBytes + off, 16), descS, k > 0);
+                }
+                MmaCommit(&sh.sFull[it & 1]);
+            };
+            auto products = [&](int32_t it) {
+                BarWait(&sh.vFull[it & 1], (it / 2) & 1, failed);
+                TcFenceAfter();
+                for (int32_t k = 0; k < kSteps; ++k) {
+                    const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
+                    MmaShared(tDp, OperandDesc(ag + off, 16), OperandDesc(av + (it & 1) * kBytes + off, 16), descDp, k > 0);
+                }
+                MmaCommit(&sh.dpFull);
+                MmaCommit(&sh.vEmpty[it & 1]);
+            };
+            BarWait(&sh.qFull, 0, failed);
+            scores(0);
+            products(0);
+            if (count > 1) {
+                scores(1);
+            }
+            for (int32_t it = 0; it < count && *failed == 0; ++it) {
+                BarWait(&sh.dsReady, it & 1, failed);
+                TcFenceAfter();
+                if (it + 1 < count) {
+                    products(it + 1);
+                }
+#pragma unroll
+                for (int32_t k = 0; k < kTile / 16; ++k) {
+                    MmaTmem(tDq, tS + (it & 1) * 128 + (k >> 2) * 64 + (k & 3) * 8,
+                            OperandDesc(ak + (it % 3) * kBytes + k * 2048, kHalfBytes), descDq, it > 0 || k > 0);
+                }
+                MmaCommit(&sh.kEmpty[it % 3]);
+                MmaCommit(&sh.dqDone);
+                if (it + 2 < count) {
+                    BarWait(&sh.dqDone, it & 1, failed); // ds(it), which the next scores go over, has been read
+                    scores(it + 2);
+                }
+            }
+            MmaCommit(&sh.allDone);
+            BarWait(&sh.allDone, 0, failed);
+            if (*failed != 0) {
+                MmaCommit(&sh.drain);
+                BarDrain(&sh.drain, 0);
+            }
+        }
+        __syncwarp();
+    } else {
+        const int32_t side = warp >> 2, r = (warp & 3) * 32 + (threadIdx.x & 31);
+        const int32_t i = i0 + r;
+        const int32_t p = i <= iLast ? n.shift + i : -1;
+        const Seen seen = SeenOf(s, p);
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+        const float factor = fabsf(s.scale) * kLog2e;
+        const int64_t row = static_cast<int64_t>(bh) * m.stride + i;
+        const float lse2 = p >= 0 ? m.lse2[row] : INFINITY, delta = p >= 0 ? m.delta[row] : 0.0f;
+        const F2 factor2 = MakeF2(factor, factor), off2 = MakeF2(-lse2, -lse2), delta2 = MakeF2(-delta, -delta);
+        RowScale range;
+        for (int32_t it = 0; it < count; ++it) {
+            const int32_t j0 = StepKey(steps, it) + 64 * side;
+            const uint32_t tx = tS + (it & 1) * 128 + 64 * side + lanes;
+            BarWait(&sh.sFull[it & 1], (it >> 1) & 1, failed);
+            if (__any_sync(0xffffffffu, *failed != 0)) {
+                break;
+            }
+            TcFenceAfter();
+            uint32_t x[64];
+            TmemLoad32(tx, x);
+            TmemLoad32(tx + 32, x + 32);
+            TmemLoadWait();
+            {
+                const bool sinkStep = it < steps.sinkSteps;
+                const int32_t from = sinkStep ? 0 : seen.first - j0;
+                const int32_t to = p < 0 ? 0 : sinkStep ? steps.sinkEnd - j0 : p - j0 + 1;
+                const int32_t sinkTo = sinkStep ? 0 : seen.sinkEnd - j0;
+                if (!__all_sync(0xffffffffu, from <= 0 && to >= 64)) {
+                    MaskColumns(x, (Below(to) & ~Below(from)) | Below(sinkTo), (Below(to - 32) & ~Below(from - 32)) | Below(sinkTo - 32));
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                float e0, e1;
+                SplitF2(Fma2(MakeF2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), factor2, off2), e0, e1);
+                x[2 * c] = __float_as_uint(Exp2(e0));
+                x[2 * c + 1] = __float_as_uint(Exp2(e1));
+            }
+            BarWait(&sh.dpFull, it & 1, failed);
+            TcFenceAfter();
+            float most = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+                uint32_t y[32];
+                TmemLoad32(tDp + 64 * side + lanes + c, y);
+                TmemLoadWait();
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const F2 d = Mul2(Add2(MakeF2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), delta2),
+                                      MakeF2(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1])));
+                    float d0, d1;
+                    SplitF2(d, d0, d1);
+                    x[c + e] = __float_as_uint(d0);
+                    x[c + e + 1] = __float_as_uint(d1);
+                    if constexpr (DType<T>::kIsHalf) {
+                        most = fmaxf(most, fmaxf(fabsf(d0), fabsf(d1)));
+                    }
+                }
+            }
+            float scale = 1.0f;
+            if constexpr (DType<T>::kIsHalf) {
+                sh.most[it & 1][side][r] = static_cast<uint8_t>(ExponentOf(most));
+                BarArrive(&sh.exchanged);
+                BarWait(&sh.exchanged, it & 1, failed);
+                const float change = range.Follow(max(ExponentOf(most), static_cast<uint32_t>(sh.most[it & 1][side ^ 1][r])));
+                scale = range.scale;
+                if (it > 0 && __any_sync(0xffffffffu, change != 1.0f)) {
+                    BarWait(&sh.dqDone, (it - 1) & 1, failed);
+                    TcFenceAfter();
+                    TmemScale<32 * HALVES>(tDq + lanes + 32 * HALVES * side, change);
+                }
+            }
+            uint32_t w[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                w[c] = PackPair(__uint_as_float(x[2 * c]) * scale, __uint_as_float(x[2 * c + 1]) * scale, static_cast<const T*>(nullptr));
+            }
+            TmemStore32(tx, w);
+            TmemStoreWait();
+            TcFenceBefore();
+            BarArrive(&sh.dsReady);
+        }
+        if (count > 0) {
+            BarWait(&sh.allDone, 0, failed);
+            TcFenceAfter();
+        }
+        T* out = i < s.lq ? OutRowOf<T>(m.a.gradQ, b, i, h) : nullptr;
+        const float last = s.scale * kWeightScale / range.scale;
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < HALVES; ++c) {
+            const int32_t d0 = 32 * (HALVES * side + c);
+            uint32_t o[32];
+            if (count > 0) {
+                TmemLoad32(tDq + lanes + d0, o);
+                TmemLoadWait();
+            }
+            float v[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                v[e] = p >= 0 ? __uint_as_float(o[e]) * last : 0.0f;
+                bad = bad || (d0 + e < s.dim && !(fabsf(v[e]) <= 3.4e38f));
+            }
+            if (out != nullptr && d0 < s.dim) {
+                StoreRow32<T>(out + d0, v, s.dim - d0, m.vecQ);
+            }
+        }
+        const uint32_t rows = __ballot_sync(0xffffffffu, bad && out != nullptr);
+        if ((threadIdx.x & 31) == 0 && rows != 0) {
+            atomicOr(&sh.bad[warp & 3], rows);
+        }
+        RowBarrier();
+        // rows that are not finite again, without the masked keys' part: the even ones by one warp, the odd ones by another
+        uint32_t again = sh.bad[warp & 3] & (side == 0 ? 0x55555555u : 0xaaaaaaaau);
+        while (again != 0) {
+            const int e = __ffs(again) - 1;
+            again &= again - 1;
+            AttnGradQRow<T>(m.a, b, h, i0 + 32 * (warp & 3) + e);
+        }
+        if (*failed != 0 && out != nullptr && side == 0) {
+            for (int32_t d = 0; d < s.dim; ++d) {
+                out[d] = DType<T>::FromF(NAN);
+            }
+        }
+    }
+    TcFenceBefore();
+    __syncthreads();
+    if (warp == 9) {
+        TcFenceAfter();
+        TmemFree(sh.tmem, 512);
+    }
+    if (threadIdx.x == 0 && sh.failed != 0) {
+        atomicAdd(&g_attentionTimeouts, 1u);
+    }
+}
+
+struct GradKvShared {
+    uint64_t kvFull, full[2], empty[2], sFull, dpFull, pReady, dsReady, dvDone, dkDone, exchanged, drain;
+    uint32_t tmem, failed, bad[4];
+    uint8_t most[2][2][kTile]; // fp16: exponents of a row's largest ds, of even and odd steps, of its two threads
+};
+
+// Tensor memory: S^T at 0 (the weights go over it), dP^T at 128 (ds goes over it), gradV at 256, gradK at 384; rows are keys, columns
+// queries. The products of a step in the order gradV(n), S(n + 1), gradK(n), dP(n + 1): the exponentials of step n + 1 run under the last
+// two, the rest of ds(n) under the first two.
+//
+// Sinks are seen by every later query. Were that left to the block of their keys, it would walk the whole sequence while the others
+// walk a window; so the queries behind the window of such a tile are shared out among farChunks further blocks. Their sums and the
+// tile's own go to `partial` ([tile][1 + farChunks][gradK, gradV][128][dim], fp32), which AttnSinkGradKernel adds up in order.
+template <typename T, int HALVES>
+__global__ void __launch_bounds__(320, 1)
+    AttnGradKvMmaKernel(const __grid_constant__ BackwardArgs m, const __grid_constant__ CUtensorMap mapQ,
+                        const __grid_constant__ CUtensorMap mapG, const __grid_constant__ CUtensorMap mapK,
+                        const __grid_constant__ CUtensorMap mapV)
+{
+    extern __shared__ unsigned char raw[];
+    __shared__ GradKvShared sh;
+    constexpr uint32_t kBytes = HALVES * kHalfBytes;
+    constexpr uint32_t kStage = 2 * kBytes + 2 * kTile * 4;
+    unsigned char* base = raw + (1024 - (SharedAddr(raw) & 1023)) % 1024;
+    unsigned char *sk = base, *sv = base + kBytes, *sqg = base + 2 * kBytes;  // two stages of Q and gradOut
+    float* stats = reinterpret_cast<float*>(base + 6 * kBytes);              // two stages of lse2 and delta
+    const AttnShape& s = m.a.s;
+    const int32_t perHead = m.kTiles + m.sinkTiles * m.farChunks;
+    const int32_t bu = blockIdx.x / perHead;
+    const int32_t b = bu / s.kvHeads, u = bu % s.kvHeads;
+    int32_t tile = blockIdx.x % perHead, chunk = -1;
+    if (tile >= m.kTiles) {
+        chunk = (tile - m.kTiles) % m.farChunks;
+        tile = (tile - m.kTiles) / m.farChunks;
+    }
+    const bool split = m.farChunks > 0 && tile < m.sinkTiles;
+    const Lengths n = LengthsOf(s, b);
+    const int32_t j0 = tile * kTile;
+    const int32_t jLast = min(j0 + kTile, n.kv) - 1;
+    const int32_t end = n.kv - 1; // position of the last query
+    // positions [low, high] of the queries that this block walks
+    int32_t low = max(j0, max(n.shift, 0)), high = min(end, jLast + s.window - 1);
+    if (chunk >= 0) {
+        low = max(low, jLast + s.window);
+        high = end;
+    } else if (j0 < s.sinks && !split) {
+        high = end;
+    }
+    if (jLast < j0) {
+        high = low - 1;
+    }
+    int32_t iBase = (low - n.shift) & ~3; // rows of the statistics are read 16 bytes at a time
+    const int32_t perGroup = high >= low ? (high - n.shift - iBase + kTile) / kTile : 0;
+    int32_t begin = 0, stop = perGroup * m.a.group;
+    if (chunk >= 0) {
+        const int32_t share = (stop + m.farChunks - 1) / m.farChunks;
+        begin = min(stop, chunk * share);
+        stop = min(stop, begin + share);
+    }
+    const int32_t count = stop - begin;
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        sh.failed = 0;
+        BarInit(&sh.kvFull, 1);
+        for (int e = 0; e < 2; ++e) {
+            BarInit(&sh.full[e], 1);
+            BarInit(&sh.empty[e], 1);
+        }
+        BarInit(&sh.sFull, 1);
+        BarInit(&sh.dpFull, 1);
+        BarInit(&sh.pReady, kRowThreads);
+        BarInit(&sh.dsReady, kRowThreads);
+        BarInit(&sh.dvDone, 1);
+        BarInit(&sh.dkDone, 1);
+        BarInit(&sh.exchanged, kRowThreads);
+        BarInit(&sh.drain, 1);
+        BarInitDone();
+    }
+    if (threadIdx.x < 4) {
+        sh.bad[threadIdx.x] = 0;
+    }
+    if (warp == 9) {
+        TmemAlloc(&sh.tmem, 512);
+    }
+    TcFenceBefore();
+    __syncthreads();
+    TcFenceAfter();
+    const uint32_t tS = sh.tmem, tDp = tS + 128, tDv = tS + 256, tDk = tS + 384;
+    volatile uint32_t* failed = &sh.failed;
+
+    if (warp == 8) {
+        if ((threadIdx.x & 31) == 0 && count > 0) {
+            auto load = [&](unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int32_t row, int32_t head) {
+#pragma unroll
+                for (int c = 0; c < HALVES; ++c) {
+                    TmaLoad4(dst + c * kHalfBytes, map, bar, 64 * c, row, head, b);
+                }
+            };
+            BarExpect(&sh.kvFull, 2 * kBytes);
+            load(sk, &mapK, &sh.kvFull, j0, u);
+            load(sv, &mapV, &sh.kvFull, j0, u);
+            int32_t it = 0;
+            for (; it < count; ++it) {
+                const int32_t st = it & 1, h = u * m.a.group + (begin + it) / perGroup;
+                const int32_t i0 = iBase + (begin + it) % perGroup * kTile;
+                if (it >= 2) {
+                    BarWait(&sh.empty[st], (it / 2 - 1) & 1, failed);
+                }
+                if (*failed != 0) {
+                    break;
+                }
+                BarExpect(&sh.full[st], kStage);
+                load(sqg + st * 2 * kBytes, &mapQ, &sh.full[st], i0, h);
+                load(sqg + st * 2 * kBytes + kBytes, &mapG, &sh.full[st], i0, h);
+                const int64_t row = (static_cast<int64_t>(b) * s.heads + h) * m.stride + i0;
+                BulkLoad(stats + st * 2 * kTile, m.lse2 + row, kTile * 4, &sh.full[st]);
+                BulkLoad(stats + st * 2 * kTile + kTile, m.delta + row, kTile * 4, &sh.full[st]);
+            }
+            BarDrain(&sh.kvFull, 0);
+            for (int32_t e = it > 2 ? it - 2 : 0; e < it; ++e) {
+                BarDrain(&sh.full[e & 1], (e / 2) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if ((threadIdx.x & 31) == 0 && count > 0) {
+            const int32_t kSteps = (s.dim + 15) / 16;
+            const uint32_t descS = ProductDesc<T>(kTile, false, s.scale < 0.0f), descDp = ProductDesc<T>(kTile, false, false);
+            const uint32_t descOut = ProductDesc<T>(kSteps * 16, true, false);
+            const uint32_t ak = SharedAddr(sk), av = SharedAddr(sv), aq = SharedAddr(sqg);
+            auto inner = [&](uint32_t d, uint32_t a, uint32_t rows, uint32_t desc, uint64_t* bar) {
+                for (int32_t k = 0; k < kSteps; ++k) {
+                    const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
+                    MmaShared(d, OperandDesc(a + off, 16), OperandDesc(rows + off, 16), desc, k > 0);
+                }
+                MmaCommit(bar);
+            };
+            auto outer = [&](uint32_t d, uint32_t a, uint32_t rows, bool add) {
+#pragma unroll
+                for (int32_t k = 0; k < kTile / 16; ++k) {
+                    MmaTmem(d, a + (k >> 2) * 64 + (k & 3) * 8, OperandDesc(rows + k * 2048, kHalfBytes), descOut, add || k > 0);
+                }
+            };
+            BarWait(&sh.kvFull, 0, failed);
+            BarWait(&sh.full[0], 0, failed);
+            TcFenceAfter();
+            inner(tS, ak, aq, descS, &sh.sFull);
+            inner(tDp, av, aq + kBytes, descDp, &sh.dpFull);
+            for (int32_t it = 0; it < count && *failed == 0; ++it) {
+                const uint32_t phase = it & 1, at = aq + (it & 1) * 2 * kBytes, next = aq + ((it + 1) & 1) * 2 * kBytes;
+                BarWait(&sh.pReady, phase, failed);
+                TcFenceAfter();
+                outer(tDv, tS, at + kBytes, it > 0);
+                MmaCommit(&sh.dvDone);
+                if (it + 1 < count) {
+                    BarWait(&sh.full[(it + 1) & 1], ((it + 1) / 2) & 1, failed);
+                    BarWait(&sh.dvDone, phase, failed); // the weights, which the next scores go over, have been read
+                    TcFenceAfter();
+                    inner(tS, ak, next, descS, &sh.sFull);
+                }
+                BarWait(&sh.dsReady, phase, failed);
+                TcFenceAfter();
+                outer(tDk, tDp, at, it > 0);
+                MmaCommit(&sh.empty[it & 1]);
+                MmaCommit(&sh.dkDone);
+                if (it + 1 < count) {
+                    BarWait(&sh.dkDone, phase, failed);
+                    TcFenceAfter();
+                    inner(tDp, av, next + kBytes, descDp, &sh.dpFull);
+                }
+            }
+            BarWait(&sh.dkDone, (count - 1) & 1, failed);
+            if (*failed != 0) {
+                MmaCommit(&sh.drain);
+                BarDrain(&sh.drain, 0);
+            }
+        }
+        __syncwarp();
+    } else {
+        const int32_t side = warp >> 2, r = (warp & 3) * 32 + (threadIdx.x & 31);
+        const int32_t j = j0 + r;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+        const float factor = fabsf(s.scale) * kLog2e;
+        const F2 factor2 = MakeF2(factor, factor);
+        // positions [from, to) of the queries that see key j, of those that this block walks
+        const int32_t from = max(j, low);
+        const int32_t to = j >= n.kv ? 0 : (j < s.sinks || s.window > high + 1 - j) ? high + 1 : j + s.window;
+        RowScale range;
+        for (int32_t it = 0; it < count; ++it) {
+            const int32_t st = it & 1;
+            const int32_t p0 = n.shift + iBase + (begin + it) % perGroup * kTile + 64 * side;
+            BarWait(&sh.full[st], (it >> 1) & 1, failed); // the statistics
+            BarWait(&sh.sFull, it & 1, failed);
+            if (__any_sync(0xffffffffu, *failed != 0)) {
+                break;
+            }
+            TcFenceAfter();
+            uint32_t x[64];
+            TmemLoad32(tS + 64 * side + lanes, x);
+            TmemLoad32(tS + 64 * side + lanes + 32, x + 32);
+            TmemLoadWait();
+            if (!__all_sync(0xffffffffu, from <= p0 && to >= p0 + 64)) {
+                MaskColumns(x, Below(to - p0) & ~Below(from - p0), Below(to - p0 - 32) & ~Below(from - p0 - 32));
+            }
+            const float4* lse = reinterpret_cast<const float4*>(stats + st * 2 * kTile + 64 * side);
+            const float4* del = reinterpret_cast<const float4*>(stats + st * 2 * kTile + kTile + 64 * side);
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 l = lse[(c + e) / 4];
+                    float z[4];
+                    SplitF2(Fma2(MakeF2(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1])), factor2, MakeF2(-l.x, -l.y)), z[0], z[1]);
+                    SplitF2(Fma2(MakeF2(__uint_as_float(x[c + e + 2]), __uint_as_float(x[c + e + 3])), factor2, MakeF2(-l.z, -l.w)), z[2],
+                            z[3]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        z[k] = Exp2(z[k]);
+                        x[c + e + k] = __float_as_uint(z[k]);
+                    }
+                    w[e / 2] = PackPair(z[0], z[1], static_cast<const T*>(nullptr));
+                    w[e / 2 + 1] = PackPair(z[2], z[3], static_cast<const T*>(nullptr));
+                }
+                TmemStore16(tS + 64 * side + lanes + c / 2, w);
+            }
+            TmemStoreWait();
+            TcFenceBefore();
+            BarArrive(&sh.pReady);
+            BarWait(&sh.dpFull, it & 1, failed);
+            TcFenceAfter();
+            float most = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+                uint32_t y[32];
+                TmemLoad32(tDp + 64 * side + lanes + c, y);
+                TmemLoadWait();
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 d = del[(c + e) / 4];
+                    float z[4];
+                    SplitF2(Mul2(Add2(MakeF2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), MakeF2(-d.x, -d.y)),
+                                 MakeF2(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1]))),
+                            z[0], z[1]);
+                    SplitF2(Mul2(Add2(MakeF2(__uint_as_float(y[e + 2]), __uint_as_float(y[e + 3])), MakeF2(-d.z, -d.w)),
+                                 MakeF2(__uint_as_float(x[c + e + 2]), __uint_as_float(x[c + e + 3]))),
+                            z[2], z[3]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        x[c + e + k] = __float_as_uint(z[k]);
+                        if constexpr (DType<T>::kIsHalf) {
+                            most = fmaxf(most, fabsf(z[k]));
+                        }
+                    }
+                }
+            }
+            float scale = 1.0f;
+            if constexpr (DType<T>::kIsHalf) {
+                sh.most[it & 1][side][r] = static_cast<uint8_t>(ExponentOf(most));
+                BarArrive(&sh.exchanged);
+                BarWait(&sh.exchanged, it & 1, failed);
+                const float change = range.Follow(max(ExponentOf(most), static_cast<uint32_t>(sh.most[it & 1][side ^ 1][r])));
+                scale = range.scale;
+                if (it > 0 && __any_sync(0xffffffffu, change != 1.0f)) {
+                    BarWait(&sh.dkDone, (it - 1) & 1, failed);
+                    TcFenceAfter();
+                    TmemScale<32 * HALVES>(tDk + lanes + 32 * HALVES * side, change);
+                }
+            }
+            uint32_t w[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                w[c] = PackPair(__uint_as_float(x[2 * c]) * scale, __uint_as_float(x[2 * c + 1]) * scale, static_cast<const T*>(nullptr));
+            }
+            TmemStore32(tDp + 64 * side + lanes, w);
+            TmemStoreWait();
+            TcFenceBefore();
+            BarArrive(&sh.dsReady);
+        }
+        if (count > 0) {
+            BarWait(&sh.dkDone, (count - 1) & 1, failed);
+            TcFenceAfter();
+        }
+        const bool lives = j < s.lk;
+        bool bad = false;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            const float last = which == 0 ? s.scale * kWeightScale / range.scale : kWeightScale;
+            const uint32_t from32 = (which == 0 ? tDk : tDv) + lanes;
+            float* part = split ? m.partial + (((static_cast<int64_t>(bu) * m.sinkTiles + tile) * (1 + m.farChunks) + 1 + chunk) * 2 + which) *
+                                                  kTile * s.dim + static_cast<int64_t>(r) * s.dim :
+                                  nullptr;
+            T* out = lives && !split ? OutRowOf<T>(which == 0 ? m.a.gradK : m.a.gradV, b, j, u) : nullptr;
+#pragma unroll
+            for (int c = 0; c < HALVES; ++c) {
+                const int32_t d0 = 32 * (HALVES * side + c);
+                uint32_t o[32];
+                if (count > 0) {
+                    TmemLoad32(from32 + d0, o);
+                    TmemLoadWait();
+                }
+                float v[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    v[e] = count > 0 && j < n.kv ? __uint_as_float(o[e]) * last : 0.0f;
+                    bad = bad || (d0 + e < s.dim && !(fabsf(v[e]) <= 3.4e38f));
+                }
+                if (out != nullptr && d0 < s.dim) {
+                    StoreRow32<T>(out + d0, v, s.dim - d0, which == 0 ? m.vecK : m.vecV);
+                }
+                if (part != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        if (d0 + e < s.dim) {
+                            part[d0 + e] = *failed != 0 ? NAN : v[e];
+                        }
+                    }
+                }
+            }
+        }
+        const uint32_t rows = __ballot_sync(0xffffffffu, bad && lives && !split);
+        if ((threadIdx.x & 31) == 0 && rows != 0) {
+            atomicOr(&sh.bad[warp & 3], rows);
+        }
+        RowBarrier();
+        uint32_t again = sh.bad[warp & 3] & (side == 0 ? 0x55555555u : 0xaaaaaaaau);
+        while (again != 0) {
+            const int e = __ffs(again) - 1;
+            again &= again - 1;
+            AttnGradKvRow<T>(m.a, b, u, j0 + 32 * (warp & 3) + e);
+        }
+        if (*failed != 0 && lives && !split && side == 0) {
+            T *gk = OutRowOf<T>(m.a.gradK, b, j, u), *gv = OutRowOf<T>(m.a.gradV, b, j, u);
+            for (int32_t d = 0; d < s.dim; ++d) {
+                gk[d] = gv[d] = DType<T>::FromF(NAN);
+            }
+        }
+    }
+    TcFenceBefore();
+    __syncthreads();
+    if (warp == 9) {
+        TcFenceAfter();
+        TmemFree(sh.tmem, 512);
+    }
+    if (threadIdx.x == 0 && sh.failed != 0) {
+        atomicAdd(&g_attentionTimeouts, 1u);
+    }
+}
+
+// gradK and gradV of the keys of tiles with sinks: the blocks' sums in order, a warp per key.
+template <typename T>
+__global__ void __launch_bounds__(128) AttnSinkGradKernel(BackwardArgs m)
+{
+    const AttnShape& s = m.a.s;
+    const int lane = threadIdx.x & 31;
+    const int64_t key = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int64_t tileIndex = key / kTile; // (batch, key head, tile)
+    const int32_t r = static_cast<int32_t>(key % kTile);
+    const int32_t tile = static_cast<int32_t>(tileIndex % m.sinkTiles);
+    const int32_t bu = static_cast<int32_t>(tileIndex / m.sinkTiles);
+    const int32_t b = bu / s.kvHeads, u = bu % s.kvHeads, j = tile * kTile + r;
+    if (bu >= s.batch * s.kvHeads || j >= s.lk) {
+        return;
+    }
+    bool bad = false;
+    for (int which = 0; which < 2; ++which) {
+        T* out = OutRowOf<T>(which == 0 ? m.a.gradK : m.a.gradV, b, j, u);
+        for (int32_t d = lane; d < s.dim; d += 32) {
+            float sum = 0.0f;
+            for (int32_t c = 0; c <= m.farChunks; ++c) {
+                sum += m.partial[((tileIndex * (1 + m.farChunks) + c) * 2 + which) * kTile * s.dim + static_cast<int64_t>(r) * s.dim + d];
+            }
+            bad = bad || !(fabsf(sum) <= 3.4e38f);
+            out[d] = DType<T>::FromF(sum);
+        }
+    }
+    if (__any_sync(0xffffffffu, bad)) {
+        __syncwarp();
+        AttnGradKvRow<T>(m.a, b, u, j);
+    }
+}
+
 // ---- launches ------------------------------------------------------------------------------------------------------------------
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -403,6 +1235,102 @@ cudaError_t AttnForwardMma(Dt dt, const AttnArgs& a, cudaStream_t stream)
         return m.halves == 1 ? launch(AttnForwardMmaKernel<__half, 1>) : launch(AttnForwardMmaKernel<__half, 2>);
     }
     return m.halves == 1 ? launch(AttnForwardMmaKernel<__nv_bfloat16, 1>) : launch(AttnForwardMmaKernel<__nv_bfloat16, 2>);
+}
+
+namespace {
+
+bool VecRows(const AttnTensor& t, int32_t dim) { return dim % 8 == 0 && Aligned(t.p, 16) && t.l % 8 == 0 && t.h % 8 == 0 && t.b % 8 == 0; }
+
+// Further blocks for the sinks' far queries (AttnGradKvMmaKernel): as many as bring their walks down to that of an ordinary block.
+struct FarPlan {
+    int32_t sinkTiles = 0, chunks = 0;
+};
+FarPlan PlanFar(const AttnShape& s)
+{
+    FarPlan f;
+    const int64_t sinks = s.sinks < s.lk ? s.sinks : s.lk;
+    const int64_t group = s.heads / s.kvHeads;
+    const int64_t near = group * (CeilDiv(static_cast<int64_t>(s.window) + kTile, kTile) + 1);
+    const int64_t far = group * CeilDiv(s.lq > s.window ? s.lq - s.window : 0, kTile);
+    if (sinks > 0 && 2 * far > near) {
+        f.sinkTiles = static_cast<int32_t>(CeilDiv(sinks, kTile));
+        const int64_t chunks = CeilDiv(far, near);
+        f.chunks = static_cast<int32_t>(chunks < 64 ? chunks : 64);
+    }
+    return f;
+}
+int64_t StatsStride(const AttnShape& s) { return CeilDiv(s.lq, 4) * 4 + kTile; }
+uint64_t StatsBytes(const AttnShape& s) { return (static_cast<uint64_t>(s.batch) * s.heads * StatsStride(s) * 4 + 255) & ~255ull; }
+
+} // namespace
+
+uint64_t AttnBackwardMmaWorkspace(const AttnShape& s)
+{
+    const FarPlan f = PlanFar(s);
+    return 2 * StatsBytes(s) + static_cast<uint64_t>(s.batch) * s.kvHeads * f.sinkTiles * (f.chunks + 1) * 2 * kTile * s.dim * 4;
+}
+
+cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStream_t stream)
+{
+    const AttnShape& s = a.s;
+    const FarPlan f = PlanFar(s);
+    BackwardArgs m{};
+    m.a = a;
+    m.qTiles = static_cast<int32_t>(CeilDiv(s.lq, kTile));
+    m.kTiles = static_cast<int32_t>(CeilDiv(s.lk, kTile));
+    m.stride = StatsStride(s);
+    m.lse2 = static_cast<float*>(workspace);
+    m.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + StatsBytes(s));
+    m.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + 2 * StatsBytes(s));
+    m.a.delta = m.delta;
+    m.a.deltaStride = m.stride;
+    m.sinkTiles = f.sinkTiles;
+    m.farChunks = f.chunks;
+    m.vecQ = VecRows(a.gradQ, s.dim);
+    m.vecK = VecRows(a.gradK, s.dim);
+    m.vecV = VecRows(a.gradV, s.dim);
+    const int64_t statBlocks = CeilDiv(static_cast<int64_t>(s.batch) * s.heads * m.stride, 16);
+    const int64_t kvBlocks = static_cast<int64_t>(s.batch) * s.kvHeads * (m.kTiles + static_cast<int64_t>(m.sinkTiles) * m.farChunks);
+    if (statBlocks > INT32_MAX || kvBlocks > INT32_MAX) {
+        return cudaErrorInvalidConfiguration;
+    }
+    CUtensorMap mq, mg, mk, mv;
+    cudaError_t e = MakeMap(&mq, dt, a.q, s.dim, s.lq, s.heads, s.batch);
+    e = e != cudaSuccess ? e : MakeMap(&mg, dt, a.gradOut, s.dim, s.lq, s.heads, s.batch);
+    e = e != cudaSuccess ? e : MakeMap(&mk, dt, a.k, s.dim, s.lk, s.kvHeads, s.batch);
+    e = e != cudaSuccess ? e : MakeMap(&mv, dt, a.v, s.dim, s.lk, s.kvHeads, s.batch);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    const int32_t halves = s.dim > 64 ? 2 : 1;
+    const int bytes = halves * static_cast<int>(kHalfBytes);
+    const int sharedQ = 7 * bytes + 1024, sharedKv = 6 * bytes + 4 * kTile * 4 + 1024;
+    const unsigned qBlocks = static_cast<unsigned>(static_cast<int64_t>(s.batch) * s.heads * m.qTiles);
+    const bool vecStats = VecRows(a.gradOut, s.dim) && VecRows(a.out, s.dim);
+    auto launch = [&](auto tag, auto gradQ, auto gradKv) {
+        using T = decltype(tag);
+        AttnStatisticsKernel<T><<<static_cast<unsigned>(statBlocks), 256, 0, stream>>>(m, vecStats);
+        cudaError_t set = cudaFuncSetAttribute(gradQ, cudaFuncAttributeMaxDynamicSharedMemorySize, sharedQ);
+        set = set != cudaSuccess ? set : cudaFuncSetAttribute(gradKv, cudaFuncAttributeMaxDynamicSharedMemorySize, sharedKv);
+        if (set != cudaSuccess) {
+            return set;
+        }
+        gradQ<<<qBlocks, 320, sharedQ, stream>>>(m, mq, mg, mk, mv);
+        gradKv<<<static_cast<unsigned>(kvBlocks), 320, sharedKv, stream>>>(m, mq, mg, mk, mv);
+        CountLaunch(3);
+        if (m.farChunks > 0) {
+            const int64_t keys = static_cast<int64_t>(s.batch) * s.kvHeads * m.sinkTiles * kTile;
+            AttnSinkGradKernel<T><<<static_cast<unsigned>(CeilDiv(keys, 4)), 128, 0, stream>>>(m);
+            CountLaunch();
+        }
+        return cudaGetLastError();
+    };
+    if (dt == Dt::F16) {
+        return halves == 1 ? launch(__half{}, AttnGradQMmaKernel<__half, 1>, AttnGradKvMmaKernel<__half, 1>) :
+                             launch(__half{}, AttnGradQMmaKernel<__half, 2>, AttnGradKvMmaKernel<__half, 2>);
+    }
+    return halves == 1 ? launch(__nv_bfloat16{}, AttnGradQMmaKernel<__nv_bfloat16, 1>, AttnGradKvMmaKernel<__nv_bfloat16, 1>) :
+                         launch(__nv_bfloat16{}, AttnGradQMmaKernel<__nv_bfloat16, 2>, AttnGradKvMmaKernel<__nv_bfloat16, 2>);
 }
 
 uint32_t AttentionTimeouts()

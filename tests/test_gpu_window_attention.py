@@ -341,6 +341,15 @@ def test_graph_and_stream(ops, dev, lq):
         assert all(torch.equal(x, y) for x, y in zip(got, step()))
 
 
+def test_no_wait_ran_out(ops, dev):
+    """After all of the above: the bounded waits inside the kernels have all ended by themselves."""
+    q, k = normal((1, 700, 2, 64), BF16, 70, dev), normal((1, 700, 1, 64), BF16, 71, dev)
+    out, lse = ops.window_attention(q, k, k, 100, 2)
+    ops.window_attention_backward(q, q, k, k, out, lse, 100, 2)
+    torch.cuda.synchronize(dev)
+    assert ops.async_copy_timeouts() == 0
+
+
 def test_block_of_a_model(ops, dev):
     """Norm, projections, rotary positions, attention and the way back, as a block of a model strings them together, against 64 bits."""
     b, n, h, hk, d, width, window, sinks = 2, 150, 4, 2, 64, 256, 40, 2
