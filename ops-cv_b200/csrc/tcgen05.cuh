@@ -58,13 +58,18 @@ __device__ __forceinline__ void BarDrain(uint64_t* bar, uint32_t parity)
 }
 
 // ---- TMA ---------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void TmaLoad4At(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int32_t c0, int32_t c1, int32_t c2,
+                                           int32_t c3)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+                     "r"(dst),
+                 "l"(map), "r"(SharedAddr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+                 : "memory");
+}
 __device__ __forceinline__ void TmaLoad4(void* dst, const CUtensorMap* map, uint64_t* bar, int32_t c0, int32_t c1, int32_t c2,
                                          int32_t c3)
 {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
-                     "r"(SharedAddr(dst)),
-                 "l"(map), "r"(SharedAddr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-                 : "memory");
+    TmaLoad4At(SharedAddr(dst), map, bar, c0, c1, c2, c3);
 }
 // `bytes` in a row; both addresses and the size multiples of 16
 __device__ __forceinline__ void BulkLoad(void* dst, const void* src, uint32_t bytes, uint64_t* bar)

@@ -93,7 +93,10 @@ cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& s, AttnTensor q, AttnTens
     a.out = out;
     a.lse = lse;
     a.group = s.heads / s.kvHeads;
-    if (s.lq > 16 && MmaTakes(dt, a)) {
+    if (s.lq <= kStepMostQueries && s.lk > 0) {
+        return AttnStep(dt, a, stream);
+    }
+    if (MmaTakes(dt, a)) {
         return AttnForwardMma(dt, a, stream);
     }
     const dim3 grid = RowGrid(s.lq, static_cast<int64_t>(s.batch) * s.heads);
@@ -128,7 +131,7 @@ cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& s, AttnTensor gradOut, At
     a.delta = delta;
     a.deltaStride = s.lq;
     a.group = s.heads / s.kvHeads;
-    if (s.lq > 16 && MmaTakes(dt, a) && AttnTmaReadable(gradOut, s.lq, s.heads, s.batch)) {
+    if (s.lq > 0 && MmaTakes(dt, a) && AttnTmaReadable(gradOut, s.lq, s.heads, s.batch)) {
         return AttnBackwardMma(dt, a, workspace, stream);
     }
     const dim3 rows = RowGrid(s.lq, static_cast<int64_t>(s.batch) * s.heads);

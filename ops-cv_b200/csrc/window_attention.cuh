@@ -7,6 +7,10 @@
 //   gradV_j += p_j gradOut, ds_j = p_j (gradOut . v_j - delta) scale, gradQ += ds_j k_j, gradK_j += ds_j q.
 #pragma once
 
+#include <cuda.h> // CUtensorMap
+
+#include <atomic>
+
 #include "launch_util.cuh"
 #include "sequence_kernels.h"
 
@@ -248,13 +252,42 @@ __device__ __noinline__ void AttnGradKvRow(const AttnArgs& a, int32_t b, int32_t
     }
 }
 
+// ---- few queries (window_attention_step.cu) ----------------------------------------------------------------------------------
+constexpr int kStepMostQueries = 8;
+cudaError_t AttnStep(Dt dt, const AttnArgs& a, cudaStream_t stream);
+uint32_t AttnStepTimeouts();
+
 // ---- tensor-core kernels (window_attention_mma.cu) ---------------------------------------------------------------------------
 bool AttnTmaReadable(const AttnTensor& t, int32_t tokens, int32_t heads, int32_t batch);
+// Boxes of 64 values by boxTokens tokens of one head, in the 128-byte swizzle; what lies outside the tensor arrives as zeros.
+cudaError_t AttnMakeMap(CUtensorMap* map, Dt dt, const AttnTensor& t, int32_t dim, int32_t tokens, int32_t heads, int32_t batch,
+                        int32_t boxTokens);
 // 16-bit tensors that boxes can be loaded from, heads of at most 128 values, scale != 0
 cudaError_t AttnForwardMma(Dt dt, const AttnArgs& a, cudaStream_t stream);
 // a.lse, a.out and a.gradOut too; the workspace holds delta and the statistics, and partial sums of the sinks' gradients
 uint64_t AttnBackwardMmaWorkspace(const AttnShape& s);
 cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStream_t stream);
 constexpr int kMmaMostDim = 128;
+
+// Asks once for each device for the shared memory (and clusters of more than 8 blocks) that a kernel takes: a call of the runtime that
+// costs as much as a launch. `asked` has a bit a device.
+template <typename Kernel>
+cudaError_t AskOnce(Kernel kernel, std::atomic<uint64_t>& asked, int shared, bool wideCluster = false)
+{
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);
+    if (e != cudaSuccess || (asked.load(std::memory_order_relaxed) & bit) != 0) {
+        return e;
+    }
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+    if (e == cudaSuccess && wideCluster) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    }
+    if (e == cudaSuccess) {
+        asked.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return e;
+}
 
 } // namespace opscv

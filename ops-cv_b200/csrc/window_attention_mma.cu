@@ -1175,8 +1175,12 @@ EncodeTiled Encoder()
     return fn;
 }
 
-// Boxes of 64 values by 128 tokens of one head; what lies outside the tensor arrives as zeros.
-cudaError_t MakeMap(CUtensorMap* map, Dt dt, const AttnTensor& t, int32_t dim, int32_t tokens, int32_t heads, int32_t batch)
+bool TmaStride(int64_t stride, int32_t extent) { return extent <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); }
+
+} // namespace
+
+cudaError_t AttnMakeMap(CUtensorMap* map, Dt dt, const AttnTensor& t, int32_t dim, int32_t tokens, int32_t heads, int32_t batch,
+                        int32_t boxTokens)
 {
     const EncodeTiled encode = Encoder();
     if (encode == nullptr) {
@@ -1188,16 +1192,12 @@ cudaError_t MakeMap(CUtensorMap* map, Dt dt, const AttnTensor& t, int32_t dim, i
     // the stride along a single token, head or sequence is of no account, but has to be a valid one
     const cuuint64_t strides[3] = {tokens > 1 ? static_cast<cuuint64_t>(t.l) * 2 : row, heads > 1 ? static_cast<cuuint64_t>(t.h) * 2 : row,
                                    batch > 1 ? static_cast<cuuint64_t>(t.b) * 2 : row};
-    const cuuint32_t box[4] = {64, kTile, 1, 1}, step[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(boxTokens), 1, 1}, step[4] = {1, 1, 1, 1};
     const CUresult r = encode(map, dt == Dt::F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                               const_cast<void*>(t.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
-
-bool TmaStride(int64_t stride, int32_t extent) { return extent <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); }
-
-} // namespace
 
 // A tensor that boxes can be loaded from: 16-byte aligned rows, heads and sequences, none of them at one address.
 bool AttnTmaReadable(const AttnTensor& t, int32_t tokens, int32_t heads, int32_t batch)
@@ -1214,16 +1214,17 @@ cudaError_t AttnForwardMma(Dt dt, const AttnArgs& a, cudaStream_t stream)
     m.halves = s.dim > 64 ? 2 : 1;
     m.vecOut = s.dim % 8 == 0 && Aligned(a.out.p, 16) && a.out.l % 8 == 0 && a.out.h % 8 == 0 && a.out.b % 8 == 0;
     CUtensorMap mq, mk, mv;
-    cudaError_t e = MakeMap(&mq, dt, a.q, s.dim, s.lq, s.heads, s.batch);
-    e = e != cudaSuccess ? e : MakeMap(&mk, dt, a.k, s.dim, s.lk, s.kvHeads, s.batch);
-    e = e != cudaSuccess ? e : MakeMap(&mv, dt, a.v, s.dim, s.lk, s.kvHeads, s.batch);
+    cudaError_t e = AttnMakeMap(&mq, dt, a.q, s.dim, s.lq, s.heads, s.batch, kTile);
+    e = e != cudaSuccess ? e : AttnMakeMap(&mk, dt, a.k, s.dim, s.lk, s.kvHeads, s.batch, kTile);
+    e = e != cudaSuccess ? e : AttnMakeMap(&mv, dt, a.v, s.dim, s.lk, s.kvHeads, s.batch, kTile);
     if (e != cudaSuccess) {
         return e;
     }
     const int shared = 3 * m.halves * static_cast<int>(kHalfBytes) + 1024;
     const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(s.batch) * s.heads * m.tiles);
-    auto launch = [&](auto kernel) {
-        const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+    static std::atomic<uint64_t> asked[4];
+    auto launch = [&](auto kernel, int which) {
+        const cudaError_t set = AskOnce(kernel, asked[which], shared);
         if (set != cudaSuccess) {
             return set;
         }
@@ -1232,9 +1233,9 @@ cudaError_t AttnForwardMma(Dt dt, const AttnArgs& a, cudaStream_t stream)
         return cudaGetLastError();
     };
     if (dt == Dt::F16) {
-        return m.halves == 1 ? launch(AttnForwardMmaKernel<__half, 1>) : launch(AttnForwardMmaKernel<__half, 2>);
+        return m.halves == 1 ? launch(AttnForwardMmaKernel<__half, 1>, 0) : launch(AttnForwardMmaKernel<__half, 2>, 1);
     }
-    return m.halves == 1 ? launch(AttnForwardMmaKernel<__nv_bfloat16, 1>) : launch(AttnForwardMmaKernel<__nv_bfloat16, 2>);
+    return m.halves == 1 ? launch(AttnForwardMmaKernel<__nv_bfloat16, 1>, 2) : launch(AttnForwardMmaKernel<__nv_bfloat16, 2>, 3);
 }
 
 namespace {
@@ -1295,10 +1296,10 @@ cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStrea
         return cudaErrorInvalidConfiguration;
     }
     CUtensorMap mq, mg, mk, mv;
-    cudaError_t e = MakeMap(&mq, dt, a.q, s.dim, s.lq, s.heads, s.batch);
-    e = e != cudaSuccess ? e : MakeMap(&mg, dt, a.gradOut, s.dim, s.lq, s.heads, s.batch);
-    e = e != cudaSuccess ? e : MakeMap(&mk, dt, a.k, s.dim, s.lk, s.kvHeads, s.batch);
-    e = e != cudaSuccess ? e : MakeMap(&mv, dt, a.v, s.dim, s.lk, s.kvHeads, s.batch);
+    cudaError_t e = AttnMakeMap(&mq, dt, a.q, s.dim, s.lq, s.heads, s.batch, kTile);
+    e = e != cudaSuccess ? e : AttnMakeMap(&mg, dt, a.gradOut, s.dim, s.lq, s.heads, s.batch, kTile);
+    e = e != cudaSuccess ? e : AttnMakeMap(&mk, dt, a.k, s.dim, s.lk, s.kvHeads, s.batch, kTile);
+    e = e != cudaSuccess ? e : AttnMakeMap(&mv, dt, a.v, s.dim, s.lk, s.kvHeads, s.batch, kTile);
     if (e != cudaSuccess) {
         return e;
     }
@@ -1307,14 +1308,16 @@ cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStrea
     const int sharedQ = 7 * bytes + 1024, sharedKv = 6 * bytes + 4 * kTile * 4 + 1024;
     const unsigned qBlocks = static_cast<unsigned>(static_cast<int64_t>(s.batch) * s.heads * m.qTiles);
     const bool vecStats = VecRows(a.gradOut, s.dim) && VecRows(a.out, s.dim);
+    static std::atomic<uint64_t> askedQ[4], askedKv[4];
+    const int which = (dt == Dt::F16 ? 0 : 2) + halves - 1;
     auto launch = [&](auto tag, auto gradQ, auto gradKv) {
         using T = decltype(tag);
-        AttnStatisticsKernel<T><<<static_cast<unsigned>(statBlocks), 256, 0, stream>>>(m, vecStats);
-        cudaError_t set = cudaFuncSetAttribute(gradQ, cudaFuncAttributeMaxDynamicSharedMemorySize, sharedQ);
-        set = set != cudaSuccess ? set : cudaFuncSetAttribute(gradKv, cudaFuncAttributeMaxDynamicSharedMemorySize, sharedKv);
+        cudaError_t set = AskOnce(gradQ, askedQ[which], sharedQ);
+        set = set != cudaSuccess ? set : AskOnce(gradKv, askedKv[which], sharedKv);
         if (set != cudaSuccess) {
             return set;
         }
+        AttnStatisticsKernel<T><<<static_cast<unsigned>(statBlocks), 256, 0, stream>>>(m, vecStats);
         gradQ<<<qBlocks, 320, sharedQ, stream>>>(m, mq, mg, mk, mv);
         gradKv<<<static_cast<unsigned>(kvBlocks), 320, sharedKv, stream>>>(m, mq, mg, mk, mv);
         CountLaunch(3);
@@ -1336,7 +1339,7 @@ cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStrea
 uint32_t AttentionTimeouts()
 {
     unsigned int v = 0;
-    return cudaMemcpyFromSymbol(&v, g_attentionTimeouts, sizeof(v)) == cudaSuccess ? v : 0xffffffffu;
+    return cudaMemcpyFromSymbol(&v, g_attentionTimeouts, sizeof(v)) == cudaSuccess ? v + AttnStepTimeouts() : 0xffffffffu;
 }
 
 } // namespace opscv
