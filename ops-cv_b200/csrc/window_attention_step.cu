@@ -90,26 +90,32 @@ __device__ __forceinline__ void JoinRows(const StepArgs& m, int32_t b, int32_t u
     }
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync(); // of one block alone where there is one
-    // the cluster's blocks: a warp has a row
+    if (m.splits > 1) {
+        cluster.sync();
+    } else {
+        __syncthreads();
+    }
+    // the cluster's blocks: a warp has a row, a lane the maximum and the sum of a block; then the blocks' values, their loads together
     for (int32_t r = split + m.splits * warp; r < count; r += m.splits * kWarps) {
         const int32_t row = r0 + r;
         if (row < rows) {
             const int32_t i = row / m.a.group, h = u * m.a.group + row % m.a.group;
             const int l = threadIdx.x & 31;
-            float most = -INFINITY, sum = 0.0f;
-            for (int32_t c = 0; c < m.splits; ++c) {
-                most = fmaxf(most, *cluster.map_shared_rank(&part.blockTop[r], c));
-            }
+            const bool has = l < m.splits;
+            const float mine = has ? *cluster.map_shared_rank(&part.blockTop[r], l) : -INFINITY;
+            float sum = has ? *cluster.map_shared_rank(&part.blockSum[r], l) : 0.0f;
+            const float most = WarpMax(mine);
+            const float fade = most == -INFINITY ? 1.0f : Exp2(mine - most);
+            sum = WarpSum(sum * fade);
             float x[kLaneDims] = {};
+#pragma unroll 8
             for (int32_t c = 0; c < m.splits; ++c) {
-                const float fade = most == -INFINITY ? 1.0f : Exp2(*cluster.map_shared_rank(&part.blockTop[r], c) - most);
-                sum = fmaf(*cluster.map_shared_rank(&part.blockSum[r], c), fade, sum);
+                const float f = __shfl_sync(0xffffffffu, fade, c);
                 const float* other = cluster.map_shared_rank(block + r * s.dim, c);
 #pragma unroll
                 for (int e = 0; e < kLaneDims; ++e) {
                     if (l + 32 * e < s.dim) {
-                        x[e] = fmaf(other[l + 32 * e], fade, x[e]);
+                        x[e] = fmaf(other[l + 32 * e], f, x[e]);
                     }
                 }
             }
@@ -133,7 +139,9 @@ __device__ __forceinline__ void JoinRows(const StepArgs& m, int32_t b, int32_t u
             }
         }
     }
-    cluster.sync(); // nobody's shared memory goes while others read it
+    if (m.splits > 1) {
+        cluster.sync(); // nobody's shared memory goes while others read it
+    }
 }
 
 // R rows a block, N chunks a lane, U keys of a lane group in flight
@@ -664,12 +672,12 @@ cudaError_t AttnStep(Dt dt, const AttnArgs& a, cudaStream_t stream)
     const int r = rows >= most ? most : (products || rows < 3 ? rows : 4);
     m.rowGroups = static_cast<int32_t>(CeilDiv(rows, r));
     const int64_t units = static_cast<int64_t>(s.batch) * s.kvHeads * m.rowGroups;
-    // Blocks of a cluster share out the keys of a unit: as many as bring about four blocks to each SM, while a block has 128 keys or
-    // more; beyond that only to use SMs that had none, down to 32 keys.
+    // Blocks of a cluster share out the keys of a unit, up to about two blocks an SM (a block's start and end cost as much as some
+    // hundred keys, so more are slower: 32 sequences of window 1024 with 8 key heads take 31 us as 256 blocks, 44 as 512 or 1024; 8 of
+    // 16384 keys 272 us as 64 blocks, 85 as 256, 113 as 512), and down to the 64 keys of one step of each warp.
     const int64_t keys = static_cast<int64_t>(s.window) + s.sinks + s.lq < s.lk ? static_cast<int64_t>(s.window) + s.sinks + s.lq : s.lk;
-    const int sms = NumSMs();
     int splits = 1;
-    while (splits < 16 && ((units * splits < 4 * sms && keys >= 2 * splits * 128) || (units * splits < sms && keys >= 2 * splits * 32))) {
+    while (splits < 16 && 2 * splits * units <= 2 * NumSMs() && keys >= 2 * splits * kStepKeys * kWarps) {
         splits *= 2;
     }
     m.splits = splits;
