@@ -777,7 +777,10 @@ PyObject* Rotary(Args a)
     if (Given(a[5])) {
         sections = IntArrayOf(a[5]);
     } else if (q.dim() >= 2) {
-        positions = positions.expand(q.sizes().slice(0, q.dim() - 2)); // one position for several tokens
+        const at::IntArrayRef lead = q.sizes().slice(0, q.dim() - 2);
+        if (positions.sizes() != lead) {
+            positions = positions.expand(lead); // one position for several tokens
+        }
     }
     const double scale = DoubleOf(a[6]);
     const at::Tensor qo = call.OutOr(a[7], q.sizes(), q.options());

@@ -1,4 +1,4 @@
-// Attention over a sliding window with sinks: which kernel a call takes, and the kernels that take a warp per row.
+// Attention over a sliding window with sinks: which kernels a call takes.
 #include "window_attention.cuh"
 
 namespace opscv {
@@ -6,17 +6,6 @@ namespace opscv {
 namespace {
 
 constexpr int kRowWarps = 4;
-
-template <typename T>
-__global__ void __launch_bounds__(32 * kRowWarps) AttnForwardRowsKernel(AttnArgs a)
-{
-    const int32_t i = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    if (i < a.s.lq) {
-        for (int32_t bh = blockIdx.y; bh < a.s.batch * a.s.heads; bh += gridDim.y) {
-            AttnForwardRow<T>(a, bh / a.s.heads, bh % a.s.heads, i);
-        }
-    }
-}
 
 // delta = gradOut . out, a warp per row
 template <typename T>
@@ -38,28 +27,6 @@ __global__ void __launch_bounds__(32 * kRowWarps) AttnDeltaKernel(AttnArgs a, fl
         s = WarpSum(s);
         if (lane == 0) {
             delta[static_cast<int64_t>(bh) * a.s.lq + i] = s;
-        }
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * kRowWarps) AttnGradQRowsKernel(AttnArgs a)
-{
-    const int32_t i = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    if (i < a.s.lq) {
-        for (int32_t bh = blockIdx.y; bh < a.s.batch * a.s.heads; bh += gridDim.y) {
-            AttnGradQRow<T>(a, bh / a.s.heads, bh % a.s.heads, i);
-        }
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * kRowWarps) AttnGradKvRowsKernel(AttnArgs a)
-{
-    const int32_t j = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    if (j < a.s.lk) {
-        for (int32_t bu = blockIdx.y; bu < a.s.batch * a.s.kvHeads; bu += gridDim.y) {
-            AttnGradKvRow<T>(a, bu / a.s.kvHeads, bu % a.s.kvHeads, j);
         }
     }
 }
@@ -99,10 +66,7 @@ cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& s, AttnTensor q, AttnTens
     if (MmaTakes(dt, a)) {
         return AttnForwardMma(dt, a, stream);
     }
-    const dim3 grid = RowGrid(s.lq, static_cast<int64_t>(s.batch) * s.heads);
-    OPSCV_DISPATCH_DT(dt, T, AttnForwardRowsKernel<T><<<grid, 32 * kRowWarps, 0, stream>>>(a));
-    CountLaunch();
-    return cudaGetLastError();
+    return AttnForwardTiles(dt, a, stream);
 }
 
 uint64_t WindowAttentionBwdWorkspace(Dt dt, const AttnShape& s)
@@ -131,23 +95,20 @@ cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& s, AttnTensor gradOut, At
     a.delta = delta;
     a.deltaStride = s.lq;
     a.group = s.heads / s.kvHeads;
-    if (s.lq > 0 && MmaTakes(dt, a) && AttnTmaReadable(gradOut, s.lq, s.heads, s.batch)) {
+    const bool queries = s.lq > 0 && s.heads > 0; // without any, the gradients of the keys are zeros
+    if (queries && MmaTakes(dt, a) && AttnTmaReadable(gradOut, s.lq, s.heads, s.batch)) {
         return AttnBackwardMma(dt, a, workspace, stream);
     }
-    const dim3 rows = RowGrid(s.lq, static_cast<int64_t>(s.batch) * s.heads);
-    const dim3 keys = RowGrid(s.lk, static_cast<int64_t>(s.batch) * s.kvHeads);
-    OPSCV_DISPATCH_DT(dt, T, {
-        if (s.lq > 0) {
-            AttnDeltaKernel<T><<<rows, 32 * kRowWarps, 0, stream>>>(a, delta);
-            AttnGradQRowsKernel<T><<<rows, 32 * kRowWarps, 0, stream>>>(a);
-            CountLaunch(2);
+    if (queries) {
+        const dim3 rows = RowGrid(s.lq, static_cast<int64_t>(s.batch) * s.heads);
+        OPSCV_DISPATCH_DT(dt, T, AttnDeltaKernel<T><<<rows, 32 * kRowWarps, 0, stream>>>(a, delta));
+        CountLaunch();
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) {
+            return e;
         }
-        if (s.lk > 0) {
-            AttnGradKvRowsKernel<T><<<keys, 32 * kRowWarps, 0, stream>>>(a);
-            CountLaunch();
-        }
-    });
-    return cudaGetLastError();
+    }
+    return AttnBackwardTiles(dt, a, stream);
 }
 
 } // namespace opscv

@@ -257,6 +257,10 @@ constexpr int kStepMostQueries = 8;
 cudaError_t AttnStep(Dt dt, const AttnArgs& a, cudaStream_t stream);
 uint32_t AttnStepTimeouts();
 
+// ---- fp32 arithmetic (window_attention_tiles.cu) -------------------------------------------------------------------------------
+cudaError_t AttnForwardTiles(Dt dt, const AttnArgs& a, cudaStream_t stream);
+cudaError_t AttnBackwardTiles(Dt dt, const AttnArgs& a, cudaStream_t stream); // a.delta is filled
+
 // ---- tensor-core kernels (window_attention_mma.cu) ---------------------------------------------------------------------------
 bool AttnTmaReadable(const AttnTensor& t, int32_t tokens, int32_t heads, int32_t batch);
 // Boxes of 64 values by boxTokens tokens of one head, in the 128-byte swizzle; what lies outside the tensor arrives as zeros.

@@ -1,0 +1,519 @@
+// Attention over a sliding window with sinks in fp32 arithmetic, tile by tile: fp32 tensors, heads of more than 128 values, and 16-bit
+// tensors that boxes cannot be loaded from.
+//
+// Bound by the fp32 pipes: 4 (forward) and 14 (backward) operations for each pair and value, of which a 4 x 4 block of a tile's products
+// in each thread's registers takes 64 for 8 reads of 16 bytes from shared memory. Tensor cores would need three products of tf32 parts for
+// each of fp32 and still lose bits that fp32 callers have. Blocks own their sums (gradQ in one kernel, gradK and gradV in another), so
+// nothing is added up in memory and the order of all sums is fixed.
+#include "window_attention.cuh"
+
+namespace opscv {
+
+namespace {
+
+constexpr int kThreads = 256; // 16 x 16
+
+// DP: values of a head, padded; ROWS: queries and keys of a tile. 64 x 64 tiles of up to 128 values, 32 x 32 ones of 256.
+template <int DP>
+struct Tile {
+    static constexpr int kRows = DP <= 128 ? 64 : 32;
+    static constexpr int kMicro = kRows / 16;  // rows (and columns) of a thread
+    static constexpr int kQuads = DP / 64;     // blocks of 4 values of a row that a thread has
+    static constexpr int kStride = DP + 4;     // floats of a row: 4 more shift neighbouring rows to other banks
+    static constexpr int kWeights = kRows + 4; // the same for the rows of weights
+    static constexpr int kTileFloats = kRows * kStride;
+    static constexpr int kWeightFloats = kRows * kWeights;
+};
+
+// Rows [from, from + ROWS) of one head as fp32, zeros for rows behind `end` and values behind dim.
+template <typename T, int DP>
+__device__ __forceinline__ void LoadTile(float* dst, const AttnTensor& t, int32_t b, int32_t h, int32_t from, int32_t end, int32_t dim,
+                                         bool vec)
+{
+    using L = Tile<DP>;
+    const T* base = RowOf<T>(t, b, 0, h);
+    if (vec) {
+        for (int e = threadIdx.x; e < L::kRows * (DP / 4); e += kThreads) {
+            const int r = e / (DP / 4), d = e % (DP / 4) * 4;
+            float v[4] = {};
+            if (from + r < end && d < dim) {
+                LoadPack<T, 4>(base + (from + r) * t.l + d, v);
+            }
+            *reinterpret_cast<float4*>(dst + r * L::kStride + d) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    } else {
+        for (int e = threadIdx.x; e < L::kRows * DP; e += kThreads) {
+            const int r = e / DP, d = e % DP;
+            dst[r * L::kStride + d] = from + r < end && d < dim ? DType<T>::ToF(base[(from + r) * t.l + d]) : 0.0f;
+        }
+    }
+}
+
+__device__ __forceinline__ float Dot4(const float4& a, const float4& b, float s)
+{
+    return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
+}
+
+// s[r][c] = row (micro * ty + r) of a . row (tx + 16 c) of b
+template <int DP>
+__device__ __forceinline__ void Inner(const float* a, const float* b, float (&s)[Tile<DP>::kMicro][Tile<DP>::kMicro])
+{
+    using L = Tile<DP>;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+    for (int r = 0; r < L::kMicro; ++r) {
+#pragma unroll
+        for (int c = 0; c < L::kMicro; ++c) {
+            s[r][c] = 0.0f;
+        }
+    }
+    const float* pa = a + L::kMicro * ty * L::kStride;
+    const float* pb = b + tx * L::kStride;
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 4) {
+        float4 x[L::kMicro], y[L::kMicro];
+#pragma unroll
+        for (int r = 0; r < L::kMicro; ++r) {
+            x[r] = *reinterpret_cast<const float4*>(pa + r * L::kStride + d);
+            y[r] = *reinterpret_cast<const float4*>(pb + 16 * r * L::kStride + d);
+        }
+#pragma unroll
+        for (int r = 0; r < L::kMicro; ++r) {
+#pragma unroll
+            for (int c = 0; c < L::kMicro; ++c) {
+                s[r][c] = Dot4(x[r], y[c], s[r][c]);
+            }
+        }
+    }
+}
+
+// o[r] += sum over j of w[micro * ty + r][j] row j of v, values 4 tx + 64 c to + 3
+template <int DP>
+__device__ __forceinline__ void Outer(const float* w, const float* v, float4 (&o)[Tile<DP>::kMicro][Tile<DP>::kQuads])
+{
+    using L = Tile<DP>;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const float* pw = w + L::kMicro * ty * L::kWeights;
+    const float* pv = v + 4 * tx;
+#pragma unroll 2
+    for (int j = 0; j < L::kRows; j += 4) {
+        float4 x[L::kMicro];
+#pragma unroll
+        for (int r = 0; r < L::kMicro; ++r) {
+            x[r] = *reinterpret_cast<const float4*>(pw + r * L::kWeights + j);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int c = 0; c < L::kQuads; ++c) {
+                const float4 y = *reinterpret_cast<const float4*>(pv + (j + k) * L::kStride + 64 * c);
+#pragma unroll
+                for (int r = 0; r < L::kMicro; ++r) {
+                    const float z = k == 0 ? x[r].x : k == 1 ? x[r].y : k == 2 ? x[r].z : x[r].w;
+                    o[r][c].x = fmaf(z, y.x, o[r][c].x);
+                    o[r][c].y = fmaf(z, y.y, o[r][c].y);
+                    o[r][c].z = fmaf(z, y.z, o[r][c].z);
+                    o[r][c].w = fmaf(z, y.w, o[r][c].w);
+                }
+            }
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ bool StoreQuad(T* out, const float4& v, int32_t d, int32_t dim) // true: not all finite
+{
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (d + e < dim) {
+            out[d + e] = DType<T>::FromF(x[e]);
+            bad = bad || !(fabsf(x[e]) <= 3.4e38f);
+        }
+    }
+    return bad;
+}
+
+__device__ __forceinline__ float RowMax16(float v) // over the 16 threads of a row
+{
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    }
+    return v;
+}
+__device__ __forceinline__ float RowSum16(float v)
+{
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    return v;
+}
+
+// Steps over the keys of queries at [low, high]: the sinks in front of the window, then the window from its first key on.
+template <int ROWS>
+struct Walk {
+    int32_t sinkEnd = 0, first = 0, sinkSteps = 0, steps = 0;
+    __device__ __forceinline__ Walk(const AttnShape& s, int32_t low, int32_t high)
+    {
+        if (high >= 0) {
+            low = low > 0 ? low : 0;
+            first = low >= s.window ? low - s.window + 1 : 0;
+            sinkEnd = s.sinks < first ? s.sinks : first;
+            sinkSteps = (sinkEnd + ROWS - 1) / ROWS;
+            steps = sinkSteps + (high - first + ROWS) / ROWS;
+        }
+    }
+    __device__ __forceinline__ int32_t Key(int32_t n) const { return n < sinkSteps ? n * ROWS : first + (n - sinkSteps) * ROWS; }
+    // whether step n is where the query at p gets key j from (a step of sinks may reach over the window's first keys)
+    __device__ __forceinline__ bool Sees(const AttnShape& s, int32_t n, int32_t p, int32_t j) const
+    {
+        return j <= p && (j > p - s.window || j < s.sinks) && (n >= sinkSteps || j < sinkEnd);
+    }
+};
+
+struct TileArgs {
+    AttnArgs a;
+    int32_t tiles;
+    bool vec; // rows can be read 4 values at a time
+};
+
+// ---- forward ---------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_constant__ TileArgs m)
+{
+    using L = Tile<DP>;
+    constexpr int R = L::kMicro;
+    extern __shared__ float shared[];
+    __shared__ uint32_t again[2];
+    float *sq = shared, *sk = sq + L::kTileFloats, *sw = sk + L::kTileFloats; // keys, then values
+    const AttnShape& s = m.a.s;
+    const int32_t tile = blockIdx.x % m.tiles, bh = blockIdx.x / m.tiles;
+    const int32_t b = bh / s.heads, h = bh % s.heads, u = h / m.a.group;
+    const Lengths n = LengthsOf(s, b);
+    const int32_t i0 = tile * L::kRows, iLast = min(i0 + L::kRows, n.q) - 1;
+    const Walk<L::kRows> walk(s, n.shift + i0, iLast >= i0 ? n.shift + iLast : -1);
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    if (threadIdx.x < 2) {
+        again[threadIdx.x] = 0;
+    }
+    LoadTile<T, DP>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
+    float4 o[R][L::kQuads] = {};
+    float top[R], total[R];
+    int32_t p[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        top[r] = -INFINITY;
+        total[r] = 0.0f;
+        const int32_t i = i0 + R * ty + r;
+        p[r] = i <= iLast ? n.shift + i : -1;
+    }
+    for (int32_t step = 0; step < walk.steps; ++step) {
+        const int32_t j0 = walk.Key(step);
+        __syncthreads(); // the values of the step before have been read
+        LoadTile<T, DP>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
+        __syncthreads();
+        float x[R][R];
+        Inner<DP>(sq, sk, x);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float most = top[r];
+#pragma unroll
+            for (int c = 0; c < R; ++c) {
+                x[r][c] = walk.Sees(s, step, p[r], j0 + tx + 16 * c) ? x[r][c] * s.scale : -INFINITY;
+                most = fmaxf(most, x[r][c]);
+            }
+            most = RowMax16(most);
+            const float base = most == -INFINITY ? 0.0f : most;
+            const float fade = expf(top[r] - base);
+            top[r] = most;
+            float sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < R; ++c) {
+                x[r][c] = expf(x[r][c] - base);
+                sum += x[r][c];
+                sw[(R * ty + r) * L::kWeights + tx + 16 * c] = x[r][c];
+            }
+            total[r] = total[r] * fade + sum;
+#pragma unroll
+            for (int c = 0; c < L::kQuads; ++c) {
+                o[r][c] = make_float4(o[r][c].x * fade, o[r][c].y * fade, o[r][c].z * fade, o[r][c].w * fade);
+            }
+        }
+        __syncthreads();
+        LoadTile<T, DP>(sk, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
+        __syncthreads();
+        Outer<DP>(sw, sk, o);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int32_t i = i0 + R * ty + r;
+        const float sum = RowSum16(total[r]);
+        const bool some = p[r] >= 0;
+        const float inverse = some ? 1.0f / sum : 0.0f; // a sum of 0 gives a NaN, and the row is formed again
+        bool bad = false;
+        if (i < s.lq) {
+            T* out = OutRowOf<T>(m.a.out, b, i, h);
+#pragma unroll
+            for (int c = 0; c < L::kQuads; ++c) {
+                const float4 v = some ? make_float4(o[r][c].x * inverse, o[r][c].y * inverse, o[r][c].z * inverse, o[r][c].w * inverse) :
+                                        make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                bad = StoreQuad<T>(out, v, 4 * tx + 64 * c, s.dim) || bad;
+            }
+            if (tx == 0 && m.a.lse != nullptr) {
+                m.a.lse[static_cast<int64_t>(bh) * s.lq + i] = some ? top[r] + logf(sum) : -INFINITY;
+            }
+        }
+        if (bad || (some && !(sum > 0.0f))) {
+            atomicOr(&again[(R * ty + r) >> 5], 1u << ((R * ty + r) & 31));
+        }
+    }
+    __syncthreads();
+    // rows that are not finite again, without the masked keys' part
+    for (int r = threadIdx.x >> 5; r < L::kRows; r += kThreads / 32) {
+        if ((again[r >> 5] >> (r & 31) & 1) != 0 && i0 + r < s.lq) {
+            AttnForwardRow<T>(m.a, b, h, i0 + r);
+        }
+    }
+}
+
+// ---- backward --------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_constant__ TileArgs m)
+{
+    using L = Tile<DP>;
+    constexpr int R = L::kMicro;
+    extern __shared__ float shared[];
+    __shared__ uint32_t again[2];
+    float *sq = shared, *sg = sq + L::kTileFloats, *sk = sg + L::kTileFloats, *sv = sk + L::kTileFloats, *sw = sv + L::kTileFloats;
+    const AttnShape& s = m.a.s;
+    const int32_t tile = blockIdx.x % m.tiles, bh = blockIdx.x / m.tiles;
+    const int32_t b = bh / s.heads, h = bh % s.heads, u = h / m.a.group;
+    const Lengths n = LengthsOf(s, b);
+    const int32_t i0 = tile * L::kRows, iLast = min(i0 + L::kRows, n.q) - 1;
+    const Walk<L::kRows> walk(s, n.shift + i0, iLast >= i0 ? n.shift + iLast : -1);
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    if (threadIdx.x < 2) {
+        again[threadIdx.x] = 0;
+    }
+    LoadTile<T, DP>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
+    LoadTile<T, DP>(sg, m.a.gradOut, b, h, i0, iLast + 1, s.dim, m.vec);
+    float4 o[R][L::kQuads] = {};
+    float lse[R], delta[R];
+    int32_t p[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int32_t i = i0 + R * ty + r;
+        p[r] = i <= iLast ? n.shift + i : -1;
+        lse[r] = p[r] >= 0 ? m.a.lse[static_cast<int64_t>(bh) * s.lq + i] : 0.0f;
+        delta[r] = p[r] >= 0 ? m.a.delta[static_cast<int64_t>(bh) * m.a.deltaStride + i] : 0.0f;
+    }
+    for (int32_t step = 0; step < walk.steps; ++step) {
+        const int32_t j0 = walk.Key(step);
+        __syncthreads();
+        LoadTile<T, DP>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
+        LoadTile<T, DP>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
+        __syncthreads();
+        float x[R][R], y[R][R];
+        Inner<DP>(sq, sk, x);
+        Inner<DP>(sg, sv, y);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int c = 0; c < R; ++c) {
+                const bool live = walk.Sees(s, step, p[r], j0 + tx + 16 * c);
+                sw[(R * ty + r) * L::kWeights + tx + 16 * c] =
+                    live ? expf(x[r][c] * s.scale - lse[r]) * (y[r][c] - delta[r]) * s.scale : 0.0f;
+            }
+        }
+        __syncthreads();
+        Outer<DP>(sw, sk, o);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int32_t i = i0 + R * ty + r;
+        bool bad = false;
+        if (i < s.lq) {
+            T* out = OutRowOf<T>(m.a.gradQ, b, i, h);
+#pragma unroll
+            for (int c = 0; c < L::kQuads; ++c) {
+                const float4 v = p[r] >= 0 ? o[r][c] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                bad = StoreQuad<T>(out, v, 4 * tx + 64 * c, s.dim) || bad;
+            }
+        }
+        if (bad) {
+            atomicOr(&again[(R * ty + r) >> 5], 1u << ((R * ty + r) & 31));
+        }
+    }
+    __syncthreads();
+    for (int r = threadIdx.x >> 5; r < L::kRows; r += kThreads / 32) {
+        if ((again[r >> 5] >> (r & 31) & 1) != 0 && i0 + r < s.lq) {
+            AttnGradQRow<T>(m.a, b, h, i0 + r);
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_constant__ TileArgs m)
+{
+    using L = Tile<DP>;
+    constexpr int R = L::kMicro;
+    extern __shared__ float shared[];
+    __shared__ uint32_t again[2];
+    __shared__ float sLse[L::kRows], sDelta[L::kRows];
+    float *sk = shared, *sv = sk + L::kTileFloats, *sq = sv + L::kTileFloats, *sg = sq + L::kTileFloats, *sw = sg + L::kTileFloats,
+          *sd = sw + L::kWeightFloats;
+    const AttnShape& s = m.a.s;
+    const int32_t tile = blockIdx.x % m.tiles, bu = blockIdx.x / m.tiles;
+    const int32_t b = bu / s.kvHeads, u = bu % s.kvHeads;
+    const Lengths n = LengthsOf(s, b);
+    const int32_t j0 = tile * L::kRows, jLast = min(j0 + L::kRows, n.kv) - 1, end = n.kv - 1;
+    // positions of the queries that see some key of the tile
+    const int32_t low = max(j0, max(n.shift, 0)), high = jLast < j0 ? -1 : j0 < s.sinks ? end : min(end, jLast + s.window - 1);
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    if (threadIdx.x < 2) {
+        again[threadIdx.x] = 0;
+    }
+    LoadTile<T, DP>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
+    LoadTile<T, DP>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
+    float4 ok[R][L::kQuads] = {}, ov[R][L::kQuads] = {};
+    for (int32_t h = u * m.a.group; h < (u + 1) * m.a.group; ++h) {
+        const int64_t head = static_cast<int64_t>(b) * s.heads + h;
+        for (int32_t p0 = low; p0 <= high; p0 += L::kRows) {
+            const int32_t i0 = p0 - n.shift;
+            __syncthreads();
+            LoadTile<T, DP>(sq, m.a.q, b, h, i0, n.q, s.dim, m.vec);
+            LoadTile<T, DP>(sg, m.a.gradOut, b, h, i0, n.q, s.dim, m.vec);
+            if (threadIdx.x < L::kRows) {
+                const int32_t i = i0 + threadIdx.x;
+                sLse[threadIdx.x] = i < n.q ? m.a.lse[head * s.lq + i] : 0.0f;
+                sDelta[threadIdx.x] = i < n.q ? m.a.delta[head * m.a.deltaStride + i] : 0.0f;
+            }
+            __syncthreads();
+            float x[R][R], y[R][R];
+            Inner<DP>(sk, sq, x);
+            Inner<DP>(sv, sg, y);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int32_t j = j0 + R * ty + r;
+#pragma unroll
+                for (int c = 0; c < R; ++c) {
+                    const int32_t e = tx + 16 * c, p = p0 + e;
+                    const bool live = j < n.kv && p <= end && j <= p && (j > p - s.window || j < s.sinks);
+                    const float w = live ? expf(x[r][c] * s.scale - sLse[e]) : 0.0f;
+                    sw[(R * ty + r) * L::kWeights + e] = w;
+                    sd[(R * ty + r) * L::kWeights + e] = live ? w * (y[r][c] - sDelta[e]) * s.scale : 0.0f;
+                }
+            }
+            __syncthreads();
+            Outer<DP>(sw, sg, ov);
+            Outer<DP>(sd, sq, ok);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int32_t j = j0 + R * ty + r;
+        bool bad = false;
+        if (j < s.lk) {
+            T *gk = OutRowOf<T>(m.a.gradK, b, j, u), *gv = OutRowOf<T>(m.a.gradV, b, j, u);
+#pragma unroll
+            for (int c = 0; c < L::kQuads; ++c) {
+                bad = StoreQuad<T>(gk, ok[r][c], 4 * tx + 64 * c, s.dim) || bad;
+                bad = StoreQuad<T>(gv, ov[r][c], 4 * tx + 64 * c, s.dim) || bad;
+            }
+        }
+        if (bad) {
+            atomicOr(&again[(R * ty + r) >> 5], 1u << ((R * ty + r) & 31));
+        }
+    }
+    __syncthreads();
+    for (int r = threadIdx.x >> 5; r < L::kRows; r += kThreads / 32) {
+        if ((again[r >> 5] >> (r & 31) & 1) != 0 && j0 + r < s.lk) {
+            AttnGradKvRow<T>(m.a, b, u, j0 + r);
+        }
+    }
+}
+
+bool ReadsByFour(Dt dt, const AttnTensor& t)
+{
+    return Aligned(t.p, 4 * DtSize(dt)) && t.b % 4 == 0 && t.l % 4 == 0 && t.h % 4 == 0;
+}
+
+template <typename T, int DP>
+cudaError_t Forward(Dt dt, const AttnArgs& a, cudaStream_t stream)
+{
+    using L = Tile<DP>;
+    const AttnShape& s = a.s;
+    TileArgs m{};
+    m.a = a;
+    m.tiles = static_cast<int32_t>(CeilDiv(s.lq, L::kRows));
+    m.vec = s.dim % 4 == 0 && ReadsByFour(dt, a.q) && ReadsByFour(dt, a.k) && ReadsByFour(dt, a.v);
+    constexpr int shared = (2 * L::kTileFloats + L::kWeightFloats) * 4;
+    static std::atomic<uint64_t> asked;
+    const int64_t blocks = static_cast<int64_t>(s.batch) * s.heads * m.tiles;
+    if (blocks > INT32_MAX) {
+        return cudaErrorInvalidConfiguration;
+    }
+    const cudaError_t e = AskOnce(AttnForwardTilesKernel<T, DP>, asked, shared);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    AttnForwardTilesKernel<T, DP><<<static_cast<unsigned>(blocks), kThreads, shared, stream>>>(m);
+    CountLaunch();
+    return cudaGetLastError();
+}
+
+template <typename T, int DP>
+cudaError_t Backward(Dt dt, const AttnArgs& a, cudaStream_t stream)
+{
+    using L = Tile<DP>;
+    const AttnShape& s = a.s;
+    TileArgs m{};
+    m.a = a;
+    m.vec = s.dim % 4 == 0 && ReadsByFour(dt, a.q) && ReadsByFour(dt, a.k) && ReadsByFour(dt, a.v) && ReadsByFour(dt, a.gradOut);
+    constexpr int sharedQ = (4 * L::kTileFloats + L::kWeightFloats) * 4, sharedKv = (4 * L::kTileFloats + 2 * L::kWeightFloats) * 4;
+    static std::atomic<uint64_t> askedQ, askedKv;
+    cudaError_t e = AskOnce(AttnGradQTilesKernel<T, DP>, askedQ, sharedQ);
+    e = e != cudaSuccess ? e : AskOnce(AttnGradKvTilesKernel<T, DP>, askedKv, sharedKv);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    const int64_t qTiles = CeilDiv(s.lq, L::kRows), kTiles = CeilDiv(s.lk, L::kRows);
+    const int64_t qBlocks = static_cast<int64_t>(s.batch) * s.heads * qTiles, kBlocks = static_cast<int64_t>(s.batch) * s.kvHeads * kTiles;
+    if (qBlocks > INT32_MAX || kBlocks > INT32_MAX) {
+        return cudaErrorInvalidConfiguration;
+    }
+    if (qBlocks > 0) {
+        m.tiles = static_cast<int32_t>(qTiles);
+        AttnGradQTilesKernel<T, DP><<<static_cast<unsigned>(qBlocks), kThreads, sharedQ, stream>>>(m);
+        CountLaunch();
+    }
+    if (kBlocks > 0) {
+        m.tiles = static_cast<int32_t>(kTiles);
+        AttnGradKvTilesKernel<T, DP><<<static_cast<unsigned>(kBlocks), kThreads, sharedKv, stream>>>(m);
+        CountLaunch();
+    }
+    return cudaGetLastError();
+}
+
+} // namespace
+
+cudaError_t AttnForwardTiles(Dt dt, const AttnArgs& a, cudaStream_t stream)
+{
+    OPSCV_DISPATCH_DT(dt, T, {
+        return a.s.dim <= 64 ? Forward<T, 64>(dt, a, stream) : a.s.dim <= 128 ? Forward<T, 128>(dt, a, stream) : Forward<T, 256>(dt, a, stream);
+    });
+    return cudaErrorInvalidValue;
+}
+
+cudaError_t AttnBackwardTiles(Dt dt, const AttnArgs& a, cudaStream_t stream)
+{
+    OPSCV_DISPATCH_DT(dt, T, {
+        return a.s.dim <= 64 ? Backward<T, 64>(dt, a, stream) : a.s.dim <= 128 ? Backward<T, 128>(dt, a, stream) : Backward<T, 256>(dt, a, stream);
+    });
+    return cudaErrorInvalidValue;
+}
+
+} // namespace opscv
