@@ -85,6 +85,15 @@ __device__ __forceinline__ float RowSum(float v, float* part)
     return v;
 }
 
+__device__ __forceinline__ float WarpSum(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    return v;
+}
+
 struct FwdArgs {
     const void *x, *residual, *weight;
     void *y, *sum;
@@ -99,27 +108,147 @@ struct FwdArgs {
     int32_t group, groups;
 };
 
+// Rows are held as they are stored (two 16-bit values a register) and taken apart where they are used: the registers of a row halve, and
+// the sum of two 16-bit values costs one instruction a pair. Its rounding is that of the fp32 sum: two values whose exponents are near
+// enough for a tie have an exact fp32 sum.
 template <typename T, int V>
-__device__ __forceinline__ void LoadSum(const T* x, const T* r, int32_t col, float (&z)[V])
+__device__ __forceinline__ Pack<T, V> AddPacks(const Pack<T, V>& a, const Pack<T, V>& b)
 {
-    LoadF<T, V>(x + col, z);
-    if (r != nullptr) {
-        float b[V];
-        LoadF<T, V>(r + col, b);
+    Pack<T, V> s;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+        using T2 = std::conditional_t<DType<T>::kIsHalf, __half2, __nv_bfloat162>;
+        const T2 *x = reinterpret_cast<const T2*>(&a), *y = reinterpret_cast<const T2*>(&b);
+        T2* z = reinterpret_cast<T2*>(&s);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            z[i] = __hadd2_rn(x[i], y[i]);
+        }
+    } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            z[i] = DType<T>::ToF(DType<T>::FromF(z[i] + b[i]));
+            s.v[i] = DType<T>::FromF(DType<T>::ToF(a.v[i]) + DType<T>::ToF(b.v[i]));
+        }
+    }
+    return s;
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> LoadSum(const T* x, const T* r, int32_t col)
+{
+    const Pack<T, V> z = *reinterpret_cast<const Pack<T, V>*>(x + col);
+    return r != nullptr ? AddPacks(z, *reinterpret_cast<const Pack<T, V>*>(r + col)) : z;
+}
+template <typename T, int V>
+__device__ __forceinline__ void StorePacked(T* p, const Pack<T, V>& z)
+{
+    *reinterpret_cast<Pack<T, V>*>(p) = z;
+}
+// v[i] = a[i] * b[i], two at a time
+template <int V>
+__device__ __forceinline__ void Times(float (&v)[V], const float (&b)[V])
+{
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            SplitF2(Mul2(MakeF2(v[i], v[i + 1]), MakeF2(b[i], b[i + 1])), v[i], v[i + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] *= b[i];
         }
     }
 }
+template <int V>
+__device__ __forceinline__ void Times(float (&v)[V], float f)
+{
+    float b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        b[i] = f;
+    }
+    Times(v, b);
+}
+// sum of a[i] * b[i], even and odd ones apart until the end
+template <int V>
+__device__ __forceinline__ void AddDot(const float (&a)[V], const float (&b)[V], F2& s)
+{
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            s = Fma2(MakeF2(a[i], a[i + 1]), MakeF2(b[i], b[i + 1]), s);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            s = Fma2(MakeF2(a[i], 0.0f), MakeF2(b[i], 0.0f), s);
+        }
+    }
+}
+// s[i] += a[i] * b[i]
+template <int V>
+__device__ __forceinline__ void AddProducts(const float (&a)[V], const float (&b)[V], float (&s)[V])
+{
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            SplitF2(Fma2(MakeF2(a[i], a[i + 1]), MakeF2(b[i], b[i + 1]), MakeF2(s[i], s[i + 1])), s[i], s[i + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            s[i] = fmaf(a[i], b[i], s[i]);
+        }
+    }
+}
+__device__ __forceinline__ float Both(F2 s)
+{
+    float a, b;
+    SplitF2(s, a, b);
+    return a + b;
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> ZeroPack()
+{
+    Pack<T, V> z;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        z.v[i] = DType<T>::FromF(0.0f);
+    }
+    return z;
+}
+
+// The weight of a row's chunks. One of the tensors' type is read before the reduction's wait, whose time covers the load's; an fp32
+// one takes twice the registers and is read after it.
+template <typename T, int V, int N>
+struct WeightOf {
+    Pack<T, V> held[N];
+    __device__ __forceinline__ void Early(const FwdArgs& a, int k, int32_t col)
+    {
+        if (a.weight != nullptr && !a.weight32) {
+            held[k] = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.weight) + col);
+        }
+    }
+    // v[i] *= rstd * weight[i]
+    __device__ __forceinline__ void Apply(const FwdArgs& a, int k, int32_t col, float rstd, float (&v)[V]) const
+    {
+        Times(v, rstd);
+        if (a.weight != nullptr) {
+            float w[V];
+            if (a.weight32) {
+                LoadWeight<T, V>(a.weight, true, col, w);
+            } else {
+                UnpackToF<T, V>(held[k], w);
+            }
+            Times(v, w);
+        }
+    }
+};
 
 // NV > 0: the row is held in NV * V values a thread. NV == 0: rows too wide for that are read again for the second pass (from L2
 // mostly), from `sum` where there is one, since it may lie over one of the terms.
 template <typename T, int V, int NV>
 __global__ void __launch_bounds__(kMaxThreads) RmsNormFwdKernel(FwdArgs a)
 {
-    // the weight is read before the reduction's wait, whose time covers the load's, where the registers hold both
-    constexpr bool kEarlyWeight = NV > 0 && NV * V <= 16;
     __shared__ float part[32];
     const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     if (row >= a.rows) { // rows of several warps have one row a block, so that no barrier is left out
@@ -132,49 +261,40 @@ __global__ void __launch_bounds__(kMaxThreads) RmsNormFwdKernel(FwdArgs a)
     const int32_t step = blockDim.x * V;
     const int32_t first = threadIdx.x * V;
     constexpr int N = NV > 0 ? NV : 1;
-    float z[N][V];
-    float w[kEarlyWeight ? N : 1][V];
-    float sq = 0.0f;
+    Pack<T, V> z[N];
+    WeightOf<T, V, N> w;
+    F2 sq = MakeF2(0.0f, 0.0f);
+    float f[V];
     if constexpr (NV > 0) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int32_t col = first + k * step;
+            z[k] = ZeroPack<T, V>();
             if (col < a.width) {
-                LoadSum<T, V>(x, r, col, z[k]);
-                if constexpr (kEarlyWeight) {
-                    LoadWeight<T, V>(a.weight, a.weight32, col, w[k]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    z[k][i] = 0.0f;
-                }
+                z[k] = LoadSum<T, V>(x, r, col);
+                w.Early(a, k, col);
             }
         }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                sq = fmaf(z[k][i], z[k][i], sq);
-            }
             const int32_t col = first + k * step;
             if (sum != nullptr && col < a.width) {
-                StoreF<T, V>(sum + col, z[k]);
+                StorePacked<T, V>(sum + col, z[k]);
             }
+            UnpackToF<T, V>(z[k], f);
+            AddDot(f, f, sq);
         }
     } else {
         for (int32_t col = first; col < a.width; col += step) {
-            LoadSum<T, V>(x, r, col, z[0]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                sq = fmaf(z[0][i], z[0][i], sq);
-            }
+            z[0] = LoadSum<T, V>(x, r, col);
             if (sum != nullptr) {
-                StoreF<T, V>(sum + col, z[0]);
+                StorePacked<T, V>(sum + col, z[0]);
             }
+            UnpackToF<T, V>(z[0], f);
+            AddDot(f, f, sq);
         }
     }
-    const float mean = RowSum(sq, part) / static_cast<float>(a.width);
+    const float mean = RowSum(Both(sq), part) / static_cast<float>(a.width);
     const float rstd = 1.0f / sqrtf(mean + a.eps);
     if (a.rstd != nullptr && threadIdx.x == 0) {
         a.rstd[row] = rstd;
@@ -184,38 +304,40 @@ __global__ void __launch_bounds__(kMaxThreads) RmsNormFwdKernel(FwdArgs a)
         for (int k = 0; k < NV; ++k) {
             const int32_t col = first + k * step;
             if (col < a.width) {
-                float(&wk)[V] = w[kEarlyWeight ? k : 0];
-                if constexpr (!kEarlyWeight) {
-                    LoadWeight<T, V>(a.weight, a.weight32, col, wk);
-                }
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    z[k][i] *= rstd * wk[i];
-                }
-                StoreF<T, V>(y + col, z[k]);
+                UnpackToF<T, V>(z[k], f);
+                w.Apply(a, k, col, rstd, f);
+                StoreF<T, V>(y + col, f);
             }
         }
     } else {
         for (int32_t col = first; col < a.width; col += step) {
-            if (sum != nullptr) {
-                LoadF<T, V>(sum + col, z[0]);
-            } else {
-                LoadSum<T, V>(x, r, col, z[0]);
-            }
-            LoadWeight<T, V>(a.weight, a.weight32, col, w[0]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                z[0][i] *= rstd * w[0][i];
-            }
-            StoreF<T, V>(y + col, z[0]);
+            z[0] = sum != nullptr ? *reinterpret_cast<const Pack<T, V>*>(sum + col) : LoadSum<T, V>(x, r, col);
+            w.Early(a, 0, col);
+            UnpackToF<T, V>(z[0], f);
+            w.Apply(a, 0, col, rstd, f);
+            StoreF<T, V>(y + col, f);
         }
     }
 }
 
 // ---- 8-bit outputs ---------------------------------------------------------------------------------------------------------
-// The largest magnitude of non-negative floats as unsigned integers, which order alike; a NaN is above all others, so a row or
-// group with one gets a NaN as its scale.
-__device__ __forceinline__ uint32_t Magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// A NaN is above all other magnitudes, so a row or group with one gets a NaN as its scale. As unsigned integers, non-negative floats
+// (and NaNs) order alike, which is what the maximum in shared memory uses.
+__device__ __forceinline__ float MaxOrNaN(float a, float b)
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+template <int V>
+__device__ __forceinline__ float Most(const float (&v)[V], float m)
+{
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        m = MaxOrNaN(m, fabsf(v[i]));
+    }
+    return m;
+}
 
 template <Q8 Q>
 struct Q8Type;
@@ -252,8 +374,8 @@ struct Q8Type<Q8::INT8> {
     }
 };
 
-// Value times this is the quantised value. A group of zeros (or one whose scale underflows) has scale 0 and zeros.
-__device__ __forceinline__ float Inverse(uint32_t most, float range) { return most == 0 ? 0.0f : range / __uint_as_float(most); }
+// Value times this is the quantised value. A group of zeros has scale 0 and zeros.
+__device__ __forceinline__ float Inverse(float most, float range) { return most == 0.0f ? 0.0f : range / most; }
 
 // LG: lanes of a group where a group lies within a warp (a power of two), 0 where groups go through shared memory, one word each.
 template <typename T, int V, int NV, Q8 Q, int LG>
@@ -261,7 +383,6 @@ __global__ void __launch_bounds__(kMaxThreads) RmsNormQuantKernel(FwdArgs a)
 {
     extern __shared__ uint32_t most[]; // [groups] (LG == 0)
     __shared__ float part[32];
-    constexpr bool kEarlyWeight = NV > 0 && NV * V <= 16;
     using QT = Q8Type<Q>;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     if (row >= a.rows) {
@@ -275,8 +396,10 @@ __global__ void __launch_bounds__(kMaxThreads) RmsNormQuantKernel(FwdArgs a)
     const int32_t step = blockDim.x * V;
     const int32_t first = threadIdx.x * V;
     constexpr int N = NV > 0 ? NV : 1;
-    float z[N][V], w[kEarlyWeight ? N : 1][V];
-    float sq = 0.0f;
+    Pack<T, V> z[N];
+    WeightOf<T, V, N> w;
+    F2 sq = MakeF2(0.0f, 0.0f);
+    float f[V];
     if constexpr (LG == 0) { // one row a block (the launcher sees to it)
         for (int32_t g = threadIdx.x; g < a.groups; g += blockDim.x) {
             most[g] = 0;
@@ -287,133 +410,97 @@ __global__ void __launch_bounds__(kMaxThreads) RmsNormQuantKernel(FwdArgs a)
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int32_t col = first + k * step;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                z[k][i] = w[kEarlyWeight ? k : 0][i] = 0.0f;
-            }
+            z[k] = ZeroPack<T, V>();
+            w.held[k] = ZeroPack<T, V>();
             if (col < a.width) {
-                LoadSum<T, V>(x, r, col, z[k]);
-                if constexpr (kEarlyWeight) {
-                    LoadWeight<T, V>(a.weight, a.weight32, col, w[k]);
-                }
+                z[k] = LoadSum<T, V>(x, r, col);
+                w.Early(a, k, col);
             }
         }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                sq = fmaf(z[k][i], z[k][i], sq);
-            }
             const int32_t col = first + k * step;
             if (sum != nullptr && col < a.width) {
-                StoreF<T, V>(sum + col, z[k]);
+                StorePacked<T, V>(sum + col, z[k]);
             }
+            UnpackToF<T, V>(z[k], f);
+            AddDot(f, f, sq);
         }
     } else {
         for (int32_t col = first; col < a.width; col += step) {
-            LoadSum<T, V>(x, r, col, z[0]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                sq = fmaf(z[0][i], z[0][i], sq);
-            }
+            z[0] = LoadSum<T, V>(x, r, col);
             if (sum != nullptr) {
-                StoreF<T, V>(sum + col, z[0]);
+                StorePacked<T, V>(sum + col, z[0]);
             }
+            UnpackToF<T, V>(z[0], f);
+            AddDot(f, f, sq);
         }
     }
-    const float rstd = 1.0f / sqrtf(RowSum(sq, part) / static_cast<float>(a.width) + a.eps);
-    if constexpr (NV > 0) {
-        uint32_t top[N]; // of this thread's values of chunk k
+    const float rstd = 1.0f / sqrtf(RowSum(Both(sq), part) / static_cast<float>(a.width) + a.eps);
+    if constexpr (NV > 0 && LG > 0) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            top[k] = 0;
             const int32_t col = first + k * step;
-            float(&wk)[V] = w[kEarlyWeight ? k : 0];
-            if constexpr (!kEarlyWeight) {
-                if (col < a.width) {
-                    LoadWeight<T, V>(a.weight, a.weight32, col, wk);
-                }
+            const bool inside = col < a.width;
+            UnpackToF<T, V>(z[k], f);
+            w.Apply(a, k, inside ? col : 0, rstd, f);
+            float top = Most(f, 0.0f);
+#pragma unroll
+            for (int o = LG / 2; o > 0; o >>= 1) {
+                top = MaxOrNaN(top, __shfl_xor_sync(0xffffffffu, top, o));
             }
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                z[k][i] *= rstd * wk[i];
-                top[k] = max(top[k], Magnitude(z[k][i]));
-            }
-            if constexpr (LG > 0) {
-#pragma unroll
-                for (int o = LG / 2; o > 0; o >>= 1) {
-                    top[k] = max(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+            if (inside) {
+                if ((threadIdx.x & (LG - 1)) == 0) {
+                    scales[col / (LG * V)] = top / QT::kMost;
                 }
-                if (col < a.width) {
-                    const float inv = Inverse(top[k], QT::kMost);
-                    if ((threadIdx.x & (LG - 1)) == 0) {
-                        scales[col / a.group] = __uint_as_float(top[k]) / QT::kMost;
-                    }
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        z[k][i] *= inv;
-                    }
-                    QT::template Store<V>(q + col, z[k]);
-                }
-            } else if (a.groups > 1 && col < a.width) {
-                atomicMax(&most[col / a.group], top[k]);
+                Times(f, Inverse(top, QT::kMost));
+                QT::template Store<V>(q + col, f);
             }
         }
-        if constexpr (LG == 0) {
-            if (a.groups == 1) {
-                uint32_t t = 0;
+        return;
+    }
+    if constexpr (LG == 0) {
+        // two passes over the row's values: largest magnitudes, then the quantised values
+        for (int pass = 0; pass < 2; ++pass) {
+            float top = 0.0f; // of all of this thread's values
+            auto chunk = [&](int k, int32_t col) {
+                UnpackToF<T, V>(z[k], f);
+                w.Apply(a, k, col, rstd, f);
+                const int32_t g = a.groups > 1 ? col / a.group : 0;
+                if (pass == 0) {
+                    if (a.groups > 1) {
+                        atomicMax(&most[g], __float_as_uint(Most(f, 0.0f)));
+                    } else {
+                        top = Most(f, top);
+                    }
+                } else {
+                    Times(f, Inverse(__uint_as_float(most[g]), QT::kMost));
+                    QT::template Store<V>(q + col, f);
+                }
+            };
+            if constexpr (NV > 0) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
-                    t = max(t, top[k]);
+                    const int32_t col = first + k * step;
+                    if (col < a.width) {
+                        chunk(k, col);
+                    }
                 }
-                t = __reduce_max_sync(0xffffffffu, t);
+            } else {
+                for (int32_t col = first; col < a.width; col += step) {
+                    z[0] = sum != nullptr ? *reinterpret_cast<const Pack<T, V>*>(sum + col) : LoadSum<T, V>(x, r, col);
+                    w.Early(a, 0, col);
+                    chunk(0, col);
+                }
+            }
+            if (pass == 0 && a.groups == 1) {
+                const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
                 if ((threadIdx.x & 31) == 0) {
                     atomicMax(&most[0], t);
                 }
             }
             __syncthreads();
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int32_t col = first + k * step;
-                if (col < a.width) {
-                    const float inv = Inverse(most[a.groups > 1 ? col / a.group : 0], QT::kMost);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        z[k][i] *= inv;
-                    }
-                    QT::template Store<V>(q + col, z[k]);
-                }
-            }
         }
-    } else {
-        static_assert(LG == 0, "wide rows use shared memory");
-        for (int pass = 0; pass < 2; ++pass) {
-            for (int32_t col = first; col < a.width; col += step) {
-                if (sum != nullptr) {
-                    LoadF<T, V>(sum + col, z[0]);
-                } else {
-                    LoadSum<T, V>(x, r, col, z[0]);
-                }
-                LoadWeight<T, V>(a.weight, a.weight32, col, w[0]);
-                const int32_t g = a.groups > 1 ? col / a.group : 0;
-                const float inv = pass == 0 ? 0.0f : Inverse(most[g], QT::kMost);
-                uint32_t t = 0;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    z[0][i] *= rstd * w[0][i];
-                    t = max(t, Magnitude(z[0][i]));
-                    z[0][i] *= inv;
-                }
-                if (pass == 0) {
-                    atomicMax(&most[g], t);
-                } else {
-                    QT::template Store<V>(q + col, z[0]);
-                }
-            }
-            __syncthreads();
-        }
-    }
-    if constexpr (LG == 0) {
         for (int32_t g = threadIdx.x; g < a.groups; g += blockDim.x) {
             scales[g] = __uint_as_float(most[g]) / QT::kMost;
         }
@@ -480,38 +567,42 @@ __global__ void __launch_bounds__(NV * V == 16 ? 512 : 1024) RmsNormBwdKernel(Bw
     }
     int turn = 0;
     for (; row < a.rows; row += gridDim.x, turn ^= 1) {
-        float g[NV][V], u[NV][V];
-        Pack<T, V> add[NV];
+        Pack<T, V> gp[NV], zp[NV], ap[NV];
         const float rstd = nextRstd;
-        float dot = 0.0f;
+        F2 dots = MakeF2(0.0f, 0.0f);
+        float g[V], u[V];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            UnpackToF<T, V>(nextG[k], g[k]);
-            UnpackToF<T, V>(nextZ[k], u[k]);
-            add[k] = nextA[k];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                u[k][i] *= rstd;
-                gw[k][i] = fmaf(g[k][i], u[k][i], gw[k][i]);
-                g[k][i] *= w[k][i];
-                dot = fmaf(g[k][i], u[k][i], dot);
-            }
+            gp[k] = nextG[k];
+            zp[k] = nextZ[k];
+            ap[k] = nextA[k];
+            UnpackToF<T, V>(gp[k], g);
+            UnpackToF<T, V>(zp[k], u);
+            Times(u, rstd);
+            AddProducts(g, u, gw[k]);
+            Times(g, w[k]);
+            AddDot(g, u, dots);
         }
         if (row + gridDim.x < a.rows) {
             fetch(row + gridDim.x);
         }
         // two sets of partial sums in turn: the next row's are written while a slow warp still reads this row's
-        const float c = RowSum(dot, part[turn]) * inverse;
+        const float c = RowSum(Both(dots), part[turn]) * inverse * rstd;
         T* out = static_cast<T*>(a.gradX) + RowAt(row, a.inner, a.xs);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int32_t col = first + k * step;
             if (col < a.width) {
                 float v[V];
-                UnpackToF<T, V>(add[k], v);
+                UnpackToF<T, V>(gp[k], g);
+                UnpackToF<T, V>(zp[k], u);
+                UnpackToF<T, V>(ap[k], v);
+                Times(g, w[k]);
+                Times(u, -c);
+                // gradSum + rstd (g - u c)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    v[i] = fmaf(rstd, g[k][i] - u[k][i] * c, v[i]);
+                    v[i] = fmaf(rstd, g[i] + u[i], v[i]);
                 }
                 StoreF<T, V>(out + col, v);
             }
@@ -589,26 +680,25 @@ __global__ void RmsNormWeightSumsKernel(BwdArgs a)
     a.scratch[static_cast<int64_t>(blockIdx.x) * a.width + col] = acc;
 }
 
-// The blocks' sums of one column, added in a fixed order: 8 warps take every eighth block, then add up.
+// The blocks' sums of one column, added in a fixed order: 32 warps take every 32nd block, then add up.
 template <typename W>
-__global__ void __launch_bounds__(256) RmsNormWeightGradKernel(const float* scratch, int32_t blocks, int32_t width, W* out)
+__global__ void __launch_bounds__(1024) RmsNormWeightGradKernel(const float* scratch, int32_t blocks, int32_t width, W* out)
 {
-    __shared__ float part[8][33];
+    __shared__ float part[32][33];
     const int32_t col = blockIdx.x * 32 + threadIdx.x;
     float acc = 0.0f;
     if (col < width) {
-        for (int32_t b = threadIdx.y; b < blocks; b += 8) {
+#pragma unroll 8
+        for (int32_t b = threadIdx.y; b < blocks; b += 32) {
             acc += scratch[static_cast<int64_t>(b) * width + col];
         }
     }
     part[threadIdx.y][threadIdx.x] = acc;
     __syncthreads();
-    if (threadIdx.y == 0 && col < width) {
-#pragma unroll
-        for (int i = 1; i < 8; ++i) {
-            acc += part[i][threadIdx.x];
-        }
-        out[col] = DType<W>::FromF(acc);
+    const float sum = WarpSum(part[threadIdx.x][threadIdx.y]); // of column threadIdx.y
+    const int32_t mine = blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && mine < width) {
+        out[mine] = DType<W>::FromF(sum);
     }
 }
 
@@ -866,7 +956,7 @@ cudaError_t RmsNormBwd(Dt dt, const NormShape& n, const void* gradY, RowStride g
     CountLaunch();
     if (gradWeight != nullptr) {
         const unsigned grid = static_cast<unsigned>(CeilDiv(n.width, 32));
-        const dim3 block(32, 8);
+        const dim3 block(32, 32);
         if (n.weight32) {
             RmsNormWeightGradKernel<float><<<grid, block, 0, s>>>(scratch, static_cast<int32_t>(p.blocks), n.width,
                                                                   static_cast<float*>(gradWeight));

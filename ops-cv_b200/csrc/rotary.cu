@@ -28,60 +28,32 @@ __device__ __forceinline__ int64_t TokenAt(int64_t token, int64_t inner, RowStri
     return token < inner ? token * s.s1 : token / inner * s.s0 + token % inner * s.s1;
 }
 
-// One item of V values of a pair's first half and V of its second (half layout), of V / 2 pairs (interleaved), or V values that
-// are copied. A thread reads all it needs of an item before it writes, so out may be in.
+// An item is V values of the pairs' first half and V of their second (half layout), V / 2 pairs (interleaved), or V values that are
+// copied. A thread reads all it needs of an item before it writes, so out may be in.
 template <typename T, int V>
-__device__ __forceinline__ void TurnItem(const Args& a, const T* in, T* out, int32_t item, int32_t turned, const float2* table)
-{
-    const int32_t half = a.r.half;
-    if (item >= turned) {
-        const int32_t c = 2 * half + (item - turned) * V;
-        *reinterpret_cast<Pack<T, V>*>(out + c) = *reinterpret_cast<const Pack<T, V>*>(in + c);
-        return;
-    }
-    if (a.r.interleaved) {
-        if constexpr (V >= 2) {
-            float v[V];
-            LoadPack<T, V>(in + item * V, v);
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-                const float2 cs = table[item * (V / 2) + i];
-                const float x = v[2 * i], y = v[2 * i + 1];
-                v[2 * i] = x * cs.x - y * cs.y;
-                v[2 * i + 1] = y * cs.x + x * cs.y;
-            }
-            StorePack<T, V>(out + item * V, v);
-        } else {
-            const float2 cs = table[item];
-            const float x = DType<T>::ToF(in[2 * item]), y = DType<T>::ToF(in[2 * item + 1]);
-            out[2 * item] = DType<T>::FromF(x * cs.x - y * cs.y);
-            out[2 * item + 1] = DType<T>::FromF(y * cs.x + x * cs.y);
+struct Item {
+    Pack<T, V> a, b;
+    __device__ __forceinline__ void Load(const T* p, int32_t at, int32_t second)
+    {
+        a = *reinterpret_cast<const Pack<T, V>*>(p + at);
+        if (second >= 0) {
+            b = *reinterpret_cast<const Pack<T, V>*>(p + second);
         }
-        return;
     }
-    float x[V], y[V];
-    const int32_t c = item * V;
-    LoadPack<T, V>(in + c, x);
-    LoadPack<T, V>(in + half + c, y);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float2 cs = table[c + i];
-        const float u = x[i] * cs.x - y[i] * cs.y;
-        y[i] = y[i] * cs.x + x[i] * cs.y;
-        x[i] = u;
-    }
-    StorePack<T, V>(out + c, x);
-    StorePack<T, V>(out + half + c, y);
-}
+};
 
+// A block has a few tokens. Threads are (item of a head) x (heads): a thread keeps its item's sines and cosines of a token in registers
+// for all the heads that it takes, a few of them at a time so that their loads are on their way together.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) RotaryKernel(Args a)
+__global__ void __launch_bounds__(kThreads) RotaryKernel(const __grid_constant__ Args a)
 {
+    constexpr int kHeads = 4; // at a time
     __shared__ float2 table[kTable];
     const int32_t half = a.r.half;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * a.tokensPerBlock;
     const int32_t tokens = static_cast<int32_t>(min(static_cast<int64_t>(a.tokensPerBlock), a.r.tokens - first));
-    for (int32_t e = threadIdx.x; e < tokens * half; e += kThreads) {
+    const int32_t threads = blockDim.x * blockDim.y;
+    for (int32_t e = threadIdx.y * blockDim.x + threadIdx.x; e < tokens * half; e += threads) {
         const int32_t t = e / half, i = e - t * half;
         int axis = 0;
         while (axis < a.r.axes - 1 && i >= a.r.ends[axis]) {
@@ -102,24 +74,78 @@ __global__ void __launch_bounds__(kThreads) RotaryKernel(Args a)
         table[e] = make_float2(cs * a.r.scale, (a.r.inverse ? -sn : sn) * a.r.scale);
     }
     __syncthreads();
-    const int32_t turned = a.r.interleaved && V > 1 ? 2 * half / V : half / V;
-    const int32_t items = turned + (a.r.dim - 2 * half) / V; // of a head
+    const bool inter = a.r.interleaved;
+    const int32_t turned = inter && V > 1 ? 2 * half / V : half / V; // items of a head that are turned
+    const int32_t items = turned + (a.r.dim - 2 * half) / V;
     const int32_t heads = a.q.heads + a.k.heads;
-    const int32_t perToken = heads * items;
-    for (int32_t e = threadIdx.x; e < tokens * perToken; e += kThreads) {
-        const int32_t t = e / perToken;
-        const int32_t rest = e - t * perToken;
-        int32_t head = rest / items;
-        const int32_t item = rest - head * items;
-        const bool ofK = head >= a.q.heads;
-        head -= ofK ? a.q.heads : 0;
-        const RotaryTensor& x = ofK ? a.k : a.q;
-        const T* in = static_cast<const T*>(x.in) + TokenAt(first + t, a.r.inner, x.inTok) + head * x.inHead;
-        T* out = static_cast<T*>(x.out) + TokenAt(first + t, a.r.inner, x.outTok) + head * x.outHead;
-        if (in == out && item >= turned) {
-            continue; // the copied part of a head that is turned in place
+    for (int32_t item = threadIdx.x; item < items; item += blockDim.x) {
+        const bool turn = item < turned;
+        // the item's values, and those of the second half (interleaved single values: the pair's second)
+        const int32_t at = !turn ? 2 * half + (item - turned) * V : inter && V == 1 ? 2 * item : item * V;
+        const int32_t second = !turn || (inter && V > 1) ? -1 : inter ? at + 1 : half + at;
+        for (int32_t t = 0; t < tokens; ++t) {
+            const int64_t token = first + t;
+            const T* qIn = static_cast<const T*>(a.q.in) + TokenAt(token, a.r.inner, a.q.inTok);
+            T* qOut = static_cast<T*>(a.q.out) + TokenAt(token, a.r.inner, a.q.outTok);
+            const T* kIn = static_cast<const T*>(a.k.in) + TokenAt(token, a.r.inner, a.k.inTok);
+            T* kOut = static_cast<T*>(a.k.out) + TokenAt(token, a.r.inner, a.k.outTok);
+            float cs[V], sn[V]; // interleaved: the first V / 2
+            if (turn) {
+                const float2* row = table + t * half + (inter && V > 1 ? item * (V / 2) : item * V);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    if (!inter || V == 1 || i < V / 2) {
+                        cs[i] = row[i].x;
+                        sn[i] = row[i].y;
+                    }
+                }
+            }
+            for (int32_t h0 = threadIdx.y; h0 < heads; h0 += kHeads * blockDim.y) {
+                Item<T, V> x[kHeads];
+#pragma unroll
+                for (int i = 0; i < kHeads; ++i) {
+                    const int32_t h = h0 + i * blockDim.y;
+                    if (h < heads) {
+                        x[i].Load(h < a.q.heads ? qIn + h * a.q.inHead : kIn + (h - a.q.heads) * a.k.inHead, at, second);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kHeads; ++i) {
+                    const int32_t h = h0 + i * blockDim.y;
+                    if (h >= heads) {
+                        break;
+                    }
+                    T* out = h < a.q.heads ? qOut + h * a.q.outHead : kOut + (h - a.q.heads) * a.k.outHead;
+                    if (!turn) {
+                        *reinterpret_cast<Pack<T, V>*>(out + at) = x[i].a;
+                        continue;
+                    }
+                    float u[V];
+                    UnpackToF<T, V>(x[i].a, u);
+                    if (second < 0) {
+                        if constexpr (V > 1) {
+#pragma unroll
+                            for (int e = 0; e < V / 2; ++e) {
+                                const float y = u[2 * e], z = u[2 * e + 1];
+                                u[2 * e] = y * cs[e] - z * sn[e];
+                                u[2 * e + 1] = z * cs[e] + y * sn[e];
+                            }
+                        }
+                    } else {
+                        float v[V];
+                        UnpackToF<T, V>(x[i].b, v);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            const float y = u[e];
+                            u[e] = y * cs[e] - v[e] * sn[e];
+                            v[e] = v[e] * cs[e] + y * sn[e];
+                        }
+                        StorePack<T, V>(out + second, v);
+                    }
+                    StorePack<T, V>(out + at, u);
+                }
+            }
         }
-        TurnItem<T, V>(a, in, out, item, turned, table + t * half);
     }
 }
 
@@ -201,10 +227,14 @@ cudaError_t RotaryTurn(Dt dt, const RotaryShape& r, const RotaryTensor& q, const
     a.k = k;
     a.positions = positions;
     a.frequencies = frequencies;
-    // Tokens per block: about four items a thread, so that the sines' time hides behind other blocks' copies, but at least a
-    // block per SM slot, and no more than the table holds.
-    const int64_t perToken = static_cast<int64_t>(q.heads + k.heads) * CeilDiv(r.dim, r.interleaved ? v : 2 * v);
-    int64_t t = CeilDiv(4 * kThreads, perToken < 1 ? 1 : perToken);
+    // Threads: the items of a head by as many heads as make up to 256. Tokens: what gives each thread about eight items, so that the
+    // sines' time hides behind other blocks' copies, but at least some blocks for each SM, and no more than the table holds.
+    const int32_t turned = r.interleaved && v > 1 ? 2 * r.half / v : r.half / v, items = turned + (r.dim - 2 * r.half) / v;
+    const int32_t heads = q.heads + k.heads;
+    const int32_t across = items < kThreads ? items : kThreads;
+    int32_t down = kThreads / across;
+    down = down < heads ? down : heads;
+    int64_t t = CeilDiv(8, CeilDiv(heads, down));
     const int64_t spread = CeilDiv(r.tokens, static_cast<int64_t>(NumSMs()) * 8);
     t = t < spread ? t : spread;
     const int64_t room = kTable / (r.half < 1 ? 1 : r.half);
@@ -216,7 +246,7 @@ cudaError_t RotaryTurn(Dt dt, const RotaryShape& r, const RotaryTensor& q, const
         return cudaErrorInvalidConfiguration;
     }
     OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
-        RotaryKernel<T, V><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(a);
+        RotaryKernel<T, V><<<static_cast<unsigned>(blocks), dim3(across, down), 0, s>>>(a);
     }));
     CountLaunch();
     return cudaGetLastError();
