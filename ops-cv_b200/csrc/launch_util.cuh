@@ -1,6 +1,7 @@
 // Launch-configuration helpers shared by the .cu files: dtype dispatch, vector-width choice, grid sizing.
 #pragma once
 
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -83,6 +84,27 @@ inline int PickVec(int elemSize, int64_t inner, std::initializer_list<const void
         }
     }
     return 1;
+}
+
+// Asks once for each device for the shared memory (and clusters of more than 8 blocks) that a kernel takes: a call of the runtime that
+// costs as much as a launch. `asked` has a bit a device.
+template <typename Kernel>
+cudaError_t AskOnce(Kernel kernel, std::atomic<uint64_t>& asked, int shared, bool wideCluster = false)
+{
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);
+    if (e != cudaSuccess || (asked.load(std::memory_order_relaxed) & bit) != 0) {
+        return e;
+    }
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+    if (e == cudaSuccess && wideCluster) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    }
+    if (e == cudaSuccess) {
+        asked.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return e;
 }
 
 #define OPSCV_DISPATCH_DT(dt, T, ...)                 \

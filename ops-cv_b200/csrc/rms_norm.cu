@@ -8,6 +8,7 @@
 // the reduction and the output (each thread owns the same columns in every pass over the row), so each value moves once.
 #include <cuda_fp8.h>
 
+#include "cp_async.cuh"
 #include "launch_util.cuh"
 #include "sequence_kernels.h"
 
@@ -377,7 +378,10 @@ struct Q8Type<Q8::INT8> {
 // Value times this is the quantised value. A group of zeros has scale 0 and zeros.
 __device__ __forceinline__ float Inverse(float most, float range) { return most == 0.0f ? 0.0f : range / most; }
 
-// LG: lanes of a group where a group lies within a warp (a power of two), 0 where groups go through shared memory, one word each.
+// LG: lanes of a group where a group lies within a warp (a power of two), 0 where groups go through shared memory, one word each, and
+// kRowScale where the row has one scale.
+constexpr int kRowScale = -1;
+
 template <typename T, int V, int NV, Q8 Q, int LG>
 __global__ void __launch_bounds__(kMaxThreads) RmsNormQuantKernel(FwdArgs a)
 {
@@ -437,6 +441,47 @@ __global__ void __launch_bounds__(kMaxThreads) RmsNormQuantKernel(FwdArgs a)
         }
     }
     const float rstd = 1.0f / sqrtf(RowSum(Both(sq), part) / static_cast<float>(a.width) + a.eps);
+    if constexpr (NV > 0 && LG == kRowScale) {
+        __shared__ float tops[32];
+        float top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int32_t col = first + k * step;
+            UnpackToF<T, V>(z[k], f);
+            w.Apply(a, k, col < a.width ? col : 0, rstd, f); // zeros behind the row
+            top = Most(f, top);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            top = MaxOrNaN(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
+        if (blockDim.x > 32) {
+            if ((threadIdx.x & 31) == 0) {
+                tops[threadIdx.x >> 5] = top;
+            }
+            __syncthreads();
+            top = static_cast<int>(threadIdx.x & 31) < static_cast<int>(blockDim.x >> 5) ? tops[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                top = MaxOrNaN(top, __shfl_xor_sync(0xffffffffu, top, o));
+            }
+        }
+        if (threadIdx.x == 0) {
+            scales[0] = top / QT::kMost;
+        }
+        const float inv = Inverse(top, QT::kMost);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int32_t col = first + k * step;
+            if (col < a.width) {
+                UnpackToF<T, V>(z[k], f);
+                w.Apply(a, k, col, rstd, f);
+                Times(f, inv);
+                QT::template Store<V>(q + col, f);
+            }
+        }
+        return;
+    }
     if constexpr (NV > 0 && LG > 0) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -522,9 +567,17 @@ struct BwdArgs {
 // A block walks rows blockIdx.x, + gridDim.x, ...; each thread keeps its columns' weight and the sum of the weight's gradient in
 // registers over all of them, so the weight's gradient costs no second pass over gradY and z. The rows' loads of one step are
 // issued before the reduction of the step before is waited for.
-template <typename T, int V, int NV>
+//
+// RING (16-byte chunks): the next rows come by asynchronous copies into slots of shared memory, each thread its own chunks, up to three
+// rows ahead; else the next row is loaded into registers, which hold one.
+constexpr int Ahead(int nv) { return nv <= 2 ? 3 : 2; } // 4 chunks a thread leave room for two rows
+constexpr int RingBytes(int nv, int threads) { return Ahead(nv) * 3 * nv * threads * 16; }
+
+template <typename T, int V, int NV, bool RING>
 __global__ void __launch_bounds__(NV * V == 16 ? 512 : 1024) RmsNormBwdKernel(BwdArgs a)
 {
+    constexpr int kAhead = Ahead(NV);
+    extern __shared__ uint4 slots[]; // [kAhead][3][NV][threads] (RING)
     __shared__ float part[2][32];
     const int32_t step = blockDim.x * V;
     const int32_t first = threadIdx.x * V;
@@ -544,38 +597,75 @@ __global__ void __launch_bounds__(NV * V == 16 ? 512 : 1024) RmsNormBwdKernel(Bw
             LoadWeight<T, V>(a.weight, a.weight32, col, w[k]);
         }
     }
-    auto fetch = [&](int64_t row) {
+    auto fetch = [&](int64_t row, int stage) {
         const T* g = static_cast<const T*>(a.gradY) + RowAt(row, a.inner, a.gs);
         const T* z = static_cast<const T*>(a.sum) + RowAt(row, a.inner, a.ss);
         const T* s = a.gradSum != nullptr ? static_cast<const T*>(a.gradSum) + RowAt(row, a.inner, a.as) : nullptr;
-        nextRstd = a.rstd[row];
+        if constexpr (!RING) {
+            nextRstd = a.rstd[row];
+        }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int32_t col = first + k * step;
             if (col < a.width) {
-                nextG[k] = *reinterpret_cast<const Pack<T, V>*>(g + col);
-                nextZ[k] = *reinterpret_cast<const Pack<T, V>*>(z + col);
-                if (s != nullptr) {
-                    nextA[k] = *reinterpret_cast<const Pack<T, V>*>(s + col);
+                if constexpr (RING) {
+                    uint4* at = slots + ((stage * 3) * NV + k) * blockDim.x + threadIdx.x;
+                    CpAsync16(at, g + col);
+                    CpAsync16(at + NV * blockDim.x, z + col);
+                    if (s != nullptr) {
+                        CpAsync16(at + 2 * NV * blockDim.x, s + col);
+                    }
+                } else {
+                    nextG[k] = *reinterpret_cast<const Pack<T, V>*>(g + col);
+                    nextZ[k] = *reinterpret_cast<const Pack<T, V>*>(z + col);
+                    if (s != nullptr) {
+                        nextA[k] = *reinterpret_cast<const Pack<T, V>*>(s + col);
+                    }
                 }
             }
         }
     };
     int64_t row = blockIdx.x;
-    if (row < a.rows) {
-        fetch(row);
+    int stage = 0;
+    if constexpr (RING) {
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+            if (row + x * static_cast<int64_t>(gridDim.x) < a.rows) {
+                fetch(row + x * static_cast<int64_t>(gridDim.x), x);
+            }
+            CpAsyncCommit();
+        }
+    } else if (row < a.rows) {
+        fetch(row, 0);
     }
     int turn = 0;
     for (; row < a.rows; row += gridDim.x, turn ^= 1) {
         Pack<T, V> gp[NV], zp[NV], ap[NV];
-        const float rstd = nextRstd;
+        float rstd;
+        if constexpr (RING) {
+            rstd = a.rstd[row];
+            CpAsyncWait<kAhead - 1>();
+        } else {
+            rstd = nextRstd;
+        }
         F2 dots = MakeF2(0.0f, 0.0f);
         float g[V], u[V];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            gp[k] = nextG[k];
-            zp[k] = nextZ[k];
-            ap[k] = nextA[k];
+            if constexpr (RING) {
+                const uint4* at = slots + ((stage * 3) * NV + k) * blockDim.x + threadIdx.x;
+                const uint4 zero = make_uint4(0, 0, 0, 0);
+                const bool inside = first + k * step < a.width;
+                const uint4 raw[3] = {inside ? at[0] : zero, inside ? at[NV * blockDim.x] : zero,
+                                      inside && a.gradSum != nullptr ? at[2 * NV * blockDim.x] : zero};
+                gp[k] = reinterpret_cast<const Pack<T, V>&>(raw[0]);
+                zp[k] = reinterpret_cast<const Pack<T, V>&>(raw[1]);
+                ap[k] = reinterpret_cast<const Pack<T, V>&>(raw[2]);
+            } else {
+                gp[k] = nextG[k];
+                zp[k] = nextZ[k];
+                ap[k] = nextA[k];
+            }
             UnpackToF<T, V>(gp[k], g);
             UnpackToF<T, V>(zp[k], u);
             Times(u, rstd);
@@ -583,8 +673,15 @@ __global__ void __launch_bounds__(NV * V == 16 ? 512 : 1024) RmsNormBwdKernel(Bw
             Times(g, w[k]);
             AddDot(g, u, dots);
         }
-        if (row + gridDim.x < a.rows) {
-            fetch(row + gridDim.x);
+        if constexpr (RING) {
+            const int64_t later = row + kAhead * static_cast<int64_t>(gridDim.x);
+            if (later < a.rows) {
+                fetch(later, stage);
+            }
+            CpAsyncCommit();
+            stage = stage == kAhead - 1 ? 0 : stage + 1;
+        } else if (row + gridDim.x < a.rows) {
+            fetch(row + gridDim.x, 0);
         }
         // two sets of partial sums in turn: the next row's are written while a slow warp still reads this row's
         const float c = RowSum(Both(dots), part[turn]) * inverse * rstd;
@@ -826,12 +923,12 @@ cudaError_t RmsNormQuant(Dt dt, const NormShape& n, const void* x, RowStride xs,
     RowShape shape = ShapeOfRow(n.width, v, 32, kMaxThreads);
     // Groups of 128 columns read with at least four to a lane lie within a warp (lanes hold consecutive chunks of a row, and a
     // warp's first chunk starts a group); others go through shared memory, with one row a block.
-    const bool inWarp = a.groups > 1 && a.group == 128 && shape.nv > 0 && v >= 4;
-    if (!inWarp) {
+    const bool inWarp = a.groups > 1 && a.group == 128 && shape.nv > 0 && v >= 4, ofRow = a.groups == 1 && shape.nv > 0;
+    if (!inWarp && !ofRow) {
         shape.rows = 1;
     }
     const int64_t blocks = CeilDiv(n.rows, shape.rows);
-    const size_t shared = inWarp ? 0 : static_cast<size_t>(a.groups) * 4;
+    const size_t shared = inWarp || ofRow ? 0 : static_cast<size_t>(a.groups) * 4;
     if (!GridFits(blocks) || shared > 40 * 1024) {
         return cudaErrorInvalidConfiguration;
     }
@@ -840,16 +937,20 @@ cudaError_t RmsNormQuant(Dt dt, const NormShape& n, const void* x, RowStride xs,
     OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
         OPSCV_DISPATCH_NV(shape.nv, NV, if constexpr (NV * V <= 32) {
             constexpr int LG = NV > 0 && V >= 4 ? 128 / V : 0;
-            if (type == Q8::E4M3) {
+            auto launch = [&](auto tag) {
+                constexpr Q8 Q = decltype(tag)::value;
                 if (inWarp) {
-                    RmsNormQuantKernel<T, V, NV, Q8::E4M3, LG><<<grid, block, shared, s>>>(a);
+                    RmsNormQuantKernel<T, V, NV, Q, LG><<<grid, block, shared, s>>>(a);
+                } else if (ofRow) {
+                    RmsNormQuantKernel<T, V, NV, Q, (NV > 0 ? kRowScale : 0)><<<grid, block, shared, s>>>(a);
                 } else {
-                    RmsNormQuantKernel<T, V, NV, Q8::E4M3, 0><<<grid, block, shared, s>>>(a);
+                    RmsNormQuantKernel<T, V, NV, Q, 0><<<grid, block, shared, s>>>(a);
                 }
-            } else if (inWarp) {
-                RmsNormQuantKernel<T, V, NV, Q8::INT8, LG><<<grid, block, shared, s>>>(a);
+            };
+            if (type == Q8::E4M3) {
+                launch(std::integral_constant<Q8, Q8::E4M3>{});
             } else {
-                RmsNormQuantKernel<T, V, NV, Q8::INT8, 0><<<grid, block, shared, s>>>(a);
+                launch(std::integral_constant<Q8, Q8::INT8>{});
             }
         });
     }));
@@ -947,11 +1048,26 @@ cudaError_t RmsNormBwd(Dt dt, const NormShape& n, const void* gradY, RowStride g
             RmsNormBwdWideKernel<T, V><<<static_cast<unsigned>(n.rows), kMaxThreads, 0, s>>>(a);
         }));
     } else {
+        cudaError_t failed = cudaSuccess;
         OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
             OPSCV_DISPATCH_NV(p.shape.nv, NV, if constexpr (NV > 0 && NV * V <= 16) {
-                RmsNormBwdKernel<T, V, NV><<<static_cast<unsigned>(p.blocks), p.shape.threads, 0, s>>>(a);
+                if constexpr (V * sizeof(T) == 16) {
+                    static std::atomic<uint64_t> asked;
+                    const int shared = RingBytes(NV, p.shape.threads);
+                    const cudaError_t e = AskOnce(RmsNormBwdKernel<T, V, NV, true>, asked, RingBytes(NV, 512));
+                    if (e != cudaSuccess) {
+                        failed = e;
+                    } else {
+                        RmsNormBwdKernel<T, V, NV, true><<<static_cast<unsigned>(p.blocks), p.shape.threads, shared, s>>>(a);
+                    }
+                } else {
+                    RmsNormBwdKernel<T, V, NV, false><<<static_cast<unsigned>(p.blocks), p.shape.threads, 0, s>>>(a);
+                }
             });
         }));
+        if (failed != cudaSuccess) {
+            return failed;
+        }
     }
     CountLaunch();
     if (gradWeight != nullptr) {

@@ -42,108 +42,107 @@ struct Item {
     }
 };
 
-// A block has a few tokens. Threads are (item of a head) x (heads): a thread keeps its item's sines and cosines of a token in registers
-// for all the heads that it takes, a few of them at a time so that their loads are on their way together.
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) RotaryKernel(const __grid_constant__ Args a)
+// Which product is rounded is written out, so that all widths and layouts give the same bits.
+__device__ __forceinline__ void TurnPair(float& x, float& y, float2 cs)
 {
-    constexpr int kHeads = 4; // at a time
-    __shared__ float2 table[kTable];
+    const float u = fmaf(x, cs.x, -Mul(y, cs.y));
+    y = fmaf(y, cs.x, Mul(x, cs.y));
+    x = u;
+}
+
+// A block has a few tokens. Threads are (item of a head) x (pairs of a token and a head); a thread has up to kPairs of the latter at a
+// time, whose loads are all on their way while the block forms the sines and cosines.
+constexpr int kPairs = 5;
+
+template <typename T, int V, bool INTER>
+__global__ void __launch_bounds__(kThreads, INTER ? 4 : 3) RotaryKernel(const __grid_constant__ Args a)
+{
+    __shared__ __align__(16) float2 table[kTable];
     const int32_t half = a.r.half;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * a.tokensPerBlock;
     const int32_t tokens = static_cast<int32_t>(min(static_cast<int64_t>(a.tokensPerBlock), a.r.tokens - first));
     const int32_t threads = blockDim.x * blockDim.y;
-    for (int32_t e = threadIdx.y * blockDim.x + threadIdx.x; e < tokens * half; e += threads) {
-        const int32_t t = e / half, i = e - t * half;
-        int axis = 0;
-        while (axis < a.r.axes - 1 && i >= a.r.ends[axis]) {
-            ++axis;
-        }
-        const int64_t at = TokenAt(first + t, a.r.inner, a.r.posTok) + axis * a.r.posAxis;
-        const double p = a.r.pos64 ? static_cast<double>(static_cast<const long long*>(a.positions)[at]) :
-                                     static_cast<double>(static_cast<const int*>(a.positions)[at]);
-        const double f = a.r.freq64 ? static_cast<const double*>(a.frequencies)[i] :
-                                      static_cast<double>(static_cast<const float*>(a.frequencies)[i]);
-        // In turns, p * f / (2 pi): the whole ones fall away, the rest keeps its leading bits in fp32. 1 / (2 pi) and the products
-        // are sums of two doubles, so that positions of 10^12 and more, whose angle in one double is off by 10^-4, keep theirs.
-        constexpr double kHigh = 0.15915494309189535, kLow = -9.839338337591243e-18; // 1 / (2 pi)
-        const double fHigh = f * kHigh, fLow = fma(f, kHigh, -fHigh) + f * kLow;
-        const double high = p * fHigh, low = fma(p, fHigh, -high) + p * fLow;
-        float sn, cs;
-        sincospif(2.0f * static_cast<float>((high - rint(high)) + low), &sn, &cs);
-        table[e] = make_float2(cs * a.r.scale, (a.r.inverse ? -sn : sn) * a.r.scale);
-    }
-    __syncthreads();
-    const bool inter = a.r.interleaved;
-    const int32_t turned = inter && V > 1 ? 2 * half / V : half / V; // items of a head that are turned
+    constexpr bool kNeighbours = INTER && V > 1; // pairs within an item
+    const int32_t turned = kNeighbours ? 2 * half / V : half / V; // items of a head that are turned
     const int32_t items = turned + (a.r.dim - 2 * half) / V;
-    const int32_t heads = a.q.heads + a.k.heads;
-    for (int32_t item = threadIdx.x; item < items; item += blockDim.x) {
-        const bool turn = item < turned;
+    const int32_t heads = a.q.heads + a.k.heads, pairs = tokens * heads;
+    bool ready = false; // the table
+    for (int32_t item0 = 0; item0 < items; item0 += blockDim.x) {
+        const int32_t item = item0 + threadIdx.x;
+        const bool inside = item < items, turn = item < turned;
         // the item's values, and those of the second half (interleaved single values: the pair's second)
-        const int32_t at = !turn ? 2 * half + (item - turned) * V : inter && V == 1 ? 2 * item : item * V;
-        const int32_t second = !turn || (inter && V > 1) ? -1 : inter ? at + 1 : half + at;
-        for (int32_t t = 0; t < tokens; ++t) {
-            const int64_t token = first + t;
-            const T* qIn = static_cast<const T*>(a.q.in) + TokenAt(token, a.r.inner, a.q.inTok);
-            T* qOut = static_cast<T*>(a.q.out) + TokenAt(token, a.r.inner, a.q.outTok);
-            const T* kIn = static_cast<const T*>(a.k.in) + TokenAt(token, a.r.inner, a.k.inTok);
-            T* kOut = static_cast<T*>(a.k.out) + TokenAt(token, a.r.inner, a.k.outTok);
-            float cs[V], sn[V]; // interleaved: the first V / 2
-            if (turn) {
-                const float2* row = table + t * half + (inter && V > 1 ? item * (V / 2) : item * V);
+        const int32_t at = !turn ? 2 * half + (item - turned) * V : INTER && V == 1 ? 2 * item : item * V;
+        const int32_t second = !turn || kNeighbours ? -1 : INTER ? at + 1 : half + at;
+        for (int32_t p0 = 0; p0 < pairs; p0 += kPairs * blockDim.y) {
+            Item<T, V> x[kPairs];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    if (!inter || V == 1 || i < V / 2) {
-                        cs[i] = row[i].x;
-                        sn[i] = row[i].y;
-                    }
+            for (int i = 0; i < kPairs; ++i) {
+                const int32_t p = p0 + threadIdx.y + i * blockDim.y;
+                if (inside && p < pairs) {
+                    const int32_t t = p / heads, h = p - t * heads;
+                    const RotaryTensor& z = h < a.q.heads ? a.q : a.k;
+                    x[i].Load(static_cast<const T*>(z.in) + TokenAt(first + t, a.r.inner, z.inTok) + (h < a.q.heads ? h : h - a.q.heads) * z.inHead,
+                              at, second);
                 }
             }
-            for (int32_t h0 = threadIdx.y; h0 < heads; h0 += kHeads * blockDim.y) {
-                Item<T, V> x[kHeads];
-#pragma unroll
-                for (int i = 0; i < kHeads; ++i) {
-                    const int32_t h = h0 + i * blockDim.y;
-                    if (h < heads) {
-                        x[i].Load(h < a.q.heads ? qIn + h * a.q.inHead : kIn + (h - a.q.heads) * a.k.inHead, at, second);
+            if (!ready) { // all threads of the block come here first with the same loop state
+                ready = true;
+                for (int32_t e = threadIdx.y * blockDim.x + threadIdx.x; e < tokens * half; e += threads) {
+                    const int32_t t = e / half, i = e - t * half;
+                    int axis = 0;
+                    while (axis < a.r.axes - 1 && i >= a.r.ends[axis]) {
+                        ++axis;
                     }
+                    const int64_t from = TokenAt(first + t, a.r.inner, a.r.posTok) + axis * a.r.posAxis;
+                    const double p = a.r.pos64 ? static_cast<double>(static_cast<const long long*>(a.positions)[from]) :
+                                                 static_cast<double>(static_cast<const int*>(a.positions)[from]);
+                    const double f = a.r.freq64 ? static_cast<const double*>(a.frequencies)[i] :
+                                                  static_cast<double>(static_cast<const float*>(a.frequencies)[i]);
+                    // In turns, p * f / (2 pi): the whole ones fall away, the rest keeps its leading bits in fp32. 1 / (2 pi) and the
+                    // products are sums of two doubles, so that positions of 10^12 and more, whose angle in one double is off by 10^-4,
+                    // keep theirs.
+                    constexpr double kHigh = 0.15915494309189535, kLow = -9.839338337591243e-18; // 1 / (2 pi)
+                    const double fHigh = f * kHigh, fLow = fma(f, kHigh, -fHigh) + f * kLow;
+                    const double high = p * fHigh, low = fma(p, fHigh, -high) + p * fLow;
+                    float sn, cs;
+                    sincospif(2.0f * static_cast<float>((high - rint(high)) + low), &sn, &cs);
+                    table[e] = make_float2(cs * a.r.scale, (a.r.inverse ? -sn : sn) * a.r.scale);
                 }
+                __syncthreads();
+            }
 #pragma unroll
-                for (int i = 0; i < kHeads; ++i) {
-                    const int32_t h = h0 + i * blockDim.y;
-                    if (h >= heads) {
-                        break;
-                    }
-                    T* out = h < a.q.heads ? qOut + h * a.q.outHead : kOut + (h - a.q.heads) * a.k.outHead;
-                    if (!turn) {
-                        *reinterpret_cast<Pack<T, V>*>(out + at) = x[i].a;
-                        continue;
-                    }
-                    float u[V];
-                    UnpackToF<T, V>(x[i].a, u);
-                    if (second < 0) {
-                        if constexpr (V > 1) {
-#pragma unroll
-                            for (int e = 0; e < V / 2; ++e) {
-                                const float y = u[2 * e], z = u[2 * e + 1];
-                                u[2 * e] = y * cs[e] - z * sn[e];
-                                u[2 * e + 1] = z * cs[e] + y * sn[e];
-                            }
-                        }
-                    } else {
-                        float v[V];
-                        UnpackToF<T, V>(x[i].b, v);
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const float y = u[e];
-                            u[e] = y * cs[e] - v[e] * sn[e];
-                            v[e] = v[e] * cs[e] + y * sn[e];
-                        }
-                        StorePack<T, V>(out + second, v);
-                    }
-                    StorePack<T, V>(out + at, u);
+            for (int i = 0; i < kPairs; ++i) {
+                const int32_t p = p0 + threadIdx.y + i * blockDim.y;
+                if (!inside || p >= pairs) {
+                    break;
                 }
+                const int32_t t = p / heads, h = p - t * heads;
+                const RotaryTensor& z = h < a.q.heads ? a.q : a.k;
+                T* out = static_cast<T*>(z.out) + TokenAt(first + t, a.r.inner, z.outTok) + (h < a.q.heads ? h : h - a.q.heads) * z.outHead;
+                if (!turn) {
+                    *reinterpret_cast<Pack<T, V>*>(out + at) = x[i].a;
+                    continue;
+                }
+                float u[V];
+                UnpackToF<T, V>(x[i].a, u);
+                if constexpr (kNeighbours) {
+                    const float2* row = table + t * half + item * (V / 2);
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) {
+                        const float2 cs = row[e];
+                        TurnPair(u[2 * e], u[2 * e + 1], cs);
+                    }
+                } else {
+                    const float2* row = table + t * half + item * V;
+                    float v[V];
+                    UnpackToF<T, V>(x[i].b, v);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        TurnPair(u[e], v[e], row[e]);
+                    }
+                    StorePack<T, V>(out + second, v);
+                }
+                StorePack<T, V>(out + at, u);
             }
         }
     }
@@ -227,15 +226,13 @@ cudaError_t RotaryTurn(Dt dt, const RotaryShape& r, const RotaryTensor& q, const
     a.k = k;
     a.positions = positions;
     a.frequencies = frequencies;
-    // Threads: the items of a head by as many heads as make up to 256. Tokens: what gives each thread about eight items, so that the
-    // sines' time hides behind other blocks' copies, but at least some blocks for each SM, and no more than the table holds.
+    // Threads: the items of a head by as many (token, head) pairs as make up to 256. Tokens: as many as the threads take at a time,
+    // but at least some blocks for each SM, and no more than the table holds.
     const int32_t turned = r.interleaved && v > 1 ? 2 * r.half / v : r.half / v, items = turned + (r.dim - 2 * r.half) / v;
     const int32_t heads = q.heads + k.heads;
-    const int32_t across = items < kThreads ? items : kThreads;
-    int32_t down = kThreads / across;
-    down = down < heads ? down : heads;
-    int64_t t = CeilDiv(8, CeilDiv(heads, down));
-    const int64_t spread = CeilDiv(r.tokens, static_cast<int64_t>(NumSMs()) * 8);
+    const int32_t across = items < kThreads ? items : kThreads, down = kThreads / across;
+    int64_t t = static_cast<int64_t>(kPairs) * down / heads;
+    const int64_t spread = CeilDiv(r.tokens, static_cast<int64_t>(NumSMs()) * 4);
     t = t < spread ? t : spread;
     const int64_t room = kTable / (r.half < 1 ? 1 : r.half);
     t = t < room ? t : room;
@@ -246,7 +243,11 @@ cudaError_t RotaryTurn(Dt dt, const RotaryShape& r, const RotaryTensor& q, const
         return cudaErrorInvalidConfiguration;
     }
     OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
-        RotaryKernel<T, V><<<static_cast<unsigned>(blocks), dim3(across, down), 0, s>>>(a);
+        if (r.interleaved) {
+            RotaryKernel<T, V, true><<<static_cast<unsigned>(blocks), dim3(across, down), 0, s>>>(a);
+        } else {
+            RotaryKernel<T, V, false><<<static_cast<unsigned>(blocks), dim3(across, down), 0, s>>>(a);
+        }
     }));
     CountLaunch();
     return cudaGetLastError();

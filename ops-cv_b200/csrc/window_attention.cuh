@@ -9,8 +9,6 @@
 
 #include <cuda.h> // CUtensorMap
 
-#include <atomic>
-
 #include "launch_util.cuh"
 #include "sequence_kernels.h"
 
@@ -272,26 +270,5 @@ cudaError_t AttnForwardMma(Dt dt, const AttnArgs& a, cudaStream_t stream);
 uint64_t AttnBackwardMmaWorkspace(const AttnShape& s);
 cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStream_t stream);
 constexpr int kMmaMostDim = 128;
-
-// Asks once for each device for the shared memory (and clusters of more than 8 blocks) that a kernel takes: a call of the runtime that
-// costs as much as a launch. `asked` has a bit a device.
-template <typename Kernel>
-cudaError_t AskOnce(Kernel kernel, std::atomic<uint64_t>& asked, int shared, bool wideCluster = false)
-{
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    const uint64_t bit = 1ull << (device & 63);
-    if (e != cudaSuccess || (asked.load(std::memory_order_relaxed) & bit) != 0) {
-        return e;
-    }
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
-    if (e == cudaSuccess && wideCluster) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    }
-    if (e == cudaSuccess) {
-        asked.fetch_or(bit, std::memory_order_relaxed);
-    }
-    return e;
-}
 
 } // namespace opscv
