@@ -33,10 +33,10 @@ __device__ __forceinline__ int64_t TokenAt(int64_t token, int64_t inner, RowStri
 template <typename T, int V>
 struct Item {
     Pack<T, V> a, b;
-    __device__ __forceinline__ void Load(const T* p, int32_t at, int32_t second)
+    __device__ __forceinline__ void Load(const T* p, int32_t second, bool both)
     {
-        a = *reinterpret_cast<const Pack<T, V>*>(p + at);
-        if (second >= 0) {
+        a = *reinterpret_cast<const Pack<T, V>*>(p);
+        if (both) {
             b = *reinterpret_cast<const Pack<T, V>*>(p + second);
         }
     }
@@ -50,99 +50,129 @@ __device__ __forceinline__ void TurnPair(float& x, float& y, float2 cs)
     x = u;
 }
 
-// A block has a few tokens. Threads are (item of a head) x (pairs of a token and a head); a thread has up to kPairs of the latter at a
-// time, whose loads are all on their way while the block forms the sines and cosines.
-constexpr int kPairs = 5;
+// A block has a few tokens. Threads are (item of a head) x (heads) x (tokens); each has kHeads heads of kTokens tokens at a time: its
+// addresses serve all the tokens, and all its loads are on their way while the block forms the sines and cosines.
+constexpr int kHeads = 3;
+constexpr int kTokens = 2;
 
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(kThreads, INTER ? 4 : 3) RotaryKernel(const __grid_constant__ Args a)
+__global__ void __launch_bounds__(kThreads) RotaryKernel(const __grid_constant__ Args a)
 {
     __shared__ __align__(16) float2 table[kTable];
     const int32_t half = a.r.half;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * a.tokensPerBlock;
     const int32_t tokens = static_cast<int32_t>(min(static_cast<int64_t>(a.tokensPerBlock), a.r.tokens - first));
-    const int32_t threads = blockDim.x * blockDim.y;
+    const int32_t threads = blockDim.x * blockDim.y * blockDim.z;
     constexpr bool kNeighbours = INTER && V > 1; // pairs within an item
     const int32_t turned = kNeighbours ? 2 * half / V : half / V; // items of a head that are turned
     const int32_t items = turned + (a.r.dim - 2 * half) / V;
-    const int32_t heads = a.q.heads + a.k.heads, pairs = tokens * heads;
+    const int32_t heads = a.q.heads + a.k.heads;
     bool ready = false; // the table
+    // all threads of the block make the same turns of these loops
     for (int32_t item0 = 0; item0 < items; item0 += blockDim.x) {
         const int32_t item = item0 + threadIdx.x;
-        const bool inside = item < items, turn = item < turned;
+        const bool turn = item < turned;
         // the item's values, and those of the second half (interleaved single values: the pair's second)
         const int32_t at = !turn ? 2 * half + (item - turned) * V : INTER && V == 1 ? 2 * item : item * V;
         const int32_t second = !turn || kNeighbours ? -1 : INTER ? at + 1 : half + at;
-        for (int32_t p0 = 0; p0 < pairs; p0 += kPairs * blockDim.y) {
-            Item<T, V> x[kPairs];
+        for (int32_t h0 = 0; h0 < heads; h0 += kHeads * blockDim.y) {
+            int64_t in[kHeads], out[kHeads];
+            bool ofQ[kHeads], inside[kHeads];
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) {
-                const int32_t p = p0 + threadIdx.y + i * blockDim.y;
-                if (inside && p < pairs) {
-                    const int32_t t = p / heads, h = p - t * heads;
-                    const RotaryTensor& z = h < a.q.heads ? a.q : a.k;
-                    x[i].Load(static_cast<const T*>(z.in) + TokenAt(first + t, a.r.inner, z.inTok) + (h < a.q.heads ? h : h - a.q.heads) * z.inHead,
-                              at, second);
-                }
+            for (int i = 0; i < kHeads; ++i) {
+                const int32_t h = h0 + threadIdx.y + i * blockDim.y;
+                inside[i] = item < items && h < heads;
+                ofQ[i] = h < a.q.heads;
+                in[i] = (ofQ[i] ? h * a.q.inHead : (h - a.q.heads) * a.k.inHead) + at;
+                out[i] = (ofQ[i] ? h * a.q.outHead : (h - a.q.heads) * a.k.outHead) + at;
             }
-            if (!ready) { // all threads of the block come here first with the same loop state
-                ready = true;
-                for (int32_t e = threadIdx.y * blockDim.x + threadIdx.x; e < tokens * half; e += threads) {
-                    const int32_t t = e / half, i = e - t * half;
-                    int axis = 0;
-                    while (axis < a.r.axes - 1 && i >= a.r.ends[axis]) {
-                        ++axis;
-                    }
-                    const int64_t from = TokenAt(first + t, a.r.inner, a.r.posTok) + axis * a.r.posAxis;
-                    const double p = a.r.pos64 ? static_cast<double>(static_cast<const long long*>(a.positions)[from]) :
-                                                 static_cast<double>(static_cast<const int*>(a.positions)[from]);
-                    const double f = a.r.freq64 ? static_cast<const double*>(a.frequencies)[i] :
-                                                  static_cast<double>(static_cast<const float*>(a.frequencies)[i]);
-                    // In turns, p * f / (2 pi): the whole ones fall away, the rest keeps its leading bits in fp32. 1 / (2 pi) and the
-                    // products are sums of two doubles, so that positions of 10^12 and more, whose angle in one double is off by 10^-4,
-                    // keep theirs.
-                    constexpr double kHigh = 0.15915494309189535, kLow = -9.839338337591243e-18; // 1 / (2 pi)
-                    const double fHigh = f * kHigh, fLow = fma(f, kHigh, -fHigh) + f * kLow;
-                    const double high = p * fHigh, low = fma(p, fHigh, -high) + p * fLow;
-                    float sn, cs;
-                    sincospif(2.0f * static_cast<float>((high - rint(high)) + low), &sn, &cs);
-                    table[e] = make_float2(cs * a.r.scale, (a.r.inverse ? -sn : sn) * a.r.scale);
-                }
-                __syncthreads();
-            }
+            for (int32_t t0 = 0; t0 < tokens; t0 += kTokens * blockDim.z) {
+                Item<T, V> x[kTokens][kHeads];
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) {
-                const int32_t p = p0 + threadIdx.y + i * blockDim.y;
-                if (!inside || p >= pairs) {
-                    break;
-                }
-                const int32_t t = p / heads, h = p - t * heads;
-                const RotaryTensor& z = h < a.q.heads ? a.q : a.k;
-                T* out = static_cast<T*>(z.out) + TokenAt(first + t, a.r.inner, z.outTok) + (h < a.q.heads ? h : h - a.q.heads) * z.outHead;
-                if (!turn) {
-                    *reinterpret_cast<Pack<T, V>*>(out + at) = x[i].a;
-                    continue;
-                }
-                float u[V];
-                UnpackToF<T, V>(x[i].a, u);
-                if constexpr (kNeighbours) {
-                    const float2* row = table + t * half + item * (V / 2);
+                for (int y = 0; y < kTokens; ++y) {
+                    const int32_t t = t0 + threadIdx.z + y * blockDim.z;
+                    if (t < tokens) {
+                        const T* q = static_cast<const T*>(a.q.in) + TokenAt(first + t, a.r.inner, a.q.inTok);
+                        const T* k = static_cast<const T*>(a.k.in) + TokenAt(first + t, a.r.inner, a.k.inTok);
 #pragma unroll
-                    for (int e = 0; e < V / 2; ++e) {
-                        const float2 cs = row[e];
-                        TurnPair(u[2 * e], u[2 * e + 1], cs);
+                        for (int i = 0; i < kHeads; ++i) {
+                            if (inside[i]) {
+                                x[y][i].Load((ofQ[i] ? q : k) + in[i], second - at, second >= 0);
+                            }
+                        }
                     }
-                } else {
-                    const float2* row = table + t * half + item * V;
-                    float v[V];
-                    UnpackToF<T, V>(x[i].b, v);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        TurnPair(u[e], v[e], row[e]);
-                    }
-                    StorePack<T, V>(out + second, v);
                 }
-                StorePack<T, V>(out + at, u);
+                if (!ready) {
+                    ready = true;
+                    const int32_t me = (threadIdx.z * blockDim.y + threadIdx.y) * blockDim.x + threadIdx.x;
+                    for (int32_t e = me; e < tokens * half; e += threads) {
+                        const int32_t t = e / half, i = e - t * half;
+                        int axis = 0;
+                        while (axis < a.r.axes - 1 && i >= a.r.ends[axis]) {
+                            ++axis;
+                        }
+                        const int64_t from = TokenAt(first + t, a.r.inner, a.r.posTok) + axis * a.r.posAxis;
+                        const double p = a.r.pos64 ? static_cast<double>(static_cast<const long long*>(a.positions)[from]) :
+                                                     static_cast<double>(static_cast<const int*>(a.positions)[from]);
+                        const double f = a.r.freq64 ? static_cast<const double*>(a.frequencies)[i] :
+                                                      static_cast<double>(static_cast<const float*>(a.frequencies)[i]);
+                        // In turns, p * f / (2 pi): the whole ones fall away, the rest keeps its leading bits in fp32. 1 / (2 pi) and
+                        // the products are sums of two doubles, so that positions of 10^12 and more, whose angle in one double is off
+                        // by 10^-4, keep theirs.
+                        constexpr double kHigh = 0.15915494309189535, kLow = -9.839338337591243e-18; // 1 / (2 pi)
+                        const double fHigh = f * kHigh, fLow = fma(f, kHigh, -fHigh) + f * kLow;
+                        const double high = p * fHigh, low = fma(p, fHigh, -high) + p * fLow;
+                        float sn, cs;
+                        sincospif(2.0f * static_cast<float>((high - rint(high)) + low), &sn, &cs);
+                        table[e] = make_float2(cs * a.r.scale, (a.r.inverse ? -sn : sn) * a.r.scale);
+                    }
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int y = 0; y < kTokens; ++y) {
+                    const int32_t t = t0 + threadIdx.z + y * blockDim.z;
+                    if (t >= tokens) {
+                        break;
+                    }
+                    T* q = static_cast<T*>(a.q.out) + TokenAt(first + t, a.r.inner, a.q.outTok);
+                    T* k = static_cast<T*>(a.k.out) + TokenAt(first + t, a.r.inner, a.k.outTok);
+                    float2 cs[kNeighbours ? V / 2 : V];
+                    if (turn) {
+                        const float2* row = table + t * half + item * (kNeighbours ? V / 2 : V);
+#pragma unroll
+                        for (int e = 0; e < (kNeighbours ? V / 2 : V); ++e) {
+                            cs[e] = row[e];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < kHeads; ++i) {
+                        if (!inside[i]) {
+                            break;
+                        }
+                        T* to = (ofQ[i] ? q : k) + out[i];
+                        if (!turn) {
+                            *reinterpret_cast<Pack<T, V>*>(to) = x[y][i].a;
+                            continue;
+                        }
+                        float u[V];
+                        UnpackToF<T, V>(x[y][i].a, u);
+                        if constexpr (kNeighbours) {
+#pragma unroll
+                            for (int e = 0; e < V / 2; ++e) {
+                                TurnPair(u[2 * e], u[2 * e + 1], cs[e]);
+                            }
+                        } else {
+                            float v[V];
+                            UnpackToF<T, V>(x[y][i].b, v);
+#pragma unroll
+                            for (int e = 0; e < V; ++e) {
+                                TurnPair(u[e], v[e], cs[e]);
+                            }
+                            StorePack<T, V>(to + (second - at), v);
+                        }
+                        StorePack<T, V>(to, u);
+                    }
+                }
             }
         }
     }
@@ -226,27 +256,33 @@ cudaError_t RotaryTurn(Dt dt, const RotaryShape& r, const RotaryTensor& q, const
     a.k = k;
     a.positions = positions;
     a.frequencies = frequencies;
-    // Threads: the items of a head by as many (token, head) pairs as make up to 256. Tokens: as many as the threads take at a time,
-    // but at least some blocks for each SM, and no more than the table holds.
+    // Threads: the items of a head by the heads, kHeads to each, by as many tokens as make up to 256. Tokens: as many as the threads take
+    // at a time, but at least some blocks for each SM, and no more than the table holds.
     const int32_t turned = r.interleaved && v > 1 ? 2 * r.half / v : r.half / v, items = turned + (r.dim - 2 * r.half) / v;
     const int32_t heads = q.heads + k.heads;
-    const int32_t across = items < kThreads ? items : kThreads, down = kThreads / across;
-    int64_t t = static_cast<int64_t>(kPairs) * down / heads;
+    const int32_t across = items < kThreads ? items : kThreads;
+    int32_t down = static_cast<int32_t>(CeilDiv(heads, kHeads));
+    down = down < kThreads / across ? down : kThreads / across;
+    int32_t deep = kThreads / (across * down);
+    int64_t t = static_cast<int64_t>(kTokens) * deep;
     const int64_t spread = CeilDiv(r.tokens, static_cast<int64_t>(NumSMs()) * 4);
     t = t < spread ? t : spread;
     const int64_t room = kTable / (r.half < 1 ? 1 : r.half);
     t = t < room ? t : room;
     t = t < 1 ? 1 : t;
     a.tokensPerBlock = static_cast<int32_t>(t);
+    deep = deep < t ? deep : static_cast<int32_t>(t);
+    deep = deep < 64 ? deep : 64; // a block's limit
+    const dim3 block(across, down, deep);
     const int64_t blocks = CeilDiv(r.tokens, t);
     if (blocks > INT32_MAX) {
         return cudaErrorInvalidConfiguration;
     }
     OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
         if (r.interleaved) {
-            RotaryKernel<T, V, true><<<static_cast<unsigned>(blocks), dim3(across, down), 0, s>>>(a);
+            RotaryKernel<T, V, true><<<static_cast<unsigned>(blocks), block, 0, s>>>(a);
         } else {
-            RotaryKernel<T, V, false><<<static_cast<unsigned>(blocks), dim3(across, down), 0, s>>>(a);
+            RotaryKernel<T, V, false><<<static_cast<unsigned>(blocks), block, 0, s>>>(a);
         }
     }));
     CountLaunch();
