@@ -47,19 +47,85 @@ __device__ __forceinline__ int32_t StepKey(const KeySteps& r, int32_t n)
 // Bits 0 to n - 1 of a word, n cut to [0, 32].
 __device__ __forceinline__ uint32_t Below(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
+constexpr int kRowThreads = 256; // two threads a row of a tile
+__device__ __forceinline__ void RowBarrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// columns of an accumulator times a factor a row
+template <int N>
+__device__ __forceinline__ void TmemScale(uint32_t addr, float f)
+{
+#pragma unroll 1
+    for (int c = 0; c < N; c += 8) {
+        uint32_t o[8];
+        TmemLoad8(addr + c, o);
+        TmemLoadWait();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+        }
+        TmemStore8(addr + c, o);
+    }
+    TmemStoreWait();
+}
+
+// 32 values of a row of an output, of which `left` exist
+template <typename T>
+__device__ __forceinline__ void StoreRow32(T* out, const float (&v)[32], int32_t left, bool vec)
+{
+    if (vec) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+            if (e < left) {
+                float w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    w[k] = v[e + k];
+                }
+                StorePack<T, 8>(out + e, w);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            if (e < left) {
+                out[e] = DType<T>::FromF(v[e]);
+            }
+        }
+    }
+}
+
+// -infinity where a column's bit is not set
+template <int N>
+__device__ __forceinline__ void MaskColumns(uint32_t* x, const uint32_t (&live)[N / 32])
+{
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        x[e] = (live[e >> 5] >> (e & 31) & 1) != 0 ? x[e] : 0xff800000u;
+    }
+}
+// the columns [from, to) and [0, sinkTo) of N
+template <int N>
+__device__ __forceinline__ void LiveColumns(uint32_t (&live)[N / 32], int32_t from, int32_t to, int32_t sinkTo)
+{
+#pragma unroll
+    for (int w = 0; w < N / 32; ++w) {
+        live[w] = (Below(to - 32 * w) & ~Below(from - 32 * w)) | Below(sinkTo - 32 * w);
+    }
+}
+
 // ---- forward -----------------------------------------------------------------------------------------------------------------
-// A block has 128 queries of a head. Warp 4's first thread loads the tiles and issues the products; warps 0 to 3 have a query a
-// thread: S = Q K^T arrives in tensor memory, the thread forms the weights of its row, writes them over S as 16-bit values, and
-// O += P V takes them from there, so that neither S nor P touches shared memory. Two blocks share an SM (256 columns of tensor memory
-// and 97 KB each): while one forms its weights, the other's products run.
+// A block has 128 queries of a head. Warp 8's first thread loads the tiles and issues the products; warps 0 to 7 have two threads a
+// query, of 64 columns each: S = Q K^T arrives in tensor memory, the threads agree on the row's maximum, form the weights, write them
+// over S as 16-bit values, and O += P V takes them from there, so that neither S nor P touches shared memory. Two blocks share an SM
+// (256 columns of tensor memory and 99 KB each): while one forms its weights, the other's products run.
 struct ForwardShared {
-    uint64_t qFull, kFull, vFull, sFull, pFull, oFull, drain;
-    uint32_t tmem;
-    uint32_t failed;
+    uint64_t qFull, kFull, vFull, sFull, pFull, oFull, drain, exchanged[4];
+    uint32_t tmem, failed, bad[4];
+    float row[2][2][kTile]; // maxima of even and odd steps (and the sums, at the end) of a row's two threads
 };
 
 template <typename T, int HALVES>
-__global__ void __launch_bounds__(160, 2)
+__global__ void __launch_bounds__(288, 2)
     AttnForwardMmaKernel(const __grid_constant__ MmaArgs m, const __grid_constant__ CUtensorMap mapQ,
                          const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV)
 {
@@ -69,7 +135,7 @@ __global__ void __launch_bounds__(160, 2)
     unsigned char* base = raw + (1024 - (SharedAddr(raw) & 1023)) % 1024;
     unsigned char *sq = base, *sk = base + kBytes, *sv = base + 2 * kBytes;
     const AttnShape& s = m.a.s;
-    const int32_t tile = blockIdx.x % m.tiles;
+    const int32_t tile = m.tiles - 1 - static_cast<int32_t>(blockIdx.x % m.tiles); // the tiles that see most keys first
     const int32_t bh = blockIdx.x / m.tiles;
     const int32_t b = bh / s.heads, h = bh % s.heads;
     const Lengths n = LengthsOf(s, b);
@@ -84,12 +150,16 @@ __global__ void __launch_bounds__(160, 2)
         BarInit(&sh.kFull, 1);
         BarInit(&sh.vFull, 1);
         BarInit(&sh.sFull, 1);
-        BarInit(&sh.pFull, 128);
+        BarInit(&sh.pFull, kRowThreads);
         BarInit(&sh.oFull, 1);
         BarInit(&sh.drain, 1);
+        for (int e = 0; e < 4; ++e) {
+            BarInit(&sh.exchanged[e], 64);
+            sh.bad[e] = 0;
+        }
         BarInitDone();
     }
-    if (warp == 4) {
+    if (warp == 8) {
         TmemAlloc(&sh.tmem, 256);
     }
     TcFenceBefore();
@@ -99,7 +169,7 @@ __global__ void __launch_bounds__(160, 2)
     const uint32_t tS = tmem, tO = tmem + 128;
     volatile uint32_t* failed = &sh.failed;
 
-    if (warp == 4) {
+    if (warp == 8) {
         if ((threadIdx.x & 31) == 0 && steps.steps > 0) {
             const int32_t u = h / m.a.group;
             auto load = [&](unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int32_t row, int32_t head) {
@@ -121,9 +191,12 @@ __global__ void __launch_bounds__(160, 2)
                 const uint32_t phase = it & 1;
                 BarWait(&sh.kFull, phase, failed);
                 TcFenceAfter();
-                for (int32_t k = 0; k < kSteps; ++k) {
-                    const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
-                    MmaShared(tS, OperandDesc(aq + off, 16), OperandDesc(ak + off, 16), descS, k > 0);
+#pragma unroll
+                for (int32_t k = 0; k < 4 * HALVES; ++k) {
+                    if (k < kSteps) {
+                        const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
+                        MmaShared(tS, OperandDesc(aq + off, 16), OperandDesc(ak + off, 16), descS, k > 0);
+                    }
                 }
                 MmaCommit(&sh.sFull);
                 BarWait(&sh.sFull, phase, failed);
@@ -148,7 +221,7 @@ __global__ void __launch_bounds__(160, 2)
                 TcFenceAfter();
 #pragma unroll
                 for (int32_t k = 0; k < kTile / 16; ++k) {
-                    MmaTmem(tO, tS + 8 * k, OperandDesc(av + k * 2048, kHalfBytes), descO, it > 0 || k > 0);
+                    MmaTmem(tO, tS + (k >> 2) * 64 + (k & 3) * 8, OperandDesc(av + k * 2048, kHalfBytes), descO, it > 0 || k > 0);
                 }
                 MmaCommit(&sh.oFull);
                 BarWait(&sh.oFull, phase, failed);
@@ -163,52 +236,49 @@ __global__ void __launch_bounds__(160, 2)
         }
         __syncwarp();
     } else {
-        const int32_t i = i0 + threadIdx.x;
+        const int32_t side = warp >> 2, quad = warp & 3, r = quad * 32 + (threadIdx.x & 31);
+        const int32_t i = i0 + r;
         const int32_t p = i <= iLast ? n.shift + i : -1;
         const Seen seen = SeenOf(s, p);
-        const uint32_t lanes = static_cast<uint32_t>(warp) << 21; // 32 warp, in the lane half of an address
+        const uint32_t lanes = static_cast<uint32_t>(quad) << 21; // 32 quad, in the lane half of an address
+        const uint32_t tx = tS + 64 * side + lanes, to32 = tO + 32 * HALVES * side + lanes;
         const float factor = fabsf(s.scale) * kLog2e;             // scores in powers of two
-        const int32_t wLow = low + 32 * warp, wHigh = wLow + 31;
+        const int32_t wLow = low + 32 * quad, wHigh = wLow + 31;
+        const bool rowsWhole = i0 + 32 * quad + 31 <= iLast;
         float top = -INFINITY, total = 0.0f;
         for (int32_t it = 0; it < steps.steps; ++it) {
-            const int32_t j0 = StepKey(steps, it);
+            const int32_t j0 = StepKey(steps, it) + 64 * side;
             BarWait(&sh.sFull, it & 1, failed);
             if (__any_sync(0xffffffffu, *failed != 0)) {
                 break;
             }
             TcFenceAfter();
-            uint32_t x[kTile];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                TmemLoad32(tS + lanes + 32 * c, x + 32 * c);
-            }
+            uint32_t x[64];
+            TmemLoad32(tx, x);
+            TmemLoad32(tx + 32, x + 32);
             TmemLoadWait();
-            const bool whole = it >= steps.sinkSteps && j0 + kTile - 1 <= wLow && j0 > wHigh - s.window && i0 + 32 * warp + 31 <= iLast;
-            if (!whole) {
-                // visible columns of the step: those of the window, or those of the sinks. A window step may hold sinks as well:
-                // those behind the block's first key, in front of the row's window.
-                const bool sinkStep = it < steps.sinkSteps;
-                const int32_t from = sinkStep ? 0 : seen.first - j0;
-                const int32_t to = p < 0 ? 0 : sinkStep ? steps.sinkEnd - j0 : p - j0 + 1;
-                const int32_t sinkTo = sinkStep ? 0 : seen.sinkEnd - j0;
-#pragma unroll
-                for (int c = 0; c < kTile; c += 32) {
-                    const uint32_t live = (Below(to - c) & ~Below(from - c)) | Below(sinkTo - c);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        x[c + e] = (live >> e & 1) != 0 ? x[c + e] : 0xff800000u;
-                    }
-                }
+            const bool sinkStep = it < steps.sinkSteps;
+            if (sinkStep || !rowsWhole || j0 + 63 > wLow || j0 <= wHigh - s.window) {
+                // Visible columns of the step: those of the window, or those of the sinks. A window step may hold sinks as well: those
+                // behind the block's first key, in front of the row's window.
+                uint32_t live[2];
+                LiveColumns<64>(live, sinkStep ? 0 : seen.first - j0, p < 0 ? 0 : sinkStep ? steps.sinkEnd - j0 : p - j0 + 1,
+                                sinkStep ? 0 : seen.sinkEnd - j0);
+                MaskColumns<64>(x, live);
             }
             float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < kTile; c += 8) {
+            for (int c = 0; c < 64; c += 8) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     part[e] = fmaxf(fmaxf(part[e], __uint_as_float(x[c + 2 * e])), __uint_as_float(x[c + 2 * e + 1]));
                 }
             }
-            const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * factor;
+            float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * factor;
+            sh.row[it & 1][side][r] = most;
+            BarArrive(&sh.exchanged[quad]);
+            BarWait(&sh.exchanged[quad], it & 1, failed);
+            most = fmaxf(most, sh.row[it & 1][side ^ 1][r]);
             const float grown = fmaxf(top, most);
             const bool grow = grown > top + kGrowth; // always from -infinity to a number
             if (it == 0) {
@@ -217,23 +287,13 @@ __global__ void __launch_bounds__(160, 2)
                 const float fade = grow ? Exp2(top - grown) : 1.0f;
                 top = grow ? grown : top;
                 total *= fade;
-#pragma unroll 1
-                for (int c = 0; c < 8 * HALVES; ++c) {
-                    uint32_t o[8];
-                    TmemLoad8(tO + lanes + 8 * c, o);
-                    TmemLoadWait();
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
-                    }
-                    TmemStore8(tO + lanes + 8 * c, o);
-                }
+                TmemScale<32 * HALVES>(to32, fade);
             }
             const float off = top == -INFINITY ? 0.0f : -top;
             const F2 factor2 = MakeF2(factor, factor), off2 = MakeF2(off, off);
             F2 sum2[2] = {MakeF2(0.0f, 0.0f), MakeF2(0.0f, 0.0f)};
 #pragma unroll
-            for (int c = 0; c < kTile; c += 32) {
+            for (int c = 0; c < 64; c += 32) {
                 uint32_t w[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -245,74 +305,61 @@ __global__ void __launch_bounds__(160, 2)
                     sum2[e & 1] = Add2(sum2[e & 1], MakeF2(e0, e1));
                     w[e] = PackPair(e0, e1, static_cast<const T*>(nullptr));
                 }
-                TmemStore16(tS + lanes + c / 2, w);
+                TmemStore16(tx + c / 2, w);
             }
-            float a0, a1;
-            SplitF2(Add2(sum2[0], sum2[1]), a0, a1);
-            total += a0 + a1;
             TmemStoreWait();
             TcFenceBefore();
             BarArrive(&sh.pFull);
+            float a0, a1;
+            SplitF2(Add2(sum2[0], sum2[1]), a0, a1);
+            total += a0 + a1;
         }
         // ---- the rows of out
         if (steps.steps > 0) {
             BarWait(&sh.oFull, (steps.steps - 1) & 1, failed);
             TcFenceAfter();
         }
+        RowBarrier(); // the last maxima have been read
+        sh.row[0][side][r] = total;
+        RowBarrier();
+        total = sh.row[0][0][r] + sh.row[0][1][r];
         const float inverse = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total; // NaN stays
         bool bad = seen.count > 0 && !(total > 0.0f && total <= 3.0e38f);
         T* out = i < s.lq ? OutRowOf<T>(m.a.out, b, i, h) : nullptr;
 #pragma unroll
-        for (int c = 0; c < 2 * HALVES; ++c) {
+        for (int c = 0; c < HALVES; ++c) {
+            const int32_t d0 = 32 * (HALVES * side + c);
             uint32_t o[32];
             if (steps.steps > 0) {
-                TmemLoad32(tO + lanes + 32 * c, o);
+                TmemLoad32(to32 + 32 * c, o);
                 TmemLoadWait();
             }
-            if (32 * c < s.dim) {
+            float v[32];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const float v = seen.count > 0 ? __uint_as_float(o[e]) * inverse : 0.0f;
-                    bad = bad || (32 * c + e < s.dim && !(fabsf(v) <= 3.4e38f));
-                    o[e] = __float_as_uint(v);
-                }
-                if (out != nullptr) {
-                    if (m.vecOut) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            if (32 * c + e < s.dim) {
-                                float v[8];
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) {
-                                    v[k] = __uint_as_float(o[e + k]);
-                                }
-                                StorePack<T, 8>(out + 32 * c + e, v);
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            if (32 * c + e < s.dim) {
-                                out[32 * c + e] = DType<T>::FromF(__uint_as_float(o[e]));
-                            }
-                        }
-                    }
-                }
+            for (int e = 0; e < 32; ++e) {
+                v[e] = seen.count > 0 ? __uint_as_float(o[e]) * inverse : 0.0f;
+                bad = bad || (d0 + e < s.dim && !(fabsf(v[e]) <= 3.4e38f));
+            }
+            if (out != nullptr && d0 < s.dim) {
+                StoreRow32<T>(out + d0, v, s.dim - d0, m.vecOut);
             }
         }
-        if (out != nullptr && m.a.lse != nullptr) {
+        if (out != nullptr && m.a.lse != nullptr && side == 0) {
             m.a.lse[(static_cast<int64_t>(b) * s.heads + h) * s.lq + i] = seen.count > 0 ? (top + log2f(total)) * kLn2 : -INFINITY;
         }
-        // rows that are not finite again, without the masked keys' part
-        uint32_t rows = __ballot_sync(0xffffffffu, bad && out != nullptr);
-        __syncwarp();
-        while (rows != 0) {
-            const int r = __ffs(rows) - 1;
-            rows &= rows - 1;
-            AttnForwardRow<T>(m.a, b, h, i0 + 32 * warp + r);
+        const uint32_t rows = __ballot_sync(0xffffffffu, bad && out != nullptr);
+        if ((threadIdx.x & 31) == 0 && rows != 0) {
+            atomicOr(&sh.bad[quad], rows);
         }
-        __syncwarp();
-        if (*failed != 0 && out != nullptr) {
+        RowBarrier();
+        // rows that are not finite again, without the masked keys' part: the even ones by one warp, the odd ones by another
+        uint32_t again = sh.bad[quad] & (side == 0 ? 0x55555555u : 0xaaaaaaaau);
+        while (again != 0) {
+            const int e = __ffs(again) - 1;
+            again &= again - 1;
+            AttnForwardRow<T>(m.a, b, h, i0 + 32 * quad + e);
+        }
+        if (*failed != 0 && out != nullptr && side == 0) {
             for (int32_t d = 0; d < s.dim; ++d) {
                 out[d] = DType<T>::FromF(NAN);
             }
@@ -320,7 +367,7 @@ __global__ void __launch_bounds__(160, 2)
     }
     TcFenceBefore();
     __syncthreads();
-    if (warp == 4) {
+    if (warp == 8) {
         TcFenceAfter();
         TmemFree(tmem, 256);
     }
@@ -337,8 +384,6 @@ __global__ void __launch_bounds__(160, 2)
 // the products. The weights are scaled by 2^8 (folded into the statistics), which keeps small ones out of fp16's subnormal range.
 constexpr float kWeightShift = 8.0f;
 constexpr float kWeightScale = 0.00390625f; // 2^-8
-constexpr int kRowThreads = 256;
-
 struct BackwardArgs {
     AttnArgs a;
     int32_t qTiles, kTiles;
@@ -350,8 +395,6 @@ struct BackwardArgs {
     float* partial;
     bool vecQ, vecK, vecV;
 };
-
-__device__ __forceinline__ void RowBarrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // delta and lse2 of a row by 16 lanes
 template <typename T>
@@ -423,60 +466,6 @@ struct RowScale {
     }
 };
 __device__ __forceinline__ uint32_t ExponentOf(float positive) { return __float_as_uint(positive) >> 23; }
-
-// columns of an accumulator times a factor a row
-template <int N>
-__device__ __forceinline__ void TmemScale(uint32_t addr, float f)
-{
-#pragma unroll 1
-    for (int c = 0; c < N; c += 8) {
-        uint32_t o[8];
-        TmemLoad8(addr + c, o);
-        TmemLoadWait();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-        }
-        TmemStore8(addr + c, o);
-    }
-    TmemStoreWait();
-}
-
-// 32 values of a row of an output, of which `left` exist
-template <typename T>
-__device__ __forceinline__ void StoreRow32(T* out, const float (&v)[32], int32_t left, bool vec)
-{
-    if (vec) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-            if (e < left) {
-                float w[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    w[k] = v[e + k];
-                }
-                StorePack<T, 8>(out + e, w);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            if (e < left) {
-                out[e] = DType<T>::FromF(v[e]);
-            }
-        }
-    }
-}
-
-// the weights of 64 columns, 0 in masked ones: exp2(factor s - lse2)
-__device__ __forceinline__ void MaskColumns(uint32_t (&x)[64], uint32_t live0, uint32_t live1)
-{
-#pragma unroll
-    for (int e = 0; e < 32; ++e) {
-        x[e] = (live0 >> e & 1) != 0 ? x[e] : 0xff800000u;
-        x[32 + e] = (live1 >> e & 1) != 0 ? x[32 + e] : 0xff800000u;
-    }
-}
 
 struct GradQShared {
     uint64_t qFull, kFull[3], kEmpty[3], vFull[2], vEmpty[2], sFull[2], dpFull, dsReady, dqDone, allDone, exchanged, drain;
@@ -666,7 +655,9 @@ __global__ void __launch_bounds__(320, 1)
                 const int32_t to = p < 0 ? 0 : sinkStep ? steps.sinkEnd - j0 : p - j0 + 1;
                 const int32_t sinkTo = sinkStep ? 0 : seen.sinkEnd - j0;
                 if (!__all_sync(0xffffffffu, from <= 0 && to >= 64)) {
-                    MaskColumns(x, (Below(to) & ~Below(from)) | Below(sinkTo), (Below(to - 32) & ~Below(from - 32)) | Below(sinkTo - 32));
+                    uint32_t live[2];
+                    LiveColumns<64>(live, from, to, sinkTo);
+                    MaskColumns<64>(x, live);
                 }
             }
 #pragma unroll
@@ -976,7 +967,9 @@ __global__ void __launch_bounds__(320, 1)
             TmemLoad32(tS + 64 * side + lanes + 32, x + 32);
             TmemLoadWait();
             if (!__all_sync(0xffffffffu, from <= p0 && to >= p0 + 64)) {
-                MaskColumns(x, Below(to - p0) & ~Below(from - p0), Below(to - p0 - 32) & ~Below(from - p0 - 32));
+                uint32_t live[2];
+                LiveColumns<64>(live, from - p0, to - p0, 0);
+                MaskColumns<64>(x, live);
             }
             const float4* lse = reinterpret_cast<const float4*>(stats + st * 2 * kTile + 64 * side);
             const float4* del = reinterpret_cast<const float4*>(stats + st * 2 * kTile + kTile + 64 * side);
@@ -1228,7 +1221,7 @@ cudaError_t AttnForwardMma(Dt dt, const AttnArgs& a, cudaStream_t stream)
         if (set != cudaSuccess) {
             return set;
         }
-        kernel<<<grid, 160, shared, stream>>>(m, mq, mk, mv);
+        kernel<<<grid, 288, shared, stream>>>(m, mq, mk, mv);
         CountLaunch();
         return cudaGetLastError();
     };
