@@ -8,7 +8,7 @@ namespace {
 
 __device__ unsigned int g_attentionTimeouts = 0;
 
-constexpr int kTile = 128;                        // queries of a block, keys of a step
+constexpr int kTile = 128;                        // rows of a tile
 constexpr uint32_t kHalfBytes = kTile * 128;      // 64 of the up to 128 values of 128 rows
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // The running maximum stays as it is while the scores outgrow it by no more than a factor of 2^8: weights up to 2^8 lose nothing in
@@ -22,27 +22,23 @@ struct MmaArgs {
     bool vecOut;    // rows of out can be written 16 bytes at a time
 };
 
-// The steps over keys of a block whose queries sit at [low, high]: first the sinks in front of the window, in steps from key 0,
-// then the window, in steps from its first key (TMA boxes may start anywhere along the tokens).
+// The steps of KEYS keys over those of a block whose queries sit at [low, high]: first the sinks in front of the window, in steps from
+// key 0, then the window, in steps from its first key (TMA boxes may start anywhere along the tokens).
+template <int KEYS>
 struct KeySteps {
-    int32_t sinkEnd, first, sinkSteps, steps;
-};
-__device__ __forceinline__ KeySteps StepsOf(const AttnShape& s, int32_t low, int32_t high)
-{
-    KeySteps r{0, 0, 0, 0};
-    if (high >= 0) {
-        low = low > 0 ? low : 0;
-        r.first = low >= s.window ? low - s.window + 1 : 0;
-        r.sinkEnd = s.sinks < r.first ? s.sinks : r.first;
-        r.sinkSteps = (r.sinkEnd + kTile - 1) / kTile;
-        r.steps = r.sinkSteps + (high - r.first + kTile) / kTile;
+    int32_t sinkEnd = 0, first = 0, sinkSteps = 0, steps = 0;
+    __device__ __forceinline__ KeySteps(const AttnShape& s, int32_t low, int32_t high)
+    {
+        if (high >= 0) {
+            low = low > 0 ? low : 0;
+            first = low >= s.window ? low - s.window + 1 : 0;
+            sinkEnd = s.sinks < first ? s.sinks : first;
+            sinkSteps = (sinkEnd + KEYS - 1) / KEYS;
+            steps = sinkSteps + (high - first + KEYS) / KEYS;
+        }
     }
-    return r;
-}
-__device__ __forceinline__ int32_t StepKey(const KeySteps& r, int32_t n)
-{
-    return n < r.sinkSteps ? n * kTile : r.first + (n - r.sinkSteps) * kTile;
-}
+    __device__ __forceinline__ int32_t Key(int32_t n) const { return n < sinkSteps ? n * KEYS : first + (n - sinkSteps) * KEYS; }
+};
 
 // Bits 0 to n - 1 of a word, n cut to [0, 32].
 __device__ __forceinline__ uint32_t Below(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
@@ -58,7 +54,6 @@ __device__ __forceinline__ void TmemScale(uint32_t addr, float f)
     for (int c = 0; c < N; c += 8) {
         uint32_t o[8];
         TmemLoad8(addr + c, o);
-        TmemLoadWait();
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
@@ -114,26 +109,36 @@ __device__ __forceinline__ void LiveColumns(uint32_t (&live)[N / 32], int32_t fr
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
-// A block has 128 queries of a head. Warp 8's first thread loads the tiles and issues the products; warps 0 to 7 have two threads a
-// query, of 64 columns each: S = Q K^T arrives in tensor memory, the threads agree on the row's maximum, form the weights, write them
-// over S as 16-bit values, and O += P V takes them from there, so that neither S nor P touches shared memory. Two blocks share an SM
-// (256 columns of tensor memory and 99 KB each): while one forms its weights, the other's products run.
+// A block has 128 queries of a head and walks its keys 64 at a time. Warp 8's first thread loads the tiles, warp 9's issues the products;
+// warps 0 to 7 have two threads a query, of 32 columns each: S = Q K^T arrives in tensor memory, the threads form the weights, write
+// them over S as 16-bit values, and O += P V takes them from there, so that neither S nor P touches shared memory. S has two places
+// (O, at most 128 columns, and twice 64), so the next step's scores are there when the threads come to them, and the products, their
+// latency and the copies stay out of the chain of the exponentials, which bound the rest. Two blocks share an SM (256 columns of tensor
+// memory, 97 KB of shared memory and 320 threads each).
+//
+// A row's weights are formed from the maximum of the steps before while the row's two threads exchange the maxima of this one; only
+// where a row has outgrown its old maximum by 2^8 (at the start, mostly) are they formed again and O rescaled.
+constexpr int kKeys = 64;
+constexpr uint32_t kKeyHalf = kKeys * 128;
+
 struct ForwardShared {
-    uint64_t qFull, kFull, vFull, sFull, pFull, oFull, drain, exchanged[4];
+    uint64_t qFull, kFull[2], vFull[2], sFull[2], pFull[2], pvDone[2], allDone, drain, exchanged[4];
     uint32_t tmem, failed, bad[4];
     float row[2][2][kTile]; // maxima of even and odd steps (and the sums, at the end) of a row's two threads
 };
 
-template <typename T, int HALVES>
-__global__ void __launch_bounds__(288, 2)
+// KS: steps of 16 values of a head.
+template <typename T, int KS>
+__global__ void __launch_bounds__(320, 2)
     AttnForwardMmaKernel(const __grid_constant__ MmaArgs m, const __grid_constant__ CUtensorMap mapQ,
                          const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV)
 {
     extern __shared__ unsigned char raw[];
     __shared__ ForwardShared sh;
-    constexpr uint32_t kBytes = HALVES * kHalfBytes;
+    constexpr int HALVES = KS > 4 ? 2 : 1;
+    constexpr uint32_t kBytes = HALVES * kHalfBytes, kKeyBytes = HALVES * kKeyHalf;
     unsigned char* base = raw + (1024 - (SharedAddr(raw) & 1023)) % 1024;
-    unsigned char *sq = base, *sk = base + kBytes, *sv = base + 2 * kBytes;
+    unsigned char *sq = base, *sk = base + kBytes, *sv = sk + 2 * kKeyBytes;
     const AttnShape& s = m.a.s;
     const int32_t tile = m.tiles - 1 - static_cast<int32_t>(blockIdx.x % m.tiles); // the tiles that see most keys first
     const int32_t bh = blockIdx.x / m.tiles;
@@ -142,16 +147,20 @@ __global__ void __launch_bounds__(288, 2)
     const int32_t i0 = tile * kTile;
     const int32_t iLast = min(i0 + kTile, n.q) - 1; // of the queries that count
     const int32_t low = n.shift + i0, high = iLast >= i0 ? n.shift + iLast : -1;
-    const KeySteps steps = StepsOf(s, low, high);
+    const KeySteps<kKeys> steps(s, low, high);
+    const int32_t count = steps.steps;
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         sh.failed = 0;
         BarInit(&sh.qFull, 1);
-        BarInit(&sh.kFull, 1);
-        BarInit(&sh.vFull, 1);
-        BarInit(&sh.sFull, 1);
-        BarInit(&sh.pFull, kRowThreads);
-        BarInit(&sh.oFull, 1);
+        for (int e = 0; e < 2; ++e) {
+            BarInit(&sh.kFull[e], 1);
+            BarInit(&sh.vFull[e], 1);
+            BarInit(&sh.sFull[e], 1);
+            BarInit(&sh.pFull[e], kRowThreads);
+            BarInit(&sh.pvDone[e], 1);
+        }
+        BarInit(&sh.allDone, 1);
         BarInit(&sh.drain, 1);
         for (int e = 0; e < 4; ++e) {
             BarInit(&sh.exchanged[e], 64);
@@ -159,78 +168,120 @@ __global__ void __launch_bounds__(288, 2)
         }
         BarInitDone();
     }
-    if (warp == 8) {
+    if (warp == 9) {
         TmemAlloc(&sh.tmem, 256);
     }
     TcFenceBefore();
     __syncthreads();
     TcFenceAfter();
-    const uint32_t tmem = sh.tmem;
-    const uint32_t tS = tmem, tO = tmem + 128;
+    const uint32_t tO = sh.tmem, tS = tO + 128; // S of even steps at 0 and of odd ones at 64 from there
     volatile uint32_t* failed = &sh.failed;
 
     if (warp == 8) {
-        if ((threadIdx.x & 31) == 0 && steps.steps > 0) {
+        if ((threadIdx.x & 31) == 0 && count > 0) {
             const int32_t u = h / m.a.group;
-            auto load = [&](unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int32_t row, int32_t head) {
-                BarExpect(bar, kBytes);
+            BarExpect(&sh.qFull, kBytes);
+#pragma unroll
+            for (int c = 0; c < HALVES; ++c) {
+                TmaLoad4(sq + c * kHalfBytes, &mapQ, &sh.qFull, 64 * c, i0, h, b);
+            }
+            auto load = [&](unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int32_t row) {
+                BarExpect(bar, kKeyBytes);
 #pragma unroll
                 for (int c = 0; c < HALVES; ++c) {
-                    TmaLoad4(dst + c * kHalfBytes, map, bar, 64 * c, row, head, b);
+                    TmaLoad4(dst + c * kKeyHalf, map, bar, 64 * c, row, u, b);
                 }
             };
-            load(sq, &mapQ, &sh.qFull, i0, h);
-            load(sk, &mapK, &sh.kFull, StepKey(steps, 0), u);
-            load(sv, &mapV, &sh.vFull, StepKey(steps, 0), u);
-            const int32_t kSteps = (s.dim + 15) / 16;
-            const uint32_t descS = ProductDesc<T>(kTile, false, s.scale < 0.0f);
-            const uint32_t descO = ProductDesc<T>(kSteps * 16, true, false);
-            const uint32_t aq = SharedAddr(sq), ak = SharedAddr(sk), av = SharedAddr(sv);
+            int32_t ks = 0, vs = 0; // loads so far
+            for (int32_t it = 0; it < count; ++it) {
+                const int32_t st = it & 1, j0 = steps.Key(it);
+                if (it >= 2) {
+                    BarWait(&sh.sFull[st], (it / 2 - 1) & 1, failed); // the scores that read the place before
+                }
+                if (*failed != 0) {
+                    break;
+                }
+                load(sk + st * kKeyBytes, &mapK, &sh.kFull[st], j0);
+                ++ks;
+                if (it >= 2) {
+                    BarWait(&sh.pvDone[st], (it / 2 - 1) & 1, failed);
+                }
+                if (*failed != 0) {
+                    break;
+                }
+                load(sv + st * kKeyBytes, &mapV, &sh.vFull[st], j0);
+                ++vs;
+            }
+            // own copies end before the block does, whatever became of the others
+            BarDrain(&sh.qFull, 0);
+            for (int32_t e = ks > 2 ? ks - 2 : 0; e < ks; ++e) {
+                BarDrain(&sh.kFull[e & 1], (e / 2) & 1);
+            }
+            for (int32_t e = vs > 2 ? vs - 2 : 0; e < vs; ++e) {
+                BarDrain(&sh.vFull[e & 1], (e / 2) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if (count > 0) {
+            const bool lead = ElectOne();
+            const uint32_t descS = ProductDesc<T>(kKeys, false, s.scale < 0.0f);
+            const uint32_t descO = ProductDesc<T>(KS * 16, true, false);
+            const uint64_t dq = OperandDesc(SharedAddr(sq), 16), dk = OperandDesc(SharedAddr(sk), 16), dv = OperandDesc(SharedAddr(sv), kKeyHalf);
+            // a descriptor's address is in units of 16 bytes
+            auto scores = [&](int32_t st) {
+                if (lead) {
+                    const uint64_t k0 = dk + st * (kKeyBytes >> 4);
+#pragma unroll
+                    for (int32_t k = 0; k < KS; ++k) {
+                        MmaShared(tS + st * kKeys, dq + ((k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2),
+                                  k0 + ((k >> 2) * (kKeyHalf >> 4) + (k & 3) * 2), descS, k > 0);
+                    }
+                    MmaCommit(&sh.sFull[st]);
+                }
+                __syncwarp();
+            };
             BarWait(&sh.qFull, 0, failed);
-            for (int32_t it = 0; it < steps.steps; ++it) {
-                const uint32_t phase = it & 1;
-                BarWait(&sh.kFull, phase, failed);
+            for (int32_t it = 0; it < 2 && it < count; ++it) {
+                BarWait(&sh.kFull[it], 0, failed);
                 TcFenceAfter();
-#pragma unroll
-                for (int32_t k = 0; k < 4 * HALVES; ++k) {
-                    if (k < kSteps) {
-                        const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
-                        MmaShared(tS, OperandDesc(aq + off, 16), OperandDesc(ak + off, 16), descS, k > 0);
-                    }
-                }
-                MmaCommit(&sh.sFull);
-                BarWait(&sh.sFull, phase, failed);
-                if (*failed != 0) {
-                    BarDrain(&sh.qFull, 0);
-                    BarDrain(&sh.kFull, phase);
-                    BarDrain(&sh.vFull, phase);
-                    break;
-                }
-                if (it + 1 < steps.steps) {
-                    load(sk, &mapK, &sh.kFull, StepKey(steps, it + 1), u);
-                }
-                BarWait(&sh.vFull, phase, failed);
-                BarWait(&sh.pFull, phase, failed);
-                if (*failed != 0) {
-                    BarDrain(&sh.vFull, phase);
-                    if (it + 1 < steps.steps) {
-                        BarDrain(&sh.kFull, phase ^ 1);
-                    }
+                scores(it);
+            }
+            for (int32_t it = 0; it < count; ++it) {
+                const int32_t st = it & 1;
+                const uint32_t phase = (it / 2) & 1;
+                BarWait(&sh.vFull[st], phase, failed);
+                BarWait(&sh.pFull[st], phase, failed);
+                if (__any_sync(0xffffffffu, *failed != 0)) {
                     break;
                 }
                 TcFenceAfter();
+                if (lead) {
+                    const uint64_t v0 = dv + st * (kKeyBytes >> 4);
 #pragma unroll
-                for (int32_t k = 0; k < kTile / 16; ++k) {
-                    MmaTmem(tO, tS + (k >> 2) * 64 + (k & 3) * 8, OperandDesc(av + k * 2048, kHalfBytes), descO, it > 0 || k > 0);
+                    for (int32_t k = 0; k < kKeys / 16; ++k) {
+                        MmaTmem(tO, tS + st * kKeys + (k >> 1) * 32 + (k & 1) * 8, v0 + k * (2048 >> 4), descO, it > 0 || k > 0);
+                    }
+                    MmaCommit(&sh.pvDone[st]);
                 }
-                MmaCommit(&sh.oFull);
-                BarWait(&sh.oFull, phase, failed);
-                if (it + 1 < steps.steps) {
-                    load(sv, &mapV, &sh.vFull, StepKey(steps, it + 1), u);
+                __syncwarp();
+                if (it + 2 < count) {
+                    BarWait(&sh.kFull[st], phase ^ 1, failed);
+                    BarWait(&sh.pvDone[st], phase, failed); // the weights, which the next scores go over, have been read
+                    TcFenceAfter();
+                    scores(st);
                 }
             }
+            if (lead) {
+                MmaCommit(&sh.allDone);
+            }
+            __syncwarp();
+            BarWait(&sh.allDone, 0, failed);
             if (*failed != 0) {
-                MmaCommit(&sh.drain);
+                if (lead) {
+                    MmaCommit(&sh.drain);
+                }
+                __syncwarp();
                 BarDrain(&sh.drain, 0);
             }
         }
@@ -241,34 +292,57 @@ __global__ void __launch_bounds__(288, 2)
         const int32_t p = i <= iLast ? n.shift + i : -1;
         const Seen seen = SeenOf(s, p);
         const uint32_t lanes = static_cast<uint32_t>(quad) << 21; // 32 quad, in the lane half of an address
-        const uint32_t tx = tS + 64 * side + lanes, to32 = tO + 32 * HALVES * side + lanes;
+        const uint32_t to32 = tO + 32 * HALVES * side + lanes;
         const float factor = fabsf(s.scale) * kLog2e;             // scores in powers of two
         const int32_t wLow = low + 32 * quad, wHigh = wLow + 31;
         const bool rowsWhole = i0 + 32 * quad + 31 <= iLast;
+        const F2 factor2 = MakeF2(factor, factor);
         float top = -INFINITY, total = 0.0f;
-        for (int32_t it = 0; it < steps.steps; ++it) {
-            const int32_t j0 = StepKey(steps, it) + 64 * side;
-            BarWait(&sh.sFull, it & 1, failed);
+        for (int32_t it = 0; it < count; ++it) {
+            const int32_t j0 = steps.Key(it) + 32 * side;
+            const uint32_t tx = tS + (it & 1) * kKeys + 32 * side + lanes;
+            BarWait(&sh.sFull[it & 1], (it / 2) & 1, failed);
             if (__any_sync(0xffffffffu, *failed != 0)) {
                 break;
             }
             TcFenceAfter();
-            uint32_t x[64];
-            TmemLoad32(tx, x);
-            TmemLoad32(tx + 32, x + 32);
-            TmemLoadWait();
             const bool sinkStep = it < steps.sinkSteps;
-            if (sinkStep || !rowsWhole || j0 + 63 > wLow || j0 <= wHigh - s.window) {
-                // Visible columns of the step: those of the window, or those of the sinks. A window step may hold sinks as well: those
-                // behind the block's first key, in front of the row's window.
-                uint32_t live[2];
-                LiveColumns<64>(live, sinkStep ? 0 : seen.first - j0, p < 0 ? 0 : sinkStep ? steps.sinkEnd - j0 : p - j0 + 1,
-                                sinkStep ? 0 : seen.sinkEnd - j0);
-                MaskColumns<64>(x, live);
-            }
+            const bool masked = sinkStep || !rowsWhole || j0 + 31 > wLow || j0 <= wHigh - s.window;
+            uint32_t x[32];
+            auto read = [&] {
+                TmemLoad32(tx, x);
+                if (masked) {
+                    // Visible columns of the step: those of the window, or those of the sinks. A window step may hold sinks as well:
+                    // those behind the block's first key, in front of the row's window.
+                    uint32_t live[1];
+                    LiveColumns<32>(live, sinkStep ? 0 : seen.first - j0, p < 0 ? 0 : sinkStep ? steps.sinkEnd - j0 : p - j0 + 1,
+                                    sinkStep ? 0 : seen.sinkEnd - j0);
+                    MaskColumns<32>(x, live);
+                }
+            };
+            uint32_t w[16];
+            float sum = 0.0f;
+            auto weigh = [&] {
+                const float off = top == -INFINITY ? 0.0f : -top;
+                const F2 off2 = MakeF2(off, off);
+                F2 sum2[2] = {MakeF2(0.0f, 0.0f), MakeF2(0.0f, 0.0f)};
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float e0, e1;
+                    SplitF2(Fma2(MakeF2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), factor2, off2), e0, e1);
+                    e0 = Exp2(e0);
+                    e1 = Exp2(e1);
+                    sum2[e & 1] = Add2(sum2[e & 1], MakeF2(e0, e1));
+                    w[e] = PackPair(e0, e1, static_cast<const T*>(nullptr));
+                }
+                float a0, a1;
+                SplitF2(Add2(sum2[0], sum2[1]), a0, a1);
+                sum = a0 + a1;
+            };
+            read();
             float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 64; c += 8) {
+            for (int c = 0; c < 32; c += 8) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     part[e] = fmaxf(fmaxf(part[e], __uint_as_float(x[c + 2 * e])), __uint_as_float(x[c + 2 * e + 1]));
@@ -277,46 +351,35 @@ __global__ void __launch_bounds__(288, 2)
             float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * factor;
             sh.row[it & 1][side][r] = most;
             BarArrive(&sh.exchanged[quad]);
+            if (it > 0) {
+                weigh();
+            }
             BarWait(&sh.exchanged[quad], it & 1, failed);
             most = fmaxf(most, sh.row[it & 1][side ^ 1][r]);
             const float grown = fmaxf(top, most);
             const bool grow = grown > top + kGrowth; // always from -infinity to a number
             if (it == 0) {
                 top = grown;
-            } else if (__any_sync(0xffffffffu, grow)) {
+                weigh();
+            } else if (__any_sync(0xffffffffu, grow)) { // in both warps of the rows alike
                 const float fade = grow ? Exp2(top - grown) : 1.0f;
                 top = grow ? grown : top;
                 total *= fade;
+                BarWait(&sh.pvDone[(it - 1) & 1], ((it - 1) / 2) & 1, failed);
+                TcFenceAfter();
                 TmemScale<32 * HALVES>(to32, fade);
+                read();
+                weigh();
             }
-            const float off = top == -INFINITY ? 0.0f : -top;
-            const F2 factor2 = MakeF2(factor, factor), off2 = MakeF2(off, off);
-            F2 sum2[2] = {MakeF2(0.0f, 0.0f), MakeF2(0.0f, 0.0f)};
-#pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-                uint32_t w[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const F2 z = Fma2(MakeF2(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])), factor2, off2);
-                    float e0, e1;
-                    SplitF2(z, e0, e1);
-                    e0 = Exp2(e0);
-                    e1 = Exp2(e1);
-                    sum2[e & 1] = Add2(sum2[e & 1], MakeF2(e0, e1));
-                    w[e] = PackPair(e0, e1, static_cast<const T*>(nullptr));
-                }
-                TmemStore16(tx + c / 2, w);
-            }
+            total += sum;
+            TmemStore16(tx, w);
             TmemStoreWait();
             TcFenceBefore();
-            BarArrive(&sh.pFull);
-            float a0, a1;
-            SplitF2(Add2(sum2[0], sum2[1]), a0, a1);
-            total += a0 + a1;
+            BarArrive(&sh.pFull[it & 1]);
         }
         // ---- the rows of out
-        if (steps.steps > 0) {
-            BarWait(&sh.oFull, (steps.steps - 1) & 1, failed);
+        if (count > 0) {
+            BarWait(&sh.allDone, 0, failed);
             TcFenceAfter();
         }
         RowBarrier(); // the last maxima have been read
@@ -330,9 +393,8 @@ __global__ void __launch_bounds__(288, 2)
         for (int c = 0; c < HALVES; ++c) {
             const int32_t d0 = 32 * (HALVES * side + c);
             uint32_t o[32];
-            if (steps.steps > 0) {
+            if (count > 0) {
                 TmemLoad32(to32 + 32 * c, o);
-                TmemLoadWait();
             }
             float v[32];
 #pragma unroll
@@ -367,9 +429,9 @@ __global__ void __launch_bounds__(288, 2)
     }
     TcFenceBefore();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 9) {
         TcFenceAfter();
-        TmemFree(tmem, 256);
+        TmemFree(sh.tmem, 256);
     }
     if (threadIdx.x == 0 && sh.failed != 0) {
         atomicAdd(&g_attentionTimeouts, 1u);
@@ -495,7 +557,7 @@ __global__ void __launch_bounds__(320, 1)
     const int32_t i0 = tile * kTile;
     const int32_t iLast = min(i0 + kTile, n.q) - 1;
     const int32_t low = n.shift + i0, high = iLast >= i0 ? n.shift + iLast : -1;
-    const KeySteps steps = StepsOf(s, low, high);
+    const KeySteps<kTile> steps(s, low, high);
     const int32_t count = steps.steps;
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
@@ -544,7 +606,7 @@ __global__ void __launch_bounds__(320, 1)
             load(sg, &mapG, &sh.qFull, i0, h);
             int32_t it = 0;
             for (; it < count; ++it) {
-                const int32_t j0 = StepKey(steps, it), ks = it % 3, vs = it & 1;
+                const int32_t j0 = steps.Key(it), ks = it % 3, vs = it & 1;
                 if (it >= 3) {
                     BarWait(&sh.kEmpty[ks], (it / 3 - 1) & 1, failed);
                 }
@@ -638,7 +700,7 @@ __global__ void __launch_bounds__(320, 1)
         const F2 factor2 = MakeF2(factor, factor), off2 = MakeF2(-lse2, -lse2), delta2 = MakeF2(-delta, -delta);
         RowScale range;
         for (int32_t it = 0; it < count; ++it) {
-            const int32_t j0 = StepKey(steps, it) + 64 * side;
+            const int32_t j0 = steps.Key(it) + 64 * side;
             const uint32_t tx = tS + (it & 1) * 128 + 64 * side + lanes;
             BarWait(&sh.sFull[it & 1], (it >> 1) & 1, failed);
             if (__any_sync(0xffffffffu, *failed != 0)) {
@@ -646,9 +708,7 @@ __global__ void __launch_bounds__(320, 1)
             }
             TcFenceAfter();
             uint32_t x[64];
-            TmemLoad32(tx, x);
-            TmemLoad32(tx + 32, x + 32);
-            TmemLoadWait();
+            TmemLoad64(tx, x);
             {
                 const bool sinkStep = it < steps.sinkSteps;
                 const int32_t from = sinkStep ? 0 : seen.first - j0;
@@ -674,7 +734,6 @@ __global__ void __launch_bounds__(320, 1)
             for (int c = 0; c < 64; c += 32) {
                 uint32_t y[32];
                 TmemLoad32(tDp + 64 * side + lanes + c, y);
-                TmemLoadWait();
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     const F2 d = Mul2(Add2(MakeF2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), delta2),
@@ -724,7 +783,6 @@ __global__ void __launch_bounds__(320, 1)
             uint32_t o[32];
             if (count > 0) {
                 TmemLoad32(tDq + lanes + d0, o);
-                TmemLoadWait();
             }
             float v[32];
 #pragma unroll
@@ -963,9 +1021,7 @@ __global__ void __launch_bounds__(320, 1)
             }
             TcFenceAfter();
             uint32_t x[64];
-            TmemLoad32(tS + 64 * side + lanes, x);
-            TmemLoad32(tS + 64 * side + lanes + 32, x + 32);
-            TmemLoadWait();
+            TmemLoad64(tS + 64 * side + lanes, x);
             if (!__all_sync(0xffffffffu, from <= p0 && to >= p0 + 64)) {
                 uint32_t live[2];
                 LiveColumns<64>(live, from - p0, to - p0, 0);
@@ -1003,7 +1059,6 @@ __global__ void __launch_bounds__(320, 1)
             for (int c = 0; c < 64; c += 32) {
                 uint32_t y[32];
                 TmemLoad32(tDp + 64 * side + lanes + c, y);
-                TmemLoadWait();
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
                     const float4 d = del[(c + e) / 4];
@@ -1066,7 +1121,6 @@ __global__ void __launch_bounds__(320, 1)
                 uint32_t o[32];
                 if (count > 0) {
                     TmemLoad32(from32 + d0, o);
-                    TmemLoadWait();
                 }
                 float v[32];
 #pragma unroll
@@ -1170,6 +1224,28 @@ EncodeTiled Encoder()
 
 bool TmaStride(int64_t stride, int32_t extent) { return extent <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); }
 
+template <typename T>
+cudaError_t LaunchForward(const MmaArgs& m, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, unsigned grid, int shared,
+                          cudaStream_t stream)
+{
+    auto launch = [&](auto kernel, std::atomic<uint64_t>& asked) {
+        const cudaError_t set = AskOnce(kernel, asked, shared);
+        if (set != cudaSuccess) {
+            return set;
+        }
+        kernel<<<grid, 320, shared, stream>>>(m, mq, mk, mv);
+        CountLaunch();
+        return cudaGetLastError();
+    };
+    static std::atomic<uint64_t> asked[5];
+    const int32_t steps = static_cast<int32_t>(CeilDiv(m.a.s.dim, 16));
+    return steps <= 2 ? launch(AttnForwardMmaKernel<T, 2>, asked[0]) :
+           steps <= 4 ? launch(AttnForwardMmaKernel<T, 4>, asked[1]) :
+           steps <= 5 ? launch(AttnForwardMmaKernel<T, 5>, asked[2]) :
+           steps <= 6 ? launch(AttnForwardMmaKernel<T, 6>, asked[3]) :
+                        launch(AttnForwardMmaKernel<T, 8>, asked[4]);
+}
+
 } // namespace
 
 cudaError_t AttnMakeMap(CUtensorMap* map, Dt dt, const AttnTensor& t, int32_t dim, int32_t tokens, int32_t heads, int32_t batch,
@@ -1208,27 +1284,17 @@ cudaError_t AttnForwardMma(Dt dt, const AttnArgs& a, cudaStream_t stream)
     m.vecOut = s.dim % 8 == 0 && Aligned(a.out.p, 16) && a.out.l % 8 == 0 && a.out.h % 8 == 0 && a.out.b % 8 == 0;
     CUtensorMap mq, mk, mv;
     cudaError_t e = AttnMakeMap(&mq, dt, a.q, s.dim, s.lq, s.heads, s.batch, kTile);
-    e = e != cudaSuccess ? e : AttnMakeMap(&mk, dt, a.k, s.dim, s.lk, s.kvHeads, s.batch, kTile);
-    e = e != cudaSuccess ? e : AttnMakeMap(&mv, dt, a.v, s.dim, s.lk, s.kvHeads, s.batch, kTile);
+    e = e != cudaSuccess ? e : AttnMakeMap(&mk, dt, a.k, s.dim, s.lk, s.kvHeads, s.batch, kKeys);
+    e = e != cudaSuccess ? e : AttnMakeMap(&mv, dt, a.v, s.dim, s.lk, s.kvHeads, s.batch, kKeys);
     if (e != cudaSuccess) {
         return e;
     }
     const int shared = 3 * m.halves * static_cast<int>(kHalfBytes) + 1024;
     const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(s.batch) * s.heads * m.tiles);
-    static std::atomic<uint64_t> asked[4];
-    auto launch = [&](auto kernel, int which) {
-        const cudaError_t set = AskOnce(kernel, asked[which], shared);
-        if (set != cudaSuccess) {
-            return set;
-        }
-        kernel<<<grid, 288, shared, stream>>>(m, mq, mk, mv);
-        CountLaunch();
-        return cudaGetLastError();
-    };
     if (dt == Dt::F16) {
-        return m.halves == 1 ? launch(AttnForwardMmaKernel<__half, 1>, 0) : launch(AttnForwardMmaKernel<__half, 2>, 1);
+        return LaunchForward<__half>(m, mq, mk, mv, grid, shared, stream);
     }
-    return m.halves == 1 ? launch(AttnForwardMmaKernel<__nv_bfloat16, 1>, 2) : launch(AttnForwardMmaKernel<__nv_bfloat16, 2>, 3);
+    return LaunchForward<__nv_bfloat16>(m, mq, mk, mv, grid, shared, stream);
 }
 
 namespace {
