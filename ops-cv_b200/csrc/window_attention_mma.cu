@@ -529,6 +529,25 @@ struct RowScale {
 };
 __device__ __forceinline__ uint32_t ExponentOf(float positive) { return __float_as_uint(positive) >> 23; }
 
+// 128 x 128 products over KS steps of 16 values, both operands with the values along their 128 bytes, halves of 64 kHalfBytes apart
+template <int KS>
+__device__ __forceinline__ void InnerProducts(uint32_t d, uint64_t a, uint64_t b, uint32_t desc)
+{
+#pragma unroll
+    for (int32_t k = 0; k < KS; ++k) {
+        const uint64_t off = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
+        MmaShared(d, a + off, b + off, desc, k > 0);
+    }
+}
+// the products of 128 weights a row (tensor memory: 64 at `a`, 64 at a + 64) with 128 rows of values
+__device__ __forceinline__ void OuterProducts(uint32_t d, uint32_t a, uint64_t rows, uint32_t desc, bool add)
+{
+#pragma unroll
+    for (int32_t k = 0; k < kTile / 16; ++k) {
+        MmaTmem(d, a + (k >> 2) * 64 + (k & 3) * 8, rows + k * (2048 >> 4), desc, add || k > 0);
+    }
+}
+
 struct GradQShared {
     uint64_t qFull, kFull[3], kEmpty[3], vFull[2], vEmpty[2], sFull[2], dpFull, dsReady, dqDone, allDone, exchanged, drain;
     uint32_t tmem, failed, bad[4];
@@ -538,7 +557,7 @@ struct GradQShared {
 // Tensor memory: S of even and odd steps at 0 and 128 (ds of a step goes over its S), dP at 256, gradQ at 384. The products of a step in
 // the order dP(n + 1), gradQ(n), S(n + 2): the row threads form the weights of step n + 1 from an S that is there already while the
 // first two run.
-template <typename T, int HALVES>
+template <typename T, int KS>
 __global__ void __launch_bounds__(320, 1)
     AttnGradQMmaKernel(const __grid_constant__ BackwardArgs m, const __grid_constant__ CUtensorMap mapQ,
                        const __grid_constant__ CUtensorMap mapG, const __grid_constant__ CUtensorMap mapK,
@@ -546,6 +565,7 @@ __global__ void __launch_bounds__(320, 1)
 {
     extern __shared__ unsigned char raw[];
     __shared__ GradQShared sh;
+    constexpr int HALVES = KS > 4 ? 2 : 1;
     constexpr uint32_t kBytes = HALVES * kHalfBytes;
     unsigned char* base = raw + (1024 - (SharedAddr(raw) & 1023)) % 1024;
     unsigned char *sq = base, *sg = base + kBytes, *sk = base + 2 * kBytes, *sv = base + 5 * kBytes;
@@ -632,58 +652,70 @@ __global__ void __launch_bounds__(320, 1)
         }
         __syncwarp();
     } else if (warp == 9) {
-        if ((threadIdx.x & 31) == 0 && count > 0) {
-            const int32_t kSteps = (s.dim + 15) / 16;
+        if (count > 0) {
+            const bool lead = ElectOne();
             const uint32_t descS = ProductDesc<T>(kTile, false, s.scale < 0.0f), descDp = ProductDesc<T>(kTile, false, false);
-            const uint32_t descDq = ProductDesc<T>(kSteps * 16, true, false);
-            const uint32_t aq = SharedAddr(sq), ag = SharedAddr(sg), ak = SharedAddr(sk), av = SharedAddr(sv);
-            auto scores = [&](int32_t it) {
-                BarWait(&sh.kFull[it % 3], (it / 3) & 1, failed);
+            const uint32_t descDq = ProductDesc<T>(KS * 16, true, false);
+            const uint64_t dq = OperandDesc(SharedAddr(sq), 16), dg = OperandDesc(SharedAddr(sg), 16);
+            const uint64_t dk = OperandDesc(SharedAddr(sk), 16), dkRows = OperandDesc(SharedAddr(sk), kHalfBytes),
+                           dv = OperandDesc(SharedAddr(sv), 16);
+            auto scores = [&](int32_t it, int32_t ks) { // ks: it modulo 3
+                BarWait(&sh.kFull[ks], (it / 3) & 1, failed);
                 TcFenceAfter();
-                for (int32_t k = 0; k < kSteps; ++k) {
-                    const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
-                    MmaShared(tS + (it & 1) * 128, OperandDesc(aq + off, 16), OperandDesc(ak + (it % 3) * kBytes + off, 16), descS, k > 0);
+                if (lead) {
+                    InnerProducts<KS>(tS + (it & 1) * 128, dq, dk + ks * (kBytes >> 4), descS);
+                    MmaCommit(&sh.sFull[it & 1]);
                 }
-                MmaCommit(&sh.sFull[it & 1]);
+                __syncwarp();
             };
             auto products = [&](int32_t it) {
                 BarWait(&sh.vFull[it & 1], (it / 2) & 1, failed);
                 TcFenceAfter();
-                for (int32_t k = 0; k < kSteps; ++k) {
-                    const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
-                    MmaShared(tDp, OperandDesc(ag + off, 16), OperandDesc(av + (it & 1) * kBytes + off, 16), descDp, k > 0);
+                if (lead) {
+                    InnerProducts<KS>(tDp, dg, dv + (it & 1) * (kBytes >> 4), descDp);
+                    MmaCommit(&sh.dpFull);
+                    MmaCommit(&sh.vEmpty[it & 1]);
                 }
-                MmaCommit(&sh.dpFull);
-                MmaCommit(&sh.vEmpty[it & 1]);
+                __syncwarp();
             };
             BarWait(&sh.qFull, 0, failed);
-            scores(0);
+            scores(0, 0);
             products(0);
             if (count > 1) {
-                scores(1);
+                scores(1, 1);
             }
-            for (int32_t it = 0; it < count && *failed == 0; ++it) {
+            int32_t ks = 0;
+            for (int32_t it = 0; it < count; ++it) {
                 BarWait(&sh.dsReady, it & 1, failed);
+                if (__any_sync(0xffffffffu, *failed != 0)) {
+                    break;
+                }
                 TcFenceAfter();
                 if (it + 1 < count) {
                     products(it + 1);
                 }
-#pragma unroll
-                for (int32_t k = 0; k < kTile / 16; ++k) {
-                    MmaTmem(tDq, tS + (it & 1) * 128 + (k >> 2) * 64 + (k & 3) * 8,
-                            OperandDesc(ak + (it % 3) * kBytes + k * 2048, kHalfBytes), descDq, it > 0 || k > 0);
+                if (lead) {
+                    OuterProducts(tDq, tS + (it & 1) * 128, dkRows + ks * (kBytes >> 4), descDq, it > 0);
+                    MmaCommit(&sh.kEmpty[ks]);
+                    MmaCommit(&sh.dqDone);
                 }
-                MmaCommit(&sh.kEmpty[it % 3]);
-                MmaCommit(&sh.dqDone);
+                __syncwarp();
                 if (it + 2 < count) {
                     BarWait(&sh.dqDone, it & 1, failed); // ds(it), which the next scores go over, has been read
-                    scores(it + 2);
+                    scores(it + 2, ks == 0 ? 2 : ks - 1);
                 }
+                ks = ks == 2 ? 0 : ks + 1;
             }
-            MmaCommit(&sh.allDone);
+            if (lead) {
+                MmaCommit(&sh.allDone);
+            }
+            __syncwarp();
             BarWait(&sh.allDone, 0, failed);
             if (*failed != 0) {
-                MmaCommit(&sh.drain);
+                if (lead) {
+                    MmaCommit(&sh.drain);
+                }
+                __syncwarp();
                 BarDrain(&sh.drain, 0);
             }
         }
@@ -836,7 +868,7 @@ struct GradKvShared {
 // Sinks are seen by every later query. Were that left to the block of their keys, it would walk the whole sequence while the others
 // walk a window; so the queries behind the window of such a tile are shared out among farChunks further blocks. Their sums and the
 // tile's own go to `partial` ([tile][1 + farChunks][gradK, gradV][128][dim], fp32), which AttnSinkGradKernel adds up in order.
-template <typename T, int HALVES>
+template <typename T, int KS>
 __global__ void __launch_bounds__(320, 1)
     AttnGradKvMmaKernel(const __grid_constant__ BackwardArgs m, const __grid_constant__ CUtensorMap mapQ,
                         const __grid_constant__ CUtensorMap mapG, const __grid_constant__ CUtensorMap mapK,
@@ -844,6 +876,7 @@ __global__ void __launch_bounds__(320, 1)
 {
     extern __shared__ unsigned char raw[];
     __shared__ GradKvShared sh;
+    constexpr int HALVES = KS > 4 ? 2 : 1;
     constexpr uint32_t kBytes = HALVES * kHalfBytes;
     constexpr uint32_t kStage = 2 * kBytes + 2 * kTile * 4;
     unsigned char* base = raw + (1024 - (SharedAddr(raw) & 1023)) % 1024;
@@ -948,55 +981,68 @@ __global__ void __launch_bounds__(320, 1)
         }
         __syncwarp();
     } else if (warp == 9) {
-        if ((threadIdx.x & 31) == 0 && count > 0) {
-            const int32_t kSteps = (s.dim + 15) / 16;
+        if (count > 0) {
+            const bool lead = ElectOne();
             const uint32_t descS = ProductDesc<T>(kTile, false, s.scale < 0.0f), descDp = ProductDesc<T>(kTile, false, false);
-            const uint32_t descOut = ProductDesc<T>(kSteps * 16, true, false);
-            const uint32_t ak = SharedAddr(sk), av = SharedAddr(sv), aq = SharedAddr(sqg);
-            auto inner = [&](uint32_t d, uint32_t a, uint32_t rows, uint32_t desc, uint64_t* bar) {
-                for (int32_t k = 0; k < kSteps; ++k) {
-                    const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
-                    MmaShared(d, OperandDesc(a + off, 16), OperandDesc(rows + off, 16), desc, k > 0);
+            const uint32_t descOut = ProductDesc<T>(KS * 16, true, false);
+            const uint64_t dk = OperandDesc(SharedAddr(sk), 16), dv = OperandDesc(SharedAddr(sv), 16);
+            // Q and gradOut as rows of values (inner products) and as columns (outer ones)
+            const uint64_t dq = OperandDesc(SharedAddr(sqg), 16), dqRows = OperandDesc(SharedAddr(sqg), kHalfBytes);
+            constexpr uint64_t kPlace = 2 * kBytes >> 4, kGrad = kBytes >> 4;
+            auto inner = [&](uint32_t d, uint64_t a, uint64_t rows, uint32_t desc, uint64_t* bar) {
+                if (lead) {
+                    InnerProducts<KS>(d, a, rows, desc);
+                    MmaCommit(bar);
                 }
-                MmaCommit(bar);
-            };
-            auto outer = [&](uint32_t d, uint32_t a, uint32_t rows, bool add) {
-#pragma unroll
-                for (int32_t k = 0; k < kTile / 16; ++k) {
-                    MmaTmem(d, a + (k >> 2) * 64 + (k & 3) * 8, OperandDesc(rows + k * 2048, kHalfBytes), descOut, add || k > 0);
-                }
+                __syncwarp();
             };
             BarWait(&sh.kvFull, 0, failed);
             BarWait(&sh.full[0], 0, failed);
             TcFenceAfter();
-            inner(tS, ak, aq, descS, &sh.sFull);
-            inner(tDp, av, aq + kBytes, descDp, &sh.dpFull);
-            for (int32_t it = 0; it < count && *failed == 0; ++it) {
-                const uint32_t phase = it & 1, at = aq + (it & 1) * 2 * kBytes, next = aq + ((it + 1) & 1) * 2 * kBytes;
+            inner(tS, dk, dq, descS, &sh.sFull);
+            inner(tDp, dv, dq + kGrad, descDp, &sh.dpFull);
+            for (int32_t it = 0; it < count; ++it) {
+                const uint32_t phase = it & 1;
+                const uint64_t at = (it & 1) * kPlace, next = ((it + 1) & 1) * kPlace;
                 BarWait(&sh.pReady, phase, failed);
+                if (__any_sync(0xffffffffu, *failed != 0)) {
+                    break;
+                }
                 TcFenceAfter();
-                outer(tDv, tS, at + kBytes, it > 0);
-                MmaCommit(&sh.dvDone);
+                if (lead) {
+                    OuterProducts(tDv, tS, dqRows + at + kGrad, descOut, it > 0);
+                    MmaCommit(&sh.dvDone);
+                }
+                __syncwarp();
                 if (it + 1 < count) {
                     BarWait(&sh.full[(it + 1) & 1], ((it + 1) / 2) & 1, failed);
                     BarWait(&sh.dvDone, phase, failed); // the weights, which the next scores go over, have been read
                     TcFenceAfter();
-                    inner(tS, ak, next, descS, &sh.sFull);
+                    inner(tS, dk, dq + next, descS, &sh.sFull);
                 }
                 BarWait(&sh.dsReady, phase, failed);
+                if (__any_sync(0xffffffffu, *failed != 0)) {
+                    break;
+                }
                 TcFenceAfter();
-                outer(tDk, tDp, at, it > 0);
-                MmaCommit(&sh.empty[it & 1]);
-                MmaCommit(&sh.dkDone);
+                if (lead) {
+                    OuterProducts(tDk, tDp, dqRows + at, descOut, it > 0);
+                    MmaCommit(&sh.empty[it & 1]);
+                    MmaCommit(&sh.dkDone);
+                }
+                __syncwarp();
                 if (it + 1 < count) {
                     BarWait(&sh.dkDone, phase, failed);
                     TcFenceAfter();
-                    inner(tDp, av, next + kBytes, descDp, &sh.dpFull);
+                    inner(tDp, dv, dq + next + kGrad, descDp, &sh.dpFull);
                 }
             }
             BarWait(&sh.dkDone, (count - 1) & 1, failed);
             if (*failed != 0) {
-                MmaCommit(&sh.drain);
+                if (lead) {
+                    MmaCommit(&sh.drain);
+                }
+                __syncwarp();
                 BarDrain(&sh.drain, 0);
             }
         }
@@ -1324,6 +1370,47 @@ uint64_t StatsBytes(const AttnShape& s) { return (static_cast<uint64_t>(s.batch)
 
 } // namespace
 
+namespace {
+
+struct BackwardLaunch {
+    const BackwardArgs& m;
+    const CUtensorMap &mq, &mg, &mk, &mv;
+    unsigned statBlocks, qBlocks, kvBlocks;
+    int sharedQ, sharedKv;
+    bool vecStats;
+};
+template <typename T>
+cudaError_t LaunchBackward(const BackwardLaunch& l, cudaStream_t stream)
+{
+    const BackwardArgs& m = l.m;
+    auto launch = [&](auto gradQ, auto gradKv, std::atomic<uint64_t>(&asked)[2]) {
+        cudaError_t set = AskOnce(gradQ, asked[0], l.sharedQ);
+        set = set != cudaSuccess ? set : AskOnce(gradKv, asked[1], l.sharedKv);
+        if (set != cudaSuccess) {
+            return set;
+        }
+        AttnStatisticsKernel<T><<<l.statBlocks, 256, 0, stream>>>(m, l.vecStats);
+        gradQ<<<l.qBlocks, 320, l.sharedQ, stream>>>(m, l.mq, l.mg, l.mk, l.mv);
+        gradKv<<<l.kvBlocks, 320, l.sharedKv, stream>>>(m, l.mq, l.mg, l.mk, l.mv);
+        CountLaunch(3);
+        if (m.farChunks > 0) {
+            const int64_t keys = static_cast<int64_t>(m.a.s.batch) * m.a.s.kvHeads * m.sinkTiles * kTile;
+            AttnSinkGradKernel<T><<<static_cast<unsigned>(CeilDiv(keys, 4)), 128, 0, stream>>>(m);
+            CountLaunch();
+        }
+        return cudaGetLastError();
+    };
+    static std::atomic<uint64_t> asked[5][2];
+    const int32_t steps = static_cast<int32_t>(CeilDiv(m.a.s.dim, 16));
+    return steps <= 2 ? launch(AttnGradQMmaKernel<T, 2>, AttnGradKvMmaKernel<T, 2>, asked[0]) :
+           steps <= 4 ? launch(AttnGradQMmaKernel<T, 4>, AttnGradKvMmaKernel<T, 4>, asked[1]) :
+           steps <= 5 ? launch(AttnGradQMmaKernel<T, 5>, AttnGradKvMmaKernel<T, 5>, asked[2]) :
+           steps <= 6 ? launch(AttnGradQMmaKernel<T, 6>, AttnGradKvMmaKernel<T, 6>, asked[3]) :
+                        launch(AttnGradQMmaKernel<T, 8>, AttnGradKvMmaKernel<T, 8>, asked[4]);
+}
+
+} // namespace
+
 uint64_t AttnBackwardMmaWorkspace(const AttnShape& s)
 {
     const FarPlan f = PlanFar(s);
@@ -1367,32 +1454,9 @@ cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStrea
     const int sharedQ = 7 * bytes + 1024, sharedKv = 6 * bytes + 4 * kTile * 4 + 1024;
     const unsigned qBlocks = static_cast<unsigned>(static_cast<int64_t>(s.batch) * s.heads * m.qTiles);
     const bool vecStats = VecRows(a.gradOut, s.dim) && VecRows(a.out, s.dim);
-    static std::atomic<uint64_t> askedQ[4], askedKv[4];
-    const int which = (dt == Dt::F16 ? 0 : 2) + halves - 1;
-    auto launch = [&](auto tag, auto gradQ, auto gradKv) {
-        using T = decltype(tag);
-        cudaError_t set = AskOnce(gradQ, askedQ[which], sharedQ);
-        set = set != cudaSuccess ? set : AskOnce(gradKv, askedKv[which], sharedKv);
-        if (set != cudaSuccess) {
-            return set;
-        }
-        AttnStatisticsKernel<T><<<static_cast<unsigned>(statBlocks), 256, 0, stream>>>(m, vecStats);
-        gradQ<<<qBlocks, 320, sharedQ, stream>>>(m, mq, mg, mk, mv);
-        gradKv<<<static_cast<unsigned>(kvBlocks), 320, sharedKv, stream>>>(m, mq, mg, mk, mv);
-        CountLaunch(3);
-        if (m.farChunks > 0) {
-            const int64_t keys = static_cast<int64_t>(s.batch) * s.kvHeads * m.sinkTiles * kTile;
-            AttnSinkGradKernel<T><<<static_cast<unsigned>(CeilDiv(keys, 4)), 128, 0, stream>>>(m);
-            CountLaunch();
-        }
-        return cudaGetLastError();
-    };
-    if (dt == Dt::F16) {
-        return halves == 1 ? launch(__half{}, AttnGradQMmaKernel<__half, 1>, AttnGradKvMmaKernel<__half, 1>) :
-                             launch(__half{}, AttnGradQMmaKernel<__half, 2>, AttnGradKvMmaKernel<__half, 2>);
-    }
-    return halves == 1 ? launch(__nv_bfloat16{}, AttnGradQMmaKernel<__nv_bfloat16, 1>, AttnGradKvMmaKernel<__nv_bfloat16, 1>) :
-                         launch(__nv_bfloat16{}, AttnGradQMmaKernel<__nv_bfloat16, 2>, AttnGradKvMmaKernel<__nv_bfloat16, 2>);
+    const BackwardLaunch l{m, mq, mg, mk, mv, static_cast<unsigned>(statBlocks), qBlocks, static_cast<unsigned>(kvBlocks), sharedQ, sharedKv,
+                           vecStats};
+    return dt == Dt::F16 ? LaunchBackward<__half>(l, stream) : LaunchBackward<__nv_bfloat16>(l, stream);
 }
 
 uint32_t AttentionTimeouts()
