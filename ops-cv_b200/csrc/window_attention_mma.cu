@@ -1,4 +1,6 @@
 // Attention over a sliding window with sinks on the tensor cores: 16-bit tensors with heads of up to 128 values.
+#include <algorithm>
+
 #include "tcgen05.cuh"
 #include "window_attention.cuh"
 
@@ -43,8 +45,12 @@ struct KeySteps {
 // Bits 0 to n - 1 of a word, n cut to [0, 32].
 __device__ __forceinline__ uint32_t Below(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-constexpr int kRowThreads = 256; // two threads a row of a tile
-__device__ __forceinline__ void RowBarrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// of the threads that have the rows
+template <int THREADS>
+__device__ __forceinline__ void RowBarrier()
+{
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
 
 // columns of an accumulator times a factor a row
 template <int N>
@@ -63,13 +69,13 @@ __device__ __forceinline__ void TmemScale(uint32_t addr, float f)
     TmemStoreWait();
 }
 
-// 32 values of a row of an output, of which `left` exist
-template <typename T>
-__device__ __forceinline__ void StoreRow32(T* out, const float (&v)[32], int32_t left, bool vec)
+// N values of a row of an output, of which `left` exist
+template <typename T, int N>
+__device__ __forceinline__ void StoreRow(T* out, const float (&v)[N], int32_t left, bool vec)
 {
     if (vec) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
+        for (int e = 0; e < N; e += 8) {
             if (e < left) {
                 float w[8];
 #pragma unroll
@@ -81,7 +87,7 @@ __device__ __forceinline__ void StoreRow32(T* out, const float (&v)[32], int32_t
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < N; ++e) {
             if (e < left) {
                 out[e] = DType<T>::FromF(v[e]);
             }
@@ -118,6 +124,7 @@ __device__ __forceinline__ void LiveColumns(uint32_t (&live)[N / 32], int32_t fr
 //
 // A row's weights are formed from the maximum of the steps before while the row's two threads exchange the maxima of this one; only
 // where a row has outgrown its old maximum by 2^8 (at the start, mostly) are they formed again and O rescaled.
+constexpr int kRowThreads = 256;
 constexpr int kKeys = 64;
 constexpr uint32_t kKeyHalf = kKeys * 128;
 
@@ -382,9 +389,9 @@ __global__ void __launch_bounds__(320, 2)
             BarWait(&sh.allDone, 0, failed);
             TcFenceAfter();
         }
-        RowBarrier(); // the last maxima have been read
+        RowBarrier<kRowThreads>(); // the last maxima have been read
         sh.row[0][side][r] = total;
-        RowBarrier();
+        RowBarrier<kRowThreads>();
         total = sh.row[0][0][r] + sh.row[0][1][r];
         const float inverse = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total; // NaN stays
         bool bad = seen.count > 0 && !(total > 0.0f && total <= 3.0e38f);
@@ -403,7 +410,7 @@ __global__ void __launch_bounds__(320, 2)
                 bad = bad || (d0 + e < s.dim && !(fabsf(v[e]) <= 3.4e38f));
             }
             if (out != nullptr && d0 < s.dim) {
-                StoreRow32<T>(out + d0, v, s.dim - d0, m.vecOut);
+                StoreRow<T>(out + d0, v, s.dim - d0, m.vecOut);
             }
         }
         if (out != nullptr && m.a.lse != nullptr && side == 0) {
@@ -413,7 +420,7 @@ __global__ void __launch_bounds__(320, 2)
         if ((threadIdx.x & 31) == 0 && rows != 0) {
             atomicOr(&sh.bad[quad], rows);
         }
-        RowBarrier();
+        RowBarrier<kRowThreads>();
         // rows that are not finite again, without the masked keys' part: the even ones by one warp, the odd ones by another
         uint32_t again = sh.bad[quad] & (side == 0 ? 0x55555555u : 0xaaaaaaaau);
         while (again != 0) {
@@ -439,21 +446,28 @@ __global__ void __launch_bounds__(320, 2)
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------
-// Two kernels, each with the sums that it owns in tensor memory, so that no sum crosses blocks but for the sinks' (below) and all are
-// formed in a fixed order: gradQ by blocks of 128 queries that walk their keys, gradK and gradV by blocks of 128 keys that walk the
-// queries that see them. S and dP are formed twice for that (7 products where one kernel would do 5 and add gradQ up in memory, in an
-// order of chance). Both have one block an SM: warps 0 to 7 have a row each two threads (64 columns each), warp 8 loads, warp 9 issues
-// the products. The weights are scaled by 2^8 (folded into the statistics), which keeps small ones out of fp16's subnormal range.
+// Two kinds of blocks, each with the sums that it owns in tensor memory, so that no sum crosses blocks but for the sinks' (below) and all
+// are formed in a fixed order: gradK and gradV by blocks of 128 keys that walk the queries that see them, gradQ by blocks of 128 queries
+// that walk their keys. S and dP are formed twice for that (7 products where one kind would do 5 and add gradQ up in memory, in an order
+// of chance). They go in one launch, the longer ones first, so that the others fill the SMs that the last of them leave. A block has an SM
+// to itself: warps 0 to 15 have a row each four threads (32 columns each), warp 16 loads, warp 17 issues the products; with two threads
+// a row, the chain of one thread's exponentials was longer than the products. The weights are scaled by 2^8 (folded into the statistics),
+// which keeps small ones out of fp16's subnormal range.
+constexpr int kSides = 4;
+constexpr int kColumns = kTile / kSides;
+constexpr int kGradThreads = kTile * kSides;
+constexpr int kLoadWarp = kGradThreads / 32, kProductWarp = kLoadWarp + 1;
 constexpr float kWeightShift = 8.0f;
 constexpr float kWeightScale = 0.00390625f; // 2^-8
 struct BackwardArgs {
     AttnArgs a;
     int32_t qTiles, kTiles;
+    uint32_t kvBlocks;
     float* lse2;  // [batch, heads, stride]: lse in powers of two less kWeightShift; +infinity where a query sees nothing, so that its
                   // weights are 0
     float* delta; // [batch, heads, stride], 0 there
     int64_t stride;
-    int32_t sinkTiles, farChunks; // see AttnGradKvMmaKernel
+    int32_t sinkTiles, farChunks; // see GradKvBlock
     float* partial;
     bool vecQ, vecK, vecV;
 };
@@ -539,39 +553,70 @@ __device__ __forceinline__ void InnerProducts(uint32_t d, uint64_t a, uint64_t b
         MmaShared(d, a + off, b + off, desc, k > 0);
     }
 }
-// the products of 128 weights a row (tensor memory: 64 at `a`, 64 at a + 64) with 128 rows of values
+// the products of 128 weights a row (tensor memory: 32 in 16 columns at `a`, the next at a + 32, ...) with 128 rows of values
 __device__ __forceinline__ void OuterProducts(uint32_t d, uint32_t a, uint64_t rows, uint32_t desc, bool add)
 {
 #pragma unroll
     for (int32_t k = 0; k < kTile / 16; ++k) {
-        MmaTmem(d, a + (k >> 2) * 64 + (k & 3) * 8, rows + k * (2048 >> 4), desc, add || k > 0);
+        MmaTmem(d, a + (k >> 1) * kColumns + (k & 1) * 8, rows + k * (2048 >> 4), desc, add || k > 0);
     }
+}
+
+// 32 weights of a row, scaled, as 16-bit values
+template <typename T>
+__device__ __forceinline__ void StoreWeights(uint32_t addr, const uint32_t (&x)[kColumns], float scale)
+{
+    uint32_t w[kColumns / 2];
+#pragma unroll
+    for (int c = 0; c < kColumns / 2; ++c) {
+        w[c] = PackPair(__uint_as_float(x[2 * c]) * scale, __uint_as_float(x[2 * c + 1]) * scale, static_cast<const T*>(nullptr));
+    }
+    TmemStore16(addr, w);
+}
+template <int N>
+__device__ __forceinline__ void TmemLoadOwn(uint32_t addr, uint32_t* o)
+{
+    if constexpr (N == 32) {
+        TmemLoad32(addr, o);
+    } else {
+        TmemLoad16(addr, o);
+    }
+}
+// The exponent of the largest of a row's threads' values.
+__device__ __forceinline__ uint32_t LargestOfRow(uint8_t (&most)[kSides][kTile], int32_t side, int32_t r, float mine, uint64_t* exchanged,
+                                                 uint32_t phase, volatile uint32_t* failed)
+{
+    most[side][r] = static_cast<uint8_t>(ExponentOf(mine));
+    BarArrive(exchanged);
+    BarWait(exchanged, phase, failed);
+    uint32_t e = 0;
+#pragma unroll
+    for (int x = 0; x < kSides; ++x) {
+        e = max(e, static_cast<uint32_t>(most[x][r]));
+    }
+    return e;
 }
 
 struct GradQShared {
     uint64_t qFull, kFull[3], kEmpty[3], vFull[2], vEmpty[2], sFull[2], dpFull, dsReady, dqDone, allDone, exchanged, drain;
     uint32_t tmem, failed, bad[4];
-    uint8_t most[2][2][kTile]; // fp16: exponents of a row's largest ds, of even and odd steps, of its two threads
+    uint8_t most[2][kSides][kTile]; // fp16: exponents of a row's largest ds, of even and odd steps, of its threads
 };
 
 // Tensor memory: S of even and odd steps at 0 and 128 (ds of a step goes over its S), dP at 256, gradQ at 384. The products of a step in
 // the order dP(n + 1), gradQ(n), S(n + 2): the row threads form the weights of step n + 1 from an S that is there already while the
 // first two run.
 template <typename T, int KS>
-__global__ void __launch_bounds__(320, 1)
-    AttnGradQMmaKernel(const __grid_constant__ BackwardArgs m, const __grid_constant__ CUtensorMap mapQ,
-                       const __grid_constant__ CUtensorMap mapG, const __grid_constant__ CUtensorMap mapK,
-                       const __grid_constant__ CUtensorMap mapV)
+__device__ __forceinline__ void GradQBlock(const BackwardArgs& m, const CUtensorMap& mapQ, const CUtensorMap& mapG, const CUtensorMap& mapK,
+                                           const CUtensorMap& mapV, uint32_t block, unsigned char* raw, GradQShared& sh)
 {
-    extern __shared__ unsigned char raw[];
-    __shared__ GradQShared sh;
     constexpr int HALVES = KS > 4 ? 2 : 1;
     constexpr uint32_t kBytes = HALVES * kHalfBytes;
     unsigned char* base = raw + (1024 - (SharedAddr(raw) & 1023)) % 1024;
     unsigned char *sq = base, *sg = base + kBytes, *sk = base + 2 * kBytes, *sv = base + 5 * kBytes;
     const AttnShape& s = m.a.s;
-    const int32_t tile = blockIdx.x % m.qTiles;
-    const int32_t bh = blockIdx.x / m.qTiles;
+    const int32_t tile = m.qTiles - 1 - static_cast<int32_t>(block % m.qTiles); // the tiles that see most keys first
+    const int32_t bh = block / m.qTiles;
     const int32_t b = bh / s.heads, h = bh % s.heads;
     const Lengths n = LengthsOf(s, b);
     const int32_t i0 = tile * kTile;
@@ -593,17 +638,17 @@ __global__ void __launch_bounds__(320, 1)
             BarInit(&sh.sFull[e], 1);
         }
         BarInit(&sh.dpFull, 1);
-        BarInit(&sh.dsReady, kRowThreads);
+        BarInit(&sh.dsReady, kGradThreads);
         BarInit(&sh.dqDone, 1);
         BarInit(&sh.allDone, 1);
-        BarInit(&sh.exchanged, kRowThreads);
+        BarInit(&sh.exchanged, kGradThreads);
         BarInit(&sh.drain, 1);
         BarInitDone();
     }
     if (threadIdx.x < 4) {
         sh.bad[threadIdx.x] = 0;
     }
-    if (warp == 9) {
+    if (warp == kProductWarp) {
         TmemAlloc(&sh.tmem, 512);
     }
     TcFenceBefore();
@@ -612,7 +657,7 @@ __global__ void __launch_bounds__(320, 1)
     const uint32_t tS = sh.tmem, tDp = tS + 256, tDq = tS + 384;
     volatile uint32_t* failed = &sh.failed;
 
-    if (warp == 8) {
+    if (warp == kLoadWarp) {
         if ((threadIdx.x & 31) == 0 && count > 0) {
             const int32_t u = h / m.a.group;
             auto load = [&](unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int32_t row, int32_t head) {
@@ -651,7 +696,7 @@ __global__ void __launch_bounds__(320, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == kProductWarp) {
         if (count > 0) {
             const bool lead = ElectOne();
             const uint32_t descS = ProductDesc<T>(kTile, false, s.scale < 0.0f), descDp = ProductDesc<T>(kTile, false, false);
@@ -721,6 +766,7 @@ __global__ void __launch_bounds__(320, 1)
         }
         __syncwarp();
     } else {
+        constexpr int kOwn = 64 * HALVES / kSides; // columns of the sums that a thread has
         const int32_t side = warp >> 2, r = (warp & 3) * 32 + (threadIdx.x & 31);
         const int32_t i = i0 + r;
         const int32_t p = i <= iLast ? n.shift + i : -1;
@@ -732,48 +778,47 @@ __global__ void __launch_bounds__(320, 1)
         const F2 factor2 = MakeF2(factor, factor), off2 = MakeF2(-lse2, -lse2), delta2 = MakeF2(-delta, -delta);
         RowScale range;
         for (int32_t it = 0; it < count; ++it) {
-            const int32_t j0 = steps.Key(it) + 64 * side;
-            const uint32_t tx = tS + (it & 1) * 128 + 64 * side + lanes;
+            const int32_t j0 = steps.Key(it) + kColumns * side;
+            const uint32_t tx = tS + (it & 1) * 128 + kColumns * side + lanes;
             BarWait(&sh.sFull[it & 1], (it >> 1) & 1, failed);
             if (__any_sync(0xffffffffu, *failed != 0)) {
                 break;
             }
             TcFenceAfter();
-            uint32_t x[64];
-            TmemLoad64(tx, x);
+            uint32_t x[kColumns];
+            TmemLoad32(tx, x);
             {
                 const bool sinkStep = it < steps.sinkSteps;
                 const int32_t from = sinkStep ? 0 : seen.first - j0;
                 const int32_t to = p < 0 ? 0 : sinkStep ? steps.sinkEnd - j0 : p - j0 + 1;
                 const int32_t sinkTo = sinkStep ? 0 : seen.sinkEnd - j0;
-                if (!__all_sync(0xffffffffu, from <= 0 && to >= 64)) {
-                    uint32_t live[2];
-                    LiveColumns<64>(live, from, to, sinkTo);
-                    MaskColumns<64>(x, live);
+                if (!__all_sync(0xffffffffu, from <= 0 && to >= kColumns)) {
+                    uint32_t live[1];
+                    LiveColumns<kColumns>(live, from, to, sinkTo);
+                    MaskColumns<kColumns>(x, live);
                 }
             }
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
+            for (int e = 0; e < kColumns; e += 2) {
                 float e0, e1;
-                SplitF2(Fma2(MakeF2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), factor2, off2), e0, e1);
-                x[2 * c] = __float_as_uint(Exp2(e0));
-                x[2 * c + 1] = __float_as_uint(Exp2(e1));
+                SplitF2(Fma2(MakeF2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), factor2, off2), e0, e1);
+                x[e] = __float_as_uint(Exp2(e0));
+                x[e + 1] = __float_as_uint(Exp2(e1));
             }
             BarWait(&sh.dpFull, it & 1, failed);
             TcFenceAfter();
             float most = 0.0f;
+            {
+                uint32_t y[kColumns];
+                TmemLoad32(tDp + kColumns * side + lanes, y);
 #pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-                uint32_t y[32];
-                TmemLoad32(tDp + 64 * side + lanes + c, y);
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
+                for (int e = 0; e < kColumns; e += 2) {
                     const F2 d = Mul2(Add2(MakeF2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), delta2),
-                                      MakeF2(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1])));
+                                      MakeF2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
                     float d0, d1;
                     SplitF2(d, d0, d1);
-                    x[c + e] = __float_as_uint(d0);
-                    x[c + e + 1] = __float_as_uint(d1);
+                    x[e] = __float_as_uint(d0);
+                    x[e + 1] = __float_as_uint(d1);
                     if constexpr (DType<T>::kIsHalf) {
                         most = fmaxf(most, fmaxf(fabsf(d0), fabsf(d1)));
                     }
@@ -781,23 +826,15 @@ __global__ void __launch_bounds__(320, 1)
             }
             float scale = 1.0f;
             if constexpr (DType<T>::kIsHalf) {
-                sh.most[it & 1][side][r] = static_cast<uint8_t>(ExponentOf(most));
-                BarArrive(&sh.exchanged);
-                BarWait(&sh.exchanged, it & 1, failed);
-                const float change = range.Follow(max(ExponentOf(most), static_cast<uint32_t>(sh.most[it & 1][side ^ 1][r])));
+                const float change = range.Follow(LargestOfRow(sh.most[it & 1], side, r, most, &sh.exchanged, it & 1, failed));
                 scale = range.scale;
-                if (it > 0 && __any_sync(0xffffffffu, change != 1.0f)) {
+                if (it > 0 && __any_sync(0xffffffffu, change != 1.0f)) { // in all warps of the rows alike
                     BarWait(&sh.dqDone, (it - 1) & 1, failed);
                     TcFenceAfter();
-                    TmemScale<32 * HALVES>(tDq + lanes + 32 * HALVES * side, change);
+                    TmemScale<kOwn>(tDq + lanes + kOwn * side, change);
                 }
             }
-            uint32_t w[32];
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-                w[c] = PackPair(__uint_as_float(x[2 * c]) * scale, __uint_as_float(x[2 * c + 1]) * scale, static_cast<const T*>(nullptr));
-            }
-            TmemStore32(tx, w);
+            StoreWeights<T>(tx, x, scale);
             TmemStoreWait();
             TcFenceBefore();
             BarArrive(&sh.dsReady);
@@ -809,30 +846,29 @@ __global__ void __launch_bounds__(320, 1)
         T* out = i < s.lq ? OutRowOf<T>(m.a.gradQ, b, i, h) : nullptr;
         const float last = s.scale * kWeightScale / range.scale;
         bool bad = false;
-#pragma unroll
-        for (int c = 0; c < HALVES; ++c) {
-            const int32_t d0 = 32 * (HALVES * side + c);
-            uint32_t o[32];
+        {
+            const int32_t d0 = kOwn * side;
+            uint32_t o[kOwn];
             if (count > 0) {
-                TmemLoad32(tDq + lanes + d0, o);
+                TmemLoadOwn<kOwn>(tDq + lanes + d0, o);
             }
-            float v[32];
+            float v[kOwn];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
+            for (int e = 0; e < kOwn; ++e) {
                 v[e] = p >= 0 ? __uint_as_float(o[e]) * last : 0.0f;
                 bad = bad || (d0 + e < s.dim && !(fabsf(v[e]) <= 3.4e38f));
             }
             if (out != nullptr && d0 < s.dim) {
-                StoreRow32<T>(out + d0, v, s.dim - d0, m.vecQ);
+                StoreRow<T>(out + d0, v, s.dim - d0, m.vecQ);
             }
         }
         const uint32_t rows = __ballot_sync(0xffffffffu, bad && out != nullptr);
         if ((threadIdx.x & 31) == 0 && rows != 0) {
             atomicOr(&sh.bad[warp & 3], rows);
         }
-        RowBarrier();
-        // rows that are not finite again, without the masked keys' part: the even ones by one warp, the odd ones by another
-        uint32_t again = sh.bad[warp & 3] & (side == 0 ? 0x55555555u : 0xaaaaaaaau);
+        RowBarrier<kGradThreads>();
+        // rows that are not finite again, without the masked keys' part, shared out among the rows' warps
+        uint32_t again = sh.bad[warp & 3] & (0x11111111u << side);
         while (again != 0) {
             const int e = __ffs(again) - 1;
             again &= again - 1;
@@ -846,7 +882,7 @@ __global__ void __launch_bounds__(320, 1)
     }
     TcFenceBefore();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kProductWarp) {
         TcFenceAfter();
         TmemFree(sh.tmem, 512);
     }
@@ -858,7 +894,7 @@ __global__ void __launch_bounds__(320, 1)
 struct GradKvShared {
     uint64_t kvFull, full[2], empty[2], sFull, dpFull, pReady, dsReady, dvDone, dkDone, exchanged, drain;
     uint32_t tmem, failed, bad[4];
-    uint8_t most[2][2][kTile]; // fp16: exponents of a row's largest ds, of even and odd steps, of its two threads
+    uint8_t most[2][kSides][kTile]; // fp16: exponents of a row's largest ds, of even and odd steps, of its threads
 };
 
 // Tensor memory: S^T at 0 (the weights go over it), dP^T at 128 (ds goes over it), gradV at 256, gradK at 384; rows are keys, columns
@@ -869,13 +905,9 @@ struct GradKvShared {
 // walk a window; so the queries behind the window of such a tile are shared out among farChunks further blocks. Their sums and the
 // tile's own go to `partial` ([tile][1 + farChunks][gradK, gradV][128][dim], fp32), which AttnSinkGradKernel adds up in order.
 template <typename T, int KS>
-__global__ void __launch_bounds__(320, 1)
-    AttnGradKvMmaKernel(const __grid_constant__ BackwardArgs m, const __grid_constant__ CUtensorMap mapQ,
-                        const __grid_constant__ CUtensorMap mapG, const __grid_constant__ CUtensorMap mapK,
-                        const __grid_constant__ CUtensorMap mapV)
+__device__ __forceinline__ void GradKvBlock(const BackwardArgs& m, const CUtensorMap& mapQ, const CUtensorMap& mapG, const CUtensorMap& mapK,
+                                            const CUtensorMap& mapV, uint32_t block, unsigned char* raw, GradKvShared& sh)
 {
-    extern __shared__ unsigned char raw[];
-    __shared__ GradKvShared sh;
     constexpr int HALVES = KS > 4 ? 2 : 1;
     constexpr uint32_t kBytes = HALVES * kHalfBytes;
     constexpr uint32_t kStage = 2 * kBytes + 2 * kTile * 4;
@@ -884,9 +916,9 @@ __global__ void __launch_bounds__(320, 1)
     float* stats = reinterpret_cast<float*>(base + 6 * kBytes);              // two stages of lse2 and delta
     const AttnShape& s = m.a.s;
     const int32_t perHead = m.kTiles + m.sinkTiles * m.farChunks;
-    const int32_t bu = blockIdx.x / perHead;
+    const int32_t bu = block / perHead;
     const int32_t b = bu / s.kvHeads, u = bu % s.kvHeads;
-    int32_t tile = blockIdx.x % perHead, chunk = -1;
+    int32_t tile = block % perHead, chunk = -1;
     if (tile >= m.kTiles) {
         chunk = (tile - m.kTiles) % m.farChunks;
         tile = (tile - m.kTiles) / m.farChunks;
@@ -926,18 +958,18 @@ __global__ void __launch_bounds__(320, 1)
         }
         BarInit(&sh.sFull, 1);
         BarInit(&sh.dpFull, 1);
-        BarInit(&sh.pReady, kRowThreads);
-        BarInit(&sh.dsReady, kRowThreads);
+        BarInit(&sh.pReady, kGradThreads);
+        BarInit(&sh.dsReady, kGradThreads);
         BarInit(&sh.dvDone, 1);
         BarInit(&sh.dkDone, 1);
-        BarInit(&sh.exchanged, kRowThreads);
+        BarInit(&sh.exchanged, kGradThreads);
         BarInit(&sh.drain, 1);
         BarInitDone();
     }
     if (threadIdx.x < 4) {
         sh.bad[threadIdx.x] = 0;
     }
-    if (warp == 9) {
+    if (warp == kProductWarp) {
         TmemAlloc(&sh.tmem, 512);
     }
     TcFenceBefore();
@@ -946,7 +978,7 @@ __global__ void __launch_bounds__(320, 1)
     const uint32_t tS = sh.tmem, tDp = tS + 128, tDv = tS + 256, tDk = tS + 384;
     volatile uint32_t* failed = &sh.failed;
 
-    if (warp == 8) {
+    if (warp == kLoadWarp) {
         if ((threadIdx.x & 31) == 0 && count > 0) {
             auto load = [&](unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int32_t row, int32_t head) {
 #pragma unroll
@@ -980,7 +1012,7 @@ __global__ void __launch_bounds__(320, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == kProductWarp) {
         if (count > 0) {
             const bool lead = ElectOne();
             const uint32_t descS = ProductDesc<T>(kTile, false, s.scale < 0.0f), descDp = ProductDesc<T>(kTile, false, false);
@@ -1048,6 +1080,7 @@ __global__ void __launch_bounds__(320, 1)
         }
         __syncwarp();
     } else {
+        constexpr int kOwn = 64 * HALVES / kSides; // columns of the sums that a thread has
         const int32_t side = warp >> 2, r = (warp & 3) * 32 + (threadIdx.x & 31);
         const int32_t j = j0 + r;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
@@ -1059,65 +1092,56 @@ __global__ void __launch_bounds__(320, 1)
         RowScale range;
         for (int32_t it = 0; it < count; ++it) {
             const int32_t st = it & 1;
-            const int32_t p0 = n.shift + iBase + (begin + it) % perGroup * kTile + 64 * side;
+            const int32_t p0 = n.shift + iBase + (begin + it) % perGroup * kTile + kColumns * side;
             BarWait(&sh.full[st], (it >> 1) & 1, failed); // the statistics
             BarWait(&sh.sFull, it & 1, failed);
             if (__any_sync(0xffffffffu, *failed != 0)) {
                 break;
             }
             TcFenceAfter();
-            uint32_t x[64];
-            TmemLoad64(tS + 64 * side + lanes, x);
-            if (!__all_sync(0xffffffffu, from <= p0 && to >= p0 + 64)) {
-                uint32_t live[2];
-                LiveColumns<64>(live, from - p0, to - p0, 0);
-                MaskColumns<64>(x, live);
+            uint32_t x[kColumns];
+            TmemLoad32(tS + kColumns * side + lanes, x);
+            if (!__all_sync(0xffffffffu, from <= p0 && to >= p0 + kColumns)) {
+                uint32_t live[1];
+                LiveColumns<kColumns>(live, from - p0, to - p0, 0);
+                MaskColumns<kColumns>(x, live);
             }
-            const float4* lse = reinterpret_cast<const float4*>(stats + st * 2 * kTile + 64 * side);
-            const float4* del = reinterpret_cast<const float4*>(stats + st * 2 * kTile + kTile + 64 * side);
+            const float4* lse = reinterpret_cast<const float4*>(stats + st * 2 * kTile + kColumns * side);
+            const float4* del = reinterpret_cast<const float4*>(stats + st * 2 * kTile + kTile + kColumns * side);
 #pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-                uint32_t w[16];
+            for (int e = 0; e < kColumns; e += 4) {
+                const float4 l = lse[e / 4];
+                float z[4];
+                SplitF2(Fma2(MakeF2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), factor2, MakeF2(-l.x, -l.y)), z[0], z[1]);
+                SplitF2(Fma2(MakeF2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), factor2, MakeF2(-l.z, -l.w)), z[2], z[3]);
 #pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    const float4 l = lse[(c + e) / 4];
-                    float z[4];
-                    SplitF2(Fma2(MakeF2(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1])), factor2, MakeF2(-l.x, -l.y)), z[0], z[1]);
-                    SplitF2(Fma2(MakeF2(__uint_as_float(x[c + e + 2]), __uint_as_float(x[c + e + 3])), factor2, MakeF2(-l.z, -l.w)), z[2],
-                            z[3]);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        z[k] = Exp2(z[k]);
-                        x[c + e + k] = __float_as_uint(z[k]);
-                    }
-                    w[e / 2] = PackPair(z[0], z[1], static_cast<const T*>(nullptr));
-                    w[e / 2 + 1] = PackPair(z[2], z[3], static_cast<const T*>(nullptr));
+                for (int k = 0; k < 4; ++k) {
+                    x[e + k] = __float_as_uint(Exp2(z[k]));
                 }
-                TmemStore16(tS + 64 * side + lanes + c / 2, w);
             }
+            StoreWeights<T>(tS + kColumns * side + lanes, x, 1.0f);
             TmemStoreWait();
             TcFenceBefore();
             BarArrive(&sh.pReady);
             BarWait(&sh.dpFull, it & 1, failed);
             TcFenceAfter();
             float most = 0.0f;
+            {
+                uint32_t y[kColumns];
+                TmemLoad32(tDp + kColumns * side + lanes, y);
 #pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-                uint32_t y[32];
-                TmemLoad32(tDp + 64 * side + lanes + c, y);
-#pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    const float4 d = del[(c + e) / 4];
+                for (int e = 0; e < kColumns; e += 4) {
+                    const float4 d = del[e / 4];
                     float z[4];
                     SplitF2(Mul2(Add2(MakeF2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), MakeF2(-d.x, -d.y)),
-                                 MakeF2(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1]))),
+                                 MakeF2(__uint_as_float(x[e]), __uint_as_float(x[e + 1]))),
                             z[0], z[1]);
                     SplitF2(Mul2(Add2(MakeF2(__uint_as_float(y[e + 2]), __uint_as_float(y[e + 3])), MakeF2(-d.z, -d.w)),
-                                 MakeF2(__uint_as_float(x[c + e + 2]), __uint_as_float(x[c + e + 3]))),
+                                 MakeF2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]))),
                             z[2], z[3]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        x[c + e + k] = __float_as_uint(z[k]);
+                        x[e + k] = __float_as_uint(z[k]);
                         if constexpr (DType<T>::kIsHalf) {
                             most = fmaxf(most, fabsf(z[k]));
                         }
@@ -1126,23 +1150,15 @@ __global__ void __launch_bounds__(320, 1)
             }
             float scale = 1.0f;
             if constexpr (DType<T>::kIsHalf) {
-                sh.most[it & 1][side][r] = static_cast<uint8_t>(ExponentOf(most));
-                BarArrive(&sh.exchanged);
-                BarWait(&sh.exchanged, it & 1, failed);
-                const float change = range.Follow(max(ExponentOf(most), static_cast<uint32_t>(sh.most[it & 1][side ^ 1][r])));
+                const float change = range.Follow(LargestOfRow(sh.most[it & 1], side, r, most, &sh.exchanged, it & 1, failed));
                 scale = range.scale;
                 if (it > 0 && __any_sync(0xffffffffu, change != 1.0f)) {
                     BarWait(&sh.dkDone, (it - 1) & 1, failed);
                     TcFenceAfter();
-                    TmemScale<32 * HALVES>(tDk + lanes + 32 * HALVES * side, change);
+                    TmemScale<kOwn>(tDk + lanes + kOwn * side, change);
                 }
             }
-            uint32_t w[32];
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-                w[c] = PackPair(__uint_as_float(x[2 * c]) * scale, __uint_as_float(x[2 * c + 1]) * scale, static_cast<const T*>(nullptr));
-            }
-            TmemStore32(tDp + 64 * side + lanes, w);
+            StoreWeights<T>(tDp + kColumns * side + lanes, x, scale);
             TmemStoreWait();
             TcFenceBefore();
             BarArrive(&sh.dsReady);
@@ -1161,28 +1177,25 @@ __global__ void __launch_bounds__(320, 1)
                                                   kTile * s.dim + static_cast<int64_t>(r) * s.dim :
                                   nullptr;
             T* out = lives && !split ? OutRowOf<T>(which == 0 ? m.a.gradK : m.a.gradV, b, j, u) : nullptr;
+            const int32_t d0 = kOwn * side;
+            uint32_t o[kOwn];
+            if (count > 0) {
+                TmemLoadOwn<kOwn>(from32 + d0, o);
+            }
+            float v[kOwn];
 #pragma unroll
-            for (int c = 0; c < HALVES; ++c) {
-                const int32_t d0 = 32 * (HALVES * side + c);
-                uint32_t o[32];
-                if (count > 0) {
-                    TmemLoad32(from32 + d0, o);
-                }
-                float v[32];
+            for (int e = 0; e < kOwn; ++e) {
+                v[e] = count > 0 && j < n.kv ? __uint_as_float(o[e]) * last : 0.0f;
+                bad = bad || (d0 + e < s.dim && !(fabsf(v[e]) <= 3.4e38f));
+            }
+            if (out != nullptr && d0 < s.dim) {
+                StoreRow<T>(out + d0, v, s.dim - d0, which == 0 ? m.vecK : m.vecV);
+            }
+            if (part != nullptr) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    v[e] = count > 0 && j < n.kv ? __uint_as_float(o[e]) * last : 0.0f;
-                    bad = bad || (d0 + e < s.dim && !(fabsf(v[e]) <= 3.4e38f));
-                }
-                if (out != nullptr && d0 < s.dim) {
-                    StoreRow32<T>(out + d0, v, s.dim - d0, which == 0 ? m.vecK : m.vecV);
-                }
-                if (part != nullptr) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        if (d0 + e < s.dim) {
-                            part[d0 + e] = *failed != 0 ? NAN : v[e];
-                        }
+                for (int e = 0; e < kOwn; ++e) {
+                    if (d0 + e < s.dim) {
+                        part[d0 + e] = *failed != 0 ? NAN : v[e];
                     }
                 }
             }
@@ -1191,8 +1204,8 @@ __global__ void __launch_bounds__(320, 1)
         if ((threadIdx.x & 31) == 0 && rows != 0) {
             atomicOr(&sh.bad[warp & 3], rows);
         }
-        RowBarrier();
-        uint32_t again = sh.bad[warp & 3] & (side == 0 ? 0x55555555u : 0xaaaaaaaau);
+        RowBarrier<kGradThreads>();
+        uint32_t again = sh.bad[warp & 3] & (0x11111111u << side);
         while (again != 0) {
             const int e = __ffs(again) - 1;
             again &= again - 1;
@@ -1207,12 +1220,30 @@ __global__ void __launch_bounds__(320, 1)
     }
     TcFenceBefore();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kProductWarp) {
         TcFenceAfter();
         TmemFree(sh.tmem, 512);
     }
     if (threadIdx.x == 0 && sh.failed != 0) {
         atomicAdd(&g_attentionTimeouts, 1u);
+    }
+}
+
+template <typename T, int KS>
+__global__ void __launch_bounds__(kGradThreads + 64, 1)
+    AttnGradMmaKernel(const __grid_constant__ BackwardArgs m, const __grid_constant__ CUtensorMap mapQ,
+                      const __grid_constant__ CUtensorMap mapG, const __grid_constant__ CUtensorMap mapK,
+                      const __grid_constant__ CUtensorMap mapV)
+{
+    extern __shared__ unsigned char raw[];
+    __shared__ union {
+        GradQShared q;
+        GradKvShared kv;
+    } sh;
+    if (blockIdx.x < m.kvBlocks) {
+        GradKvBlock<T, KS>(m, mapQ, mapG, mapK, mapV, blockIdx.x, raw, sh.kv);
+    } else {
+        GradQBlock<T, KS>(m, mapQ, mapG, mapK, mapV, blockIdx.x - m.kvBlocks, raw, sh.q);
     }
 }
 
@@ -1347,7 +1378,7 @@ namespace {
 
 bool VecRows(const AttnTensor& t, int32_t dim) { return dim % 8 == 0 && Aligned(t.p, 16) && t.l % 8 == 0 && t.h % 8 == 0 && t.b % 8 == 0; }
 
-// Further blocks for the sinks' far queries (AttnGradKvMmaKernel): as many as bring their walks down to that of an ordinary block.
+// Further blocks for the sinks' far queries (GradKvBlock): as many as bring their walks down to that of an ordinary block.
 struct FarPlan {
     int32_t sinkTiles = 0, chunks = 0;
 };
@@ -1375,24 +1406,22 @@ namespace {
 struct BackwardLaunch {
     const BackwardArgs& m;
     const CUtensorMap &mq, &mg, &mk, &mv;
-    unsigned statBlocks, qBlocks, kvBlocks;
-    int sharedQ, sharedKv;
+    unsigned statBlocks, blocks;
+    int shared;
     bool vecStats;
 };
 template <typename T>
 cudaError_t LaunchBackward(const BackwardLaunch& l, cudaStream_t stream)
 {
     const BackwardArgs& m = l.m;
-    auto launch = [&](auto gradQ, auto gradKv, std::atomic<uint64_t>(&asked)[2]) {
-        cudaError_t set = AskOnce(gradQ, asked[0], l.sharedQ);
-        set = set != cudaSuccess ? set : AskOnce(gradKv, asked[1], l.sharedKv);
+    auto launch = [&](auto kernel, std::atomic<uint64_t>& asked) {
+        const cudaError_t set = AskOnce(kernel, asked, l.shared);
         if (set != cudaSuccess) {
             return set;
         }
         AttnStatisticsKernel<T><<<l.statBlocks, 256, 0, stream>>>(m, l.vecStats);
-        gradQ<<<l.qBlocks, 320, l.sharedQ, stream>>>(m, l.mq, l.mg, l.mk, l.mv);
-        gradKv<<<l.kvBlocks, 320, l.sharedKv, stream>>>(m, l.mq, l.mg, l.mk, l.mv);
-        CountLaunch(3);
+        kernel<<<l.blocks, kGradThreads + 64, l.shared, stream>>>(m, l.mq, l.mg, l.mk, l.mv);
+        CountLaunch(2);
         if (m.farChunks > 0) {
             const int64_t keys = static_cast<int64_t>(m.a.s.batch) * m.a.s.kvHeads * m.sinkTiles * kTile;
             AttnSinkGradKernel<T><<<static_cast<unsigned>(CeilDiv(keys, 4)), 128, 0, stream>>>(m);
@@ -1400,13 +1429,13 @@ cudaError_t LaunchBackward(const BackwardLaunch& l, cudaStream_t stream)
         }
         return cudaGetLastError();
     };
-    static std::atomic<uint64_t> asked[5][2];
+    static std::atomic<uint64_t> asked[5];
     const int32_t steps = static_cast<int32_t>(CeilDiv(m.a.s.dim, 16));
-    return steps <= 2 ? launch(AttnGradQMmaKernel<T, 2>, AttnGradKvMmaKernel<T, 2>, asked[0]) :
-           steps <= 4 ? launch(AttnGradQMmaKernel<T, 4>, AttnGradKvMmaKernel<T, 4>, asked[1]) :
-           steps <= 5 ? launch(AttnGradQMmaKernel<T, 5>, AttnGradKvMmaKernel<T, 5>, asked[2]) :
-           steps <= 6 ? launch(AttnGradQMmaKernel<T, 6>, AttnGradKvMmaKernel<T, 6>, asked[3]) :
-                        launch(AttnGradQMmaKernel<T, 8>, AttnGradKvMmaKernel<T, 8>, asked[4]);
+    return steps <= 2 ? launch(AttnGradMmaKernel<T, 2>, asked[0]) :
+           steps <= 4 ? launch(AttnGradMmaKernel<T, 4>, asked[1]) :
+           steps <= 5 ? launch(AttnGradMmaKernel<T, 5>, asked[2]) :
+           steps <= 6 ? launch(AttnGradMmaKernel<T, 6>, asked[3]) :
+                        launch(AttnGradMmaKernel<T, 8>, asked[4]);
 }
 
 } // namespace
@@ -1451,11 +1480,14 @@ cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStrea
     }
     const int32_t halves = s.dim > 64 ? 2 : 1;
     const int bytes = halves * static_cast<int>(kHalfBytes);
-    const int sharedQ = 7 * bytes + 1024, sharedKv = 6 * bytes + 4 * kTile * 4 + 1024;
-    const unsigned qBlocks = static_cast<unsigned>(static_cast<int64_t>(s.batch) * s.heads * m.qTiles);
+    const int shared = std::max(7 * bytes, 6 * bytes + 4 * kTile * 4) + 1024; // gradQ's tiles, gradK's and gradV's with two places of statistics
+    const int64_t blocks = kvBlocks + static_cast<int64_t>(s.batch) * s.heads * m.qTiles;
+    if (blocks > INT32_MAX) {
+        return cudaErrorInvalidConfiguration;
+    }
+    m.kvBlocks = static_cast<uint32_t>(kvBlocks);
     const bool vecStats = VecRows(a.gradOut, s.dim) && VecRows(a.out, s.dim);
-    const BackwardLaunch l{m, mq, mg, mk, mv, static_cast<unsigned>(statBlocks), qBlocks, static_cast<unsigned>(kvBlocks), sharedQ, sharedKv,
-                           vecStats};
+    const BackwardLaunch l{m, mq, mg, mk, mv, static_cast<unsigned>(statBlocks), static_cast<unsigned>(blocks), shared, vecStats};
     return dt == Dt::F16 ? LaunchBackward<__half>(l, stream) : LaunchBackward<__nv_bfloat16>(l, stream);
 }
 
