@@ -71,9 +71,9 @@ cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& s, AttnTensor q, AttnTens
 
 uint64_t WindowAttentionBwdWorkspace(Dt dt, const AttnShape& s)
 {
-    const uint64_t rows = static_cast<uint64_t>(s.batch) * s.heads * s.lq * 4;
+    const uint64_t tiles = AttnBackwardTilesWorkspace(s);
     const uint64_t mma = dt != Dt::F32 && s.dim <= kMmaMostDim ? AttnBackwardMmaWorkspace(s) : 0;
-    return rows > mma ? rows : mma; // which kernels a call takes is known only with the pointers
+    return tiles > mma ? tiles : mma; // which kernels a call takes is known only with the pointers
 }
 
 cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& s, AttnTensor gradOut, AttnTensor q, AttnTensor k, AttnTensor v, AttnTensor out,
@@ -108,7 +108,7 @@ cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& s, AttnTensor gradOut, At
             return e;
         }
     }
-    return AttnBackwardTiles(dt, a, stream);
+    return AttnBackwardTiles(dt, a, workspace, stream);
 }
 
 } // namespace opscv

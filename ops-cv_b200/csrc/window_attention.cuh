@@ -257,7 +257,9 @@ uint32_t AttnStepTimeouts();
 
 // ---- fp32 arithmetic (window_attention_tiles.cu) -------------------------------------------------------------------------------
 cudaError_t AttnForwardTiles(Dt dt, const AttnArgs& a, cudaStream_t stream);
-cudaError_t AttnBackwardTiles(Dt dt, const AttnArgs& a, cudaStream_t stream); // a.delta is filled
+// a.delta is the start of the workspace, and filled
+uint64_t AttnBackwardTilesWorkspace(const AttnShape& s);
+cudaError_t AttnBackwardTiles(Dt dt, const AttnArgs& a, void* workspace, cudaStream_t stream);
 
 // ---- tensor-core kernels (window_attention_mma.cu) ---------------------------------------------------------------------------
 bool AttnTmaReadable(const AttnTensor& t, int32_t tokens, int32_t heads, int32_t batch);

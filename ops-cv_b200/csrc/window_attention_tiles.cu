@@ -14,11 +14,12 @@ namespace {
 constexpr int kThreads = 256; // 16 x 16
 
 // DP: values of a head, padded; ROWS: queries and keys of a tile. 64 x 64 tiles of up to 128 values, 32 x 32 ones of 256.
+// DP is a multiple of 32.
 template <int DP>
 struct Tile {
     static constexpr int kRows = DP <= 128 ? 64 : 32;
     static constexpr int kMicro = kRows / 16;  // rows (and columns) of a thread
-    static constexpr int kQuads = DP / 64;     // blocks of 4 values of a row that a thread has
+    static constexpr int kPairs = DP / 32;     // pairs of values of a row that a thread has
     static constexpr int kStride = DP + 4;     // floats of a row: 4 more shift neighbouring rows to other banks
     static constexpr int kWeights = kRows + 4; // the same for the rows of weights
     static constexpr int kTileFloats = kRows * kStride;
@@ -87,14 +88,14 @@ __device__ __forceinline__ void Inner(const float* a, const float* b, float (&s)
     }
 }
 
-// o[r] += sum over j of w[micro * ty + r][j] row j of v, values 4 tx + 64 c to + 3
+// o[r] += sum over j of w[micro * ty + r][j] row j of v, values 2 tx + 32 c and the next
 template <int DP>
-__device__ __forceinline__ void Outer(const float* w, const float* v, float4 (&o)[Tile<DP>::kMicro][Tile<DP>::kQuads])
+__device__ __forceinline__ void Outer(const float* w, const float* v, float2 (&o)[Tile<DP>::kMicro][Tile<DP>::kPairs])
 {
     using L = Tile<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const float* pw = w + L::kMicro * ty * L::kWeights;
-    const float* pv = v + 4 * tx;
+    const float* pv = v + 2 * tx;
 #pragma unroll 2
     for (int j = 0; j < L::kRows; j += 4) {
         float4 x[L::kMicro];
@@ -105,15 +106,13 @@ __device__ __forceinline__ void Outer(const float* w, const float* v, float4 (&o
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
 #pragma unroll
-            for (int c = 0; c < L::kQuads; ++c) {
-                const float4 y = *reinterpret_cast<const float4*>(pv + (j + k) * L::kStride + 64 * c);
+            for (int c = 0; c < L::kPairs; ++c) {
+                const float2 y = *reinterpret_cast<const float2*>(pv + (j + k) * L::kStride + 32 * c);
 #pragma unroll
                 for (int r = 0; r < L::kMicro; ++r) {
                     const float z = k == 0 ? x[r].x : k == 1 ? x[r].y : k == 2 ? x[r].z : x[r].w;
                     o[r][c].x = fmaf(z, y.x, o[r][c].x);
                     o[r][c].y = fmaf(z, y.y, o[r][c].y);
-                    o[r][c].z = fmaf(z, y.z, o[r][c].z);
-                    o[r][c].w = fmaf(z, y.w, o[r][c].w);
                 }
             }
         }
@@ -121,16 +120,16 @@ __device__ __forceinline__ void Outer(const float* w, const float* v, float4 (&o
 }
 
 template <typename T>
-__device__ __forceinline__ bool StoreQuad(T* out, const float4& v, int32_t d, int32_t dim) // true: not all finite
+__device__ __forceinline__ bool StorePair(T* out, const float2& v, int32_t d, int32_t dim) // true: not all finite
 {
-    const float x[4] = {v.x, v.y, v.z, v.w};
     bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (d + e < dim) {
-            out[d + e] = DType<T>::FromF(x[e]);
-            bad = bad || !(fabsf(x[e]) <= 3.4e38f);
-        }
+    if (d < dim) {
+        out[d] = DType<T>::FromF(v.x);
+        bad = !(fabsf(v.x) <= 3.4e38f);
+    }
+    if (d + 1 < dim) {
+        out[d + 1] = DType<T>::FromF(v.y);
+        bad = bad || !(fabsf(v.y) <= 3.4e38f);
     }
     return bad;
 }
@@ -178,7 +177,18 @@ struct TileArgs {
     AttnArgs a;
     int32_t tiles;
     bool vec; // rows can be read 4 values at a time
+    // gradK and gradV, see there
+    bool perHead;
+    int32_t sinkTiles, chunks;
+    float* partial; // null: blocks write the results
 };
+// Where a block's sums start: the tiles of a unit (a head or key head), each with its chunks behind it where it has sinks.
+__device__ __forceinline__ int64_t PartialSlot(const TileArgs& m, int32_t unit, int32_t tile, int32_t slot, int32_t rows)
+{
+    const int64_t perUnit = m.tiles + static_cast<int64_t>(m.sinkTiles) * m.chunks;
+    const int64_t at = tile + static_cast<int64_t>(min(tile, m.sinkTiles)) * m.chunks + slot;
+    return (unit * perUnit + at) * 2 * rows * m.a.s.dim;
+}
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP>
@@ -200,7 +210,7 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
         again[threadIdx.x] = 0;
     }
     LoadTile<T, DP>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
-    float4 o[R][L::kQuads] = {};
+    float2 o[R][L::kPairs] = {};
     float top[R], total[R];
     int32_t p[R];
 #pragma unroll
@@ -238,8 +248,8 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
             }
             total[r] = total[r] * fade + sum;
 #pragma unroll
-            for (int c = 0; c < L::kQuads; ++c) {
-                o[r][c] = make_float4(o[r][c].x * fade, o[r][c].y * fade, o[r][c].z * fade, o[r][c].w * fade);
+            for (int c = 0; c < L::kPairs; ++c) {
+                o[r][c] = make_float2(o[r][c].x * fade, o[r][c].y * fade);
             }
         }
         __syncthreads();
@@ -257,10 +267,9 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
         if (i < s.lq) {
             T* out = OutRowOf<T>(m.a.out, b, i, h);
 #pragma unroll
-            for (int c = 0; c < L::kQuads; ++c) {
-                const float4 v = some ? make_float4(o[r][c].x * inverse, o[r][c].y * inverse, o[r][c].z * inverse, o[r][c].w * inverse) :
-                                        make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                bad = StoreQuad<T>(out, v, 4 * tx + 64 * c, s.dim) || bad;
+            for (int c = 0; c < L::kPairs; ++c) {
+                const float2 v = some ? make_float2(o[r][c].x * inverse, o[r][c].y * inverse) : make_float2(0.0f, 0.0f);
+                bad = StorePair<T>(out, v, 2 * tx + 32 * c, s.dim) || bad;
             }
             if (tx == 0 && m.a.lse != nullptr) {
                 m.a.lse[static_cast<int64_t>(bh) * s.lq + i] = some ? top[r] + logf(sum) : -INFINITY;
@@ -300,7 +309,7 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
     }
     LoadTile<T, DP>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
     LoadTile<T, DP>(sg, m.a.gradOut, b, h, i0, iLast + 1, s.dim, m.vec);
-    float4 o[R][L::kQuads] = {};
+    float2 o[R][L::kPairs] = {};
     float lse[R], delta[R];
     int32_t p[R];
 #pragma unroll
@@ -338,9 +347,9 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
         if (i < s.lq) {
             T* out = OutRowOf<T>(m.a.gradQ, b, i, h);
 #pragma unroll
-            for (int c = 0; c < L::kQuads; ++c) {
-                const float4 v = p[r] >= 0 ? o[r][c] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                bad = StoreQuad<T>(out, v, 4 * tx + 64 * c, s.dim) || bad;
+            for (int c = 0; c < L::kPairs; ++c) {
+                const float2 v = p[r] >= 0 ? o[r][c] : make_float2(0.0f, 0.0f);
+                bad = StorePair<T>(out, v, 2 * tx + 32 * c, s.dim) || bad;
             }
         }
         if (bad) {
@@ -355,6 +364,10 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
     }
 }
 
+// A block has a tile of keys and the query heads of its key head. Where those blocks are too few for the SMs (`perHead`), a block has one
+// query head instead; and where sinks are seen by many more queries than a window's, these are shared out among `chunks` further blocks
+// of their tile. In both cases the blocks' sums go to `partial` in fp32 ([batch, heads or key heads, 1 + chunks of a tile with sinks,
+// gradK and gradV, rows of the tile, dim]), and AttnGradKvSumKernel adds them up in order.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_constant__ TileArgs m)
 {
@@ -366,20 +379,35 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
     float *sk = shared, *sv = sk + L::kTileFloats, *sq = sv + L::kTileFloats, *sg = sq + L::kTileFloats, *sw = sg + L::kTileFloats,
           *sd = sw + L::kWeightFloats;
     const AttnShape& s = m.a.s;
-    const int32_t tile = blockIdx.x % m.tiles, bu = blockIdx.x / m.tiles;
-    const int32_t b = bu / s.kvHeads, u = bu % s.kvHeads;
+    const int32_t perUnit = m.tiles + m.sinkTiles * m.chunks;
+    int32_t tile = blockIdx.x % perUnit, chunk = -1;
+    const int32_t unit = blockIdx.x / perUnit, units = m.perHead ? s.heads : s.kvHeads;
+    if (tile >= m.tiles) {
+        chunk = (tile - m.tiles) % m.chunks;
+        tile = (tile - m.tiles) / m.chunks;
+    }
+    const int32_t b = unit / units, u = m.perHead ? unit % units / m.a.group : unit % units;
+    const int32_t hFirst = m.perHead ? unit % units : u * m.a.group, hEnd = m.perHead ? hFirst + 1 : hFirst + m.a.group;
+    const bool far = m.chunks > 0 && tile < m.sinkTiles; // its far queries are others'
     const Lengths n = LengthsOf(s, b);
     const int32_t j0 = tile * L::kRows, jLast = min(j0 + L::kRows, n.kv) - 1, end = n.kv - 1;
-    // positions of the queries that see some key of the tile
-    const int32_t low = max(j0, max(n.shift, 0)), high = jLast < j0 ? -1 : j0 < s.sinks ? end : min(end, jLast + s.window - 1);
+    // positions of the queries that this block walks
+    int32_t low = max(j0, max(n.shift, 0)), high = jLast < j0 ? -1 : j0 < s.sinks && !far ? end : min(end, jLast + s.window - 1);
+    if (chunk >= 0) {
+        low = max(low, jLast + s.window);
+        const int32_t steps = end >= low ? (end - low + L::kRows) / L::kRows : 0, share = (steps + m.chunks - 1) / m.chunks;
+        high = jLast < j0 ? -1 : static_cast<int32_t>(min(static_cast<int64_t>(end), low + static_cast<int64_t>(chunk + 1) * share * L::kRows - 1));
+        low += chunk * share * L::kRows;
+    }
+    const int32_t stop = high; // queries behind it are another block's
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     if (threadIdx.x < 2) {
         again[threadIdx.x] = 0;
     }
     LoadTile<T, DP>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
     LoadTile<T, DP>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
-    float4 ok[R][L::kQuads] = {}, ov[R][L::kQuads] = {};
-    for (int32_t h = u * m.a.group; h < (u + 1) * m.a.group; ++h) {
+    float2 ok[R][L::kPairs] = {}, ov[R][L::kPairs] = {};
+    for (int32_t h = hFirst; h < hEnd; ++h) {
         const int64_t head = static_cast<int64_t>(b) * s.heads + h;
         for (int32_t p0 = low; p0 <= high; p0 += L::kRows) {
             const int32_t i0 = p0 - n.shift;
@@ -401,7 +429,7 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
 #pragma unroll
                 for (int c = 0; c < R; ++c) {
                     const int32_t e = tx + 16 * c, p = p0 + e;
-                    const bool live = j < n.kv && p <= end && j <= p && (j > p - s.window || j < s.sinks);
+                    const bool live = j < n.kv && p <= stop && j <= p && (j > p - s.window || j < s.sinks);
                     const float w = live ? expf(x[r][c] * s.scale - sLse[e]) : 0.0f;
                     sw[(R * ty + r) * L::kWeights + e] = w;
                     sd[(R * ty + r) * L::kWeights + e] = live ? w * (y[r][c] - sDelta[e]) * s.scale : 0.0f;
@@ -412,6 +440,19 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
             Outer<DP>(sd, sq, ok);
         }
     }
+    if (m.partial != nullptr) {
+        float* part = m.partial + PartialSlot(m, unit, tile, 1 + chunk, L::kRows);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int c = 0; c < L::kPairs; ++c) {
+                const int32_t at = (R * ty + r) * s.dim, d = 2 * tx + 32 * c;
+                StorePair<float>(part + at, ok[r][c], d, s.dim);
+                StorePair<float>(part + L::kRows * s.dim + at, ov[r][c], d, s.dim);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int32_t j = j0 + R * ty + r;
@@ -419,9 +460,9 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
         if (j < s.lk) {
             T *gk = OutRowOf<T>(m.a.gradK, b, j, u), *gv = OutRowOf<T>(m.a.gradV, b, j, u);
 #pragma unroll
-            for (int c = 0; c < L::kQuads; ++c) {
-                bad = StoreQuad<T>(gk, ok[r][c], 4 * tx + 64 * c, s.dim) || bad;
-                bad = StoreQuad<T>(gv, ov[r][c], 4 * tx + 64 * c, s.dim) || bad;
+            for (int c = 0; c < L::kPairs; ++c) {
+                bad = StorePair<T>(gk, ok[r][c], 2 * tx + 32 * c, s.dim) || bad;
+                bad = StorePair<T>(gv, ov[r][c], 2 * tx + 32 * c, s.dim) || bad;
             }
         }
         if (bad) {
@@ -433,6 +474,39 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
         if ((again[r >> 5] >> (r & 31) & 1) != 0 && j0 + r < s.lk) {
             AttnGradKvRow<T>(m.a, b, u, j0 + r);
         }
+    }
+}
+
+// A warp per key.
+template <typename T>
+__global__ void __launch_bounds__(128) AttnGradKvSumKernel(const __grid_constant__ TileArgs m, int32_t rows)
+{
+    const AttnShape& s = m.a.s;
+    const int lane = threadIdx.x & 31;
+    const int64_t key = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5); // (batch, key head, key)
+    if (key >= static_cast<int64_t>(s.batch) * s.kvHeads * s.lk) {
+        return;
+    }
+    const int32_t j = static_cast<int32_t>(key % s.lk), bu = static_cast<int32_t>(key / s.lk), b = bu / s.kvHeads, u = bu % s.kvHeads;
+    const int32_t tile = j / rows, slots = tile < m.sinkTiles ? 1 + m.chunks : 1;
+    const int32_t first = m.perHead ? b * s.heads + u * m.a.group : bu, units = m.perHead ? m.a.group : 1;
+    bool bad = false;
+    for (int which = 0; which < 2; ++which) {
+        T* out = OutRowOf<T>(which == 0 ? m.a.gradK : m.a.gradV, b, j, u);
+        for (int32_t d = lane; d < s.dim; d += 32) {
+            float sum = 0.0f;
+            for (int32_t x = 0; x < units; ++x) {
+                for (int32_t c = 0; c < slots; ++c) {
+                    sum += m.partial[PartialSlot(m, first + x, tile, c, rows) + (which * rows + j % rows) * static_cast<int64_t>(s.dim) + d];
+                }
+            }
+            bad = bad || !(fabsf(sum) <= 3.4e38f);
+            out[d] = DType<T>::FromF(sum);
+        }
+    }
+    if (__any_sync(0xffffffffu, bad)) {
+        __syncwarp();
+        AttnGradKvRow<T>(m.a, b, u, j);
     }
 }
 
@@ -465,8 +539,35 @@ cudaError_t Forward(Dt dt, const AttnArgs& a, cudaStream_t stream)
     return cudaGetLastError();
 }
 
+// The blocks of gradK and gradV (see the kernel), from the sizes alone: the workspace holds their sums.
+struct KvPlan {
+    int32_t rows = 64, tiles = 0, sinkTiles = 0, chunks = 0;
+    bool perHead = false;
+    int64_t units = 0;
+    int64_t Blocks() const { return units * (tiles + static_cast<int64_t>(sinkTiles) * chunks); }
+    bool Partial() const { return perHead || chunks > 0; }
+};
+KvPlan PlanKv(const AttnShape& s)
+{
+    KvPlan p;
+    p.rows = s.dim <= 128 ? 64 : 32;
+    p.tiles = static_cast<int32_t>(CeilDiv(s.lk, p.rows));
+    const int64_t group = s.heads / s.kvHeads;
+    p.perHead = group > 1 && static_cast<int64_t>(s.batch) * s.kvHeads * p.tiles < 2 * kNumSMsFallback;
+    p.units = static_cast<int64_t>(s.batch) * (p.perHead ? s.heads : s.kvHeads);
+    const int64_t near = CeilDiv(static_cast<int64_t>(s.window) + p.rows, p.rows), far = CeilDiv(s.lq > s.window ? s.lq - s.window : 0, p.rows);
+    const int64_t sinks = s.sinks < s.lk ? s.sinks : s.lk;
+    if (sinks > 0 && s.heads > 0 && 2 * far > near) {
+        p.sinkTiles = static_cast<int32_t>(CeilDiv(sinks, p.rows));
+        const int64_t chunks = CeilDiv(far, near);
+        p.chunks = static_cast<int32_t>(chunks < 64 ? chunks : 64);
+    }
+    return p;
+}
+uint64_t DeltaBytes(const AttnShape& s) { return (static_cast<uint64_t>(s.batch) * s.heads * s.lq * 4 + 255) & ~255ull; }
+
 template <typename T, int DP>
-cudaError_t Backward(Dt dt, const AttnArgs& a, cudaStream_t stream)
+cudaError_t Backward(Dt dt, const AttnArgs& a, void* workspace, cudaStream_t stream)
 {
     using L = Tile<DP>;
     const AttnShape& s = a.s;
@@ -480,9 +581,10 @@ cudaError_t Backward(Dt dt, const AttnArgs& a, cudaStream_t stream)
     if (e != cudaSuccess) {
         return e;
     }
-    const int64_t qTiles = CeilDiv(s.lq, L::kRows), kTiles = CeilDiv(s.lk, L::kRows);
-    const int64_t qBlocks = static_cast<int64_t>(s.batch) * s.heads * qTiles, kBlocks = static_cast<int64_t>(s.batch) * s.kvHeads * kTiles;
-    if (qBlocks > INT32_MAX || kBlocks > INT32_MAX) {
+    const KvPlan plan = PlanKv(s);
+    const int64_t qTiles = CeilDiv(s.lq, L::kRows), qBlocks = static_cast<int64_t>(s.batch) * s.heads * qTiles, kBlocks = plan.Blocks();
+    const int64_t keys = static_cast<int64_t>(s.batch) * s.kvHeads * s.lk;
+    if (qBlocks > INT32_MAX || kBlocks > INT32_MAX || CeilDiv(keys, 4) > INT32_MAX || plan.rows != L::kRows) {
         return cudaErrorInvalidConfiguration;
     }
     if (qBlocks > 0) {
@@ -491,9 +593,17 @@ cudaError_t Backward(Dt dt, const AttnArgs& a, cudaStream_t stream)
         CountLaunch();
     }
     if (kBlocks > 0) {
-        m.tiles = static_cast<int32_t>(kTiles);
+        m.tiles = plan.tiles;
+        m.perHead = plan.perHead;
+        m.sinkTiles = plan.sinkTiles;
+        m.chunks = plan.chunks;
+        m.partial = plan.Partial() ? reinterpret_cast<float*>(static_cast<char*>(workspace) + DeltaBytes(s)) : nullptr;
         AttnGradKvTilesKernel<T, DP><<<static_cast<unsigned>(kBlocks), kThreads, sharedKv, stream>>>(m);
         CountLaunch();
+        if (m.partial != nullptr) {
+            AttnGradKvSumKernel<T><<<static_cast<unsigned>(CeilDiv(keys, 4)), 128, 0, stream>>>(m, L::kRows);
+            CountLaunch();
+        }
     }
     return cudaGetLastError();
 }
@@ -502,16 +612,30 @@ cudaError_t Backward(Dt dt, const AttnArgs& a, cudaStream_t stream)
 
 cudaError_t AttnForwardTiles(Dt dt, const AttnArgs& a, cudaStream_t stream)
 {
+    const int32_t d = a.s.dim;
     OPSCV_DISPATCH_DT(dt, T, {
-        return a.s.dim <= 64 ? Forward<T, 64>(dt, a, stream) : a.s.dim <= 128 ? Forward<T, 128>(dt, a, stream) : Forward<T, 256>(dt, a, stream);
+        return d <= 64 ? Forward<T, 64>(dt, a, stream) :
+               d <= 96 ? Forward<T, 96>(dt, a, stream) :
+               d <= 128 ? Forward<T, 128>(dt, a, stream) :
+                          Forward<T, 256>(dt, a, stream);
     });
     return cudaErrorInvalidValue;
 }
 
-cudaError_t AttnBackwardTiles(Dt dt, const AttnArgs& a, cudaStream_t stream)
+uint64_t AttnBackwardTilesWorkspace(const AttnShape& s)
 {
+    const KvPlan p = PlanKv(s);
+    return DeltaBytes(s) + (p.Partial() ? static_cast<uint64_t>(p.Blocks()) * 2 * p.rows * s.dim * 4 : 0);
+}
+
+cudaError_t AttnBackwardTiles(Dt dt, const AttnArgs& a, void* workspace, cudaStream_t stream)
+{
+    const int32_t d = a.s.dim;
     OPSCV_DISPATCH_DT(dt, T, {
-        return a.s.dim <= 64 ? Backward<T, 64>(dt, a, stream) : a.s.dim <= 128 ? Backward<T, 128>(dt, a, stream) : Backward<T, 256>(dt, a, stream);
+        return d <= 64 ? Backward<T, 64>(dt, a, workspace, stream) :
+               d <= 96 ? Backward<T, 96>(dt, a, workspace, stream) :
+               d <= 128 ? Backward<T, 128>(dt, a, workspace, stream) :
+                          Backward<T, 256>(dt, a, workspace, stream);
     });
     return cudaErrorInvalidValue;
 }
