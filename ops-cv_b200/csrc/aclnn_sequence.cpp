@@ -116,44 +116,41 @@ class LeadMerge {
 public:
     explicit LeadMerge(size_t lead) : lead_(lead) {}
     // strides of t's dimensions [from, from + lead); `to` gets the result
-    void Add(const aclTensor* t, size_t from, RowStride* to) { uses_.push_back({t, from, to}); }
+    void Add(const aclTensor* t, size_t from, RowStride* to) { uses_[used_++] = {t, from, to}; } // at most five
     bool Run(Lead& out)
     {
-        struct Level {
-            int64_t n;
-            size_t last; // the dimension whose stride the level has
-        };
-        std::vector<Level> levels;
-        const aclTensor* t0 = uses_[0].t;
+        int64_t extent[2] = {1, 1}; // of the levels, and the dimension whose stride each has
+        size_t last[2] = {0, 0};
+        int count = 0;
+        const Use& u0 = uses_[0];
         for (size_t i = 0; i < lead_; ++i) {
-            const int64_t n = t0->dims[uses_[0].from + i];
+            const int64_t n = u0.t->dims[u0.from + i];
             if (n == 1) {
                 continue;
             }
-            bool joins = !levels.empty();
-            for (const Use& u : uses_) {
+            bool joins = count > 0;
+            for (int x = 0; x < used_; ++x) {
+                const Use& u = uses_[x];
                 if (joins) {
-                    joins = u.t->strides[u.from + levels.back().last] == u.t->strides[u.from + i] * n;
+                    joins = u.t->strides[u.from + last[count - 1]] == u.t->strides[u.from + i] * n;
                 }
             }
             if (joins) {
-                levels.back().n *= n;
-                levels.back().last = i;
+                extent[count - 1] *= n;
+                last[count - 1] = i;
+            } else if (count == 2) {
+                return false;
             } else {
-                levels.push_back({n, i});
+                extent[count] = n;
+                last[count++] = i;
             }
         }
-        if (levels.size() > 2) {
-            return false;
-        }
-        out.total = 1;
-        for (const Level& l : levels) {
-            out.total *= l.n;
-        }
-        out.inner = levels.empty() ? 1 : levels.back().n;
-        for (const Use& u : uses_) {
-            u.to->s1 = levels.empty() ? 0 : u.t->strides[u.from + levels.back().last];
-            u.to->s0 = levels.size() == 2 ? u.t->strides[u.from + levels[0].last] : 0;
+        out.total = extent[0] * extent[1];
+        out.inner = count > 0 ? extent[count - 1] : 1;
+        for (int x = 0; x < used_; ++x) {
+            const Use& u = uses_[x];
+            u.to->s1 = count > 0 ? u.t->strides[u.from + last[count - 1]] : 0;
+            u.to->s0 = count == 2 ? u.t->strides[u.from + last[0]] : 0;
         }
         return true;
     }
@@ -165,7 +162,8 @@ private:
         RowStride* to;
     };
     size_t lead_;
-    std::vector<Use> uses_;
+    Use uses_[5];
+    int used_ = 0;
 };
 
 // Gives every operand its buffer: itself, or a staged copy where `stage` says so (or where it has to be).
