@@ -13,39 +13,39 @@ namespace {
 
 constexpr int kThreads = 256; // 16 x 16
 
-// DP: values of a head, padded; ROWS: queries and keys of a tile. 64 x 64 tiles of up to 128 values, 32 x 32 ones of 256.
-// DP is a multiple of 32.
-template <int DP>
+// DP: values of a head, padded to a multiple of 32. Rows of a tile as `a` (whose sums a block owns, A of them) and as `b` (that it walks, B
+// of them): a thread has kA rows of a, from kA * ty on, and rows tx + 16 c of b.
+template <int DP, int A, int B>
 struct Tile {
-    static constexpr int kRows = DP <= 128 ? 64 : 32;
-    static constexpr int kMicro = kRows / 16;  // rows (and columns) of a thread
-    static constexpr int kPairs = DP / 32;     // pairs of values of a row that a thread has
-    static constexpr int kStride = DP + 4;     // floats of a row: 4 more shift neighbouring rows to other banks
-    static constexpr int kWeights = kRows + 4; // the same for the rows of weights
-    static constexpr int kTileFloats = kRows * kStride;
-    static constexpr int kWeightFloats = kRows * kWeights;
+    static constexpr int kA = A / 16, kB = B / 16;
+    static constexpr int kPairs = DP / 32;    // pairs of values of a row that a thread has
+    static constexpr int kStride = DP + 4;    // floats of a row: 4 more shift neighbouring rows to other banks
+    static constexpr int kWeights = B + 4;    // the same for the rows of weights
+    static constexpr int kFloatsA = A * kStride, kFloatsB = B * kStride;
+    static constexpr int kWeightFloats = A * kWeights;
 };
 
 // Rows [from, from + ROWS) of one head as fp32, zeros for rows behind `end` and values behind dim.
-template <typename T, int DP>
+template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void LoadTile(float* dst, const AttnTensor& t, int32_t b, int32_t h, int32_t from, int32_t end, int32_t dim,
                                          bool vec)
 {
-    using L = Tile<DP>;
+    constexpr int kStride = DP + 4;
     const T* base = RowOf<T>(t, b, 0, h);
     if (vec) {
-        for (int e = threadIdx.x; e < L::kRows * (DP / 4); e += kThreads) {
+#pragma unroll 4
+        for (int e = threadIdx.x; e < ROWS * (DP / 4); e += kThreads) {
             const int r = e / (DP / 4), d = e % (DP / 4) * 4;
             float v[4] = {};
             if (from + r < end && d < dim) {
                 LoadPack<T, 4>(base + (from + r) * t.l + d, v);
             }
-            *reinterpret_cast<float4*>(dst + r * L::kStride + d) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(dst + r * kStride + d) = make_float4(v[0], v[1], v[2], v[3]);
         }
     } else {
-        for (int e = threadIdx.x; e < L::kRows * DP; e += kThreads) {
+        for (int e = threadIdx.x; e < ROWS * DP; e += kThreads) {
             const int r = e / DP, d = e % DP;
-            dst[r * L::kStride + d] = from + r < end && d < dim ? DType<T>::ToF(base[(from + r) * t.l + d]) : 0.0f;
+            dst[r * kStride + d] = from + r < end && d < dim ? DType<T>::ToF(base[(from + r) * t.l + d]) : 0.0f;
         }
     }
 }
@@ -55,52 +55,53 @@ __device__ __forceinline__ float Dot4(const float4& a, const float4& b, float s)
     return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
 }
 
-// s[r][c] = row (micro * ty + r) of a . row (tx + 16 c) of b
-template <int DP>
-__device__ __forceinline__ void Inner(const float* a, const float* b, float (&s)[Tile<DP>::kMicro][Tile<DP>::kMicro])
+// s[r][c] = row (kA * ty + r) of a . row (tx + 16 c) of b
+template <typename L, int DP>
+__device__ __forceinline__ void Inner(const float* a, const float* b, float (&s)[L::kA][L::kB])
 {
-    using L = Tile<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 #pragma unroll
-    for (int r = 0; r < L::kMicro; ++r) {
+    for (int r = 0; r < L::kA; ++r) {
 #pragma unroll
-        for (int c = 0; c < L::kMicro; ++c) {
+        for (int c = 0; c < L::kB; ++c) {
             s[r][c] = 0.0f;
         }
     }
-    const float* pa = a + L::kMicro * ty * L::kStride;
+    const float* pa = a + L::kA * ty * L::kStride;
     const float* pb = b + tx * L::kStride;
 #pragma unroll 4
     for (int d = 0; d < DP; d += 4) {
-        float4 x[L::kMicro], y[L::kMicro];
+        float4 x[L::kA], y[L::kB];
 #pragma unroll
-        for (int r = 0; r < L::kMicro; ++r) {
+        for (int r = 0; r < L::kA; ++r) {
             x[r] = *reinterpret_cast<const float4*>(pa + r * L::kStride + d);
-            y[r] = *reinterpret_cast<const float4*>(pb + 16 * r * L::kStride + d);
         }
 #pragma unroll
-        for (int r = 0; r < L::kMicro; ++r) {
+        for (int c = 0; c < L::kB; ++c) {
+            y[c] = *reinterpret_cast<const float4*>(pb + 16 * c * L::kStride + d);
+        }
 #pragma unroll
-            for (int c = 0; c < L::kMicro; ++c) {
+        for (int r = 0; r < L::kA; ++r) {
+#pragma unroll
+            for (int c = 0; c < L::kB; ++c) {
                 s[r][c] = Dot4(x[r], y[c], s[r][c]);
             }
         }
     }
 }
 
-// o[r] += sum over j of w[micro * ty + r][j] row j of v, values 2 tx + 32 c and the next
-template <int DP>
-__device__ __forceinline__ void Outer(const float* w, const float* v, float2 (&o)[Tile<DP>::kMicro][Tile<DP>::kPairs])
+// o[r] += sum over j of w[kA * ty + r][j] row j of v (B rows), values 2 tx + 32 c and the next
+template <typename L, int B>
+__device__ __forceinline__ void Outer(const float* w, const float* v, float2 (&o)[L::kA][L::kPairs])
 {
-    using L = Tile<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const float* pw = w + L::kMicro * ty * L::kWeights;
+    const float* pw = w + L::kA * ty * L::kWeights;
     const float* pv = v + 2 * tx;
 #pragma unroll 2
-    for (int j = 0; j < L::kRows; j += 4) {
-        float4 x[L::kMicro];
+    for (int j = 0; j < B; j += 4) {
+        float4 x[L::kA];
 #pragma unroll
-        for (int r = 0; r < L::kMicro; ++r) {
+        for (int r = 0; r < L::kA; ++r) {
             x[r] = *reinterpret_cast<const float4*>(pw + r * L::kWeights + j);
         }
 #pragma unroll
@@ -109,7 +110,7 @@ __device__ __forceinline__ void Outer(const float* w, const float* v, float2 (&o
             for (int c = 0; c < L::kPairs; ++c) {
                 const float2 y = *reinterpret_cast<const float2*>(pv + (j + k) * L::kStride + 32 * c);
 #pragma unroll
-                for (int r = 0; r < L::kMicro; ++r) {
+                for (int r = 0; r < L::kA; ++r) {
                     const float z = k == 0 ? x[r].x : k == 1 ? x[r].y : k == 2 ? x[r].z : x[r].w;
                     o[r][c].x = fmaf(z, y.x, o[r][c].x);
                     o[r][c].y = fmaf(z, y.y, o[r][c].y);
@@ -191,25 +192,25 @@ __device__ __forceinline__ int64_t PartialSlot(const TileArgs& m, int32_t unit, 
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DP>
+template <typename T, int DP, int A, int B>
 __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_constant__ TileArgs m)
 {
-    using L = Tile<DP>;
-    constexpr int R = L::kMicro;
+    using L = Tile<DP, A, B>;
+    constexpr int R = L::kA, C = L::kB;
     extern __shared__ float shared[];
     __shared__ uint32_t again[2];
-    float *sq = shared, *sk = sq + L::kTileFloats, *sw = sk + L::kTileFloats; // keys, then values
+    float *sq = shared, *sk = sq + L::kFloatsA, *sw = sk + L::kFloatsB; // keys, then values
     const AttnShape& s = m.a.s;
     const int32_t tile = blockIdx.x % m.tiles, bh = blockIdx.x / m.tiles;
     const int32_t b = bh / s.heads, h = bh % s.heads, u = h / m.a.group;
     const Lengths n = LengthsOf(s, b);
-    const int32_t i0 = tile * L::kRows, iLast = min(i0 + L::kRows, n.q) - 1;
-    const Walk<L::kRows> walk(s, n.shift + i0, iLast >= i0 ? n.shift + iLast : -1);
+    const int32_t i0 = tile * A, iLast = min(i0 + A, n.q) - 1;
+    const Walk<B> walk(s, n.shift + i0, iLast >= i0 ? n.shift + iLast : -1);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     if (threadIdx.x < 2) {
         again[threadIdx.x] = 0;
     }
-    LoadTile<T, DP>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
+    LoadTile<T, DP, A>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
     float2 o[R][L::kPairs] = {};
     float top[R], total[R];
     int32_t p[R];
@@ -223,15 +224,15 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
     for (int32_t step = 0; step < walk.steps; ++step) {
         const int32_t j0 = walk.Key(step);
         __syncthreads(); // the values of the step before have been read
-        LoadTile<T, DP>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
+        LoadTile<T, DP, B>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
         __syncthreads();
-        float x[R][R];
-        Inner<DP>(sq, sk, x);
+        float x[R][C];
+        Inner<L, DP>(sq, sk, x);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float most = top[r];
 #pragma unroll
-            for (int c = 0; c < R; ++c) {
+            for (int c = 0; c < C; ++c) {
                 x[r][c] = walk.Sees(s, step, p[r], j0 + tx + 16 * c) ? x[r][c] * s.scale : -INFINITY;
                 most = fmaxf(most, x[r][c]);
             }
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
             top[r] = most;
             float sum = 0.0f;
 #pragma unroll
-            for (int c = 0; c < R; ++c) {
+            for (int c = 0; c < C; ++c) {
                 x[r][c] = expf(x[r][c] - base);
                 sum += x[r][c];
                 sw[(R * ty + r) * L::kWeights + tx + 16 * c] = x[r][c];
@@ -253,9 +254,9 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
             }
         }
         __syncthreads();
-        LoadTile<T, DP>(sk, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
+        LoadTile<T, DP, B>(sk, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
         __syncthreads();
-        Outer<DP>(sw, sk, o);
+        Outer<L, B>(sw, sk, o);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
     }
     __syncthreads();
     // rows that are not finite again, without the masked keys' part
-    for (int r = threadIdx.x >> 5; r < L::kRows; r += kThreads / 32) {
+    for (int r = threadIdx.x >> 5; r < A; r += kThreads / 32) {
         if ((again[r >> 5] >> (r & 31) & 1) != 0 && i0 + r < s.lq) {
             AttnForwardRow<T>(m.a, b, h, i0 + r);
         }
@@ -289,26 +290,26 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------------------
-template <typename T, int DP>
+template <typename T, int DP, int A, int B>
 __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_constant__ TileArgs m)
 {
-    using L = Tile<DP>;
-    constexpr int R = L::kMicro;
+    using L = Tile<DP, A, B>;
+    constexpr int R = L::kA, C = L::kB;
     extern __shared__ float shared[];
     __shared__ uint32_t again[2];
-    float *sq = shared, *sg = sq + L::kTileFloats, *sk = sg + L::kTileFloats, *sv = sk + L::kTileFloats, *sw = sv + L::kTileFloats;
+    float *sq = shared, *sg = sq + L::kFloatsA, *sk = sg + L::kFloatsA, *sv = sk + L::kFloatsB, *sw = sv + L::kFloatsB;
     const AttnShape& s = m.a.s;
     const int32_t tile = blockIdx.x % m.tiles, bh = blockIdx.x / m.tiles;
     const int32_t b = bh / s.heads, h = bh % s.heads, u = h / m.a.group;
     const Lengths n = LengthsOf(s, b);
-    const int32_t i0 = tile * L::kRows, iLast = min(i0 + L::kRows, n.q) - 1;
-    const Walk<L::kRows> walk(s, n.shift + i0, iLast >= i0 ? n.shift + iLast : -1);
+    const int32_t i0 = tile * A, iLast = min(i0 + A, n.q) - 1;
+    const Walk<B> walk(s, n.shift + i0, iLast >= i0 ? n.shift + iLast : -1);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     if (threadIdx.x < 2) {
         again[threadIdx.x] = 0;
     }
-    LoadTile<T, DP>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
-    LoadTile<T, DP>(sg, m.a.gradOut, b, h, i0, iLast + 1, s.dim, m.vec);
+    LoadTile<T, DP, A>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
+    LoadTile<T, DP, A>(sg, m.a.gradOut, b, h, i0, iLast + 1, s.dim, m.vec);
     float2 o[R][L::kPairs] = {};
     float lse[R], delta[R];
     int32_t p[R];
@@ -322,23 +323,23 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
     for (int32_t step = 0; step < walk.steps; ++step) {
         const int32_t j0 = walk.Key(step);
         __syncthreads();
-        LoadTile<T, DP>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
-        LoadTile<T, DP>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
+        LoadTile<T, DP, B>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
+        LoadTile<T, DP, B>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
         __syncthreads();
-        float x[R][R], y[R][R];
-        Inner<DP>(sq, sk, x);
-        Inner<DP>(sg, sv, y);
+        float x[R][C], y[R][C];
+        Inner<L, DP>(sq, sk, x);
+        Inner<L, DP>(sg, sv, y);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
-            for (int c = 0; c < R; ++c) {
+            for (int c = 0; c < C; ++c) {
                 const bool live = walk.Sees(s, step, p[r], j0 + tx + 16 * c);
                 sw[(R * ty + r) * L::kWeights + tx + 16 * c] =
                     live ? expf(x[r][c] * s.scale - lse[r]) * (y[r][c] - delta[r]) * s.scale : 0.0f;
             }
         }
         __syncthreads();
-        Outer<DP>(sw, sk, o);
+        Outer<L, B>(sw, sk, o);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -357,7 +358,7 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
         }
     }
     __syncthreads();
-    for (int r = threadIdx.x >> 5; r < L::kRows; r += kThreads / 32) {
+    for (int r = threadIdx.x >> 5; r < A; r += kThreads / 32) {
         if ((again[r >> 5] >> (r & 31) & 1) != 0 && i0 + r < s.lq) {
             AttnGradQRow<T>(m.a, b, h, i0 + r);
         }
@@ -368,15 +369,15 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
 // query head instead; and where sinks are seen by many more queries than a window's, these are shared out among `chunks` further blocks
 // of their tile. In both cases the blocks' sums go to `partial` in fp32 ([batch, heads or key heads, 1 + chunks of a tile with sinks,
 // gradK and gradV, rows of the tile, dim]), and AttnGradKvSumKernel adds them up in order.
-template <typename T, int DP>
+template <typename T, int DP, int A, int B>
 __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_constant__ TileArgs m)
 {
-    using L = Tile<DP>;
-    constexpr int R = L::kMicro;
+    using L = Tile<DP, A, B>;
+    constexpr int R = L::kA, C = L::kB;
     extern __shared__ float shared[];
     __shared__ uint32_t again[2];
-    __shared__ float sLse[L::kRows], sDelta[L::kRows];
-    float *sk = shared, *sv = sk + L::kTileFloats, *sq = sv + L::kTileFloats, *sg = sq + L::kTileFloats, *sw = sg + L::kTileFloats,
+    __shared__ float sLse[B], sDelta[B];
+    float *sk = shared, *sv = sk + L::kFloatsA, *sq = sv + L::kFloatsA, *sg = sq + L::kFloatsB, *sw = sg + L::kFloatsB,
           *sd = sw + L::kWeightFloats;
     const AttnShape& s = m.a.s;
     const int32_t perUnit = m.tiles + m.sinkTiles * m.chunks;
@@ -390,44 +391,44 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
     const int32_t hFirst = m.perHead ? unit % units : u * m.a.group, hEnd = m.perHead ? hFirst + 1 : hFirst + m.a.group;
     const bool far = m.chunks > 0 && tile < m.sinkTiles; // its far queries are others'
     const Lengths n = LengthsOf(s, b);
-    const int32_t j0 = tile * L::kRows, jLast = min(j0 + L::kRows, n.kv) - 1, end = n.kv - 1;
+    const int32_t j0 = tile * A, jLast = min(j0 + A, n.kv) - 1, end = n.kv - 1;
     // positions of the queries that this block walks
     int32_t low = max(j0, max(n.shift, 0)), high = jLast < j0 ? -1 : j0 < s.sinks && !far ? end : min(end, jLast + s.window - 1);
     if (chunk >= 0) {
         low = max(low, jLast + s.window);
-        const int32_t steps = end >= low ? (end - low + L::kRows) / L::kRows : 0, share = (steps + m.chunks - 1) / m.chunks;
-        high = jLast < j0 ? -1 : static_cast<int32_t>(min(static_cast<int64_t>(end), low + static_cast<int64_t>(chunk + 1) * share * L::kRows - 1));
-        low += chunk * share * L::kRows;
+        const int32_t steps = end >= low ? (end - low + B) / B : 0, share = (steps + m.chunks - 1) / m.chunks;
+        high = jLast < j0 ? -1 : static_cast<int32_t>(min(static_cast<int64_t>(end), low + static_cast<int64_t>(chunk + 1) * share * B - 1));
+        low += chunk * share * B;
     }
     const int32_t stop = high; // queries behind it are another block's
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     if (threadIdx.x < 2) {
         again[threadIdx.x] = 0;
     }
-    LoadTile<T, DP>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
-    LoadTile<T, DP>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
+    LoadTile<T, DP, A>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
+    LoadTile<T, DP, A>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
     float2 ok[R][L::kPairs] = {}, ov[R][L::kPairs] = {};
     for (int32_t h = hFirst; h < hEnd; ++h) {
         const int64_t head = static_cast<int64_t>(b) * s.heads + h;
-        for (int32_t p0 = low; p0 <= high; p0 += L::kRows) {
+        for (int32_t p0 = low; p0 <= high; p0 += B) {
             const int32_t i0 = p0 - n.shift;
             __syncthreads();
-            LoadTile<T, DP>(sq, m.a.q, b, h, i0, n.q, s.dim, m.vec);
-            LoadTile<T, DP>(sg, m.a.gradOut, b, h, i0, n.q, s.dim, m.vec);
-            if (threadIdx.x < L::kRows) {
+            LoadTile<T, DP, B>(sq, m.a.q, b, h, i0, n.q, s.dim, m.vec);
+            LoadTile<T, DP, B>(sg, m.a.gradOut, b, h, i0, n.q, s.dim, m.vec);
+            if (threadIdx.x < B) {
                 const int32_t i = i0 + threadIdx.x;
                 sLse[threadIdx.x] = i < n.q ? m.a.lse[head * s.lq + i] : 0.0f;
                 sDelta[threadIdx.x] = i < n.q ? m.a.delta[head * m.a.deltaStride + i] : 0.0f;
             }
             __syncthreads();
-            float x[R][R], y[R][R];
-            Inner<DP>(sk, sq, x);
-            Inner<DP>(sv, sg, y);
+            float x[R][C], y[R][C];
+            Inner<L, DP>(sk, sq, x);
+            Inner<L, DP>(sv, sg, y);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const int32_t j = j0 + R * ty + r;
 #pragma unroll
-                for (int c = 0; c < R; ++c) {
+                for (int c = 0; c < C; ++c) {
                     const int32_t e = tx + 16 * c, p = p0 + e;
                     const bool live = j < n.kv && p <= stop && j <= p && (j > p - s.window || j < s.sinks);
                     const float w = live ? expf(x[r][c] * s.scale - sLse[e]) : 0.0f;
@@ -436,19 +437,19 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
                 }
             }
             __syncthreads();
-            Outer<DP>(sw, sg, ov);
-            Outer<DP>(sd, sq, ok);
+            Outer<L, B>(sw, sg, ov);
+            Outer<L, B>(sd, sq, ok);
         }
     }
     if (m.partial != nullptr) {
-        float* part = m.partial + PartialSlot(m, unit, tile, 1 + chunk, L::kRows);
+        float* part = m.partial + PartialSlot(m, unit, tile, 1 + chunk, A);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
             for (int c = 0; c < L::kPairs; ++c) {
                 const int32_t at = (R * ty + r) * s.dim, d = 2 * tx + 32 * c;
                 StorePair<float>(part + at, ok[r][c], d, s.dim);
-                StorePair<float>(part + L::kRows * s.dim + at, ov[r][c], d, s.dim);
+                StorePair<float>(part + A * s.dim + at, ov[r][c], d, s.dim);
             }
         }
         return;
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
         }
     }
     __syncthreads();
-    for (int r = threadIdx.x >> 5; r < L::kRows; r += kThreads / 32) {
+    for (int r = threadIdx.x >> 5; r < A; r += kThreads / 32) {
         if ((again[r >> 5] >> (r & 31) & 1) != 0 && j0 + r < s.lk) {
             AttnGradKvRow<T>(m.a, b, u, j0 + r);
         }
@@ -495,10 +496,10 @@ __global__ void __launch_bounds__(128) AttnGradKvSumKernel(const __grid_constant
         T* out = OutRowOf<T>(which == 0 ? m.a.gradK : m.a.gradV, b, j, u);
         for (int32_t d = lane; d < s.dim; d += 32) {
             float sum = 0.0f;
-            for (int32_t x = 0; x < units; ++x) {
-                for (int32_t c = 0; c < slots; ++c) {
-                    sum += m.partial[PartialSlot(m, first + x, tile, c, rows) + (which * rows + j % rows) * static_cast<int64_t>(s.dim) + d];
-                }
+            const int64_t within = (which * rows + j % rows) * static_cast<int64_t>(s.dim) + d;
+#pragma unroll 4
+            for (int32_t x = 0; x < units * slots; ++x) { // by head, then by block
+                sum += m.partial[PartialSlot(m, first + x / slots, tile, x % slots, rows) + within];
             }
             bad = bad || !(fabsf(sum) <= 3.4e38f);
             out[d] = DType<T>::FromF(sum);
@@ -515,26 +516,33 @@ bool ReadsByFour(Dt dt, const AttnTensor& t)
     return Aligned(t.p, 4 * DtSize(dt)) && t.b % 4 == 0 && t.l % 4 == 0 && t.h % 4 == 0;
 }
 
-template <typename T, int DP>
+// Rows of the tiles that blocks own: 64 (32 of more than 128 values), or 32 where that leaves SMs with one block: a block's loads and waits
+// then hide behind another's products (2 x 777 tokens, 6 heads of 72: forward 94 us with 64 rows, 64 us with 32).
+int OwnRows(const AttnShape& s, int64_t units, int64_t tokens)
+{
+    return s.dim > 128 || units * CeilDiv(tokens, 64) < 2 * kNumSMsFallback ? 32 : 64;
+}
+
+template <typename T, int DP, int A, int B>
 cudaError_t Forward(Dt dt, const AttnArgs& a, cudaStream_t stream)
 {
-    using L = Tile<DP>;
+    using L = Tile<DP, A, B>;
     const AttnShape& s = a.s;
     TileArgs m{};
     m.a = a;
-    m.tiles = static_cast<int32_t>(CeilDiv(s.lq, L::kRows));
+    m.tiles = static_cast<int32_t>(CeilDiv(s.lq, A));
     m.vec = s.dim % 4 == 0 && ReadsByFour(dt, a.q) && ReadsByFour(dt, a.k) && ReadsByFour(dt, a.v);
-    constexpr int shared = (2 * L::kTileFloats + L::kWeightFloats) * 4;
+    constexpr int shared = (L::kFloatsA + L::kFloatsB + L::kWeightFloats) * 4;
     static std::atomic<uint64_t> asked;
     const int64_t blocks = static_cast<int64_t>(s.batch) * s.heads * m.tiles;
     if (blocks > INT32_MAX) {
         return cudaErrorInvalidConfiguration;
     }
-    const cudaError_t e = AskOnce(AttnForwardTilesKernel<T, DP>, asked, shared);
+    const cudaError_t e = AskOnce(AttnForwardTilesKernel<T, DP, A, B>, asked, shared);
     if (e != cudaSuccess) {
         return e;
     }
-    AttnForwardTilesKernel<T, DP><<<static_cast<unsigned>(blocks), kThreads, shared, stream>>>(m);
+    AttnForwardTilesKernel<T, DP, A, B><<<static_cast<unsigned>(blocks), kThreads, shared, stream>>>(m);
     CountLaunch();
     return cudaGetLastError();
 }
@@ -550,62 +558,108 @@ struct KvPlan {
 KvPlan PlanKv(const AttnShape& s)
 {
     KvPlan p;
-    p.rows = s.dim <= 128 ? 64 : 32;
-    p.tiles = static_cast<int32_t>(CeilDiv(s.lk, p.rows));
     const int64_t group = s.heads / s.kvHeads;
-    p.perHead = group > 1 && static_cast<int64_t>(s.batch) * s.kvHeads * p.tiles < 2 * kNumSMsFallback;
+    p.perHead = group > 1 && static_cast<int64_t>(s.batch) * s.kvHeads * CeilDiv(s.lk, 64) < 2 * kNumSMsFallback;
     p.units = static_cast<int64_t>(s.batch) * (p.perHead ? s.heads : s.kvHeads);
-    const int64_t near = CeilDiv(static_cast<int64_t>(s.window) + p.rows, p.rows), far = CeilDiv(s.lq > s.window ? s.lq - s.window : 0, p.rows);
+    p.rows = OwnRows(s, p.units, s.lk);
+    p.tiles = static_cast<int32_t>(CeilDiv(s.lk, p.rows));
+    const int64_t step = s.dim <= 128 ? 64 : 32;
+    const int64_t near = CeilDiv(static_cast<int64_t>(s.window) + p.rows, step), far = CeilDiv(s.lq > s.window ? s.lq - s.window : 0, step);
     const int64_t sinks = s.sinks < s.lk ? s.sinks : s.lk;
     if (sinks > 0 && s.heads > 0 && 2 * far > near) {
         p.sinkTiles = static_cast<int32_t>(CeilDiv(sinks, p.rows));
-        const int64_t chunks = CeilDiv(far, near);
+        const int64_t chunks = CeilDiv(far, near > 1 ? near : 1);
         p.chunks = static_cast<int32_t>(chunks < 64 ? chunks : 64);
     }
     return p;
 }
 uint64_t DeltaBytes(const AttnShape& s) { return (static_cast<uint64_t>(s.batch) * s.heads * s.lq * 4 + 255) & ~255ull; }
 
+template <typename T, int DP, int A, int B>
+cudaError_t GradQ(const TileArgs& args, cudaStream_t stream)
+{
+    using L = Tile<DP, A, B>;
+    TileArgs m = args;
+    const AttnShape& s = m.a.s;
+    constexpr int shared = (2 * L::kFloatsA + 2 * L::kFloatsB + L::kWeightFloats) * 4;
+    static std::atomic<uint64_t> asked;
+    m.tiles = static_cast<int32_t>(CeilDiv(s.lq, A));
+    const int64_t blocks = static_cast<int64_t>(s.batch) * s.heads * m.tiles;
+    if (blocks > INT32_MAX) {
+        return cudaErrorInvalidConfiguration;
+    }
+    const cudaError_t e = AskOnce(AttnGradQTilesKernel<T, DP, A, B>, asked, shared);
+    if (e != cudaSuccess || blocks == 0) {
+        return e;
+    }
+    AttnGradQTilesKernel<T, DP, A, B><<<static_cast<unsigned>(blocks), kThreads, shared, stream>>>(m);
+    CountLaunch();
+    return cudaGetLastError();
+}
+
+template <typename T, int DP, int A, int B>
+cudaError_t GradKv(const TileArgs& args, const KvPlan& plan, float* partial, cudaStream_t stream)
+{
+    using L = Tile<DP, A, B>;
+    TileArgs m = args;
+    const AttnShape& s = m.a.s;
+    constexpr int shared = (2 * L::kFloatsA + 2 * L::kFloatsB + 2 * L::kWeightFloats) * 4;
+    static std::atomic<uint64_t> asked;
+    const int64_t blocks = plan.Blocks(), keys = static_cast<int64_t>(s.batch) * s.kvHeads * s.lk;
+    if (blocks > INT32_MAX || CeilDiv(keys, 4) > INT32_MAX) {
+        return cudaErrorInvalidConfiguration;
+    }
+    cudaError_t e = AskOnce(AttnGradKvTilesKernel<T, DP, A, B>, asked, shared);
+    if (e != cudaSuccess || keys == 0) {
+        return e;
+    }
+    m.tiles = plan.tiles;
+    m.perHead = plan.perHead;
+    m.sinkTiles = plan.sinkTiles;
+    m.chunks = plan.chunks;
+    m.partial = plan.Partial() ? partial : nullptr;
+    if (blocks > 0) {
+        AttnGradKvTilesKernel<T, DP, A, B><<<static_cast<unsigned>(blocks), kThreads, shared, stream>>>(m);
+        CountLaunch();
+    }
+    if (m.partial != nullptr) {
+        AttnGradKvSumKernel<T><<<static_cast<unsigned>(CeilDiv(keys, 4)), 128, 0, stream>>>(m, A);
+        CountLaunch();
+    }
+    return cudaGetLastError();
+}
+
 template <typename T, int DP>
 cudaError_t Backward(Dt dt, const AttnArgs& a, void* workspace, cudaStream_t stream)
 {
-    using L = Tile<DP>;
     const AttnShape& s = a.s;
     TileArgs m{};
     m.a = a;
     m.vec = s.dim % 4 == 0 && ReadsByFour(dt, a.q) && ReadsByFour(dt, a.k) && ReadsByFour(dt, a.v) && ReadsByFour(dt, a.gradOut);
-    constexpr int sharedQ = (4 * L::kTileFloats + L::kWeightFloats) * 4, sharedKv = (4 * L::kTileFloats + 2 * L::kWeightFloats) * 4;
-    static std::atomic<uint64_t> askedQ, askedKv;
-    cudaError_t e = AskOnce(AttnGradQTilesKernel<T, DP>, askedQ, sharedQ);
-    e = e != cudaSuccess ? e : AskOnce(AttnGradKvTilesKernel<T, DP>, askedKv, sharedKv);
-    if (e != cudaSuccess) {
-        return e;
-    }
     const KvPlan plan = PlanKv(s);
-    const int64_t qTiles = CeilDiv(s.lq, L::kRows), qBlocks = static_cast<int64_t>(s.batch) * s.heads * qTiles, kBlocks = plan.Blocks();
-    const int64_t keys = static_cast<int64_t>(s.batch) * s.kvHeads * s.lk;
-    if (qBlocks > INT32_MAX || kBlocks > INT32_MAX || CeilDiv(keys, 4) > INT32_MAX || plan.rows != L::kRows) {
-        return cudaErrorInvalidConfiguration;
+    float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + DeltaBytes(s));
+    const bool few = OwnRows(s, static_cast<int64_t>(s.batch) * s.heads, s.lq) == 32;
+    cudaError_t e;
+    if constexpr (DP <= 128) {
+        e = few ? GradQ<T, DP, 32, 64>(m, stream) : GradQ<T, DP, 64, 64>(m, stream);
+        return e != cudaSuccess ? e :
+               plan.rows == 32  ? GradKv<T, DP, 32, 64>(m, plan, partial, stream) :
+                                  GradKv<T, DP, 64, 64>(m, plan, partial, stream);
+    } else {
+        e = GradQ<T, DP, 32, 32>(m, stream);
+        return e != cudaSuccess ? e : GradKv<T, DP, 32, 32>(m, plan, partial, stream);
     }
-    if (qBlocks > 0) {
-        m.tiles = static_cast<int32_t>(qTiles);
-        AttnGradQTilesKernel<T, DP><<<static_cast<unsigned>(qBlocks), kThreads, sharedQ, stream>>>(m);
-        CountLaunch();
+}
+
+template <typename T, int DP>
+cudaError_t ForwardBySize(Dt dt, const AttnArgs& a, cudaStream_t stream)
+{
+    if constexpr (DP <= 128) {
+        return OwnRows(a.s, static_cast<int64_t>(a.s.batch) * a.s.heads, a.s.lq) == 32 ? Forward<T, DP, 32, 64>(dt, a, stream) :
+                                                                                       Forward<T, DP, 64, 64>(dt, a, stream);
+    } else {
+        return Forward<T, DP, 32, 32>(dt, a, stream);
     }
-    if (kBlocks > 0) {
-        m.tiles = plan.tiles;
-        m.perHead = plan.perHead;
-        m.sinkTiles = plan.sinkTiles;
-        m.chunks = plan.chunks;
-        m.partial = plan.Partial() ? reinterpret_cast<float*>(static_cast<char*>(workspace) + DeltaBytes(s)) : nullptr;
-        AttnGradKvTilesKernel<T, DP><<<static_cast<unsigned>(kBlocks), kThreads, sharedKv, stream>>>(m);
-        CountLaunch();
-        if (m.partial != nullptr) {
-            AttnGradKvSumKernel<T><<<static_cast<unsigned>(CeilDiv(keys, 4)), 128, 0, stream>>>(m, L::kRows);
-            CountLaunch();
-        }
-    }
-    return cudaGetLastError();
 }
 
 } // namespace
@@ -614,10 +668,10 @@ cudaError_t AttnForwardTiles(Dt dt, const AttnArgs& a, cudaStream_t stream)
 {
     const int32_t d = a.s.dim;
     OPSCV_DISPATCH_DT(dt, T, {
-        return d <= 64 ? Forward<T, 64>(dt, a, stream) :
-               d <= 96 ? Forward<T, 96>(dt, a, stream) :
-               d <= 128 ? Forward<T, 128>(dt, a, stream) :
-                          Forward<T, 256>(dt, a, stream);
+        return d <= 64 ? ForwardBySize<T, 64>(dt, a, stream) :
+               d <= 96 ? ForwardBySize<T, 96>(dt, a, stream) :
+               d <= 128 ? ForwardBySize<T, 128>(dt, a, stream) :
+                          ForwardBySize<T, 256>(dt, a, stream);
     });
     return cudaErrorInvalidValue;
 }
