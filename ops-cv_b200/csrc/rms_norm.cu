@@ -820,14 +820,16 @@ int VecOfRows(int elem, const NormShape& n, std::initializer_list<RowUse> uses)
     return v;
 }
 
-// Threads of a row and chunks of V values per thread. Rows of up to 4 chunks a lane take one warp each, 4 rows a block; wider
+// Threads of a row and chunks of V values per thread. Where rows are many, 256 threads with more chunks each: what a thread spends once a
+// row is shared by more values (8192 x 4096 bf16 forward: 46 us against 49 with 512). Rows of up to 4 chunks a lane take one warp each, 4 rows a block; wider
 // ones a block of their own with as few chunks per thread as 512 threads allow, and up to 1024 threads with the most chunks that
 // `values` a thread allow. nv 0: too wide for that.
 struct RowShape {
     int nv, threads, rows;
 };
-RowShape ShapeOfRow(int32_t width, int v, int values, int mostThreads)
+RowShape ShapeOfRow(int32_t width, int v, int values, int mostThreads, int64_t rows)
 {
+    const int32_t wide = rows >= 4 * NumSMs() ? 256 : 512;
     const int32_t chunks = (width + v - 1) / v;
     if (chunks <= 32 * 4) {
         const int nv = chunks <= 32 ? 1 : (chunks <= 64 ? 2 : 4);
@@ -838,7 +840,7 @@ RowShape ShapeOfRow(int32_t width, int v, int values, int mostThreads)
     for (int nv = 1; nv <= 8 && nv * v <= values; nv *= 2) {
         const bool last = nv == 8 || 2 * nv * v > values;
         const int32_t threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
-        if (threads <= (last ? mostThreads : 512)) {
+        if (threads <= (last ? mostThreads : wide)) {
             return {nv, threads, 1};
         }
     }
@@ -892,7 +894,7 @@ cudaError_t RmsNormFwd(Dt dt, const NormShape& n, const void* x, RowStride xs, c
     a.rstd = rstd;
     const int v = VecOfRows(DtSize(dt), n,
                             {{x, xs}, {residual, rs}, {y, ys}, {sum, ss}, {n.weight32 ? nullptr : weight, {}}});
-    const RowShape shape = ShapeOfRow(n.width, v, 32, kMaxThreads);
+    const RowShape shape = ShapeOfRow(n.width, v, 32, kMaxThreads, n.rows);
     const int64_t blocks = CeilDiv(n.rows, shape.rows);
     if (!GridFits(blocks)) {
         return cudaErrorInvalidConfiguration;
@@ -920,10 +922,12 @@ cudaError_t RmsNormQuant(Dt dt, const NormShape& n, const void* x, RowStride xs,
     while (v > 1 && !(n.width % v == 0 && Aligned(q, v))) {
         v >>= 1;
     }
-    RowShape shape = ShapeOfRow(n.width, v, 32, kMaxThreads);
+    const bool small = a.groups > 1 && a.group == 128 && v >= 4;
+    // with groups in a warp, 512 threads a row are a little faster (8192 x 5120 bf16: 64 us against 68 with 256)
+    RowShape shape = ShapeOfRow(n.width, v, 32, kMaxThreads, small ? 0 : n.rows);
     // Groups of 128 columns read with at least four to a lane lie within a warp (lanes hold consecutive chunks of a row, and a
     // warp's first chunk starts a group); others go through shared memory, with one row a block.
-    const bool inWarp = a.groups > 1 && a.group == 128 && shape.nv > 0 && v >= 4, ofRow = a.groups == 1 && shape.nv > 0;
+    const bool inWarp = small && shape.nv > 0, ofRow = a.groups == 1 && shape.nv > 0;
     if (!inWarp && !ofRow) {
         shape.rows = 1;
     }
@@ -971,7 +975,7 @@ BwdPlan PlanBwd(int v, const NormShape& n)
 {
     BwdPlan p{};
     p.v = v;
-    p.shape = ShapeOfRow(n.width, v, 16, v >= 4 ? 512 : kMaxThreads);
+    p.shape = ShapeOfRow(n.width, v, 16, v >= 4 ? 512 : kMaxThreads, 0);
     if (p.shape.nv > 0 && p.shape.threads == 32 && p.shape.rows > 1) {
         // one row a block here too, of as many warps as give each lane one chunk
         const int32_t chunks = (n.width + v - 1) / v;

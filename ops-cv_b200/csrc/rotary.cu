@@ -43,22 +43,24 @@ struct Item {
 };
 
 // Which product is rounded is written out, so that all widths and layouts give the same bits.
-__device__ __forceinline__ void TurnPair(float& x, float& y, float2 cs)
+__device__ __forceinline__ void TurnPair(float& x, float& y, float cs, float sn)
 {
-    const float u = fmaf(x, cs.x, -Mul(y, cs.y));
-    y = fmaf(y, cs.x, Mul(x, cs.y));
+    const float u = fmaf(x, cs, -Mul(y, sn));
+    y = fmaf(y, cs, Mul(x, sn));
     x = u;
 }
 
-// A block has a few tokens. Threads are (item of a head) x (heads) x (tokens); each has kHeads heads of kTokens tokens at a time: its
+// A block has a few tokens. Threads are (item of a head) x (heads) x (tokens); each has kHeads heads of one or two tokens at a time: its
 // addresses serve all the tokens, and all its loads are on their way while the block forms the sines and cosines.
 constexpr int kHeads = 3;
-constexpr int kTokens = 2;
+// two tokens at a time, one where a pair's values lie apart and take twice the registers
+constexpr int TokensAtATime(bool interleaved) { return interleaved ? 2 : 1; }
 
 template <typename T, int V, bool INTER>
 __global__ void __launch_bounds__(kThreads) RotaryKernel(const __grid_constant__ Args a)
 {
-    __shared__ __align__(16) float2 table[kTable];
+    __shared__ __align__(16) float cosines[kTable], sines[kTable]; // [token][frequency]
+    constexpr int kTokens = TokensAtATime(INTER);
     const int32_t half = a.r.half;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * a.tokensPerBlock;
     const int32_t tokens = static_cast<int32_t>(min(static_cast<int64_t>(a.tokensPerBlock), a.r.tokens - first));
@@ -124,7 +126,8 @@ __global__ void __launch_bounds__(kThreads) RotaryKernel(const __grid_constant__
                         const double high = p * fHigh, low = fma(p, fHigh, -high) + p * fLow;
                         float sn, cs;
                         sincospif(2.0f * static_cast<float>((high - rint(high)) + low), &sn, &cs);
-                        table[e] = make_float2(cs * a.r.scale, (a.r.inverse ? -sn : sn) * a.r.scale);
+                        cosines[e] = cs * a.r.scale;
+                        sines[e] = (a.r.inverse ? -sn : sn) * a.r.scale;
                     }
                     __syncthreads();
                 }
@@ -136,12 +139,19 @@ __global__ void __launch_bounds__(kThreads) RotaryKernel(const __grid_constant__
                     }
                     T* q = static_cast<T*>(a.q.out) + TokenAt(first + t, a.r.inner, a.q.outTok);
                     T* k = static_cast<T*>(a.k.out) + TokenAt(first + t, a.r.inner, a.k.outTok);
-                    float2 cs[kNeighbours ? V / 2 : V];
+                    constexpr int kOwn = kNeighbours ? V / 2 : V;
+                    float cs[kOwn], sn[kOwn];
                     if (turn) {
-                        const float2* row = table + t * half + item * (kNeighbours ? V / 2 : V);
+                        const int32_t from = t * half + item * kOwn;
+                        if (half % kOwn == 0) { // aligned to the item's frequencies
+                            *reinterpret_cast<Pack<float, kOwn>*>(cs) = *reinterpret_cast<const Pack<float, kOwn>*>(cosines + from);
+                            *reinterpret_cast<Pack<float, kOwn>*>(sn) = *reinterpret_cast<const Pack<float, kOwn>*>(sines + from);
+                        } else {
 #pragma unroll
-                        for (int e = 0; e < (kNeighbours ? V / 2 : V); ++e) {
-                            cs[e] = row[e];
+                            for (int e = 0; e < kOwn; ++e) {
+                                cs[e] = cosines[from + e];
+                                sn[e] = sines[from + e];
+                            }
                         }
                     }
 #pragma unroll
@@ -159,14 +169,14 @@ __global__ void __launch_bounds__(kThreads) RotaryKernel(const __grid_constant__
                         if constexpr (kNeighbours) {
 #pragma unroll
                             for (int e = 0; e < V / 2; ++e) {
-                                TurnPair(u[2 * e], u[2 * e + 1], cs[e]);
+                                TurnPair(u[2 * e], u[2 * e + 1], cs[e], sn[e]);
                             }
                         } else {
                             float v[V];
                             UnpackToF<T, V>(x[y][i].b, v);
 #pragma unroll
                             for (int e = 0; e < V; ++e) {
-                                TurnPair(u[e], v[e], cs[e]);
+                                TurnPair(u[e], v[e], cs[e], sn[e]);
                             }
                             StorePack<T, V>(to + (second - at), v);
                         }
@@ -264,7 +274,7 @@ cudaError_t RotaryTurn(Dt dt, const RotaryShape& r, const RotaryTensor& q, const
     int32_t down = static_cast<int32_t>(CeilDiv(heads, kHeads));
     down = down < kThreads / across ? down : kThreads / across;
     int32_t deep = kThreads / (across * down);
-    int64_t t = static_cast<int64_t>(kTokens) * deep;
+    int64_t t = static_cast<int64_t>(TokensAtATime(r.interleaved)) * deep;
     const int64_t spread = CeilDiv(r.tokens, static_cast<int64_t>(NumSMs()) * 4);
     t = t < spread ? t : spread;
     const int64_t room = kTable / (r.half < 1 ? 1 : r.half);
