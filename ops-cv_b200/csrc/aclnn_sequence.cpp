@@ -54,6 +54,14 @@ aclnnStatus Guarded(const char* api, uint64_t* workspaceSize, aclOpExecutor** ex
         }                                                                      \
     } while (0)
 
+#define OPSCV_TRY(expr)                     \
+    do {                                    \
+        const aclnnStatus st_ = (expr);     \
+        if (st_ != ACLNN_SUCCESS) {         \
+            return st_;                     \
+        }                                   \
+    } while (0)
+
 int64_t Last(const aclTensor* t) { return t->dims[t->dims.size() - 1]; }
 
 bool LeadEqual(const aclTensor* a, const aclTensor* b, size_t lead)
@@ -87,6 +95,18 @@ bool LastContiguous(const aclTensor* t)
 }
 
 char* DataOf(const aclTensor* t, int elem) { return static_cast<char*>(t->data) + t->offset * elem; }
+
+// A tensor with elements has an address: a kernel would fault on none.
+bool HasData(const aclTensor* t) { return t == nullptr || t->data != nullptr || IsEmpty(t); }
+aclnnStatus CheckData(const char* api, std::initializer_list<const aclTensor*> ts)
+{
+    for (const aclTensor* t : ts) {
+        if (!HasData(t)) {
+            return Fail(ACLNN_ERR_PARAM_NULLPTR, "%s: a tensor has no data", api);
+        }
+    }
+    return ACLNN_SUCCESS;
+}
 
 // One floating tensor of a call, as the kernels get it: the view itself, or a contiguous copy in the workspace.
 struct Operand {
@@ -261,14 +281,6 @@ aclnnStatus CheckPerRow(const char* api, const aclTensor* x, const aclTensor* t,
     return ACLNN_SUCCESS;
 }
 
-#define OPSCV_TRY(expr)                     \
-    do {                                    \
-        const aclnnStatus st_ = (expr);     \
-        if (st_ != ACLNN_SUCCESS) {         \
-            return st_;                     \
-        }                                   \
-    } while (0)
-
 bool EpsOk(double eps) { return std::isfinite(eps) && eps >= 0.0; }
 
 NormShape ShapeOf(const aclTensor* x, const aclTensor* weight, double eps)
@@ -331,6 +343,7 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
     OPSCV_REQUIRE(Last(q) <= (1 << 20) && heads <= (1 << 20) && kHeads <= (1 << 20) && (heads + kHeads) * Last(q) <= (1 << 24),
                   "%s: a token of more than 2^24 values is not supported", api);
     OPSCV_REQUIRE(WritesApart(qOut) && (kOut == nullptr || WritesApart(kOut)), "%s: an output's elements overlap", api);
+    OPSCV_TRY(CheckData(api, {q, k, positions, frequencies, qOut, kOut}));
     if (Numel(q) == 0 && (k == nullptr || Numel(k) == 0)) {
         return ACLNN_SUCCESS;
     }
@@ -472,6 +485,7 @@ aclnnStatus aclnnResidualRmsNormGetWorkspaceSize(const aclTensor* x, const aclTe
         OPSCV_TRY(CheckPerRow(api, x, rstd, 0, "rstd"));
         OPSCV_REQUIRE(EpsOk(eps), "%s: eps must be finite and not negative", api);
         OPSCV_REQUIRE(WritesApart(y) && (sum == nullptr || WritesApart(sum)), "%s: an output's elements overlap", api);
+        OPSCV_TRY(CheckData(api, {x, residual, weight, y, sum, rstd}));
         if (Numel(x) == 0) {
             return ACLNN_SUCCESS;
         }
@@ -538,6 +552,7 @@ aclnnStatus aclnnResidualRmsNormBackwardGetWorkspaceSize(const aclTensor* gradY,
                           "%s: gradWeight must be contiguous, of weight's type and shape", api);
         }
         OPSCV_REQUIRE(WritesApart(gradX), "%s: an output's elements overlap", api);
+        OPSCV_TRY(CheckData(api, {gradY, sum, rstd, weight, gradSum, gradX, gradWeight}));
         NormShape n = ShapeOf(sum, weight, 0.0);
         const Dt dt = ToDt(sum->dtype);
         void* gwAt = gradWeight != nullptr ? DataOf(gradWeight, ElemSize(gradWeight->dtype)) : nullptr;
@@ -613,6 +628,7 @@ aclnnStatus aclnnResidualRmsNormQuantGetWorkspaceSize(const aclTensor* x, const 
         OPSCV_REQUIRE(groups <= 10240, "%s: more than 10240 groups a row are not supported", api);
         OPSCV_TRY(CheckPerRow(api, x, scales, groups, "scales"));
         OPSCV_REQUIRE(sum == nullptr || WritesApart(sum), "%s: an output's elements overlap", api);
+        OPSCV_TRY(CheckData(api, {x, residual, weight, out, scales, sum}));
         if (Numel(x) == 0) {
             return ACLNN_SUCCESS;
         }
@@ -716,6 +732,7 @@ aclnnStatus aclnnRotaryFrequenciesGetWorkspaceSize(double base, int64_t scaling,
         OPSCV_REQUIRE(out->dims.size() == 1 && Dense(out) && out->dims[0] <= (1 << 20),
                       "%s: out must be one contiguous dimension", api);
         const int32_t half = static_cast<int32_t>(out->dims[0]);
+        OPSCV_TRY(CheckData(api, {out}));
         if (half == 0) {
             return ACLNN_SUCCESS;
         }
@@ -748,16 +765,16 @@ aclnnStatus aclnnWindowAttentionGetWorkspaceSize(const aclTensor* q, const aclTe
         if (lse != nullptr) {
             OPSCV_TRY(CheckLse(api, q, lse));
         }
+        OPSCV_TRY(CheckData(api, {q, k, v, qLengths, kvLengths, out, lse}));
         if (Numel(q) == 0) {
             return ACLNN_SUCCESS;
         }
         Operand oq = In(q), ok = In(k), ov = In(v), oo = Out(out);
         OPSCV_TRY(Place(api, {&oq, &ok, &ov, &oo}, false, ex, ws));
         const Dt dt = ToDt(q->dtype);
-        const uint64_t own = ws.Alloc(WindowAttentionFwdWorkspace(dt, shape));
         float* lseAt = lse != nullptr ? reinterpret_cast<float*>(DataOf(lse, 4)) : nullptr;
         ex.steps.push_back([=](char* w, cudaStream_t s) {
-            return WindowAttentionFwd(dt, shape, AttnOf(oq, w), AttnOf(ok, w), AttnOf(ov, w), AttnOf(oo, w), lseAt, w + own, s);
+            return WindowAttentionFwd(dt, shape, AttnOf(oq, w), AttnOf(ok, w), AttnOf(ov, w), AttnOf(oo, w), lseAt, s);
         });
         Finish({&oo}, ex);
         return ACLNN_SUCCESS;
@@ -790,6 +807,7 @@ aclnnStatus aclnnWindowAttentionBackwardGetWorkspaceSize(const aclTensor* gradOu
         }
         OPSCV_TRY(CheckLse(api, q, lse));
         OPSCV_REQUIRE(WritesApart(gradQ) && WritesApart(gradK) && WritesApart(gradV), "%s: an output's elements overlap", api);
+        OPSCV_TRY(CheckData(api, {gradOut, q, k, v, out, lse, qLengths, kvLengths, gradQ, gradK, gradV}));
         if (Numel(q) == 0 && Numel(k) == 0) {
             return ACLNN_SUCCESS;
         }
@@ -797,7 +815,8 @@ aclnnStatus aclnnWindowAttentionBackwardGetWorkspaceSize(const aclTensor* gradOu
         Operand gq = Out(gradQ), gk = Out(gradK), gv = Out(gradV);
         OPSCV_TRY(Place(api, {&og, &oq, &ok, &ov, &oo, &gq, &gk, &gv}, false, ex, ws));
         const Dt dt = ToDt(q->dtype);
-        const uint64_t own = ws.Alloc(WindowAttentionBwdWorkspace(dt, shape));
+        const uint64_t own = ws.Alloc(WindowAttentionBwdWorkspace(dt, shape, AttnOf(og, nullptr), AttnOf(oq, nullptr), AttnOf(ok, nullptr),
+                                                                  AttnOf(ov, nullptr)));
         const float* lseAt = reinterpret_cast<const float*>(DataOf(lse, 4));
         ex.steps.push_back([=](char* w, cudaStream_t s) {
             return WindowAttentionBwd(dt, shape, AttnOf(og, w), AttnOf(oq, w), AttnOf(ok, w), AttnOf(ov, w), AttnOf(oo, w), lseAt,

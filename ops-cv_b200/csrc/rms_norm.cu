@@ -375,8 +375,10 @@ struct Q8Type<Q8::INT8> {
     }
 };
 
-// Value times this is the quantised value. A group of zeros has scale 0 and zeros.
-__device__ __forceinline__ float Inverse(float most, float range) { return most == 0.0f ? 0.0f : range / most; }
+// Value times this is the quantised value. A group of zeros has scale 0 and zeros; so has one whose inverse would overflow.
+constexpr float kLeast = 1e-35f;
+__device__ __forceinline__ float Inverse(float most, float range) { return most < kLeast ? 0.0f : range / most; }
+__device__ __forceinline__ float ScaleOf(float most, float range) { return most < kLeast ? 0.0f : most / range; }
 
 // LG: lanes of a group where a group lies within a warp (a power of two), 0 where groups go through shared memory, one word each, and
 // kRowScale where the row has one scale.
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(kMaxThreads) RmsNormQuantKernel(FwdArgs a)
             }
         }
         if (threadIdx.x == 0) {
-            scales[0] = top / QT::kMost;
+            scales[0] = ScaleOf(top, QT::kMost);
         }
         const float inv = Inverse(top, QT::kMost);
 #pragma unroll
@@ -496,7 +498,7 @@ __global__ void __launch_bounds__(kMaxThreads) RmsNormQuantKernel(FwdArgs a)
             }
             if (inside) {
                 if ((threadIdx.x & (LG - 1)) == 0) {
-                    scales[col / (LG * V)] = top / QT::kMost;
+                    scales[col / (LG * V)] = ScaleOf(top, QT::kMost);
                 }
                 Times(f, Inverse(top, QT::kMost));
                 QT::template Store<V>(q + col, f);
@@ -547,7 +549,7 @@ __global__ void __launch_bounds__(kMaxThreads) RmsNormQuantKernel(FwdArgs a)
             __syncthreads();
         }
         for (int32_t g = threadIdx.x; g < a.groups; g += blockDim.x) {
-            scales[g] = __uint_as_float(most[g]) / QT::kMost;
+            scales[g] = ScaleOf(__uint_as_float(most[g]), QT::kMost);
         }
     }
 }

@@ -78,10 +78,11 @@ struct AttnShape {
 constexpr int kMaxAttnDim = 256;
 
 // out and lse ([batch, heads, lq] contiguous) of queries over keys and values.
-uint64_t WindowAttentionFwdWorkspace(Dt dt, const AttnShape& a);
 cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& a, AttnTensor q, AttnTensor k, AttnTensor v, AttnTensor out, float* lse,
-                               void* workspace, cudaStream_t s);
-uint64_t WindowAttentionBwdWorkspace(Dt dt, const AttnShape& a);
+                               cudaStream_t s);
+// The strides and the alignment of the addresses decide which kernels a call takes; tensors in the workspace may be given by their
+// offsets in it.
+uint64_t WindowAttentionBwdWorkspace(Dt dt, const AttnShape& a, AttnTensor gradOut, AttnTensor q, AttnTensor k, AttnTensor v);
 cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& a, AttnTensor gradOut, AttnTensor q, AttnTensor k, AttnTensor v,
                                AttnTensor out, const float* lse, AttnTensor gradQ, AttnTensor gradK, AttnTensor gradV,
                                void* workspace, cudaStream_t s);

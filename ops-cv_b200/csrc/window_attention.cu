@@ -45,11 +45,15 @@ bool MmaTakes(Dt dt, const AttnArgs& a)
            AttnTmaReadable(a.k, s.lk, s.kvHeads, s.batch) && AttnTmaReadable(a.v, s.lk, s.kvHeads, s.batch);
 }
 
+bool BackwardTakesMma(Dt dt, const AttnArgs& a)
+{
+    const AttnShape& s = a.s;
+    return s.lq > 0 && s.heads > 0 && MmaTakes(dt, a) && AttnTmaReadable(a.gradOut, s.lq, s.heads, s.batch);
+}
+
 } // namespace
 
-uint64_t WindowAttentionFwdWorkspace(Dt, const AttnShape&) { return 0; }
-
-cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& s, AttnTensor q, AttnTensor k, AttnTensor v, AttnTensor out, float* lse, void*,
+cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& s, AttnTensor q, AttnTensor k, AttnTensor v, AttnTensor out, float* lse,
                                cudaStream_t stream)
 {
     AttnArgs a{};
@@ -69,11 +73,15 @@ cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& s, AttnTensor q, AttnTens
     return AttnForwardTiles(dt, a, stream);
 }
 
-uint64_t WindowAttentionBwdWorkspace(Dt dt, const AttnShape& s)
+uint64_t WindowAttentionBwdWorkspace(Dt dt, const AttnShape& s, AttnTensor gradOut, AttnTensor q, AttnTensor k, AttnTensor v)
 {
-    const uint64_t tiles = AttnBackwardTilesWorkspace(s);
-    const uint64_t mma = dt != Dt::F32 && s.dim <= kMmaMostDim ? AttnBackwardMmaWorkspace(s) : 0;
-    return tiles > mma ? tiles : mma; // which kernels a call takes is known only with the pointers
+    AttnArgs a{};
+    a.s = s;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.gradOut = gradOut;
+    return BackwardTakesMma(dt, a) ? AttnBackwardMmaWorkspace(s) : AttnBackwardTilesWorkspace(s);
 }
 
 cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& s, AttnTensor gradOut, AttnTensor q, AttnTensor k, AttnTensor v, AttnTensor out,
@@ -95,11 +103,10 @@ cudaError_t WindowAttentionBwd(Dt dt, const AttnShape& s, AttnTensor gradOut, At
     a.delta = delta;
     a.deltaStride = s.lq;
     a.group = s.heads / s.kvHeads;
-    const bool queries = s.lq > 0 && s.heads > 0; // without any, the gradients of the keys are zeros
-    if (queries && MmaTakes(dt, a) && AttnTmaReadable(gradOut, s.lq, s.heads, s.batch)) {
+    if (BackwardTakesMma(dt, a)) {
         return AttnBackwardMma(dt, a, workspace, stream);
     }
-    if (queries) {
+    if (s.lq > 0 && s.heads > 0) { // without queries, the gradients of the keys are zeros
         const dim3 rows = RowGrid(s.lq, static_cast<int64_t>(s.batch) * s.heads);
         OPSCV_DISPATCH_DT(dt, T, AttnDeltaKernel<T><<<rows, 32 * kRowWarps, 0, stream>>>(a, delta));
         CountLaunch();

@@ -11,7 +11,9 @@ STEP32 = 2.0 ** -24
 CHAIN = 64
 # rows, width: one value, one vector, a warp's row, odd ones, rows of a block, rows of 512 and 1024 threads, rows too wide for them
 SHAPES = [(1, 1), (3, 2), (5, 7), (1, 8), (17, 64), (9, 255), (4, 256), (33, 1000), (2, 1143), (6, 1152), (3, 4096), (2, 4097),
-          (5, 5120), (2, 8190), (2, 8191), (3, 8192), (2, 16384), (2, 16388), (2, 32768), (2, 32776), (1, 70001)]
+          (5, 5120), (2, 8190), (2, 8191), (3, 8192), (2, 16384), (2, 16388), (2, 32768), (2, 32776), (1, 70001),
+          # many rows take fewer threads each
+          (600, 4096), (601, 5120), (640, 8200)]
 
 
 def inputs(shape, t, seed, dev, count=2):
@@ -152,6 +154,18 @@ def test_quant_of_zeros_and_non_finite_rows(ops, dev, dtype, group):
     if group:
         assert scales[3, 0] == 0 and (q[3, :128].float() == 0).all() and scales[3, 1] > 0
     assert scales[4].isfinite().all() and (scales[4] > 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("group", [0, 32, 128])
+def test_quant_of_tiny_rows(ops, dev, dtype, group):
+    """Magnitudes whose scale has no finite inverse become zeros with scale 0."""
+    x = torch.ones(2, 256, device=dev)
+    q, scales, _ = ops.residual_rms_norm_quant(x, None, torch.full((256,), 1e-37, device=dev), dtype=dtype, group=group)
+    assert (scales == 0).all() and (q.float() == 0).all()
+    q, scales, _ = ops.residual_rms_norm_quant(x, None, torch.full((256,), 1e-33, device=dev), dtype=dtype, group=group)
+    back = q.double() * scales.double().repeat_interleave(group or 256, -1)
+    assert ((back - 1e-33).abs() < 1e-33 * 2.0 ** -4).all()
 
 
 def test_non_finite_rows_stay_in_their_rows(ops, dev):

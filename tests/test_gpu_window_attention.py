@@ -139,6 +139,43 @@ def test_against_64_bits(ops, dev, t, b, lq, lk, h, hk, d, window, sinks):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("b,lq,lk,h,hk,d,window,sinks", [
+    (1, 2000, 2000, 2, 1, 64, 130, 200),   # several tiles of sinks, whose far queries go to blocks of their own
+    (2, 900, 900, 4, 4, 72, 100, 70), (1, 1100, 1300, 3, 1, 128, 64, 1), (40, 70, 70, 8, 4, 32, 20, 2),  # many blocks, few blocks
+    (1, 9, 2000, 4, 2, 64, 500, 3), (1, 600, 600, 2, 1, 200, 90, 40),
+])
+def test_more_shapes(ops, dev, t, b, lq, lk, h, hk, d, window, sinks):
+    q, k, v, g = normal((b, lq, h, d), t, 41, dev), normal((b, lk, hk, d), t, 42, dev), normal((b, lk, hk, d), t, 43, dev), normal(
+        (b, lq, h, d), t, 44, dev)
+    check(ops, q, k, v, window, sinks, g=g)
+    kn = torch.tensor([lk - 7 * i % lk for i in range(b)], device=dev)
+    check(ops, q, k, v, window, sinks, kn=kn, g=g)
+
+
+def test_two_streams(ops, dev):
+    """Calls of different sizes that run side by side on two streams, each with a workspace of its own."""
+    work = []
+    for n, (lq, lk, d) in enumerate(((700, 700, 128), (1, 900, 64), (300, 600, 64))):
+        q, k, v, g = normal((2, lq, 4, d), BF16, 50 + n, dev), normal((2, lk, 2, d), BF16, 60 + n, dev), normal(
+            (2, lk, 2, d), BF16, 70 + n, dev), normal((2, lq, 4, d), BF16, 80 + n, dev)
+        out, lse = ops.window_attention(q, k, v, 200, 3)
+        work.append((q, k, v, g, out, lse) + tuple(ops.window_attention_backward(g, q, k, v, out, lse, 200, 3)))
+    torch.cuda.synchronize(dev)
+    streams = [torch.cuda.Stream(dev), torch.cuda.Stream(dev)]
+    spaces = [ops.Workspace(dev), ops.Workspace(dev)]
+    got = []
+    for turn in range(6):
+        for s, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                q, k, v, g, *want = work[(turn + s) % 3]
+                out, lse = ops.window_attention(q, k, v, 200, 3, workspace=spaces[s])
+                got.append(((out, lse) + tuple(ops.window_attention_backward(g, q, k, v, out, lse, 200, 3, workspace=spaces[s])), want))
+    torch.cuda.synchronize(dev)
+    for have, want in got:
+        assert all(torch.equal(x, y) for x, y in zip(have, want))
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("lq,lk,d", [(1, 300, 64), (5, 300, 128), (130, 130, 80), (300, 300, 128), (90, 400, 64)])
 def test_lengths(ops, dev, t, lq, lk, d):
     """Sequences of all lengths, empty ones and ones with more queries than keys; what lies behind the lengths is NaN and infinity."""

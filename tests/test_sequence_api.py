@@ -191,6 +191,31 @@ def test_attention_refuses(ops):
         att(q[0, 0], k, k, 3)
 
 
+def test_tensors_without_data(ops):
+    """A tensor with elements and no address is refused before a kernel could read it; an empty one needs none."""
+    L = ops.lib()
+
+    def tensor(*shape, dtype=ops.ACL_FLOAT, data=None):
+        dims = (ctypes.c_int64 * len(shape))(*shape)
+        return ctypes.c_void_p(L.aclCreateTensor(dims, len(shape), dtype, None, 0, ops.ACL_FORMAT_ND, dims, len(shape), data))
+
+    n, e = ctypes.c_uint64(0), ctypes.c_void_p(None)
+    some = ctypes.c_void_p(4096)
+    for rows, status in ((3, NULLPTR), (0, 0)):
+        x, y, bare = tensor(rows, 8, data=some), tensor(rows, 8, data=some), tensor(rows, 8)
+        for args in ((x, None, None, y), (bare, None, None, y), (x, bare, None, y), (x, None, None, bare)):
+            got = L.aclnnResidualRmsNormGetWorkspaceSize(args[0], args[1], args[2], 1e-6, args[3], None, None, ctypes.byref(n), ctypes.byref(e))
+            assert got == (status if bare in args else 0)
+            if got == 0:
+                L.aclDestroyAclOpExecutor(e)
+    q, k, bare = tensor(1, 2, 2, 8, data=some), tensor(1, 4, 1, 8, data=some), tensor(1, 4, 1, 8)
+    got = L.aclnnWindowAttentionGetWorkspaceSize(q, k, bare, None, None, 3, 0, 1.0, q, None, ctypes.byref(n), ctypes.byref(e))
+    assert got == NULLPTR
+    got = L.aclnnRotaryEmbeddingGetWorkspaceSize(q, None, tensor(1, 2, dtype=ops.ACL_INT64), tensor(4, data=some), None, False, 1.0, q, None,
+                                                 ctypes.byref(n), ctypes.byref(e))
+    assert got == NULLPTR
+
+
 def test_tensors_of_two_devices(ops):
     x = torch.zeros(2, 8)
     with pytest.raises(ValueError, match="one device"):
