@@ -57,7 +57,7 @@ constexpr int kHeads = 3;
 constexpr int TokensAtATime(bool interleaved) { return interleaved ? 2 : 1; }
 
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(kThreads) RotaryKernel(const __grid_constant__ Args a)
+__global__ void __launch_bounds__(kThreads, INTER ? 4 : 3) RotaryKernel(const __grid_constant__ Args a)
 {
     __shared__ __align__(16) float cosines[kTable], sines[kTable]; // [token][frequency]
     constexpr int kTokens = TokensAtATime(INTER);

@@ -472,51 +472,58 @@ struct BackwardArgs {
     bool vecQ, vecK, vecV;
 };
 
-// delta and lse2 of a row by 16 lanes
+// delta and lse2 of the rows of a head (blockIdx.y), a row by 16 lanes, kStatRows rows by each at a time.
+constexpr int kStatRows = 4;
 template <typename T>
-__global__ void __launch_bounds__(256) AttnStatisticsKernel(BackwardArgs m, bool vec)
+__global__ void __launch_bounds__(256) AttnStatisticsKernel(const __grid_constant__ BackwardArgs m, bool vec)
 {
     const AttnShape& s = m.a.s;
-    const int32_t lane = threadIdx.x & 15;
-    const int64_t total = static_cast<int64_t>(s.batch) * s.heads * m.stride;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-    const bool inside = row < total;
-    const int64_t bh = inside ? row / m.stride : 0;
-    const int32_t i = inside ? static_cast<int32_t>(row - bh * m.stride) : s.lq;
-    float sum = 0.0f;
-    float lse = INFINITY;
-    if (i < s.lq) {
-        const int32_t b = static_cast<int32_t>(bh / s.heads), h = static_cast<int32_t>(bh % s.heads);
+    const int32_t lane = threadIdx.x & 15, first = blockIdx.x * (16 * kStatRows) + (threadIdx.x >> 4);
+    for (int32_t bh = blockIdx.y; bh < s.batch * s.heads; bh += gridDim.y) {
+        const int32_t b = bh / s.heads, h = bh - b * s.heads;
         const Lengths n = LengthsOf(s, b);
-        if (i < n.q && n.shift + i >= 0) {
-            const T* g = RowOf<T>(m.a.gradOut, b, i, h);
-            const T* o = RowOf<T>(m.a.out, b, i, h);
-            if (vec) {
-                const int32_t d = lane * 8;
-                if (d < s.dim) {
-                    float x[8], y[8];
-                    LoadPack<T, 8>(g + d, x);
-                    LoadPack<T, 8>(o + d, y);
+        const T* g = RowOf<T>(m.a.gradOut, b, 0, h);
+        const T* o = RowOf<T>(m.a.out, b, 0, h);
+        const int64_t stats = bh * m.stride, rows = static_cast<int64_t>(bh) * s.lq;
+        float sum[kStatRows], lse[kStatRows];
+        Pack<T, 8> x[kStatRows], y[kStatRows];
+        bool live[kStatRows];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        sum = fmaf(x[e], y[e], sum);
-                    }
+        for (int r = 0; r < kStatRows; ++r) {
+            const int32_t i = first + 16 * r;
+            live[r] = i < n.q && n.shift + i >= 0;
+            lse[r] = live[r] ? m.a.lse[rows + i] : INFINITY;
+            sum[r] = 0.0f;
+            if (vec && live[r] && lane * 8 < s.dim) {
+                x[r] = *reinterpret_cast<const Pack<T, 8>*>(g + i * m.a.gradOut.l + lane * 8);
+                y[r] = *reinterpret_cast<const Pack<T, 8>*>(o + i * m.a.out.l + lane * 8);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kStatRows; ++r) {
+            const int32_t i = first + 16 * r;
+            if (vec && live[r] && lane * 8 < s.dim) {
+                float u[8], v[8];
+                UnpackToF<T, 8>(x[r], u);
+                UnpackToF<T, 8>(y[r], v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    sum[r] = fmaf(u[e], v[e], sum[r]);
                 }
-            } else {
+            } else if (!vec && live[r]) {
                 for (int32_t d = lane; d < s.dim; d += 16) {
-                    sum = fmaf(DType<T>::ToF(g[d]), DType<T>::ToF(o[d]), sum);
+                    sum[r] = fmaf(DType<T>::ToF(g[i * m.a.gradOut.l + d]), DType<T>::ToF(o[i * m.a.out.l + d]), sum[r]);
                 }
             }
-            lse = fmaf(m.a.lse[bh * s.lq + i], kLog2e, -kWeightShift);
-        }
-    }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    }
-    if (inside && lane == 0) {
-        m.lse2[row] = lse;
-        m.delta[row] = sum;
+            for (int e = 8; e > 0; e >>= 1) {
+                sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], e);
+            }
+            if (lane == 0 && i < m.stride) {
+                m.lse2[stats + i] = live[r] ? fmaf(lse[r], kLog2e, -kWeightShift) : INFINITY;
+                m.delta[stats + i] = sum[r];
+            }
+        }
     }
 }
 
@@ -1194,7 +1201,7 @@ __device__ __forceinline__ void GradKvBlock(const BackwardArgs& m, const CUtenso
             if (part != nullptr) {
 #pragma unroll
                 for (int e = 0; e < kOwn; ++e) {
-                    if (d0 + e < s.dim) {
+                    if (d0 + e < s.dim && (chunk < 0 || j < s.sinks)) { // further blocks have sums of sinks alone
                         part[d0 + e] = *failed != 0 ? NAN : v[e];
                     }
                 }
@@ -1247,9 +1254,9 @@ __global__ void __launch_bounds__(kGradThreads + 64, 1)
     }
 }
 
-// gradK and gradV of the keys of tiles with sinks: the blocks' sums in order, a warp per key.
+// gradK and gradV of the keys of tiles with sinks: the blocks' sums in order, a warp per key, a lane per four values of both.
 template <typename T>
-__global__ void __launch_bounds__(128) AttnSinkGradKernel(BackwardArgs m)
+__global__ void __launch_bounds__(128) AttnSinkGradKernel(const __grid_constant__ BackwardArgs m)
 {
     const AttnShape& s = m.a.s;
     const int lane = threadIdx.x & 31;
@@ -1262,16 +1269,28 @@ __global__ void __launch_bounds__(128) AttnSinkGradKernel(BackwardArgs m)
     if (bu >= s.batch * s.kvHeads || j >= s.lk) {
         return;
     }
-    bool bad = false;
-    for (int which = 0; which < 2; ++which) {
-        T* out = OutRowOf<T>(which == 0 ? m.a.gradK : m.a.gradV, b, j, u);
-        for (int32_t d = lane; d < s.dim; d += 32) {
-            float sum = 0.0f;
-            for (int32_t c = 0; c <= m.farChunks; ++c) {
-                sum += m.partial[((tileIndex * (1 + m.farChunks) + c) * 2 + which) * kTile * s.dim + static_cast<int64_t>(r) * s.dim + d];
+    const int32_t slots = j < s.sinks ? 1 + m.farChunks : 1;
+    const float* part = m.partial + tileIndex * (1 + m.farChunks) * 2 * kTile * s.dim + static_cast<int64_t>(r) * s.dim;
+    const int64_t other = static_cast<int64_t>(kTile) * s.dim; // from gradK to gradV
+    float sum[2][4] = {};
+#pragma unroll 4
+    for (int32_t c = 0; c < slots; ++c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (lane + 32 * e < s.dim) {
+                sum[0][e] += part[2 * c * other + lane + 32 * e];
+                sum[1][e] += part[(2 * c + 1) * other + lane + 32 * e];
             }
-            bad = bad || !(fabsf(sum) <= 3.4e38f);
-            out[d] = DType<T>::FromF(sum);
+        }
+    }
+    T *gk = OutRowOf<T>(m.a.gradK, b, j, u), *gv = OutRowOf<T>(m.a.gradV, b, j, u);
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (lane + 32 * e < s.dim) {
+            gk[lane + 32 * e] = DType<T>::FromF(sum[0][e]);
+            gv[lane + 32 * e] = DType<T>::FromF(sum[1][e]);
+            bad = bad || !(fabsf(sum[0][e]) <= 3.4e38f) || !(fabsf(sum[1][e]) <= 3.4e38f);
         }
     }
     if (__any_sync(0xffffffffu, bad)) {
@@ -1406,7 +1425,8 @@ namespace {
 struct BackwardLaunch {
     const BackwardArgs& m;
     const CUtensorMap &mq, &mg, &mk, &mv;
-    unsigned statBlocks, blocks;
+    dim3 statBlocks;
+    unsigned blocks;
     int shared;
     bool vecStats;
 };
@@ -1419,7 +1439,7 @@ cudaError_t LaunchBackward(const BackwardLaunch& l, cudaStream_t stream)
         if (set != cudaSuccess) {
             return set;
         }
-        AttnStatisticsKernel<T><<<l.statBlocks, 256, 0, stream>>>(m, l.vecStats);
+        AttnStatisticsKernel<T><<<l.statBlocks, 256, 0, stream>>>(m, l.vecStats); // rows x heads
         kernel<<<l.blocks, kGradThreads + 64, l.shared, stream>>>(m, l.mq, l.mg, l.mk, l.mv);
         CountLaunch(2);
         if (m.farChunks > 0) {
@@ -1465,9 +1485,10 @@ cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStrea
     m.vecQ = VecRows(a.gradQ, s.dim);
     m.vecK = VecRows(a.gradK, s.dim);
     m.vecV = VecRows(a.gradV, s.dim);
-    const int64_t statBlocks = CeilDiv(static_cast<int64_t>(s.batch) * s.heads * m.stride, 16);
+    const int64_t heads = static_cast<int64_t>(s.batch) * s.heads;
+    const dim3 statBlocks(static_cast<unsigned>(CeilDiv(m.stride, 16 * kStatRows)), static_cast<unsigned>(heads < 65535 ? heads : 65535));
     const int64_t kvBlocks = static_cast<int64_t>(s.batch) * s.kvHeads * (m.kTiles + static_cast<int64_t>(m.sinkTiles) * m.farChunks);
-    if (statBlocks > INT32_MAX || kvBlocks > INT32_MAX) {
+    if (kvBlocks > INT32_MAX) {
         return cudaErrorInvalidConfiguration;
     }
     CUtensorMap mq, mg, mk, mv;
@@ -1487,7 +1508,7 @@ cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStrea
     }
     m.kvBlocks = static_cast<uint32_t>(kvBlocks);
     const bool vecStats = VecRows(a.gradOut, s.dim) && VecRows(a.out, s.dim);
-    const BackwardLaunch l{m, mq, mg, mk, mv, static_cast<unsigned>(statBlocks), static_cast<unsigned>(blocks), shared, vecStats};
+    const BackwardLaunch l{m, mq, mg, mk, mv, statBlocks, static_cast<unsigned>(blocks), shared, vecStats};
     return dt == Dt::F16 ? LaunchBackward<__half>(l, stream) : LaunchBackward<__nv_bfloat16>(l, stream);
 }
 
