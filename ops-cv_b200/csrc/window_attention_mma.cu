@@ -124,19 +124,18 @@ __device__ __forceinline__ void LiveColumns(uint32_t (&live)[N / 32], int32_t fr
 //
 // A row's weights are formed from the maximum of the steps before while the row's two threads exchange the maxima of this one; only
 // where a row has outgrown its old maximum by 2^8 (at the start, mostly) are they formed again and O rescaled.
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;
 constexpr int kKeys = 64;
 constexpr uint32_t kKeyHalf = kKeys * 128;
 
 struct ForwardShared {
-    uint64_t qFull, kFull[2], vFull[2], sFull[2], pFull[2], pvDone[2], allDone, drain, exchanged[4];
-    uint32_t tmem, failed, bad[4];
-    float row[2][2][kTile]; // maxima of even and odd steps (and the sums, at the end) of a row's two threads
+    uint64_t qFull, kFull[2], vFull[2], sFull[2], pFull[2], pvDone[2], allDone, drain;
+    uint32_t tmem, failed;
 };
 
 // KS: steps of 16 values of a head.
 template <typename T, int KS>
-__global__ void __launch_bounds__(320, 2)
+__global__ void __launch_bounds__(192, 2)
     AttnForwardMmaKernel(const __grid_constant__ MmaArgs m, const __grid_constant__ CUtensorMap mapQ,
                          const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV)
 {
@@ -169,13 +168,9 @@ __global__ void __launch_bounds__(320, 2)
         }
         BarInit(&sh.allDone, 1);
         BarInit(&sh.drain, 1);
-        for (int e = 0; e < 4; ++e) {
-            BarInit(&sh.exchanged[e], 64);
-            sh.bad[e] = 0;
-        }
         BarInitDone();
     }
-    if (warp == 9) {
+    if (warp == 5) {
         TmemAlloc(&sh.tmem, 256);
     }
     TcFenceBefore();
@@ -184,7 +179,7 @@ __global__ void __launch_bounds__(320, 2)
     const uint32_t tO = sh.tmem, tS = tO + 128; // S of even steps at 0 and of odd ones at 64 from there
     volatile uint32_t* failed = &sh.failed;
 
-    if (warp == 8) {
+    if (warp == 4) {
         if ((threadIdx.x & 31) == 0 && count > 0) {
             const int32_t u = h / m.a.group;
             BarExpect(&sh.qFull, kBytes);
@@ -229,7 +224,7 @@ __global__ void __launch_bounds__(320, 2)
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == 5) {
         if (count > 0) {
             const bool lead = ElectOne();
             const uint32_t descS = ProductDesc<T>(kKeys, false, s.scale < 0.0f);
@@ -267,7 +262,7 @@ __global__ void __launch_bounds__(320, 2)
                     const uint64_t v0 = dv + st * (kKeyBytes >> 4);
 #pragma unroll
                     for (int32_t k = 0; k < kKeys / 16; ++k) {
-                        MmaTmem(tO, tS + st * kKeys + (k >> 1) * 32 + (k & 1) * 8, v0 + k * (2048 >> 4), descO, it > 0 || k > 0);
+                        MmaTmem(tO, tS + st * kKeys + k * 8, v0 + k * (2048 >> 4), descO, it > 0 || k > 0);
                     }
                     MmaCommit(&sh.pvDone[st]);
                 }
@@ -294,47 +289,48 @@ __global__ void __launch_bounds__(320, 2)
         }
         __syncwarp();
     } else {
-        const int32_t side = warp >> 2, quad = warp & 3, r = quad * 32 + (threadIdx.x & 31);
+        const int32_t quad = warp & 3, r = quad * 32 + (threadIdx.x & 31);
         const int32_t i = i0 + r;
         const int32_t p = i <= iLast ? n.shift + i : -1;
         const Seen seen = SeenOf(s, p);
         const uint32_t lanes = static_cast<uint32_t>(quad) << 21; // 32 quad, in the lane half of an address
-        const uint32_t to32 = tO + 32 * HALVES * side + lanes;
+        const uint32_t to32 = tO + lanes;
         const float factor = fabsf(s.scale) * kLog2e;             // scores in powers of two
         const int32_t wLow = low + 32 * quad, wHigh = wLow + 31;
         const bool rowsWhole = i0 + 32 * quad + 31 <= iLast;
         const F2 factor2 = MakeF2(factor, factor);
         float top = -INFINITY, total = 0.0f;
         for (int32_t it = 0; it < count; ++it) {
-            const int32_t j0 = steps.Key(it) + 32 * side;
-            const uint32_t tx = tS + (it & 1) * kKeys + 32 * side + lanes;
+            const int32_t j0 = steps.Key(it);
+            const uint32_t tx = tS + (it & 1) * kKeys + lanes;
             BarWait(&sh.sFull[it & 1], (it / 2) & 1, failed);
             if (__any_sync(0xffffffffu, *failed != 0)) {
                 break;
             }
             TcFenceAfter();
             const bool sinkStep = it < steps.sinkSteps;
-            const bool masked = sinkStep || !rowsWhole || j0 + 31 > wLow || j0 <= wHigh - s.window;
-            uint32_t x[32];
+            const bool masked = sinkStep || !rowsWhole || j0 + kKeys - 1 > wLow || j0 <= wHigh - s.window;
+            uint32_t x[64];
             auto read = [&] {
                 TmemLoad32(tx, x);
+                TmemLoad32(tx + 32, x + 32);
                 if (masked) {
                     // Visible columns of the step: those of the window, or those of the sinks. A window step may hold sinks as well:
                     // those behind the block's first key, in front of the row's window.
-                    uint32_t live[1];
-                    LiveColumns<32>(live, sinkStep ? 0 : seen.first - j0, p < 0 ? 0 : sinkStep ? steps.sinkEnd - j0 : p - j0 + 1,
+                    uint32_t live[2];
+                    LiveColumns<64>(live, sinkStep ? 0 : seen.first - j0, p < 0 ? 0 : sinkStep ? steps.sinkEnd - j0 : p - j0 + 1,
                                     sinkStep ? 0 : seen.sinkEnd - j0);
-                    MaskColumns<32>(x, live);
+                    MaskColumns<64>(x, live);
                 }
             };
-            uint32_t w[16];
+            uint32_t w[32];
             float sum = 0.0f;
             auto weigh = [&] {
                 const float off = top == -INFINITY ? 0.0f : -top;
                 const F2 off2 = MakeF2(off, off);
                 F2 sum2[2] = {MakeF2(0.0f, 0.0f), MakeF2(0.0f, 0.0f)};
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
+                for (int e = 0; e < 32; ++e) {
                     float e0, e1;
                     SplitF2(Fma2(MakeF2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), factor2, off2), e0, e1);
                     e0 = Exp2(e0);
@@ -349,37 +345,28 @@ __global__ void __launch_bounds__(320, 2)
             read();
             float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 32; c += 8) {
+            for (int c = 0; c < 64; c += 8) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     part[e] = fmaxf(fmaxf(part[e], __uint_as_float(x[c + 2 * e])), __uint_as_float(x[c + 2 * e + 1]));
                 }
             }
-            float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * factor;
-            sh.row[it & 1][side][r] = most;
-            BarArrive(&sh.exchanged[quad]);
-            if (it > 0) {
-                weigh();
-            }
-            BarWait(&sh.exchanged[quad], it & 1, failed);
-            most = fmaxf(most, sh.row[it & 1][side ^ 1][r]);
+            const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * factor;
             const float grown = fmaxf(top, most);
             const bool grow = grown > top + kGrowth; // always from -infinity to a number
             if (it == 0) {
                 top = grown;
-                weigh();
-            } else if (__any_sync(0xffffffffu, grow)) { // in both warps of the rows alike
+            } else if (__any_sync(0xffffffffu, grow)) {
                 const float fade = grow ? Exp2(top - grown) : 1.0f;
                 top = grow ? grown : top;
                 total *= fade;
                 BarWait(&sh.pvDone[(it - 1) & 1], ((it - 1) / 2) & 1, failed);
                 TcFenceAfter();
-                TmemScale<32 * HALVES>(to32, fade);
-                read();
-                weigh();
+                TmemScale<64 * HALVES>(to32, fade);
             }
+            weigh();
             total += sum;
-            TmemStore16(tx, w);
+            TmemStore32(tx, w);
             TmemStoreWait();
             TcFenceBefore();
             BarArrive(&sh.pFull[it & 1]);
@@ -389,16 +376,12 @@ __global__ void __launch_bounds__(320, 2)
             BarWait(&sh.allDone, 0, failed);
             TcFenceAfter();
         }
-        RowBarrier<kRowThreads>(); // the last maxima have been read
-        sh.row[0][side][r] = total;
-        RowBarrier<kRowThreads>();
-        total = sh.row[0][0][r] + sh.row[0][1][r];
         const float inverse = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total; // NaN stays
         bool bad = seen.count > 0 && !(total > 0.0f && total <= 3.0e38f);
         T* out = i < s.lq ? OutRowOf<T>(m.a.out, b, i, h) : nullptr;
 #pragma unroll
-        for (int c = 0; c < HALVES; ++c) {
-            const int32_t d0 = 32 * (HALVES * side + c);
+        for (int c = 0; c < 2 * HALVES; ++c) {
+            const int32_t d0 = 32 * c;
             uint32_t o[32];
             if (count > 0) {
                 TmemLoad32(to32 + 32 * c, o);
@@ -413,22 +396,19 @@ __global__ void __launch_bounds__(320, 2)
                 StoreRow<T>(out + d0, v, s.dim - d0, m.vecOut);
             }
         }
-        if (out != nullptr && m.a.lse != nullptr && side == 0) {
+        if (out != nullptr && m.a.lse != nullptr) {
             m.a.lse[(static_cast<int64_t>(b) * s.heads + h) * s.lq + i] = seen.count > 0 ? (top + log2f(total)) * kLn2 : -INFINITY;
         }
         const uint32_t rows = __ballot_sync(0xffffffffu, bad && out != nullptr);
-        if ((threadIdx.x & 31) == 0 && rows != 0) {
-            atomicOr(&sh.bad[quad], rows);
-        }
-        RowBarrier<kRowThreads>();
-        // rows that are not finite again, without the masked keys' part: the even ones by one warp, the odd ones by another
-        uint32_t again = sh.bad[quad] & (side == 0 ? 0x55555555u : 0xaaaaaaaau);
+        __syncwarp();
+        // rows that are not finite again, without the masked keys' part
+        uint32_t again = rows;
         while (again != 0) {
             const int e = __ffs(again) - 1;
             again &= again - 1;
             AttnForwardRow<T>(m.a, b, h, i0 + 32 * quad + e);
         }
-        if (*failed != 0 && out != nullptr && side == 0) {
+        if (*failed != 0 && out != nullptr) {
             for (int32_t d = 0; d < s.dim; ++d) {
                 out[d] = DType<T>::FromF(NAN);
             }
@@ -436,7 +416,7 @@ __global__ void __launch_bounds__(320, 2)
     }
     TcFenceBefore();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 5) {
         TcFenceAfter();
         TmemFree(sh.tmem, 256);
     }
@@ -1329,7 +1309,7 @@ cudaError_t LaunchForward(const MmaArgs& m, const CUtensorMap& mq, const CUtenso
         if (set != cudaSuccess) {
             return set;
         }
-        kernel<<<grid, 320, shared, stream>>>(m, mq, mk, mv);
+        kernel<<<grid, 192, shared, stream>>>(m, mq, mk, mv);
         CountLaunch();
         return cudaGetLastError();
     };
