@@ -312,8 +312,7 @@ __global__ void __launch_bounds__(192, 2)
             const bool masked = sinkStep || !rowsWhole || j0 + kKeys - 1 > wLow || j0 <= wHigh - s.window;
             uint32_t x[64];
             auto read = [&] {
-                TmemLoad32(tx, x);
-                TmemLoad32(tx + 32, x + 32);
+                TmemLoad64(tx, x);
                 if (masked) {
                     // Visible columns of the step: those of the window, or those of the sinks. A window step may hold sinks as well:
                     // those behind the block's first key, in front of the row's window.
