@@ -5,6 +5,7 @@
 // in each thread's registers takes 64 for 8 reads of 16 bytes from shared memory. Tensor cores would need three products of tf32 parts for
 // each of fp32 and still lose bits that fp32 callers have. Blocks own their sums (gradQ in one kernel, gradK and gradV in another), so
 // nothing is added up in memory and the order of all sums is fixed.
+#include "cp_async.cuh"
 #include "window_attention.cuh"
 
 namespace opscv {
@@ -25,13 +26,27 @@ struct Tile {
     static constexpr int kWeightFloats = A * kWeights;
 };
 
-// Rows [from, from + ROWS) of one head as fp32, zeros for rows behind `end` and values behind dim.
+// Rows [from, from + ROWS) of one head as fp32, zeros for rows behind `end` and values behind dim. fp32 rows that can be read 16 bytes at a
+// time are copied asynchronously: the caller commits and waits, and the copies of the next step run under the products of this one.
 template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void LoadTile(float* dst, const AttnTensor& t, int32_t b, int32_t h, int32_t from, int32_t end, int32_t dim,
                                          bool vec)
 {
     constexpr int kStride = DP + 4;
     const T* base = RowOf<T>(t, b, 0, h);
+    if constexpr (sizeof(T) == 4) {
+        if (vec) {
+            const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+            for (int e = threadIdx.x; e < ROWS * (DP / 4); e += kThreads) {
+                const int r = e / (DP / 4), d = e % (DP / 4) * 4;
+                const bool live = from + r < end && d < dim;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (r * kStride + d) * 4),
+                             "l"(live ? base + (from + r) * t.l + d : base), "r"(live ? 16 : 0)
+                             : "memory");
+            }
+            return;
+        }
+    }
     if (vec) {
 #pragma unroll 4
         for (int e = threadIdx.x; e < ROWS * (DP / 4); e += kThreads) {
@@ -199,7 +214,7 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
     constexpr int R = L::kA, C = L::kB;
     extern __shared__ float shared[];
     __shared__ uint32_t again[2];
-    float *sq = shared, *sk = sq + L::kFloatsA, *sw = sk + L::kFloatsB; // keys, then values
+    float *sq = shared, *sk = sq + L::kFloatsA, *sv = sk + L::kFloatsB, *sw = sv + L::kFloatsB;
     const AttnShape& s = m.a.s;
     const int32_t tile = blockIdx.x % m.tiles, bh = blockIdx.x / m.tiles;
     const int32_t b = bh / s.heads, h = bh % s.heads, u = h / m.a.group;
@@ -210,7 +225,15 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
     if (threadIdx.x < 2) {
         again[threadIdx.x] = 0;
     }
+    auto fetch = [&](float* to, const AttnTensor& x, int32_t step) {
+        if (step < walk.steps) {
+            LoadTile<T, DP, B>(to, x, b, u, walk.Key(step), n.kv, s.dim, m.vec);
+        }
+        CpAsyncCommit();
+    };
     LoadTile<T, DP, A>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
+    fetch(sk, m.a.k, 0);
+    fetch(sv, m.a.v, 0);
     float2 o[R][L::kPairs] = {};
     float top[R], total[R];
     int32_t p[R];
@@ -223,8 +246,7 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
     }
     for (int32_t step = 0; step < walk.steps; ++step) {
         const int32_t j0 = walk.Key(step);
-        __syncthreads(); // the values of the step before have been read
-        LoadTile<T, DP, B>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
+        CpAsyncWait<1>(); // the keys; the values may still be on their way
         __syncthreads();
         float x[R][C];
         Inner<L, DP>(sq, sk, x);
@@ -253,10 +275,13 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
                 o[r][c] = make_float2(o[r][c].x * fade, o[r][c].y * fade);
             }
         }
+        __syncthreads(); // the keys have been read, the weights written
+        fetch(sk, m.a.k, step + 1);
+        CpAsyncWait<1>();
         __syncthreads();
-        LoadTile<T, DP, B>(sk, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
+        Outer<L, B>(sw, sv, o);
         __syncthreads();
-        Outer<L, B>(sw, sk, o);
+        fetch(sv, m.a.v, step + 1);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -310,6 +335,14 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
     }
     LoadTile<T, DP, A>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
     LoadTile<T, DP, A>(sg, m.a.gradOut, b, h, i0, iLast + 1, s.dim, m.vec);
+    auto fetch = [&](float* to, const AttnTensor& x, int32_t step) {
+        if (step < walk.steps) {
+            LoadTile<T, DP, B>(to, x, b, u, walk.Key(step), n.kv, s.dim, m.vec);
+        }
+        CpAsyncCommit();
+    };
+    fetch(sv, m.a.v, 0);
+    fetch(sk, m.a.k, 0);
     float2 o[R][L::kPairs] = {};
     float lse[R], delta[R];
     int32_t p[R];
@@ -322,13 +355,15 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
     }
     for (int32_t step = 0; step < walk.steps; ++step) {
         const int32_t j0 = walk.Key(step);
-        __syncthreads();
-        LoadTile<T, DP, B>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
-        LoadTile<T, DP, B>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
+        CpAsyncWait<1>();
         __syncthreads();
         float x[R][C], y[R][C];
-        Inner<L, DP>(sq, sk, x);
         Inner<L, DP>(sg, sv, y);
+        __syncthreads();
+        fetch(sv, m.a.v, step + 1); // under the products with the keys
+        CpAsyncWait<1>();
+        __syncthreads();
+        Inner<L, DP>(sq, sk, x);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -340,6 +375,8 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
         }
         __syncthreads();
         Outer<L, B>(sw, sk, o);
+        __syncthreads();
+        fetch(sk, m.a.k, step + 1); // under the next products with the values
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -408,38 +445,50 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
     LoadTile<T, DP, A>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
     LoadTile<T, DP, A>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
     float2 ok[R][L::kPairs] = {}, ov[R][L::kPairs] = {};
-    for (int32_t h = hFirst; h < hEnd; ++h) {
-        const int64_t head = static_cast<int64_t>(b) * s.heads + h;
-        for (int32_t p0 = low; p0 <= high; p0 += B) {
-            const int32_t i0 = p0 - n.shift;
-            __syncthreads();
-            LoadTile<T, DP, B>(sq, m.a.q, b, h, i0, n.q, s.dim, m.vec);
-            LoadTile<T, DP, B>(sg, m.a.gradOut, b, h, i0, n.q, s.dim, m.vec);
-            if (threadIdx.x < B) {
-                const int32_t i = i0 + threadIdx.x;
-                sLse[threadIdx.x] = i < n.q ? m.a.lse[head * s.lq + i] : 0.0f;
-                sDelta[threadIdx.x] = i < n.q ? m.a.delta[head * m.a.deltaStride + i] : 0.0f;
-            }
-            __syncthreads();
-            float x[R][C], y[R][C];
-            Inner<L, DP>(sk, sq, x);
-            Inner<L, DP>(sv, sg, y);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int32_t j = j0 + R * ty + r;
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const int32_t e = tx + 16 * c, p = p0 + e;
-                    const bool live = j < n.kv && p <= stop && j <= p && (j > p - s.window || j < s.sinks);
-                    const float w = live ? expf(x[r][c] * s.scale - sLse[e]) : 0.0f;
-                    sw[(R * ty + r) * L::kWeights + e] = w;
-                    sd[(R * ty + r) * L::kWeights + e] = live ? w * (y[r][c] - sDelta[e]) * s.scale : 0.0f;
-                }
-            }
-            __syncthreads();
-            Outer<L, B>(sw, sg, ov);
-            Outer<L, B>(sd, sq, ok);
+    // steps over the heads and their queries
+    const int32_t perHead = high >= low ? (high - low + B) / B : 0, steps = perHead * (hEnd - hFirst);
+    auto fetch = [&](float* to, const AttnTensor& x, int32_t step) {
+        if (step < steps) {
+            LoadTile<T, DP, B>(to, x, b, hFirst + step / perHead, low + step % perHead * B - n.shift, n.q, s.dim, m.vec);
         }
+        CpAsyncCommit();
+    };
+    fetch(sg, m.a.gradOut, 0);
+    fetch(sq, m.a.q, 0);
+    for (int32_t step = 0; step < steps; ++step) {
+        const int64_t head = static_cast<int64_t>(b) * s.heads + hFirst + step / perHead;
+        const int32_t p0 = low + step % perHead * B, i0 = p0 - n.shift;
+        if (threadIdx.x < B) {
+            const int32_t i = i0 + threadIdx.x;
+            sLse[threadIdx.x] = i < n.q ? m.a.lse[head * s.lq + i] : 0.0f;
+            sDelta[threadIdx.x] = i < n.q ? m.a.delta[head * m.a.deltaStride + i] : 0.0f;
+        }
+        CpAsyncWait<1>();
+        __syncthreads();
+        float x[R][C], y[R][C];
+        Inner<L, DP>(sv, sg, y);
+        CpAsyncWait<0>();
+        __syncthreads();
+        Inner<L, DP>(sk, sq, x);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int32_t j = j0 + R * ty + r;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int32_t e = tx + 16 * c, p = p0 + e;
+                const bool live = j < n.kv && p <= stop && j <= p && (j > p - s.window || j < s.sinks);
+                const float w = live ? expf(x[r][c] * s.scale - sLse[e]) : 0.0f;
+                sw[(R * ty + r) * L::kWeights + e] = w;
+                sd[(R * ty + r) * L::kWeights + e] = live ? w * (y[r][c] - sDelta[e]) * s.scale : 0.0f;
+            }
+        }
+        __syncthreads();
+        Outer<L, B>(sw, sg, ov);
+        __syncthreads();
+        fetch(sg, m.a.gradOut, step + 1); // under the other outer products
+        Outer<L, B>(sd, sq, ok);
+        __syncthreads();
+        fetch(sq, m.a.q, step + 1); // under the next products with the values
     }
     if (m.partial != nullptr) {
         float* part = m.partial + PartialSlot(m, unit, tile, 1 + chunk, A);
@@ -532,7 +581,7 @@ cudaError_t Forward(Dt dt, const AttnArgs& a, cudaStream_t stream)
     m.a = a;
     m.tiles = static_cast<int32_t>(CeilDiv(s.lq, A));
     m.vec = s.dim % 4 == 0 && ReadsByFour(dt, a.q) && ReadsByFour(dt, a.k) && ReadsByFour(dt, a.v);
-    constexpr int shared = (L::kFloatsA + L::kFloatsB + L::kWeightFloats) * 4;
+    constexpr int shared = (L::kFloatsA + 2 * L::kFloatsB + L::kWeightFloats) * 4;
     static std::atomic<uint64_t> asked;
     const int64_t blocks = static_cast<int64_t>(s.batch) * s.heads * m.tiles;
     if (blocks > INT32_MAX) {
