@@ -115,15 +115,15 @@ __device__ __forceinline__ void LiveColumns(uint32_t (&live)[N / 32], int32_t fr
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
-// A block has 128 queries of a head and walks its keys 64 at a time. Warp 8's first thread loads the tiles, warp 9's issues the products;
-// warps 0 to 7 have two threads a query, of 32 columns each: S = Q K^T arrives in tensor memory, the threads form the weights, write
-// them over S as 16-bit values, and O += P V takes them from there, so that neither S nor P touches shared memory. S has two places
-// (O, at most 128 columns, and twice 64), so the next step's scores are there when the threads come to them, and the products, their
-// latency and the copies stay out of the chain of the exponentials, which bound the rest. Two blocks share an SM (256 columns of tensor
-// memory, 97 KB of shared memory and 320 threads each).
+// A block has 128 queries of a head and walks its keys 64 at a time. Warp 4's first thread loads the tiles, warp 5 issues the products;
+// warps 0 to 3 have a thread a query, with all 64 scores of a step in its registers: S = Q K^T arrives in tensor memory, the thread forms
+// the weights, writes them over S as 16-bit values, and O += P V takes them from there, so that neither S nor P touches shared memory and
+// a row's maximum and sum need no exchange (two threads a row: 333 us at 8192 tokens without a window, one: 301). S has two places (O, at
+// most 128 columns, and twice 64), so the next step's scores are there when the threads come to them. Two blocks share an SM (256 columns
+// of tensor memory, 97 KB of shared memory and 192 threads each), one's exponentials under the other's products.
 //
-// A row's weights are formed from the maximum of the steps before while the row's two threads exchange the maxima of this one; only
-// where a row has outgrown its old maximum by 2^8 (at the start, mostly) are they formed again and O rescaled.
+// Bound by the chain of a row's thread: scores from tensor memory, their maximum, 64 exponentials, weights back. The running maximum moves
+// only where a row has outgrown it by 2^8 (at the start, mostly); O is rescaled then and not otherwise.
 constexpr int kRowThreads = 128;
 constexpr int kKeys = 64;
 constexpr uint32_t kKeyHalf = kKeys * 128;
