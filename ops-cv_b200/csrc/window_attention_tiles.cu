@@ -12,36 +12,42 @@ namespace opscv {
 
 namespace {
 
-constexpr int kThreads = 256; // 16 x 16
-
 // DP: values of a head, padded to a multiple of 32. Rows of a tile as `a` (whose sums a block owns, A of them) and as `b` (that it walks, B
-// of them): a thread has kA rows of a, from kA * ty on, and rows tx + 16 c of b.
+// of them): a thread has rows ty + kRows r of a and tx + kCols c of b. Reads of shared memory are the limit, so a thread has as many rows of
+// both as registers and the number of warps allow: 4 x 4 of 64 rows; 2 x 8 of 32 (16 x 16 threads with 2 x 4 each: 56 us against 43 at 2 x 777
+// tokens, 6 heads of 72 on 2; 2 x 8 of 64 rows: 564 us against 463 of 4 x 4 at 2 x 1500 tokens, 16 heads of 128 on 4, window 512).
 template <int DP, int A, int B>
 struct Tile {
-    static constexpr int kA = A / 16, kB = B / 16;
-    static constexpr int kPairs = DP / 32;    // pairs of values of a row that a thread has
-    static constexpr int kStride = DP + 4;    // floats of a row: 4 more shift neighbouring rows to other banks
-    static constexpr int kWeights = B + 4;    // the same for the rows of weights
+    static constexpr int kCols = A == 32 && DP <= 128 ? 8 : 16; // threads along b's rows
+    static constexpr int kA = A == 64 ? 4 : 2, kB = B / kCols;
+    static constexpr int kRows = A / kA; // threads along a's rows
+    static constexpr int kThreads = kCols * kRows;
+    static constexpr int kChunks = DP / 32, kPairs = 16 / kCols; // a thread's pairs of values of a row
+    static constexpr int kStride = DP + 4; // floats of a row: 4 more shift neighbouring rows to other banks
+    static constexpr int kWeights = B + 4; // the same for the rows of weights
     static constexpr int kFloatsA = A * kStride, kFloatsB = B * kStride;
     static constexpr int kWeightFloats = A * kWeights;
 };
 
-// Rows [from, from + ROWS) of one head as fp32, zeros for rows behind `end` and values behind dim. fp32 rows that can be read 16 bytes at a
+// Rows of one head as fp32, zeros for rows behind `end` and values behind dim: `from` and the next, those from `split` on `jump` rows
+// further down (a walk's sinks and its window). fp32 rows that can be read 16 bytes at a
 // time are copied asynchronously: the caller commits and waits, and the copies of the next step run under the products of this one.
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, int THREADS>
 __device__ __forceinline__ void LoadTile(float* dst, const AttnTensor& t, int32_t b, int32_t h, int32_t from, int32_t end, int32_t dim,
-                                         bool vec)
+                                         bool vec, int32_t split = 0, int32_t jump = 0)
 {
     constexpr int kStride = DP + 4;
     const T* base = RowOf<T>(t, b, 0, h);
+    auto rowAt = [&](int r) { return from + r < split ? from + r : from + r + jump; };
     if constexpr (sizeof(T) == 4) {
         if (vec) {
             const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
-            for (int e = threadIdx.x; e < ROWS * (DP / 4); e += kThreads) {
+            for (int e = threadIdx.x; e < ROWS * (DP / 4); e += THREADS) {
                 const int r = e / (DP / 4), d = e % (DP / 4) * 4;
-                const bool live = from + r < end && d < dim;
+                const int32_t row = rowAt(r);
+                const bool live = row < end && d < dim;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (r * kStride + d) * 4),
-                             "l"(live ? base + (from + r) * t.l + d : base), "r"(live ? 16 : 0)
+                             "l"(live ? base + row * t.l + d : base), "r"(live ? 16 : 0)
                              : "memory");
             }
             return;
@@ -49,143 +55,208 @@ __device__ __forceinline__ void LoadTile(float* dst, const AttnTensor& t, int32_
     }
     if (vec) {
 #pragma unroll 4
-        for (int e = threadIdx.x; e < ROWS * (DP / 4); e += kThreads) {
+        for (int e = threadIdx.x; e < ROWS * (DP / 4); e += THREADS) {
             const int r = e / (DP / 4), d = e % (DP / 4) * 4;
+            const int32_t row = rowAt(r);
             float v[4] = {};
-            if (from + r < end && d < dim) {
-                LoadPack<T, 4>(base + (from + r) * t.l + d, v);
+            if (row < end && d < dim) {
+                LoadPack<T, 4>(base + row * t.l + d, v);
             }
             *reinterpret_cast<float4*>(dst + r * kStride + d) = make_float4(v[0], v[1], v[2], v[3]);
         }
     } else {
-        for (int e = threadIdx.x; e < ROWS * DP; e += kThreads) {
+        for (int e = threadIdx.x; e < ROWS * DP; e += THREADS) {
             const int r = e / DP, d = e % DP;
-            dst[r * kStride + d] = from + r < end && d < dim ? DType<T>::ToF(base[(from + r) * t.l + d]) : 0.0f;
+            const int32_t row = rowAt(r);
+            dst[r * kStride + d] = row < end && d < dim ? DType<T>::ToF(base[row * t.l + d]) : 0.0f;
         }
     }
 }
 
-__device__ __forceinline__ float Dot4(const float4& a, const float4& b, float s)
+__device__ __forceinline__ void ReadQuad(const float* p, F2 (&v)[2])
 {
-    return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
+    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(p);
+    v[0].r = x.x;
+    v[1].r = x.y;
 }
 
-// s[r][c] = row (kA * ty + r) of a . row (tx + 16 c) of b
-template <typename L, int DP>
-__device__ __forceinline__ void Inner(const float* a, const float* b, float (&s)[L::kA][L::kB])
+// s[r][c] = row (ty + kRows r) of a . row (tx + kCols c) of b, over the dim values (the rows hold zeros behind them); even and odd values
+// are summed apart
+template <typename L>
+__device__ __forceinline__ void Inner(const float* a, const float* b, int32_t dim, float (&s)[L::kA][L::kB])
 {
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tx = threadIdx.x % L::kCols, ty = threadIdx.x / L::kCols;
+    F2 sum[L::kA][L::kB];
 #pragma unroll
     for (int r = 0; r < L::kA; ++r) {
 #pragma unroll
         for (int c = 0; c < L::kB; ++c) {
-            s[r][c] = 0.0f;
+            sum[r][c] = MakeF2(0.0f, 0.0f);
         }
     }
-    const float* pa = a + L::kA * ty * L::kStride;
+    const float* pa = a + ty * L::kStride;
     const float* pb = b + tx * L::kStride;
-#pragma unroll 4
-    for (int d = 0; d < DP; d += 4) {
-        float4 x[L::kA], y[L::kB];
+#pragma unroll 2
+    for (int d = 0; d < dim; d += 4) {
+        F2 x[L::kA][2], y[L::kB][2];
 #pragma unroll
         for (int r = 0; r < L::kA; ++r) {
-            x[r] = *reinterpret_cast<const float4*>(pa + r * L::kStride + d);
+            ReadQuad(pa + L::kRows * r * L::kStride + d, x[r]);
         }
 #pragma unroll
         for (int c = 0; c < L::kB; ++c) {
-            y[c] = *reinterpret_cast<const float4*>(pb + 16 * c * L::kStride + d);
+            ReadQuad(pb + L::kCols * c * L::kStride + d, y[c]);
         }
 #pragma unroll
-        for (int r = 0; r < L::kA; ++r) {
+        for (int k = 0; k < 2; ++k) {
 #pragma unroll
-            for (int c = 0; c < L::kB; ++c) {
-                s[r][c] = Dot4(x[r], y[c], s[r][c]);
+            for (int r = 0; r < L::kA; ++r) {
+#pragma unroll
+                for (int c = 0; c < L::kB; ++c) {
+                    sum[r][c] = Fma2(x[r][k], y[c][k], sum[r][c]);
+                }
             }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < L::kA; ++r) {
+#pragma unroll
+        for (int c = 0; c < L::kB; ++c) {
+            float even, odd;
+            SplitF2(sum[r][c], even, odd);
+            s[r][c] = even + odd;
         }
     }
 }
 
-// o[r] += sum over j of w[kA * ty + r][j] row j of v (B rows), values 2 tx + 32 c and the next
+// A thread's sums of a row: kPairs pairs of values from 2 kPairs tx + 32 c on.
+template <typename L>
+struct Sums {
+    F2 v[L::kA][L::kChunks][L::kPairs];
+    __device__ __forceinline__ Sums()
+    {
+#pragma unroll
+        for (int r = 0; r < L::kA; ++r) {
+#pragma unroll
+            for (int c = 0; c < L::kChunks; ++c) {
+                for (int e = 0; e < L::kPairs; ++e) {
+                    v[r][c][e] = MakeF2(0.0f, 0.0f);
+                }
+            }
+        }
+    }
+};
+
+// o[r] += sum over j of w[ty + kRows r][j] row j of v (B rows)
 template <typename L, int B>
-__device__ __forceinline__ void Outer(const float* w, const float* v, float2 (&o)[L::kA][L::kPairs])
+__device__ __forceinline__ void Outer(const float* w, const float* v, Sums<L>& o)
 {
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const float* pw = w + L::kA * ty * L::kWeights;
-    const float* pv = v + 2 * tx;
+    const int tx = threadIdx.x % L::kCols, ty = threadIdx.x / L::kCols;
+    const float* pw = w + ty * L::kWeights;
+    const float* pv = v + 2 * L::kPairs * tx;
 #pragma unroll 2
     for (int j = 0; j < B; j += 4) {
         float4 x[L::kA];
 #pragma unroll
         for (int r = 0; r < L::kA; ++r) {
-            x[r] = *reinterpret_cast<const float4*>(pw + r * L::kWeights + j);
+            x[r] = *reinterpret_cast<const float4*>(pw + L::kRows * r * L::kWeights + j);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
+            F2 z[L::kA];
 #pragma unroll
-            for (int c = 0; c < L::kPairs; ++c) {
-                const float2 y = *reinterpret_cast<const float2*>(pv + (j + k) * L::kStride + 32 * c);
+            for (int r = 0; r < L::kA; ++r) {
+                const float one = k == 0 ? x[r].x : k == 1 ? x[r].y : k == 2 ? x[r].z : x[r].w;
+                z[r] = MakeF2(one, one);
+            }
+#pragma unroll
+            for (int c = 0; c < L::kChunks; ++c) {
+                F2 y[L::kPairs];
+                const float* at = pv + (j + k) * L::kStride + 32 * c;
+                if constexpr (L::kPairs == 2) {
+                    ReadQuad(at, y);
+                } else {
+                    y[0].r = *reinterpret_cast<const unsigned long long*>(at);
+                }
 #pragma unroll
                 for (int r = 0; r < L::kA; ++r) {
-                    const float z = k == 0 ? x[r].x : k == 1 ? x[r].y : k == 2 ? x[r].z : x[r].w;
-                    o[r][c].x = fmaf(z, y.x, o[r][c].x);
-                    o[r][c].y = fmaf(z, y.y, o[r][c].y);
+#pragma unroll
+                    for (int e = 0; e < L::kPairs; ++e) {
+                        o.v[r][c][e] = Fma2(z[r], y[e], o.v[r][c][e]);
+                    }
                 }
             }
         }
     }
 }
 
-template <typename T>
-__device__ __forceinline__ bool StorePair(T* out, const float2& v, int32_t d, int32_t dim) // true: not all finite
+// A thread's sums of its row r, times a factor; true: not all finite.
+template <typename T, typename L>
+__device__ __forceinline__ bool StoreSums(T* row, const Sums<L>& o, int r, float factor, int32_t dim, bool some = true)
 {
+    const int tx = threadIdx.x % L::kCols;
     bool bad = false;
-    if (d < dim) {
-        out[d] = DType<T>::FromF(v.x);
-        bad = !(fabsf(v.x) <= 3.4e38f);
-    }
-    if (d + 1 < dim) {
-        out[d + 1] = DType<T>::FromF(v.y);
-        bad = bad || !(fabsf(v.y) <= 3.4e38f);
+#pragma unroll
+    for (int c = 0; c < L::kChunks; ++c) {
+        float v[2 * L::kPairs];
+#pragma unroll
+        for (int e = 0; e < L::kPairs; ++e) {
+            SplitF2(o.v[r][c][e], v[2 * e], v[2 * e + 1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2 * L::kPairs; ++e) {
+            const int32_t d = 2 * L::kPairs * tx + 32 * c + e;
+            if (d < dim) {
+                v[e] = some ? v[e] * factor : 0.0f; // a masked NaN times a weight of 0 is one
+                row[d] = DType<T>::FromF(v[e]);
+                bad = bad || !(fabsf(v[e]) <= 3.4e38f);
+            }
+        }
     }
     return bad;
 }
 
-__device__ __forceinline__ float RowMax16(float v) // over the 16 threads of a row
+// over the N threads of a row
+template <int N>
+__device__ __forceinline__ float RowMax(float v)
 {
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
+    for (int o = 1; o < N; o <<= 1) {
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     }
     return v;
 }
-__device__ __forceinline__ float RowSum16(float v)
+template <int N>
+__device__ __forceinline__ float RowSum(float v)
 {
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
+    for (int o = 1; o < N; o <<= 1) {
         v += __shfl_xor_sync(0xffffffffu, v, o);
     }
     return v;
 }
 
-// Steps over the keys of queries at [low, high]: the sinks in front of the window, then the window from its first key on.
+// Steps over the keys of queries at [low, high], the sinks in front of the window and then the window, without a gap: a few sinks take
+// places of the window's first step, not a step.
 template <int ROWS>
 struct Walk {
-    int32_t sinkEnd = 0, first = 0, sinkSteps = 0, steps = 0;
+    int32_t sinkEnd = 0, jump = 0, steps = 0;
     __device__ __forceinline__ Walk(const AttnShape& s, int32_t low, int32_t high)
     {
         if (high >= 0) {
             low = low > 0 ? low : 0;
-            first = low >= s.window ? low - s.window + 1 : 0;
+            const int32_t first = low >= s.window ? low - s.window + 1 : 0;
             sinkEnd = s.sinks < first ? s.sinks : first;
-            sinkSteps = (sinkEnd + ROWS - 1) / ROWS;
-            steps = sinkSteps + (high - first + ROWS) / ROWS;
+            jump = first - sinkEnd;
+            steps = (sinkEnd + (high - first) + ROWS) / ROWS;
         }
     }
-    __device__ __forceinline__ int32_t Key(int32_t n) const { return n < sinkSteps ? n * ROWS : first + (n - sinkSteps) * ROWS; }
-    // whether step n is where the query at p gets key j from (a step of sinks may reach over the window's first keys)
-    __device__ __forceinline__ bool Sees(const AttnShape& s, int32_t n, int32_t p, int32_t j) const
+    // the key at a place of the walk
+    __device__ __forceinline__ int32_t Key(int32_t at) const { return at < sinkEnd ? at : at + jump; }
+    __device__ __forceinline__ bool Sees(const AttnShape& s, int32_t p, int32_t at) const
     {
-        return j <= p && (j > p - s.window || j < s.sinks) && (n >= sinkSteps || j < sinkEnd);
+        const int32_t j = Key(at);
+        return j <= p && (j > p - s.window || j < s.sinks);
     }
 };
 
@@ -208,7 +279,7 @@ __device__ __forceinline__ int64_t PartialSlot(const TileArgs& m, int32_t unit, 
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int A, int B>
-__global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_constant__ TileArgs m)
+__global__ void __launch_bounds__(Tile<DP, A, B>::kThreads) AttnForwardTilesKernel(const __grid_constant__ TileArgs m)
 {
     using L = Tile<DP, A, B>;
     constexpr int R = L::kA, C = L::kB;
@@ -221,44 +292,43 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
     const Lengths n = LengthsOf(s, b);
     const int32_t i0 = tile * A, iLast = min(i0 + A, n.q) - 1;
     const Walk<B> walk(s, n.shift + i0, iLast >= i0 ? n.shift + iLast : -1);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tx = threadIdx.x % L::kCols, ty = threadIdx.x / L::kCols;
     if (threadIdx.x < 2) {
         again[threadIdx.x] = 0;
     }
     auto fetch = [&](float* to, const AttnTensor& x, int32_t step) {
         if (step < walk.steps) {
-            LoadTile<T, DP, B>(to, x, b, u, walk.Key(step), n.kv, s.dim, m.vec);
+            LoadTile<T, DP, B, L::kThreads>(to, x, b, u, step * B, n.kv, s.dim, m.vec, walk.sinkEnd, walk.jump);
         }
         CpAsyncCommit();
     };
-    LoadTile<T, DP, A>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
+    LoadTile<T, DP, A, L::kThreads>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
     fetch(sk, m.a.k, 0);
     fetch(sv, m.a.v, 0);
-    float2 o[R][L::kPairs] = {};
+    Sums<L> o;
     float top[R], total[R];
     int32_t p[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         top[r] = -INFINITY;
         total[r] = 0.0f;
-        const int32_t i = i0 + R * ty + r;
+        const int32_t i = i0 + ty + L::kRows * r;
         p[r] = i <= iLast ? n.shift + i : -1;
     }
     for (int32_t step = 0; step < walk.steps; ++step) {
-        const int32_t j0 = walk.Key(step);
         CpAsyncWait<1>(); // the keys; the values may still be on their way
         __syncthreads();
         float x[R][C];
-        Inner<L, DP>(sq, sk, x);
+        Inner<L>(sq, sk, s.dim, x);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float most = top[r];
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                x[r][c] = walk.Sees(s, step, p[r], j0 + tx + 16 * c) ? x[r][c] * s.scale : -INFINITY;
+                x[r][c] = walk.Sees(s, p[r], step * B + tx + L::kCols * c) ? x[r][c] * s.scale : -INFINITY;
                 most = fmaxf(most, x[r][c]);
             }
-            most = RowMax16(most);
+            most = RowMax<L::kCols>(most);
             const float base = most == -INFINITY ? 0.0f : most;
             const float fade = expf(top[r] - base);
             top[r] = most;
@@ -267,12 +337,16 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
             for (int c = 0; c < C; ++c) {
                 x[r][c] = expf(x[r][c] - base);
                 sum += x[r][c];
-                sw[(R * ty + r) * L::kWeights + tx + 16 * c] = x[r][c];
+                sw[(ty + L::kRows * r) * L::kWeights + tx + L::kCols * c] = x[r][c];
             }
             total[r] = total[r] * fade + sum;
+            const F2 fade2 = MakeF2(fade, fade);
 #pragma unroll
-            for (int c = 0; c < L::kPairs; ++c) {
-                o[r][c] = make_float2(o[r][c].x * fade, o[r][c].y * fade);
+            for (int c = 0; c < L::kChunks; ++c) {
+#pragma unroll
+                for (int e = 0; e < L::kPairs; ++e) {
+                    o.v[r][c][e] = Mul2(o.v[r][c][e], fade2);
+                }
             }
         }
         __syncthreads(); // the keys have been read, the weights written
@@ -283,31 +357,28 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
         __syncthreads();
         fetch(sv, m.a.v, step + 1);
     }
+    CpAsyncWait<0>(); // a block without a step has its first copies under way
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int32_t i = i0 + R * ty + r;
-        const float sum = RowSum16(total[r]);
+        const int32_t i = i0 + ty + L::kRows * r;
+        const float sum = RowSum<L::kCols>(total[r]);
         const bool some = p[r] >= 0;
         const float inverse = some ? 1.0f / sum : 0.0f; // a sum of 0 gives a NaN, and the row is formed again
         bool bad = false;
         if (i < s.lq) {
             T* out = OutRowOf<T>(m.a.out, b, i, h);
-#pragma unroll
-            for (int c = 0; c < L::kPairs; ++c) {
-                const float2 v = some ? make_float2(o[r][c].x * inverse, o[r][c].y * inverse) : make_float2(0.0f, 0.0f);
-                bad = StorePair<T>(out, v, 2 * tx + 32 * c, s.dim) || bad;
-            }
+            bad = StoreSums<T>(out, o, r, inverse, s.dim, some);
             if (tx == 0 && m.a.lse != nullptr) {
                 m.a.lse[static_cast<int64_t>(bh) * s.lq + i] = some ? top[r] + logf(sum) : -INFINITY;
             }
         }
         if (bad || (some && !(sum > 0.0f))) {
-            atomicOr(&again[(R * ty + r) >> 5], 1u << ((R * ty + r) & 31));
+            atomicOr(&again[(ty + L::kRows * r) >> 5], 1u << ((ty + L::kRows * r) & 31));
         }
     }
     __syncthreads();
     // rows that are not finite again, without the masked keys' part
-    for (int r = threadIdx.x >> 5; r < A; r += kThreads / 32) {
+    for (int r = threadIdx.x >> 5; r < A; r += L::kThreads / 32) {
         if ((again[r >> 5] >> (r & 31) & 1) != 0 && i0 + r < s.lq) {
             AttnForwardRow<T>(m.a, b, h, i0 + r);
         }
@@ -316,7 +387,7 @@ __global__ void __launch_bounds__(kThreads) AttnForwardTilesKernel(const __grid_
 
 // ---- backward --------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int A, int B>
-__global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_constant__ TileArgs m)
+__global__ void __launch_bounds__(Tile<DP, A, B>::kThreads) AttnGradQTilesKernel(const __grid_constant__ TileArgs m)
 {
     using L = Tile<DP, A, B>;
     constexpr int R = L::kA, C = L::kB;
@@ -329,47 +400,46 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
     const Lengths n = LengthsOf(s, b);
     const int32_t i0 = tile * A, iLast = min(i0 + A, n.q) - 1;
     const Walk<B> walk(s, n.shift + i0, iLast >= i0 ? n.shift + iLast : -1);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tx = threadIdx.x % L::kCols, ty = threadIdx.x / L::kCols;
     if (threadIdx.x < 2) {
         again[threadIdx.x] = 0;
     }
-    LoadTile<T, DP, A>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
-    LoadTile<T, DP, A>(sg, m.a.gradOut, b, h, i0, iLast + 1, s.dim, m.vec);
+    LoadTile<T, DP, A, L::kThreads>(sq, m.a.q, b, h, i0, iLast + 1, s.dim, m.vec);
+    LoadTile<T, DP, A, L::kThreads>(sg, m.a.gradOut, b, h, i0, iLast + 1, s.dim, m.vec);
     auto fetch = [&](float* to, const AttnTensor& x, int32_t step) {
         if (step < walk.steps) {
-            LoadTile<T, DP, B>(to, x, b, u, walk.Key(step), n.kv, s.dim, m.vec);
+            LoadTile<T, DP, B, L::kThreads>(to, x, b, u, step * B, n.kv, s.dim, m.vec, walk.sinkEnd, walk.jump);
         }
         CpAsyncCommit();
     };
     fetch(sv, m.a.v, 0);
     fetch(sk, m.a.k, 0);
-    float2 o[R][L::kPairs] = {};
+    Sums<L> o;
     float lse[R], delta[R];
     int32_t p[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int32_t i = i0 + R * ty + r;
+        const int32_t i = i0 + ty + L::kRows * r;
         p[r] = i <= iLast ? n.shift + i : -1;
         lse[r] = p[r] >= 0 ? m.a.lse[static_cast<int64_t>(bh) * s.lq + i] : 0.0f;
         delta[r] = p[r] >= 0 ? m.a.delta[static_cast<int64_t>(bh) * m.a.deltaStride + i] : 0.0f;
     }
     for (int32_t step = 0; step < walk.steps; ++step) {
-        const int32_t j0 = walk.Key(step);
         CpAsyncWait<1>();
         __syncthreads();
         float x[R][C], y[R][C];
-        Inner<L, DP>(sg, sv, y);
+        Inner<L>(sg, sv, s.dim, y);
         __syncthreads();
         fetch(sv, m.a.v, step + 1); // under the products with the keys
         CpAsyncWait<1>();
         __syncthreads();
-        Inner<L, DP>(sq, sk, x);
+        Inner<L>(sq, sk, s.dim, x);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const bool live = walk.Sees(s, step, p[r], j0 + tx + 16 * c);
-                sw[(R * ty + r) * L::kWeights + tx + 16 * c] =
+                const bool live = walk.Sees(s, p[r], step * B + tx + L::kCols * c);
+                sw[(ty + L::kRows * r) * L::kWeights + tx + L::kCols * c] =
                     live ? expf(x[r][c] * s.scale - lse[r]) * (y[r][c] - delta[r]) * s.scale : 0.0f;
             }
         }
@@ -378,24 +448,21 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
         __syncthreads();
         fetch(sk, m.a.k, step + 1); // under the next products with the values
     }
+    CpAsyncWait<0>();
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int32_t i = i0 + R * ty + r;
+        const int32_t i = i0 + ty + L::kRows * r;
         bool bad = false;
         if (i < s.lq) {
             T* out = OutRowOf<T>(m.a.gradQ, b, i, h);
-#pragma unroll
-            for (int c = 0; c < L::kPairs; ++c) {
-                const float2 v = p[r] >= 0 ? o[r][c] : make_float2(0.0f, 0.0f);
-                bad = StorePair<T>(out, v, 2 * tx + 32 * c, s.dim) || bad;
-            }
+            bad = StoreSums<T>(out, o, r, 1.0f, s.dim, p[r] >= 0);
         }
         if (bad) {
-            atomicOr(&again[(R * ty + r) >> 5], 1u << ((R * ty + r) & 31));
+            atomicOr(&again[(ty + L::kRows * r) >> 5], 1u << ((ty + L::kRows * r) & 31));
         }
     }
     __syncthreads();
-    for (int r = threadIdx.x >> 5; r < A; r += kThreads / 32) {
+    for (int r = threadIdx.x >> 5; r < A; r += L::kThreads / 32) {
         if ((again[r >> 5] >> (r & 31) & 1) != 0 && i0 + r < s.lq) {
             AttnGradQRow<T>(m.a, b, h, i0 + r);
         }
@@ -407,7 +474,7 @@ __global__ void __launch_bounds__(kThreads) AttnGradQTilesKernel(const __grid_co
 // of their tile. In both cases the blocks' sums go to `partial` in fp32 ([batch, heads or key heads, 1 + chunks of a tile with sinks,
 // gradK and gradV, rows of the tile, dim]), and AttnGradKvSumKernel adds them up in order.
 template <typename T, int DP, int A, int B>
-__global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_constant__ TileArgs m)
+__global__ void __launch_bounds__(Tile<DP, A, B>::kThreads) AttnGradKvTilesKernel(const __grid_constant__ TileArgs m)
 {
     using L = Tile<DP, A, B>;
     constexpr int R = L::kA, C = L::kB;
@@ -438,18 +505,18 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
         low += chunk * share * B;
     }
     const int32_t stop = high; // queries behind it are another block's
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tx = threadIdx.x % L::kCols, ty = threadIdx.x / L::kCols;
     if (threadIdx.x < 2) {
         again[threadIdx.x] = 0;
     }
-    LoadTile<T, DP, A>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
-    LoadTile<T, DP, A>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
-    float2 ok[R][L::kPairs] = {}, ov[R][L::kPairs] = {};
+    LoadTile<T, DP, A, L::kThreads>(sk, m.a.k, b, u, j0, n.kv, s.dim, m.vec);
+    LoadTile<T, DP, A, L::kThreads>(sv, m.a.v, b, u, j0, n.kv, s.dim, m.vec);
+    Sums<L> ok, ov;
     // steps over the heads and their queries
     const int32_t perHead = high >= low ? (high - low + B) / B : 0, steps = perHead * (hEnd - hFirst);
     auto fetch = [&](float* to, const AttnTensor& x, int32_t step) {
         if (step < steps) {
-            LoadTile<T, DP, B>(to, x, b, hFirst + step / perHead, low + step % perHead * B - n.shift, n.q, s.dim, m.vec);
+            LoadTile<T, DP, B, L::kThreads>(to, x, b, hFirst + step / perHead, low + step % perHead * B - n.shift, n.q, s.dim, m.vec);
         }
         CpAsyncCommit();
     };
@@ -466,20 +533,20 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
         CpAsyncWait<1>();
         __syncthreads();
         float x[R][C], y[R][C];
-        Inner<L, DP>(sv, sg, y);
+        Inner<L>(sv, sg, s.dim, y);
         CpAsyncWait<0>();
         __syncthreads();
-        Inner<L, DP>(sk, sq, x);
+        Inner<L>(sk, sq, s.dim, x);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int32_t j = j0 + R * ty + r;
+            const int32_t j = j0 + ty + L::kRows * r;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const int32_t e = tx + 16 * c, p = p0 + e;
+                const int32_t e = tx + L::kCols * c, p = p0 + e;
                 const bool live = j < n.kv && p <= stop && j <= p && (j > p - s.window || j < s.sinks);
                 const float w = live ? expf(x[r][c] * s.scale - sLse[e]) : 0.0f;
-                sw[(R * ty + r) * L::kWeights + e] = w;
-                sd[(R * ty + r) * L::kWeights + e] = live ? w * (y[r][c] - sDelta[e]) * s.scale : 0.0f;
+                sw[(ty + L::kRows * r) * L::kWeights + e] = w;
+                sd[(ty + L::kRows * r) * L::kWeights + e] = live ? w * (y[r][c] - sDelta[e]) * s.scale : 0.0f;
             }
         }
         __syncthreads();
@@ -490,37 +557,32 @@ __global__ void __launch_bounds__(kThreads) AttnGradKvTilesKernel(const __grid_c
         __syncthreads();
         fetch(sq, m.a.q, step + 1); // under the next products with the values
     }
+    CpAsyncWait<0>();
     if (m.partial != nullptr) {
         float* part = m.partial + PartialSlot(m, unit, tile, 1 + chunk, A);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-#pragma unroll
-            for (int c = 0; c < L::kPairs; ++c) {
-                const int32_t at = (R * ty + r) * s.dim, d = 2 * tx + 32 * c;
-                StorePair<float>(part + at, ok[r][c], d, s.dim);
-                StorePair<float>(part + A * s.dim + at, ov[r][c], d, s.dim);
-            }
+            const int32_t at = (ty + L::kRows * r) * s.dim;
+            StoreSums<float>(part + at, ok, r, 1.0f, s.dim);
+            StoreSums<float>(part + A * s.dim + at, ov, r, 1.0f, s.dim);
         }
         return;
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int32_t j = j0 + R * ty + r;
+        const int32_t j = j0 + ty + L::kRows * r;
         bool bad = false;
         if (j < s.lk) {
             T *gk = OutRowOf<T>(m.a.gradK, b, j, u), *gv = OutRowOf<T>(m.a.gradV, b, j, u);
-#pragma unroll
-            for (int c = 0; c < L::kPairs; ++c) {
-                bad = StorePair<T>(gk, ok[r][c], 2 * tx + 32 * c, s.dim) || bad;
-                bad = StorePair<T>(gv, ov[r][c], 2 * tx + 32 * c, s.dim) || bad;
-            }
+            bad = StoreSums<T>(gk, ok, r, 1.0f, s.dim);
+            bad = StoreSums<T>(gv, ov, r, 1.0f, s.dim) || bad;
         }
         if (bad) {
-            atomicOr(&again[(R * ty + r) >> 5], 1u << ((R * ty + r) & 31));
+            atomicOr(&again[(ty + L::kRows * r) >> 5], 1u << ((ty + L::kRows * r) & 31));
         }
     }
     __syncthreads();
-    for (int r = threadIdx.x >> 5; r < A; r += kThreads / 32) {
+    for (int r = threadIdx.x >> 5; r < A; r += L::kThreads / 32) {
         if ((again[r >> 5] >> (r & 31) & 1) != 0 && j0 + r < s.lk) {
             AttnGradKvRow<T>(m.a, b, u, j0 + r);
         }
@@ -592,7 +654,7 @@ cudaError_t Forward(Dt dt, const AttnArgs& a, cudaStream_t stream)
     if (e != cudaSuccess) {
         return e;
     }
-    AttnForwardTilesKernel<T, DP, A, B><<<static_cast<unsigned>(blocks), kThreads, shared, stream>>>(m);
+    AttnForwardTilesKernel<T, DP, A, B><<<static_cast<unsigned>(blocks), L::kThreads, shared, stream>>>(m);
     CountLaunch();
     return cudaGetLastError();
 }
@@ -642,7 +704,7 @@ cudaError_t GradQ(const TileArgs& args, cudaStream_t stream)
     if (e != cudaSuccess || blocks == 0) {
         return e;
     }
-    AttnGradQTilesKernel<T, DP, A, B><<<static_cast<unsigned>(blocks), kThreads, shared, stream>>>(m);
+    AttnGradQTilesKernel<T, DP, A, B><<<static_cast<unsigned>(blocks), L::kThreads, shared, stream>>>(m);
     CountLaunch();
     return cudaGetLastError();
 }
@@ -669,7 +731,7 @@ cudaError_t GradKv(const TileArgs& args, const KvPlan& plan, float* partial, cud
     m.chunks = plan.chunks;
     m.partial = plan.Partial() ? partial : nullptr;
     if (blocks > 0) {
-        AttnGradKvTilesKernel<T, DP, A, B><<<static_cast<unsigned>(blocks), kThreads, shared, stream>>>(m);
+        AttnGradKvTilesKernel<T, DP, A, B><<<static_cast<unsigned>(blocks), L::kThreads, shared, stream>>>(m);
         CountLaunch();
     }
     if (m.partial != nullptr) {
