@@ -273,4 +273,16 @@ uint64_t AttnBackwardMmaWorkspace(const AttnShape& s);
 cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStream_t stream);
 constexpr int kMmaMostDim = 128;
 
+// Blocks that share out the far queries of a tile with sinks, of the `wanted` that bring their walks down to an ordinary one's; 0: the
+// tile's own block walks them. Each costs memory for its sums, so where sinks fill tiles enough for the SMs, there are fewer or none.
+inline int32_t AttnFarChunks(int64_t units, int32_t sinkTiles, int64_t wanted)
+{
+    int64_t most = 64;
+    if (sinkTiles >= 4) {
+        const int64_t enough = 8 * kNumSMsFallback / (units * sinkTiles > 0 ? units * sinkTiles : 1);
+        most = enough < most ? enough : most;
+    }
+    return static_cast<int32_t>(wanted < most ? wanted : most);
+}
+
 } // namespace opscv

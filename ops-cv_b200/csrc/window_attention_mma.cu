@@ -1390,7 +1390,8 @@ FarPlan PlanFar(const AttnShape& s)
     if (sinks > 0 && 2 * far > near) {
         f.sinkTiles = static_cast<int32_t>(CeilDiv(sinks, kTile));
         const int64_t chunks = CeilDiv(far, near);
-        f.chunks = static_cast<int32_t>(chunks < 64 ? chunks : 64);
+        f.chunks = AttnFarChunks(static_cast<int64_t>(s.batch) * s.kvHeads, f.sinkTiles, chunks);
+        f.sinkTiles = f.chunks > 0 ? f.sinkTiles : 0;
     }
     return f;
 }
@@ -1482,7 +1483,7 @@ cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStrea
     const int bytes = halves * static_cast<int>(kHalfBytes);
     const int shared = std::max(7 * bytes, 6 * bytes + 4 * kTile * 4) + 1024; // gradQ's tiles, gradK's and gradV's with two places of statistics
     const int64_t blocks = kvBlocks + static_cast<int64_t>(s.batch) * s.heads * m.qTiles;
-    if (blocks > INT32_MAX) {
+    if (blocks > INT32_MAX || static_cast<int64_t>(s.batch) * s.kvHeads * m.sinkTiles * (kTile / 4) > INT32_MAX) {
         return cudaErrorInvalidConfiguration;
     }
     m.kvBlocks = static_cast<uint32_t>(kvBlocks);

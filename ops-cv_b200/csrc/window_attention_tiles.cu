@@ -5,6 +5,8 @@
 // in each thread's registers takes 64 for 8 reads of 16 bytes from shared memory. Tensor cores would need three products of tf32 parts for
 // each of fp32 and still lose bits that fp32 callers have. Blocks own their sums (gradQ in one kernel, gradK and gradV in another), so
 // nothing is added up in memory and the order of all sums is fixed.
+#include <algorithm>
+
 #include "cp_async.cuh"
 #include "window_attention.cuh"
 
@@ -267,12 +269,14 @@ struct TileArgs {
     // gradK and gradV, see there
     bool perHead;
     int32_t sinkTiles, chunks;
-    float* partial; // null: blocks write the results
+    float* partial;
 };
+// Tiles whose blocks leave sums: all with a block a query head, otherwise those with sinks.
+__host__ __device__ __forceinline__ int32_t PartialTiles(bool perHead, int32_t tiles, int32_t sinkTiles) { return perHead ? tiles : sinkTiles; }
 // Where a block's sums start: the tiles of a unit (a head or key head), each with its chunks behind it where it has sinks.
 __device__ __forceinline__ int64_t PartialSlot(const TileArgs& m, int32_t unit, int32_t tile, int32_t slot, int32_t rows)
 {
-    const int64_t perUnit = m.tiles + static_cast<int64_t>(m.sinkTiles) * m.chunks;
+    const int64_t perUnit = PartialTiles(m.perHead, m.tiles, m.sinkTiles) + static_cast<int64_t>(m.sinkTiles) * m.chunks;
     const int64_t at = tile + static_cast<int64_t>(min(tile, m.sinkTiles)) * m.chunks + slot;
     return (unit * perUnit + at) * 2 * rows * m.a.s.dim;
 }
@@ -471,7 +475,7 @@ __global__ void __launch_bounds__(Tile<DP, A, B>::kThreads) AttnGradQTilesKernel
 
 // A block has a tile of keys and the query heads of its key head. Where those blocks are too few for the SMs (`perHead`), a block has one
 // query head instead; and where sinks are seen by many more queries than a window's, these are shared out among `chunks` further blocks
-// of their tile. In both cases the blocks' sums go to `partial` in fp32 ([batch, heads or key heads, 1 + chunks of a tile with sinks,
+// of their tile. The sums of such blocks go to `partial` in fp32 ([batch, heads or key heads, tiles, 1 + chunks of one with sinks,
 // gradK and gradV, rows of the tile, dim]), and AttnGradKvSumKernel adds them up in order.
 template <typename T, int DP, int A, int B>
 __global__ void __launch_bounds__(Tile<DP, A, B>::kThreads) AttnGradKvTilesKernel(const __grid_constant__ TileArgs m)
@@ -558,7 +562,7 @@ __global__ void __launch_bounds__(Tile<DP, A, B>::kThreads) AttnGradKvTilesKerne
         fetch(sq, m.a.q, step + 1); // under the next products with the values
     }
     CpAsyncWait<0>();
-    if (m.partial != nullptr) {
+    if (tile < PartialTiles(m.perHead, m.tiles, m.sinkTiles)) {
         float* part = m.partial + PartialSlot(m, unit, tile, 1 + chunk, A);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -589,17 +593,18 @@ __global__ void __launch_bounds__(Tile<DP, A, B>::kThreads) AttnGradKvTilesKerne
     }
 }
 
-// A warp per key.
+// A warp per key of the tiles with sums.
 template <typename T>
 __global__ void __launch_bounds__(128) AttnGradKvSumKernel(const __grid_constant__ TileArgs m, int32_t rows)
 {
     const AttnShape& s = m.a.s;
     const int lane = threadIdx.x & 31;
     const int64_t key = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5); // (batch, key head, key)
-    if (key >= static_cast<int64_t>(s.batch) * s.kvHeads * s.lk) {
+    const int32_t perUnit = m.perHead ? s.lk : min(s.lk, m.sinkTiles * rows);
+    if (key >= static_cast<int64_t>(s.batch) * s.kvHeads * perUnit) {
         return;
     }
-    const int32_t j = static_cast<int32_t>(key % s.lk), bu = static_cast<int32_t>(key / s.lk), b = bu / s.kvHeads, u = bu % s.kvHeads;
+    const int32_t j = static_cast<int32_t>(key % perUnit), bu = static_cast<int32_t>(key / perUnit), b = bu / s.kvHeads, u = bu % s.kvHeads;
     const int32_t tile = j / rows, slots = tile < m.sinkTiles ? 1 + m.chunks : 1;
     const int32_t first = m.perHead ? b * s.heads + u * m.a.group : bu, units = m.perHead ? m.a.group : 1;
     bool bad = false;
@@ -665,7 +670,7 @@ struct KvPlan {
     bool perHead = false;
     int64_t units = 0;
     int64_t Blocks() const { return units * (tiles + static_cast<int64_t>(sinkTiles) * chunks); }
-    bool Partial() const { return perHead || chunks > 0; }
+    int64_t Partials() const { return units * (PartialTiles(perHead, tiles, sinkTiles) + static_cast<int64_t>(sinkTiles) * chunks); }
 };
 KvPlan PlanKv(const AttnShape& s)
 {
@@ -681,7 +686,8 @@ KvPlan PlanKv(const AttnShape& s)
     if (sinks > 0 && s.heads > 0 && 2 * far > near) {
         p.sinkTiles = static_cast<int32_t>(CeilDiv(sinks, p.rows));
         const int64_t chunks = CeilDiv(far, near > 1 ? near : 1);
-        p.chunks = static_cast<int32_t>(chunks < 64 ? chunks : 64);
+        p.chunks = AttnFarChunks(p.units, p.sinkTiles, chunks);
+        p.sinkTiles = p.chunks > 0 ? p.sinkTiles : 0;
     }
     return p;
 }
@@ -717,24 +723,26 @@ cudaError_t GradKv(const TileArgs& args, const KvPlan& plan, float* partial, cud
     const AttnShape& s = m.a.s;
     constexpr int shared = (2 * L::kFloatsA + 2 * L::kFloatsB + 2 * L::kWeightFloats) * 4;
     static std::atomic<uint64_t> asked;
-    const int64_t blocks = plan.Blocks(), keys = static_cast<int64_t>(s.batch) * s.kvHeads * s.lk;
+    const int64_t blocks = plan.Blocks();
+    const int64_t summed = plan.perHead ? s.lk : std::min<int64_t>(s.lk, static_cast<int64_t>(plan.sinkTiles) * A);
+    const int64_t keys = static_cast<int64_t>(s.batch) * s.kvHeads * summed; // whose gradients are put together from blocks' sums
     if (blocks > INT32_MAX || CeilDiv(keys, 4) > INT32_MAX) {
         return cudaErrorInvalidConfiguration;
     }
     cudaError_t e = AskOnce(AttnGradKvTilesKernel<T, DP, A, B>, asked, shared);
-    if (e != cudaSuccess || keys == 0) {
+    if (e != cudaSuccess) {
         return e;
     }
     m.tiles = plan.tiles;
     m.perHead = plan.perHead;
     m.sinkTiles = plan.sinkTiles;
     m.chunks = plan.chunks;
-    m.partial = plan.Partial() ? partial : nullptr;
+    m.partial = partial;
     if (blocks > 0) {
         AttnGradKvTilesKernel<T, DP, A, B><<<static_cast<unsigned>(blocks), L::kThreads, shared, stream>>>(m);
         CountLaunch();
     }
-    if (m.partial != nullptr) {
+    if (keys > 0) {
         AttnGradKvSumKernel<T><<<static_cast<unsigned>(CeilDiv(keys, 4)), 128, 0, stream>>>(m, A);
         CountLaunch();
     }
@@ -791,7 +799,7 @@ cudaError_t AttnForwardTiles(Dt dt, const AttnArgs& a, cudaStream_t stream)
 uint64_t AttnBackwardTilesWorkspace(const AttnShape& s)
 {
     const KvPlan p = PlanKv(s);
-    return DeltaBytes(s) + (p.Partial() ? static_cast<uint64_t>(p.Blocks()) * 2 * p.rows * s.dim * 4 : 0);
+    return DeltaBytes(s) + static_cast<uint64_t>(p.Partials()) * 2 * p.rows * s.dim * 4;
 }
 
 cudaError_t AttnBackwardTiles(Dt dt, const AttnArgs& a, void* workspace, cudaStream_t stream)

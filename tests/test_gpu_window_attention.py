@@ -247,6 +247,23 @@ def test_scales(ops, dev, t, scale, lq):
     check(ops, q, k, v, 70, 2, scale, g=g)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d", [40, 128, 136])
+@pytest.mark.parametrize("sinks,window", [(1, 5), (31, 33), (63, 64), (64, 65), (65, 1), (130, 100), (300, 7)])
+def test_sinks_at_the_ends_of_steps(ops, dev, t, d, sinks, window):
+    q, g = normal((1, 190, 4, d), t, 111, dev), normal((1, 190, 4, d), t, 114, dev)
+    k, v = normal((1, 333, 2, d), t, 112, dev), normal((1, 333, 2, d), t, 113, dev)
+    check(ops, q, k, v, window, sinks, g=g)
+
+
+@pytest.mark.parametrize("t,d", [(F32, 64), (BF16, 64), (F16, 40)])
+@pytest.mark.parametrize("b,hk,lq,sinks", [(32, 4, 700, 700), (24, 4, 1300, 600), (2, 2, 1500, 10 ** 9)])
+def test_sinks_of_many_tiles(ops, dev, t, d, b, hk, lq, sinks):
+    q, g = normal((b, lq, hk, d), t, 121, dev), normal((b, lq, hk, d), t, 124, dev)
+    k, v = normal((b, lq, hk, d), t, 122, dev), normal((b, lq, hk, d), t, 123, dev)
+    check(ops, q, k, v, 40, sinks, g=g)
+
+
 @pytest.mark.parametrize("lq", [1, 140])
 def test_fp16_gradients_of_any_size(ops, dev, lq):
     """Gradients a million times smaller or a thousand times larger (and values of 1000) keep their precision in fp16."""

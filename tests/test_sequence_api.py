@@ -216,6 +216,25 @@ def test_tensors_without_data(ops):
     assert got == NULLPTR
 
 
+@pytest.mark.parametrize("code", ["ACL_BF16", "ACL_FLOAT"])
+@pytest.mark.parametrize("sinks", [0, 4, 1000, 2 ** 20, 2 ** 40])
+def test_workspace_of_many_sinks(ops, code, sinks):
+    """However many sinks there are, the sums of the blocks that share their queries stay small (the tensors take 4 GiB and more)."""
+    L = ops.lib()
+
+    def tensor(*shape, dtype):
+        dims = (ctypes.c_int64 * len(shape))(*shape)
+        return ctypes.c_void_p(L.aclCreateTensor(dims, len(shape), dtype, None, 0, ops.ACL_FORMAT_ND, dims, len(shape), ctypes.c_void_p(4096)))
+
+    dtype, tokens, heads, kv, d = getattr(ops, code), 2 ** 20, 16, 4, 128
+    q, k = tensor(1, tokens, heads, d, dtype=dtype), tensor(1, tokens, kv, d, dtype=dtype)
+    lse = tensor(1, heads, tokens, dtype=ops.ACL_FLOAT)
+    n, e = ctypes.c_uint64(0), ctypes.c_void_p(None)
+    got = L.aclnnWindowAttentionBackwardGetWorkspaceSize(q, q, k, k, q, lse, None, None, 64, sinks, 0.1, q, k, k, ctypes.byref(n), ctypes.byref(e))
+    assert got == 0 and n.value < 2 ** 30
+    L.aclDestroyAclOpExecutor(e)
+
+
 def test_tensors_of_two_devices(ops):
     x = torch.zeros(2, 8)
     with pytest.raises(ValueError, match="one device"):
