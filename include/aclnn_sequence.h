@@ -52,7 +52,8 @@ ACLNN_API aclnnStatus aclnnResidualRmsNormBackward(void* workspace, uint64_t wor
 /* The same norm with y in 8 bits: each row (group = 0) or each `group` columns of a row (a multiple of 32; the last group may be
  * shorter) are divided by a scale of their own, max|y| / 448 for out of type ACL_FLOAT8_E4M3FN and max|y| / 127 for ACL_INT8, and
  * rounded to nearest even; y is about out * scale. The division is of the fp32 values, before any rounding of y. A group of zeros
- * (or of magnitudes below 1e-35) has scale 0 and zeros; one that holds a NaN or an infinity has a NaN or infinity as its scale, and its values say nothing.
+ * (or of magnitudes below 1e-35) has scale 0 and zeros; one that holds a NaN or an infinity has a NaN or infinity as its scale,
+ * and its values say nothing.
  * out: x's shape, contiguous. scales: [..., groups], ACL_FLOAT, contiguous. sum: as above, may be null. */
 ACLNN_API aclnnStatus aclnnResidualRmsNormQuantGetWorkspaceSize(const aclTensor* x, const aclTensor* residual,
                                                                 const aclTensor* weight, double eps, int64_t group,

@@ -6,6 +6,8 @@
 //
 // Bound by HBM: the forward moves two rows in and two out, the backward three in and one out. A row stays in registers between
 // the reduction and the output (each thread owns the same columns in every pass over the row), so each value moves once.
+// 8192 x 4096 bf16: forward 46 us (5.85 TB/s), backward 48 us and 5 more for the weight's sums (5.0 TB/s over both); to e4m3 in groups of
+// 128, 8192 x 5120: 63 us (4.65 TB/s), where the scaling of each value fills 59 % of the issue slots. 16 rows of 4096: 2.6 us.
 #include <cuda_fp8.h>
 
 #include "cp_async.cuh"
@@ -823,9 +825,9 @@ int VecOfRows(int elem, const NormShape& n, std::initializer_list<RowUse> uses)
 }
 
 // Threads of a row and chunks of V values per thread. Where rows are many, 256 threads with more chunks each: what a thread spends once a
-// row is shared by more values (8192 x 4096 bf16 forward: 46 us against 49 with 512). Rows of up to 4 chunks a lane take one warp each, 4 rows a block; wider
-// ones a block of their own with as few chunks per thread as 512 threads allow, and up to 1024 threads with the most chunks that
-// `values` a thread allow. nv 0: too wide for that.
+// row is shared by more values (8192 x 4096 bf16 forward: 46 us against 49 with 512). Rows of up to 4 chunks a lane take one warp each, 4
+// rows a block; wider ones a block of their own with as few chunks per thread as 512 threads allow, and up to 1024 threads with the most
+// chunks that `values` a thread allow. nv 0: too wide for that.
 struct RowShape {
     int nv, threads, rows;
 };
