@@ -64,7 +64,7 @@ cudaError_t WindowAttentionFwd(Dt dt, const AttnShape& s, AttnTensor q, AttnTens
     a.out = out;
     a.lse = lse;
     a.group = s.heads / s.kvHeads;
-    if (s.lq <= kStepMostQueries && s.lk > 0) {
+    if (AttnStepTakes(dt, a)) {
         return AttnStep(dt, a, stream);
     }
     if (MmaTakes(dt, a)) {

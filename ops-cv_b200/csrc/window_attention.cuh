@@ -251,7 +251,7 @@ __device__ __noinline__ void AttnGradKvRow(const AttnArgs& a, int32_t b, int32_t
 }
 
 // ---- few queries (window_attention_step.cu) ----------------------------------------------------------------------------------
-constexpr int kStepMostQueries = 8;
+bool AttnStepTakes(Dt dt, const AttnArgs& a);
 cudaError_t AttnStep(Dt dt, const AttnArgs& a, cudaStream_t stream);
 uint32_t AttnStepTimeouts();
 

@@ -1,4 +1,4 @@
-// Attention of few queries (a decoding step) over long keys.
+// Attention of few queries (a decoding step, a short chunk or draft) over long keys.
 //
 // Bound by reading the visible keys and values once: with one query a sequence there are only heads / kvHeads rows to share a key, too
 // few for the 128 of tcgen05. A block has rows of one key head and a share of the keys, and each warp keeps a softmax of its own keys
@@ -656,23 +656,61 @@ cudaError_t LaunchFor(const StepArgs& m, int r, int n, bool vec, int64_t units, 
 
 } // namespace
 
+namespace {
+
+// Rows a block, and which kernel: `products` of a warp, or fp32 arithmetic with n chunks a lane.
+struct StepPlan {
+    bool vec, products;
+    int n, r;
+    int64_t rowGroups;
+};
+StepPlan PlanStep(Dt dt, const AttnArgs& a)
+{
+    const AttnShape& s = a.s;
+    StepPlan p;
+    const int64_t rows = static_cast<int64_t>(s.lq) * a.group;
+    const int v = dt == Dt::F32 ? 4 : 8;
+    const int n = static_cast<int>(CeilDiv(s.dim, 8 * v)); // chunks a lane
+    p.n = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
+    const int values = p.n * v; // a lane, of q and of the sums, for each row
+    auto rowsApart = [&](const AttnTensor& x) { return Aligned(x.p, 16) && x.b % v == 0 && x.l % v == 0 && x.h % v == 0; };
+    p.vec = s.dim % v == 0 && rowsApart(a.q) && rowsApart(a.k) && rowsApart(a.v);
+    p.products = dt != Dt::F32 && s.dim % 2 == 0 && s.dim <= kMmaMostDim && rowsApart(a.q) &&
+                 AttnTmaReadable(a.k, s.lk, s.kvHeads, s.batch) && AttnTmaReadable(a.v, s.lk, s.kvHeads, s.batch);
+    const int most = p.products ? kMostRows : values > 16 ? 2 : 4;
+    p.r = rows >= most ? most : static_cast<int>(p.products || rows < 3 ? rows : 4);
+    p.rowGroups = CeilDiv(rows, p.r > 0 ? p.r : 1);
+    return p;
+}
+
+} // namespace
+
+// Up to 8 queries always. More where the blocks of the other kernels, which walk all keys of 32 to 128 queries, leave most of the SMs
+// idle: as long as there are few groups of rows (each reads the keys again) and keys enough to share out. bf16, heads of 128, 32 on 8, one
+// sequence of 32768 keys: 16 queries (32 groups) 94 us against 517, 64 (128 groups) 326 against 515, 128 (256 groups) 633 against 516;
+// 8 sequences of 8192: 9 queries (192 groups) 172 against 152. fp32, 16 heads of 64, 4096 keys: 64 queries (256 groups) 136 us against 274,
+// 128 queries (512 groups) 275 against 274; wider heads, whose tiles are slower: 32 of 128 on 8, 32768 keys, 64 queries (512 groups) 2768
+// us against 3712; bf16, 8 heads of 256, 8192 keys, 128 queries (512 groups) 578 us against 2128.
+bool AttnStepTakes(Dt dt, const AttnArgs& a)
+{
+    const AttnShape& s = a.s;
+    if (s.lk == 0 || s.lq <= 8) {
+        return s.lk > 0;
+    }
+    const int64_t keys = std::min<int64_t>(s.lk, static_cast<int64_t>(s.window) + s.sinks + s.lq);
+    const StepPlan p = PlanStep(dt, a);
+    return keys >= 1024 && p.rowGroups * s.batch * s.kvHeads <= (p.products ? 128 : s.dim > 64 ? 512 : 256);
+}
+
 cudaError_t AttnStep(Dt dt, const AttnArgs& a, cudaStream_t stream)
 {
     const AttnShape& s = a.s;
     StepArgs m{};
     m.a = a;
-    const int32_t rows = s.lq * a.group;
-    const int v = dt == Dt::F32 ? 4 : 8;
-    int n = static_cast<int>(CeilDiv(s.dim, 8 * v)); // chunks a lane
-    n = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
-    const int values = n * v; // a lane, of q and of the sums, for each row
-    auto rowsApart = [&](const AttnTensor& x) { return Aligned(x.p, 16) && x.b % v == 0 && x.l % v == 0 && x.h % v == 0; };
-    const bool vec = s.dim % v == 0 && rowsApart(a.q) && rowsApart(a.k) && rowsApart(a.v);
-    const bool products = dt != Dt::F32 && s.dim % 2 == 0 && s.dim <= kMmaMostDim && rowsApart(a.q) &&
-                          AttnTmaReadable(a.k, s.lk, s.kvHeads, s.batch) && AttnTmaReadable(a.v, s.lk, s.kvHeads, s.batch);
-    const int most = products ? kMostRows : values > 16 ? 2 : 4;
-    const int r = rows >= most ? most : (products || rows < 3 ? rows : 4);
-    m.rowGroups = static_cast<int32_t>(CeilDiv(rows, r));
+    const StepPlan plan = PlanStep(dt, a);
+    const bool vec = plan.vec, products = plan.products;
+    const int n = plan.n, r = plan.r;
+    m.rowGroups = static_cast<int32_t>(plan.rowGroups);
     const int64_t units = static_cast<int64_t>(s.batch) * s.kvHeads * m.rowGroups;
     // Blocks of a cluster share out the keys of a unit, up to about two blocks an SM (a block's start and end cost as much as some
     // hundred keys, so more are slower: 32 sequences of window 1024 with 8 key heads take 31 us as 256 blocks, 44 as 512 or 1024; 8 of

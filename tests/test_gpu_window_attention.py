@@ -256,6 +256,25 @@ def test_sinks_at_the_ends_of_steps(ops, dev, t, d, sinks, window):
     check(ops, q, k, v, window, sinks, g=g)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("lq,lk,h,hk,d,window,sinks", [
+    (9, 1024, 4, 2, 64, 10 ** 6, 0), (17, 1500, 8, 1, 128, 2000, 3), (33, 3001, 6, 2, 80, 1100, 40), (100, 1111, 3, 3, 40, 990, 130),
+    (150, 2500, 2, 1, 128, 1000, 0), (300, 2000, 2, 1, 96, 1500, 1700), (16, 1300, 4, 1, 200, 1290, 5), (70, 1800, 2, 2, 256, 5000, 0)])
+def test_some_queries_over_many_keys(ops, dev, t, lq, lk, h, hk, d, window, sinks):
+    b = 3
+    q, g = normal((b, lq, h, d), t, 131, dev), normal((b, lq, h, d), t, 134, dev)
+    k, v = normal((b, lk, hk, d), t, 132, dev), normal((b, lk, hk, d), t, 133, dev)
+    check(ops, q, k, v, window, sinks, g=g)
+    qn, kn = torch.tensor([lq, lq // 2, lq], device=dev), torch.tensor([lk, lk - 7, lq - 3], device=dev)
+    check(ops, q, k, v, window, sinks, qn=qn, kn=kn, g=g)
+    wide = torch.full((b, lk + 50, hk, d), math.nan, dtype=t, device=dev)  # keys behind the sequences hold anything
+    wide_v = wide.clone()
+    wide[:, :lk], wide_v[:, :lk] = k, v
+    got = ops.window_attention(q, wide, wide_v, window, sinks, kv_lengths=torch.full((b,), lk, device=dev))[0]
+    ref = Reference(q, k, v, window, sinks)
+    close("out", got, ref.out, ref.out_bound)
+
+
 @pytest.mark.parametrize("t,d", [(F32, 64), (BF16, 64), (F16, 40)])
 @pytest.mark.parametrize("b,hk,lq,sinks", [(32, 4, 700, 700), (24, 4, 1300, 600), (2, 2, 1500, 10 ** 9)])
 def test_sinks_of_many_tiles(ops, dev, t, d, b, hk, lq, sinks):
