@@ -196,3 +196,17 @@ def test_frequencies(ops, dev, scaling, half, base):
     assert ((got - want).abs() <= 1e-14 * want).all()
     got = ops.rotary_frequencies(2 * half, base, scaling, device=dev, **how).cpu()
     assert ((got.double() - want).abs() <= (2.0 ** -24 + 1e-14) * want).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d", [33, 40, 48, 56, 72, 100, 136])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_values_behind_the_pairs_are_copied(ops, dev, t, d, interleaved):
+    q, k = normal((2, 19, 5, d), t, 21, dev), normal((2, 19, 2, d), t, 22, dev)
+    f, p = frequencies(16, dev), torch.arange(19, device=dev) + 300
+    whole = ops.rotary_embedding(q[..., :32].contiguous(), k[..., :32].contiguous(), p.expand(2, 19), f, interleaved)
+    into = q.clone(), k.clone()
+    for got in (ops.rotary_embedding(q, k, p.expand(2, 19), f, interleaved),
+                ops.rotary_embedding(*into, p.expand(2, 19), f, interleaved, q_out=into[0], k_out=into[1])):
+        for x, y, w in zip((q, k), got, whole):
+            assert torch.equal(y[..., 32:], x[..., 32:]) and torch.equal(y[..., :32], w)
