@@ -21,7 +21,7 @@ namespace opscv {
 
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4; // of a block; twice that where blocks are few (AttnStep)
 constexpr int kThreads = 32 * kWarps;
 
 struct StepArgs {
@@ -55,31 +55,32 @@ __device__ __forceinline__ void LoadRow(const T* p, int32_t lane, int32_t dim, b
 
 // Maxima (of scores in powers of two) and sums of the block's rows: of its warps, and of all of them.
 constexpr int kMostRows = 16;
+template <int W>
 struct RowParts {
-    float warpTop[kWarps][kMostRows], warpSum[kWarps][kMostRows], blockTop[kMostRows], blockSum[kMostRows];
+    float warpTop[W][kMostRows], warpSum[W][kMostRows], blockTop[kMostRows], blockSum[kMostRows];
 };
 
-// The warps' parts of `count` rows (weighted values [kWarps][count][dim] in `shared`, which has room for [count][dim] more) to the
+// The warps' parts of `count` rows (weighted values [W][count][dim] in `shared`, which has room for [count][dim] more) to the
 // results, by all threads of all blocks of the cluster.
-template <typename T>
+template <typename T, int W>
 __device__ __forceinline__ void JoinRows(const StepArgs& m, int32_t b, int32_t u, int32_t r0, int32_t count, const Lengths& n,
-                                         float* shared, RowParts& part)
+                                         float* shared, RowParts<W>& part)
 {
     const AttnShape& s = m.a.s;
     const int32_t rows = s.lq * m.a.group, split = blockIdx.x % m.splits;
     const int warp = threadIdx.x >> 5;
     __syncthreads();
-    // the block's four warps: thread t has columns t, t + 128, ... of the rows
-    float* block = shared + kWarps * count * s.dim;
-    for (int32_t e = threadIdx.x; e < count * s.dim; e += kThreads) {
+    // the block's warps: a thread has every 32 W-th column of the rows
+    float* block = shared + W * count * s.dim;
+    for (int32_t e = threadIdx.x; e < count * s.dim; e += 32 * W) {
         const int32_t r = e / s.dim;
         float most = -INFINITY, sum = 0.0f, x = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < W; ++w) {
             most = fmaxf(most, part.warpTop[w][r]);
         }
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float fade = most == -INFINITY ? 1.0f : Exp2(part.warpTop[w][r] - most);
             sum = fmaf(part.warpSum[w][r], fade, sum);
             x = fmaf(shared[w * count * s.dim + e], fade, x);
@@ -98,7 +99,7 @@ __device__ __forceinline__ void JoinRows(const StepArgs& m, int32_t b, int32_t u
         __syncthreads();
     }
     // the cluster's blocks: a warp has a row, a lane the maximum and the sum of a block; then the blocks' values, their loads together
-    for (int32_t r = split + m.splits * warp; r < count; r += m.splits * kWarps) {
+    for (int32_t r = split + m.splits * warp; r < count; r += m.splits * W) {
         const int32_t row = r0 + r;
         if (row < rows) {
             const int32_t i = row / m.a.group, h = u * m.a.group + row % m.a.group;
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kThreads) AttnStepKernel(const __grid_constant
 {
     constexpr int V = 16 / sizeof(T);
     extern __shared__ float shared[]; // [kWarps][R][dim] weighted values, then [R][dim] of the block
-    __shared__ RowParts part;
+    __shared__ RowParts<kWarps> part;
     const AttnShape& s = m.a.s;
     const int32_t split = blockIdx.x % m.splits;
     int32_t unit = blockIdx.x / m.splits;
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(kThreads) AttnStepKernel(const __grid_constant
             part.warpSum[warp][r] = sum;
         }
     }
-    JoinRows<T>(m, b, u, r0, R, n, shared, part);
+    JoinRows<T, kWarps>(m, b, u, r0, R, n, shared, part);
 }
 
 // ---- 16-bit rows on the warp's products ------------------------------------------------------------------------------------
@@ -364,14 +365,14 @@ constexpr uint32_t kBox = kStepKeys * 128; // 64 values of 16 keys
 
 // B64: blocks of 64 dims (1 or 2). In a lane, g = lane / 4 and c = lane % 4 stand for the row and the pair of columns that the products'
 // layout gives it.
-template <typename T, int B64>
-__global__ void __launch_bounds__(kThreads, 3)
+template <typename T, int B64, int W>
+__global__ void __launch_bounds__(32 * W, W == kWarps ? 3 : 1)
     AttnStepMmaKernel(const __grid_constant__ StepArgs m, int32_t mostRows, const __grid_constant__ CUtensorMap mapK,
                       const __grid_constant__ CUtensorMap mapV)
 {
     extern __shared__ __align__(1024) float shared[];
-    __shared__ RowParts part;
-    __shared__ uint64_t full[kWarps][kStages];
+    __shared__ RowParts<W> part;
+    __shared__ uint64_t full[W][kStages];
     __shared__ uint32_t failure;
     const AttnShape& s = m.a.s;
     const int32_t split = blockIdx.x % m.splits;
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 3)
             TmaLoad4At(at + (B64 + e) * kBox, &mapV, &full[warp][stage], 64 * e, j, u, b);
         }
     };
-    const int32_t first = split * kWarps + warp, stride = m.splits * kWarps;
+    const int32_t first = split * W + warp, stride = m.splits * W;
     if (lane == 0) {
         for (int x = 0; x < kStages; ++x) {
             if (first + x * stride < steps) {
@@ -591,22 +592,24 @@ __global__ void __launch_bounds__(kThreads, 3)
             }
         }
     }
-    JoinRows<T>(m, b, u, r0, mostRows, n, shared, part);
+    JoinRows<T, W>(m, b, u, r0, mostRows, n, shared, part);
 }
 
 // Shared memory of any of these: the rows of 16 (of at most 128 values) or 4 (256), the rings.
-constexpr size_t kRing = static_cast<size_t>(kWarps) * kStages * 2 * kBox; // per block of 64 dims
-constexpr size_t kMostShared = 2 * kRing + 1024;
-static_assert((kWarps + 1) * 16 * 128 * 4 <= kMostShared && (kWarps + 1) * 4 * 256 * 4 <= kMostShared, "rows fit");
+constexpr size_t kRing = static_cast<size_t>(kStages) * 2 * kBox; // of a warp, per block of 64 dims
+constexpr size_t MostShared(int warps) { return 2 * kRing * warps + 1024; }
+static_assert((kWarps + 1) * 16 * 128 * 4 <= MostShared(kWarps) && (kWarps + 1) * 4 * 256 * 4 <= MostShared(kWarps) &&
+                  (2 * kWarps + 1) * 16 * 128 * 4 <= MostShared(2 * kWarps),
+              "rows fit");
 
 template <typename Kernel, typename... More>
-cudaError_t Launch(Kernel kernel, std::atomic<uint64_t>& asked, const StepArgs& m, int r, size_t ring, int64_t units, cudaStream_t stream,
-                   const More&... more)
+cudaError_t Launch(Kernel kernel, std::atomic<uint64_t>& asked, const StepArgs& m, int r, int warps, size_t ring, int64_t units,
+                   cudaStream_t stream, const More&... more)
 {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(units * m.splits));
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = std::max(static_cast<size_t>(kWarps + 1) * r * m.a.s.dim * 4, ring);
+    config.blockDim = dim3(32 * warps);
+    config.dynamicSmemBytes = std::max(static_cast<size_t>(warps + 1) * r * m.a.s.dim * 4, ring);
     config.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -614,7 +617,7 @@ cudaError_t Launch(Kernel kernel, std::atomic<uint64_t>& asked, const StepArgs& 
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    const cudaError_t ask = AskOnce(kernel, asked, static_cast<int>(kMostShared), true);
+    const cudaError_t ask = AskOnce(kernel, asked, static_cast<int>(MostShared(warps)), true);
     if (ask != cudaSuccess) {
         return ask;
     }
@@ -630,8 +633,8 @@ cudaError_t LaunchFor(const StepArgs& m, int r, int n, bool vec, int64_t units, 
 #define OPSCV_STEP(R, N, U)                                                                                       \
     if (r == R && n == N) {                                                                                       \
         static std::atomic<uint64_t> asked[2];                                                                    \
-        return vec ? Launch(AttnStepKernel<T, R, N, U, true>, asked[0], m, r, 0, units, stream) :                 \
-                     Launch(AttnStepKernel<T, R, N, U, false>, asked[1], m, r, 0, units, stream);                 \
+        return vec ? Launch(AttnStepKernel<T, R, N, U, true>, asked[0], m, r, kWarps, 0, units, stream) :                 \
+                     Launch(AttnStepKernel<T, R, N, U, false>, asked[1], m, r, kWarps, 0, units, stream);                 \
     }
     OPSCV_STEP(1, 1, 4)
     OPSCV_STEP(2, 1, 4)
@@ -731,15 +734,25 @@ cudaError_t AttnStep(Dt dt, const AttnArgs& a, cudaStream_t stream)
         if (e != cudaSuccess) {
             return e;
         }
-        static std::atomic<uint64_t> asked[4];
-        const bool wide = s.dim > 64;
-        const size_t ring = (wide ? 2 : 1) * kRing + 1024;
+        // Where the blocks take at most half of the SMs, they have twice the warps: the chain of a warp's steps, not memory, is their limit
+        // (32768 keys, 16 heads of 128 on 4, 64 blocks: 26.5 us against 41.8; of 64 on 2, 65536 keys, 32 blocks: 30.8 against 47.2). With more
+        // blocks, clusters of 16 such large ones wait for one another's SMs (8192 keys, 32 heads of 128 on 8, 128 blocks: 24.6 against 18.5).
+        const bool more = 2 * units * splits <= NumSMs() && keys >= static_cast<int64_t>(splits) * kStepKeys * 8 * kWarps;
+        const int warps = more ? 2 * kWarps : kWarps;
+        const size_t ring = (s.dim > 64 ? 2 : 1) * kRing * warps + 1024;
+        auto launch = [&](auto wide, auto narrow, auto wideMore, auto narrowMore, std::atomic<uint64_t>* asked) {
+            return warps == kWarps ? (s.dim > 64 ? Launch(wide, asked[0], m, r, warps, ring, units, stream, r, mk, mv) :
+                                                   Launch(narrow, asked[1], m, r, warps, ring, units, stream, r, mk, mv)) :
+                                     (s.dim > 64 ? Launch(wideMore, asked[2], m, r, warps, ring, units, stream, r, mk, mv) :
+                                                   Launch(narrowMore, asked[3], m, r, warps, ring, units, stream, r, mk, mv));
+        };
+        static std::atomic<uint64_t> asked[8];
         if (dt == Dt::F16) {
-            return wide ? Launch(AttnStepMmaKernel<__half, 2>, asked[0], m, r, ring, units, stream, r, mk, mv) :
-                          Launch(AttnStepMmaKernel<__half, 1>, asked[1], m, r, ring, units, stream, r, mk, mv);
+            return launch(AttnStepMmaKernel<__half, 2, kWarps>, AttnStepMmaKernel<__half, 1, kWarps>,
+                          AttnStepMmaKernel<__half, 2, 2 * kWarps>, AttnStepMmaKernel<__half, 1, 2 * kWarps>, asked);
         }
-        return wide ? Launch(AttnStepMmaKernel<__nv_bfloat16, 2>, asked[2], m, r, ring, units, stream, r, mk, mv) :
-                      Launch(AttnStepMmaKernel<__nv_bfloat16, 1>, asked[3], m, r, ring, units, stream, r, mk, mv);
+        return launch(AttnStepMmaKernel<__nv_bfloat16, 2, kWarps>, AttnStepMmaKernel<__nv_bfloat16, 1, kWarps>,
+                      AttnStepMmaKernel<__nv_bfloat16, 2, 2 * kWarps>, AttnStepMmaKernel<__nv_bfloat16, 1, 2 * kWarps>, asked + 4);
     }
     switch (dt) {
         case Dt::F32: return LaunchFor<float>(m, r, n, vec, units, stream);

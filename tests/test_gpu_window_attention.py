@@ -258,6 +258,24 @@ def test_sinks_at_the_ends_of_steps(ops, dev, t, d, sinks, window):
 
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("lq,lk,h,hk,d,window,sinks", [
+    (1, 9000, 4, 1, 128, 10 ** 6, 0), (1, 5000, 2, 2, 64, 4000, 5), (5, 3001, 6, 2, 80, 10 ** 6, 0), (8, 2500, 8, 1, 40, 2100, 70),
+    (2, 700, 2, 1, 64, 600, 33), (16, 6000, 4, 1, 128, 10 ** 6, 0)])
+def test_few_blocks(ops, dev, t, lq, lk, h, hk, d, window, sinks):
+    """So few that they take twice the warps; the sequence ends inside a step, and what lies behind it says nothing."""
+    q = normal((1, lq, h, d), t, 141, dev)
+    k, v = normal((1, lk, hk, d), t, 142, dev), normal((1, lk, hk, d), t, 143, dev)
+    check(ops, q, k, v, window, sinks)
+    n = torch.tensor([lk - 61], device=dev)
+    want = Reference(q, k, v, window, sinks, kn=n)
+    k, v = k.clone(), v.clone()
+    k[:, lk - 61:], v[:, lk - 61:] = math.nan, math.inf
+    got, lse = ops.window_attention(q, k, v, window, sinks, kv_lengths=n)
+    close("out", got, want.out, want.out_bound)
+    close_lse(lse, want)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("lq,lk,h,hk,d,window,sinks", [
     (9, 1024, 4, 2, 64, 10 ** 6, 0), (17, 1500, 8, 1, 128, 2000, 3), (33, 3001, 6, 2, 80, 1100, 40), (100, 1111, 3, 3, 40, 990, 130),
     (150, 2500, 2, 1, 128, 1000, 0), (300, 2000, 2, 1, 96, 1500, 1700), (16, 1300, 4, 1, 200, 1290, 5), (70, 1800, 2, 2, 256, 5000, 0)])
 def test_some_queries_over_many_keys(ops, dev, t, lq, lk, h, hk, d, window, sinks):
