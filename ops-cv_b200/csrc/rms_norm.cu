@@ -576,9 +576,12 @@ struct BwdArgs {
 // rows ahead; else the next row is loaded into registers, which hold one.
 constexpr int Ahead(int nv) { return nv <= 2 ? 3 : 2; } // 4 chunks a thread leave room for two rows
 constexpr int RingBytes(int nv, int threads) { return Ahead(nv) * 3 * nv * threads * 16; }
+// 16 values a thread are the most whose weight, sums and rows fit its registers, and only with 512 threads a block.
+constexpr int kBwdValues = 16;
+constexpr int BwdThreads(int nv, int v) { return nv * v == kBwdValues ? 512 : kMaxThreads; }
 
 template <typename T, int V, int NV, bool RING>
-__global__ void __launch_bounds__(NV * V == 16 ? 512 : 1024) RmsNormBwdKernel(BwdArgs a)
+__global__ void __launch_bounds__(BwdThreads(NV, V)) RmsNormBwdKernel(BwdArgs a)
 {
     constexpr int kAhead = Ahead(NV);
     extern __shared__ uint4 slots[]; // [kAhead][3][NV][threads] (RING)
@@ -979,7 +982,8 @@ BwdPlan PlanBwd(int v, const NormShape& n)
 {
     BwdPlan p{};
     p.v = v;
-    p.shape = ShapeOfRow(n.width, v, 16, v >= 4 ? 512 : kMaxThreads, 0);
+    const int mostNv = v >= kBwdValues / 8 ? kBwdValues / v : 8;
+    p.shape = ShapeOfRow(n.width, v, kBwdValues, BwdThreads(mostNv, v), 0);
     if (p.shape.nv > 0 && p.shape.threads == 32 && p.shape.rows > 1) {
         // one row a block here too, of as many warps as give each lane one chunk
         const int32_t chunks = (n.width + v - 1) / v;
@@ -1050,6 +1054,10 @@ cudaError_t RmsNormBwd(Dt dt, const NormShape& n, const void* gradY, RowStride g
         if (a.scratch != nullptr) { // before gradX, which may lie over gradY
             const dim3 grid(static_cast<unsigned>(p.blocks), static_cast<unsigned>(CeilDiv(n.width, 256)));
             OPSCV_DISPATCH_DT(dt, T, RmsNormWeightSumsKernel<T><<<grid, 256, 0, s>>>(a));
+            const cudaError_t e = cudaGetLastError();
+            if (e != cudaSuccess) {
+                return e;
+            }
             CountLaunch();
         }
         OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
@@ -1058,7 +1066,7 @@ cudaError_t RmsNormBwd(Dt dt, const NormShape& n, const void* gradY, RowStride g
     } else {
         cudaError_t failed = cudaSuccess;
         OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
-            OPSCV_DISPATCH_NV(p.shape.nv, NV, if constexpr (NV > 0 && NV * V <= 16) {
+            OPSCV_DISPATCH_NV(p.shape.nv, NV, if constexpr (NV > 0 && NV * V <= kBwdValues) {
                 if constexpr (V * sizeof(T) == 16) {
                     static std::atomic<uint64_t> asked;
                     const int shared = RingBytes(NV, p.shape.threads);
@@ -1076,6 +1084,10 @@ cudaError_t RmsNormBwd(Dt dt, const NormShape& n, const void* gradY, RowStride g
         if (failed != cudaSuccess) {
             return failed;
         }
+    }
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) { // no sums to make gradWeight of
+        return e;
     }
     CountLaunch();
     if (gradWeight != nullptr) {

@@ -273,3 +273,22 @@ def test_graph_and_stream(ops, dev):
             a.copy_(b)
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,width,wide", [(2, 8194, 8194), (3, 10002, 10002), (3, 12290, 12290), (2, 16382, 16382), (300, 8198, 8198),
+                                             (2, 12288, 12290), (2, 16384, 16386)])
+def test_backward_of_wide_rows_in_pairs(ops, dev, t, rows, width, wide):
+    """Rows of more than 8192 values that can only be read two at a time, by their width or by their distance."""
+    z, gy, gs, _ = (x[:, :width] for x in inputs((rows, wide), t, 22, dev, 4))
+    w = weights(width, t, 23, dev)
+    y, rstd = forward64(z, w, 1e-6)
+    got = ops.residual_rms_norm(z, None, w)[0]
+    close(got, y, (half_step(t) + 2 * CHAIN * STEP32) * y.abs() + torch.finfo(t).tiny)
+    gx, gw = ops.residual_rms_norm_backward(gy, z, rstd.float().squeeze(-1), w, gs)
+    u, g = z.double() * rstd, gy.double() * w.double()
+    want = gs.double() + rstd * (g - u * (g * u).mean(-1, keepdim=True))
+    terms = gs.double().abs() + rstd * (g.abs() + u.abs() * (g * u).abs().mean(-1, keepdim=True))
+    close(gx, want, half_step(t) * want.abs() + 2 * CHAIN * STEP32 * terms + torch.finfo(t).tiny)
+    want = (gy.double() * u).sum(0)
+    close(gw, want, half_step(t) * want.abs() + (rows + CHAIN) * STEP32 * (gy.double() * u).abs().sum(0) + torch.finfo(t).tiny)
