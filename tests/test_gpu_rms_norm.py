@@ -292,3 +292,17 @@ def test_backward_of_wide_rows_in_pairs(ops, dev, t, rows, width, wide):
     close(gx, want, half_step(t) * want.abs() + 2 * CHAIN * STEP32 * terms + torch.finfo(t).tiny)
     want = (gy.double() * u).sum(0)
     close(gw, want, half_step(t) * want.abs() + (rows + CHAIN) * STEP32 * (gy.double() * u).abs().sum(0) + torch.finfo(t).tiny)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("width", [40, 200, 1144, 5000])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_quant_of_a_weight_that_is_not_finite(ops, dev, t, width, bad):
+    """It reaches the scale of its own group and no other, the shorter last one least of all."""
+    x = inputs((3, width), t, 24, dev)[0]
+    for w in (torch.ones(width, device=dev), torch.ones(width, dtype=t, device=dev)):
+        clean = [ops.residual_rms_norm_quant(x, None, w, group=group)[1] for group in (32, 128)]
+        w[0] = bad
+        for group, want in zip((32, 128), clean):
+            got = ops.residual_rms_norm_quant(x, None, w, group=group)[1]
+            assert not got[:, 0].isfinite().any() and torch.equal(got[:, 1:], want[:, 1:])
