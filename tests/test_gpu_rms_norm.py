@@ -306,3 +306,21 @@ def test_quant_of_a_weight_that_is_not_finite(ops, dev, t, width, bad):
         for group, want in zip((32, 128), clean):
             got = ops.residual_rms_norm_quant(x, None, w, group=group)[1]
             assert not got[:, 0].isfinite().any() and torch.equal(got[:, 1:], want[:, 1:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("rows,width", [(256, 4096), (64, 5120), (300, 96), (37, 1143), (9, 40000)])
+@pytest.mark.parametrize("group", [0, 32, 128, 160])
+def test_quant_divides_the_fp32_values(ops, dev, rows, width, dtype, group):
+    """The 8-bit values are those of y / scale, divided in fp32 and rounded to nearest even (y of fp32 tensors comes out as it is)."""
+    x = inputs((rows, width), torch.float32, 25, dev)[0]
+    w = weights(width, torch.float32, 26, dev)
+    y = ops.residual_rms_norm(x, None, w)[0]
+    q, scales, _ = ops.residual_rms_norm_quant(x, None, w, dtype=dtype, group=group)
+    range_ = 127.0 if dtype == torch.int8 else 448.0
+    g = group if 0 < group < width else width
+    tops = torch.stack([p.abs().amax(-1) for p in torch.split(y, g, -1)], -1)
+    assert torch.equal(scales, tops / torch.full_like(tops, range_))  # by a tensor: torch takes a number's inverse
+    want = y / torch.repeat_interleave(scales, g, -1)[:, :width]
+    want = want.round() if dtype == torch.int8 else want.clamp(-448, 448).to(dtype).float()
+    assert torch.equal(q.float(), want)
