@@ -293,6 +293,23 @@ NormShape ShapeOf(const aclTensor* x, const aclTensor* weight, double eps)
 }
 
 // ---- rotary ------------------------------------------------------------------------------------------------------------------
+// Positions that broadcast along a dimension between others do not merge with them; such go through a copy. Those that stand for
+// themselves in three dimensions or more do not: the kernel reads two.
+bool PositionsStageable(const aclTensor* positions, size_t axesDim)
+{
+    int levels = 0;
+    int64_t last = 0;
+    for (size_t i = axesDim; i < positions->dims.size(); ++i) {
+        const int64_t n = positions->dims[i], stride = positions->strides[i];
+        if (n == 1 || stride == 0) {
+            continue;
+        }
+        levels += levels == 0 || last != stride * n ? 1 : 0;
+        last = stride;
+    }
+    return levels <= 2 && ViewStageable(positions);
+}
+
 aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, const aclTensor* positions,
                        const aclTensor* frequencies, const aclIntArray* sections, bool interleaved, double scale, bool inverse,
                        aclTensor* qOut, aclTensor* kOut, aclOpExecutor& ex, WsPlan& ws)
@@ -348,6 +365,7 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
         return ACLNN_SUCCESS;
     }
     Operand oq = In(q), ok = In(k), oqo = Out(qOut), oko = Out(kOut);
+    aclTensor pos = *positions;
     RotaryTensor tq, tk;
     Lead merged;
     auto addAll = [&](LeadMerge& m) {
@@ -357,15 +375,35 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
             m.Add(&ok.view, 0, &tk.inTok);
             m.Add(&oko.view, 0, &tk.outTok);
         }
-        m.Add(positions, axesDim, &r.posTok);
+        m.Add(&pos, axesDim, &r.posTok);
     };
     const auto all = {&oq, &ok, &oqo, &oko};
+    // the views as they are; with copied positions; with copies of the others; with copies of all
     bool merges = MergesAsGiven(all, lead, addAll, merged);
+    const aclTensor copied = ContiguousLike(positions);
+    const bool mayCopy = !merges && PositionsStageable(positions, axesDim);
+    bool copies = false;
+    if (mayCopy) {
+        pos = copied;
+        merges = copies = MergesAsGiven(all, lead, addAll, merged);
+        pos = copies ? copied : *positions;
+    }
     OPSCV_TRY(Place(api, all, !merges, ex, ws));
     if (!merges) {
-        LeadMerge m(lead);
-        addAll(m);
-        OPSCV_REQUIRE(m.Run(merged), "%s: positions with more than two strided leading dimensions are not supported", api);
+        LeadMerge asGiven(lead), withCopy(lead);
+        addAll(asGiven);
+        if (!asGiven.Run(merged)) {
+            OPSCV_REQUIRE(mayCopy, "%s: positions with more than two strided leading dimensions are not supported", api);
+            copies = true;
+            pos = copied;
+            addAll(withCopy);
+            withCopy.Run(merged); // contiguous tensors merge to one
+        }
+    }
+    BufRef posBuf;
+    posBuf.base = DataOf(positions, ElemSize(positions->dtype));
+    if (copies) {
+        posBuf = StageInput(positions, ws, &ex);
     }
     r.tokens = merged.total;
     r.inner = merged.inner;
@@ -375,7 +413,7 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
     r.inverse = inverse;
     r.freq64 = frequencies->dtype == ACL_DOUBLE;
     r.pos64 = positions->dtype == ACL_INT64;
-    r.posAxis = axesDim != 0 ? positions->strides[0] : 0;
+    r.posAxis = axesDim != 0 ? pos.strides[0] : 0;
     r.scale = static_cast<float>(scale);
     tq.heads = static_cast<int32_t>(heads);
     tq.inHead = oq.view.strides[lead];
@@ -385,7 +423,6 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
         tk.inHead = ok.view.strides[lead];
         tk.outHead = oko.view.strides[lead];
     }
-    const void* pos = DataOf(positions, r.pos64 ? 8 : 4);
     const void* freq = DataOf(frequencies, r.freq64 ? 8 : 4);
     const Dt dt = ToDt(q->dtype);
     const BufRef bq = oq.buf, bk = ok.buf, bqo = oqo.buf, bko = oko.buf;
@@ -397,7 +434,7 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
             b.in = bk.At(w);
             b.out = bko.At(w);
         }
-        return RotaryTurn(dt, r, a, b, pos, freq, s);
+        return RotaryTurn(dt, r, a, b, posBuf.At(w), freq, s);
     });
     Finish(all, ex);
     return ACLNN_SUCCESS;

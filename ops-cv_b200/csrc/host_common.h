@@ -116,7 +116,10 @@ inline int64_t Numel(const aclTensor* t)
 bool IsContiguous(const aclTensor* t);
 bool DtypeSupported(aclDataType d); // fp32 / fp16 / bf16
 Dt ToDt(aclDataType d);
-inline int ElemSize(aclDataType d) { return d == ACL_FLOAT ? 4 : 2; }
+inline int ElemSize(aclDataType d) // of tensors that may be staged
+{
+    return d == ACL_INT64 || d == ACL_DOUBLE ? 8 : d == ACL_FLOAT || d == ACL_INT32 ? 4 : 2;
+}
 const char* DtypeName(aclDataType d);
 const char* FormatName(aclFormat f);
 int64_t GetDeterministic(); // thread-local ACL_OPT_DETERMINISTIC

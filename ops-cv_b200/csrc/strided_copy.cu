@@ -241,7 +241,9 @@ cudaError_t StridedCopy(int elemSize, void* contiguous, void* viewBase, View4 v,
     if (total == 0) {
         return cudaSuccess;
     }
-    if (elemSize == 4) {
+    if (elemSize == 8) {
+        LaunchStridedCopy<uint64_t>(static_cast<uint64_t*>(contiguous), static_cast<uint64_t*>(viewBase), v, toView, s);
+    } else if (elemSize == 4) {
         LaunchStridedCopy<uint32_t>(static_cast<uint32_t*>(contiguous), static_cast<uint32_t*>(viewBase), v, toView, s);
     } else {
         LaunchStridedCopy<uint16_t>(static_cast<uint16_t*>(contiguous), static_cast<uint16_t*>(viewBase), v, toView, s);

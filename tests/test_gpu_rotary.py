@@ -210,3 +210,25 @@ def test_values_behind_the_pairs_are_copied(ops, dev, t, d, interleaved):
                 ops.rotary_embedding(*into, p.expand(2, 19), f, interleaved, q_out=into[0], k_out=into[1])):
         for x, y, w in zip((q, k), got, whole):
             assert torch.equal(y[..., 32:], x[..., 32:]) and torch.equal(y[..., :32], w)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_positions_that_broadcast(ops, dev, t, kind):
+    """Stride 0 along any of the leading dimensions, between others too, with and without axes; views of q that need copies as well."""
+    q, k = normal((2, 3, 5, 4, 24), t, 23, dev), normal((2, 3, 5, 2, 24), t, 24, dev)
+    f = frequencies(8, dev)
+    whole = torch.randint(0, 9000, (3, 2, 3, 5), generator=torch.Generator().manual_seed(25)).to(kind).to(dev)
+    for cut in ((0, 0, 0), (1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (1, 1, 0), (0, 1, 1), (1, 1, 1)):
+        p = whole[(slice(None), *(slice(0, 1) if c else slice(None) for c in cut))].contiguous().expand(3, 2, 3, 5)
+        full = p.contiguous()
+        for at, flat, sections in ((p[0], full[0], None), (p, full, (3, 4, 1)), (p[:1], full[:1], (8,))):
+            want = ops.rotary_embedding(q, k, flat, f, sections=sections)
+            check(want[0], q, flat, f, False, sections, 1.0)
+            got = ops.rotary_embedding(q, k, at, f, sections=sections)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+            apart = torch.zeros(2, 4, 3, 6, 4, 24, dtype=t, device=dev)[:, ::2, :, 1:].transpose(1, 2)[:, :, 0]
+            apart.copy_(q)
+            assert torch.equal(ops.rotary_embedding(apart, k, at, f, sections=sections, q_out=apart)[0], want[0])
+            back = ops.rotary_embedding_backward(q, k, at, f, sections=sections)
+            assert torch.equal(back[0], ops.rotary_embedding_backward(q, k, flat, f, sections=sections)[0])

@@ -239,3 +239,10 @@ def test_tensors_of_two_devices(ops):
     x = torch.zeros(2, 8)
     with pytest.raises(ValueError, match="one device"):
         ops.residual_rms_norm(x, torch.zeros(2, 8, device="meta"))
+
+
+def test_rotary_accepts_positions_that_broadcast(ops):
+    q, f = torch.zeros(2, 3, 4, 2, 8), torch.zeros(4)
+    for shape in ((2, 1, 1), (1, 3, 1), (1, 1, 4), (2, 1, 4), (2, 3, 1), (1, 3, 4), (3, 1), (1, 1, 1)):
+        for t in (torch.int32, torch.int64):
+            accepted(lambda: ops.rotary_embedding(q, None, torch.zeros(shape, dtype=t), f))
