@@ -781,10 +781,18 @@ PyObject* Rotary(Args a)
     aclIntArray sections;
     if (Given(a[5])) {
         sections = IntArrayOf(a[5]);
-    } else if (q.dim() >= 2) {
+    }
+    if (q.dim() >= 2) { // one position for several tokens
         const at::IntArrayRef lead = q.sizes().slice(0, q.dim() - 2);
-        if (positions.sizes() != lead) {
-            positions = positions.expand(lead); // one position for several tokens
+        if (!Given(a[5])) {
+            positions = positions.sizes() == lead ? positions : positions.expand(lead);
+        } else if (positions.dim() >= 1 && positions.sizes().slice(1) != lead) {
+            std::vector<int64_t> shape = lead.vec();
+            shape.insert(shape.begin(), positions.size(0));
+            while (positions.dim() < static_cast<int64_t>(shape.size())) {
+                positions = positions.unsqueeze(1); // behind the axes
+            }
+            positions = positions.expand(shape);
         }
     }
     const double scale = DoubleOf(a[6]);

@@ -34,8 +34,8 @@ def residual_rms_norm_quant(x, residual=None, weight=None, eps=1e-6, dtype=torch
 def rotary_embedding(q, k, positions, frequencies, interleaved=False, sections=None, scale=1.0, q_out=None, k_out=None,
                      workspace=None):
     """(q', k') with the first 2 * len(frequencies) values of each head turned by position * frequency; k may be None.
-    q is [..., heads, dim]; positions has (or broadcasts to) its leading dimensions, with an axis in front for each of `sections`
-    where these are given. Pairs are (i, half + i), or neighbours where `interleaved`. q_out may be q and k_out k."""
+    q is [..., heads, dim]; positions has (or broadcasts to) its leading dimensions, behind a dimension of the axes where `sections`
+    are given: [axes, tokens] serves all sequences of q [batch, tokens, heads, dim]. Pairs are (i, half + i), or neighbours where `interleaved`. q_out may be q and k_out k."""
     return native().rotary_embedding(q, k, positions, frequencies, interleaved, sections, scale, q_out, k_out, workspace, False)
 
 

@@ -232,3 +232,15 @@ def test_positions_that_broadcast(ops, dev, t, kind):
             assert torch.equal(ops.rotary_embedding(apart, k, at, f, sections=sections, q_out=apart)[0], want[0])
             back = ops.rotary_embedding_backward(q, k, at, f, sections=sections)
             assert torch.equal(back[0], ops.rotary_embedding_backward(q, k, flat, f, sections=sections)[0])
+
+
+def test_axes_of_a_table_for_all_sequences(ops, dev):
+    q, k = normal((4, 9, 3, 40), torch.float16, 26, dev), normal((4, 9, 1, 40), torch.float16, 27, dev)
+    f, sections = frequencies(16, dev), (6, 5, 5)
+    p = torch.randint(0, 5000, (3, 9), generator=torch.Generator().manual_seed(28)).to(dev)
+    full = p[:, None].expand(3, 4, 9).contiguous()
+    want = ops.rotary_embedding(q, k, full, f, sections=sections)
+    for at in (p, p[:, None]):
+        got = ops.rotary_embedding(q, k, at, f, sections=sections)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    check(want[0], q, full, f, False, sections, 1.0)

@@ -246,3 +246,16 @@ def test_rotary_accepts_positions_that_broadcast(ops):
     for shape in ((2, 1, 1), (1, 3, 1), (1, 1, 4), (2, 1, 4), (2, 3, 1), (1, 3, 4), (3, 1), (1, 1, 1)):
         for t in (torch.int32, torch.int64):
             accepted(lambda: ops.rotary_embedding(q, None, torch.zeros(shape, dtype=t), f))
+
+
+def test_rotary_positions_by_axes_broadcast(ops):
+    q, f = torch.zeros(2, 5, 4, 16), torch.zeros(8)
+    for shape in ((3, 5), (3, 1, 5), (3, 2, 1), (3, 1), (3,), (3, 2, 5)):
+        accepted(lambda: ops.rotary_embedding(q, None, torch.zeros(shape, dtype=torch.int64), f, sections=(4, 2, 2)))
+        accepted(lambda: ops.rotary_embedding_backward(q, None, torch.zeros(shape, dtype=torch.int32), f, sections=(4, 2, 2)))
+        refused(ops, lambda: ops.rotary_embedding(q, None, torch.zeros(shape, dtype=torch.int64), f, sections=(4, 4)), "positions must be")
+    accepted(lambda: ops.rotary_embedding(q[0, 0], None, torch.zeros(2, dtype=torch.int64), f, sections=(4, 4)))
+    for shape in ((3, 4), (3, 5, 2), (3, 2, 2, 5)):
+        with pytest.raises(RuntimeError, match="expand"):
+            ops.rotary_embedding(q, None, torch.zeros(shape, dtype=torch.int64), f, sections=(4, 2, 2))
+    refused(ops, lambda: ops.rotary_embedding(q, None, torch.tensor(3), f, sections=(8,)), "positions must be")
