@@ -798,21 +798,21 @@ __global__ void __launch_bounds__(kMaxThreads) RmsNormBwdWideKernel(BwdArgs a)
         StoreF<T, V>(out + col, v);
     }
 }
-// and the sums of the weight's gradient: a thread per column, a block per (columns, share of the rows).
+// and the sums of the weight's gradient: a thread per column, a block per (columns, share of the rows); the shares, 64 at most, along y.
 template <typename T>
 __global__ void RmsNormWeightSumsKernel(BwdArgs a)
 {
-    const int32_t col = blockIdx.y * blockDim.x + threadIdx.x;
+    const int32_t col = blockIdx.x * blockDim.x + threadIdx.x;
     if (col >= a.width) {
         return;
     }
     float acc = 0.0f;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const float g = DType<T>::ToF(static_cast<const T*>(a.gradY)[RowAt(row, a.inner, a.gs) + col]);
         const float z = DType<T>::ToF(static_cast<const T*>(a.sum)[RowAt(row, a.inner, a.ss) + col]);
         acc = fmaf(g, z * a.rstd[row], acc);
     }
-    a.scratch[static_cast<int64_t>(blockIdx.x) * a.width + col] = acc;
+    a.scratch[static_cast<int64_t>(blockIdx.y) * a.width + col] = acc;
 }
 
 // The blocks' sums of one column, added in a fixed order: 32 warps take every 32nd block, then add up.
@@ -1083,7 +1083,7 @@ cudaError_t RmsNormBwd(Dt dt, const NormShape& n, const void* gradY, RowStride g
             return cudaErrorInvalidConfiguration;
         }
         if (a.scratch != nullptr) { // before gradX, which may lie over gradY
-            const dim3 grid(static_cast<unsigned>(p.blocks), static_cast<unsigned>(CeilDiv(n.width, 256)));
+            const dim3 grid(static_cast<unsigned>(CeilDiv(n.width, 256)), static_cast<unsigned>(p.blocks));
             OPSCV_DISPATCH_DT(dt, T, RmsNormWeightSumsKernel<T><<<grid, 256, 0, s>>>(a));
             const cudaError_t e = cudaGetLastError();
             if (e != cudaSuccess) {

@@ -324,3 +324,19 @@ def test_quant_divides_the_fp32_values(ops, dev, rows, width, dtype, group):
     want = y / torch.repeat_interleave(scales, g, -1)[:, :width]
     want = want.round() if dtype == torch.int8 else want.clamp(-448, 448).to(dtype).float()
     assert torch.equal(q.float(), want)
+
+
+def test_backward_of_rows_of_16_million_values(ops, dev):
+    """More columns than a grid's second dimension has blocks for."""
+    width, t = 65535 * 256 + 4, torch.bfloat16
+    z, gy = ((torch.randn(2, width, generator=torch.Generator(device=dev).manual_seed(s), device=dev)).to(t) for s in (27, 28))
+    w = z[0].abs() + 0.5
+    _, rstd = forward64(z, w, 1e-6)
+    gx, gw = ops.residual_rms_norm_backward(gy, z, rstd.float().squeeze(-1), w)
+    u, g = z.double() * rstd, gy.double() * w.double()
+    want = (gy.double() * u).sum(0)
+    close(gw, want, half_step(t) * want.abs() + CHAIN * STEP32 * (gy.double() * u).abs().sum(0) + torch.finfo(t).tiny)
+    want = rstd * (g - u * (g * u).mean(-1, keepdim=True))
+    terms = rstd * (g.abs() + u.abs() * (g * u).abs().mean(-1, keepdim=True))
+    chain = width // 1024 + CHAIN  # a thread adds up its share of the row in turn
+    close(gx, want, half_step(t) * want.abs() + 2 * chain * STEP32 * terms + torch.finfo(t).tiny)
