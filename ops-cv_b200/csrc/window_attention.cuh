@@ -7,6 +7,8 @@
 //   gradV_j += p_j gradOut, ds_j = p_j (gradOut . v_j - delta) scale, gradQ += ds_j k_j, gradK_j += ds_j q.
 #pragma once
 
+#include <algorithm>
+
 #include <cuda.h> // CUtensorMap
 
 #include "launch_util.cuh"
@@ -274,15 +276,15 @@ cudaError_t AttnBackwardMma(Dt dt, const AttnArgs& a, void* workspace, cudaStrea
 constexpr int kMmaMostDim = 128;
 
 // Blocks that share out the far queries of a tile with sinks, of the `wanted` that bring their walks down to an ordinary one's; 0: the
-// tile's own block walks them. Each costs memory for its sums, so where sinks fill tiles enough for the SMs, there are fewer or none.
+// tile's own block walks them. Each costs memory for its sums, so there are no more than four of them an SM over all units and tiles:
+// longer walks then end with the others, and the sums take some 150 MB at most. Backward, heads of 128, bf16, with 4, 8 and 16 an SM:
+// 32 sequences of 2048, 8 heads, window 128, 300 sinks 904, 1266 and 1568 us; 64 of 4096, window 64, 4 sinks 3176, 3192 and 3246 (3438
+// and 805 MB without a limit). Nor more than 64 a tile: 65536 tokens, one head, window 256: 144 us, 165 with 128; fp32, 16384 tokens,
+// window 64: 171 us, 189 with 128, 194 with 32. The SMs are a constant, not the device's, because both phases have to come to one plan.
 inline int32_t AttnFarChunks(int64_t units, int32_t sinkTiles, int64_t wanted)
 {
-    int64_t most = 64;
-    if (sinkTiles >= 4) {
-        const int64_t enough = 8 * kNumSMsFallback / (units * sinkTiles > 0 ? units * sinkTiles : 1);
-        most = enough < most ? enough : most;
-    }
-    return static_cast<int32_t>(wanted < most ? wanted : most);
+    const int64_t enough = 4 * kNumSMsFallback / (units * sinkTiles > 0 ? units * sinkTiles : 1);
+    return static_cast<int32_t>(std::min({wanted, enough, static_cast<int64_t>(64)}));
 }
 
 } // namespace opscv

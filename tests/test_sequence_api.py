@@ -259,3 +259,23 @@ def test_rotary_positions_by_axes_broadcast(ops):
         with pytest.raises(RuntimeError, match="expand"):
             ops.rotary_embedding(q, None, torch.zeros(shape, dtype=torch.int64), f, sections=(4, 2, 2))
     refused(ops, lambda: ops.rotary_embedding(q, None, torch.tensor(3), f, sections=(8,)), "positions must be")
+
+
+@pytest.mark.parametrize("code", ["ACL_BF16", "ACL_FLOAT"])
+@pytest.mark.parametrize("batch,tokens,kv,group,sinks", [(64, 4096, 8, 1, 4), (64, 4096, 8, 4, 130), (256, 2048, 16, 1, 1), (16, 32768, 8, 1, 300)])
+def test_workspace_of_many_sequences(ops, code, batch, tokens, kv, group, sinks):
+    """However many sequences have sinks, the sums of the blocks that share their queries take less than the gradient of the keys."""
+    L = ops.lib()
+
+    def tensor(*shape, dtype):
+        dims = (ctypes.c_int64 * len(shape))(*shape)
+        return ctypes.c_void_p(L.aclCreateTensor(dims, len(shape), dtype, None, 0, ops.ACL_FORMAT_ND, dims, len(shape), ctypes.c_void_p(4096)))
+
+    dtype, d, elem = getattr(ops, code), 128, 2 if code == "ACL_BF16" else 4
+    q, k = tensor(batch, tokens, kv * group, d, dtype=dtype), tensor(batch, tokens, kv, d, dtype=dtype)
+    lse = tensor(batch, kv * group, tokens, dtype=ops.ACL_FLOAT)
+    n, e = ctypes.c_uint64(0), ctypes.c_void_p(None)
+    got = L.aclnnWindowAttentionBackwardGetWorkspaceSize(q, q, k, k, q, lse, None, None, 64, sinks, 0.1, q, k, k, ctypes.byref(n), ctypes.byref(e))
+    statistics = 2 * 4 * batch * kv * group * (tokens + 256)
+    assert got == 0 and n.value - statistics < batch * tokens * kv * d * elem
+    L.aclDestroyAclOpExecutor(e)
