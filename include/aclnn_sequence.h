@@ -99,7 +99,7 @@ ACLNN_API aclnnStatus aclnnRotaryEmbeddingBackward(void* workspace, uint64_t wor
  *   3 wavelength: frequencies that turn `high` times or more within originalLength tokens stay, those that turn `low` times or
  *     less are divided by factor, the ones between are blended by their turns (0 <= low < high);
  *   4 ramp: the same, blended linearly over i between the (real-valued) indices that turn `high` and `low` times, rounded
- *     outwards (0 < low < high).
+ *     outwards and cut to [0, 2 half - 1] (0 < low < high).
  * originalLength > 0, low and high are read for scaling 3 and 4 only. */
 ACLNN_API aclnnStatus aclnnRotaryFrequenciesGetWorkspaceSize(double base, int64_t scaling, double factor,
                                                              double originalLength, double low, double high,

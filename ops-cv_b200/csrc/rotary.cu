@@ -221,13 +221,13 @@ __global__ void RotaryFrequenciesKernel(void* out, bool is64, int32_t half, doub
         keep = keep < 0.0 ? 0.0 : (keep > 1.0 ? 1.0 : keep);
         f = f * keep + f / factor * (1.0 - keep);
     } else if (kind == RotaryScaling::RAMP) {
-        // the same, blended linearly over the frequencies' indices between those that turn `high` and `low` times
+        // the same, blended linearly over the frequencies' indices between those that turn `high` and `low` times, as far as there are
+        // such indices
         const double first = floor(half * log(originalLength / (high * 2.0 * pi)) / log(base));
         const double last = ceil(half * log(originalLength / (low * 2.0 * pi)) / log(base));
         const double a = first < 0.0 ? 0.0 : first;
-        double b = last > 2.0 * half - 1.0 ? 2.0 * half - 1.0 : last;
-        b = b <= a ? a + 0.001 : b;
-        double stretch = (i - a) / (b - a);
+        const double b = last > 2.0 * half - 1.0 ? 2.0 * half - 1.0 : last;
+        double stretch = b > a ? (i - a) / (b - a) : i > b ? 1.0 : 0.0; // b < a: all turn less than `low` times, or all more than `high`
         stretch = stretch < 0.0 ? 0.0 : (stretch > 1.0 ? 1.0 : stretch);
         f = f * (1.0 - stretch) + f / factor * stretch;
     }

@@ -244,3 +244,18 @@ def test_axes_of_a_table_for_all_sequences(ops, dev):
         got = ops.rotary_embedding(q, k, at, f, sections=sections)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     check(want[0], q, full, f, False, sections, 1.0)
+
+
+@pytest.mark.parametrize("half", [4, 64])
+def test_ramp_without_frequencies_between(ops, dev, half):
+    """Contexts so short that every frequency turns far less than `low` times are divided throughout, so long that all turn more than `high`
+    times are left as they are; where both bounds fall on one index, it stays."""
+    plain = ops.rotary_frequencies(2 * half, 10000.0, dtype=torch.float64, device=dev)
+    but_first = torch.cat((plain[:1], plain[1:] / 8))
+    for length, low, high in ((2.0, 1.0, 32.0), (6.0, 1.0, 2.0), (0.5, 1.0, 4.0), (1e12, 1.0, 32.0)):
+        last = math.ceil(half * math.log(length / (low * 2 * math.pi)) / math.log(10000.0))  # an index in (-1, 0) is rounded outwards to 0
+        want = plain / 8 if last < 0 else but_first if last == 0 else plain
+        got = ops.rotary_frequencies(2 * half, 10000.0, "ramp", 8.0, length, low, high, torch.float64, dev)
+        assert ((got - want).abs() <= 1e-14 * want).all()
+    got = ops.rotary_frequencies(2 * half, 10000.0, "ramp", 8.0, 2 * math.pi * 1.5, 1.5, 1.5 + 1e-13, torch.float64, dev)
+    assert ((got[1:] - plain[1:] / 8).abs() <= 1e-14 * plain[1:]).all()
