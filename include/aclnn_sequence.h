@@ -25,8 +25,9 @@ extern "C" {
 /* ---- ResidualRmsNorm -------------------------------------------------------------------------------------------------------
  * sum = x + residual, rounded to the tensors' type; rstd = 1 / sqrt(mean(sum^2) + eps) over the last dimension;
  * y = sum * rstd * weight.
- * x, residual, y, sum: the same shape [..., width], width >= 1. residual may be null (sum is then x; `sum` may be null, and is a
- * copy of x where it is given). weight: [width] of the tensors' type or ACL_FLOAT, or null (ones). eps: finite, >= 0.
+ * x, residual, y, sum: the same shape [..., width], 1 <= width < 2^30. residual may be null (sum is then x; `sum` may be null, and is a
+ * copy of x where it is given). weight: [width] of the tensors' type or ACL_FLOAT, or null (ones). eps: taken in fp32, where it has to
+ * be finite, and >= 0.
  * sum, rstd ([...], ACL_FLOAT, contiguous): null where they are not wanted; the backward reads both.
  * y may lie over x or residual, and sum over x or residual (each over another one). */
 ACLNN_API aclnnStatus aclnnResidualRmsNormGetWorkspaceSize(const aclTensor* x, const aclTensor* residual,
@@ -54,7 +55,7 @@ ACLNN_API aclnnStatus aclnnResidualRmsNormBackward(void* workspace, uint64_t wor
  * rounded to nearest even; y is about out * scale. The division is of the fp32 values, before any rounding of y. A group of zeros
  * (or of magnitudes below 1e-35) has scale 0 and zeros; one that holds a NaN or an infinity has a NaN or infinity as its scale,
  * and its values say nothing.
- * out: x's shape, contiguous. scales: [..., groups], ACL_FLOAT, contiguous. sum: as above, may be null. */
+ * out: x's shape, contiguous. scales: [..., groups], ACL_FLOAT, contiguous, at most 10240 groups. sum: as above, may be null. */
 ACLNN_API aclnnStatus aclnnResidualRmsNormQuantGetWorkspaceSize(const aclTensor* x, const aclTensor* residual,
                                                                 const aclTensor* weight, double eps, int64_t group,
                                                                 aclTensor* out, aclTensor* scales, aclTensor* sum,
@@ -64,7 +65,9 @@ ACLNN_API aclnnStatus aclnnResidualRmsNormQuant(void* workspace, uint64_t worksp
 
 /* ---- RotaryEmbedding ---------------------------------------------------------------------------------------------------------
  * q: [..., heads, dim], k: [..., kvHeads, dim] with the same leading dimensions, or null. The first rotary = 2 * half values of a
- * head are turned by the angles position * frequencies[i], i < half, and multiplied by `scale`; the others are copied.
+ * head are turned by the angles position * frequencies[i], i < half, and multiplied by `scale` (taken in fp32, where it has to be
+ * finite); the others are copied. A token of more than 2^24 values, of q and k together, is refused, and so are more than 2^20 heads
+ * or values of a head.
  * Pair i is values (i, half + i), or (2i, 2i + 1) where `interleaved`.
  * frequencies: [half] of ACL_DOUBLE or ACL_FLOAT, contiguous, 1 <= half <= dim / 2 and half <= 2048. The angle is formed in
  * 64 bits.
@@ -116,7 +119,8 @@ ACLNN_API aclnnStatus aclnnRotaryFrequencies(void* workspace, uint64_t workspace
  * kvLengths, qLengths: [batch], ACL_INT32 or ACL_INT64, contiguous, or null (all keys, all queries): how many keys and queries of
  * each sequence count; values outside [0, keys] and [0, queries] are cut to it. Query i of a sequence sits at position
  * p = kvLength - qLength + i, so that the last query sits at the last key; it sees the keys j <= p with j > p - window
- * (window >= 1) or j < sinks (sinks >= 0; both are cut to 2^30). scale multiplies the scores.
+ * (window >= 1) or j < sinks (sinks >= 0; both are cut to 2^30). scale multiplies the scores; it is taken in fp32,
+ * where it has to be finite.
  * out = softmax(scale q.k over the keys seen) v; lse: [batch, heads, queries], ACL_FLOAT, contiguous, the natural logarithm of the
  * softmax's sum, or null. A query behind its sequence's length, or that sees no key, has out 0 and lse -infinity.
  * What lies in keys that a query does not see, NaN and infinities included, does not reach its result. */

@@ -281,7 +281,9 @@ aclnnStatus CheckPerRow(const char* api, const aclTensor* x, const aclTensor* t,
     return ACLNN_SUCCESS;
 }
 
-bool EpsOk(double eps) { return std::isfinite(eps) && eps >= 0.0; }
+// The kernels take eps and scales in fp32.
+bool Finite32(double v) { return std::isfinite(static_cast<float>(v)); }
+bool EpsOk(double eps) { return Finite32(eps) && eps >= 0.0; }
 
 NormShape ShapeOf(const aclTensor* x, const aclTensor* weight, double eps)
 {
@@ -336,7 +338,7 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
     const int64_t half = frequencies->dims[0];
     OPSCV_REQUIRE(half >= 1 && 2 * half <= Last(q) && half <= 2048, "%s: %ld frequencies do not fit a head of %ld values", api,
                   (long)half, (long)Last(q));
-    OPSCV_REQUIRE(std::isfinite(scale), "%s: scale must be finite", api);
+    OPSCV_REQUIRE(Finite32(scale), "%s: scale must be finite in fp32", api);
     const size_t axesDim = sections != nullptr ? 1 : 0;
     RotaryShape r;
     if (sections != nullptr) {
@@ -465,7 +467,7 @@ aclnnStatus CheckAttention(const char* api, const aclTensor* q, const aclTensor*
     }
     OPSCV_REQUIRE(window >= 1, "%s: window must be at least 1, got %ld", api, (long)window);
     OPSCV_REQUIRE(sinks >= 0, "%s: sinks must not be negative, got %ld", api, (long)sinks);
-    OPSCV_REQUIRE(std::isfinite(scale), "%s: scale must be finite", api);
+    OPSCV_REQUIRE(Finite32(scale), "%s: scale must be finite in fp32", api);
     s.batch = static_cast<int32_t>(q->dims[0]);
     s.lq = static_cast<int32_t>(q->dims[1]);
     s.lk = static_cast<int32_t>(k->dims[1]);
@@ -520,7 +522,7 @@ aclnnStatus aclnnResidualRmsNormGetWorkspaceSize(const aclTensor* x, const aclTe
         OPSCV_TRY(CheckNormTensor(api, x, y, "y"));
         OPSCV_TRY(CheckNormTensor(api, x, sum, "sum"));
         OPSCV_TRY(CheckPerRow(api, x, rstd, 0, "rstd"));
-        OPSCV_REQUIRE(EpsOk(eps), "%s: eps must be finite and not negative", api);
+        OPSCV_REQUIRE(EpsOk(eps), "%s: eps must be finite in fp32 and not negative", api);
         OPSCV_REQUIRE(WritesApart(y) && (sum == nullptr || WritesApart(sum)), "%s: an output's elements overlap", api);
         OPSCV_TRY(CheckData(api, {x, residual, weight, y, sum, rstd}));
         if (Numel(x) == 0) {
@@ -654,7 +656,7 @@ aclnnStatus aclnnResidualRmsNormQuantGetWorkspaceSize(const aclTensor* x, const 
         OPSCV_TRY(CheckNorm(api, x, weight));
         OPSCV_TRY(CheckNormTensor(api, x, residual, "residual"));
         OPSCV_TRY(CheckNormTensor(api, x, sum, "sum"));
-        OPSCV_REQUIRE(EpsOk(eps), "%s: eps must be finite and not negative", api);
+        OPSCV_REQUIRE(EpsOk(eps), "%s: eps must be finite in fp32 and not negative", api);
         OPSCV_REQUIRE(group == 0 || (group >= 32 && group % 32 == 0), "%s: group must be 0 or a multiple of 32, got %ld", api,
                       (long)group);
         OPSCV_REQUIRE(out->dtype == ACL_FLOAT8_E4M3FN || out->dtype == ACL_INT8, "%s: out must be FLOAT8_E4M3FN or INT8, got %s",

@@ -279,3 +279,19 @@ def test_workspace_of_many_sequences(ops, code, batch, tokens, kv, group, sinks)
     statistics = 2 * 4 * batch * kv * group * (tokens + 256)
     assert got == 0 and n.value - statistics < batch * tokens * kv * d * elem
     L.aclDestroyAclOpExecutor(e)
+
+
+def test_scalars_beyond_fp32(ops):
+    """Finite in 64 bits is not enough: the kernels take them in 32."""
+    x, q, f, p = torch.zeros(2, 3, 8), torch.zeros(2, 5, 4, 16), torch.zeros(8), torch.arange(5)
+    for big in (1e39, 1e300):
+        refused(ops, lambda: ops.residual_rms_norm(x, eps=big), "eps")
+        refused(ops, lambda: ops.residual_rms_norm_quant(x, eps=big), "eps")
+        for sign in (1, -1):
+            refused(ops, lambda: ops.rotary_embedding(q, None, p, f, scale=sign * big), "scale")
+            refused(ops, lambda: ops.rotary_embedding_backward(q, None, p, f, scale=sign * big), "scale")
+            refused(ops, lambda: ops.window_attention(q, q, q, 3, scale=sign * big), "scale")
+            refused(ops, lambda: ops.window_attention_backward(q, q, q, q, q, torch.zeros(2, 4, 5), 3, scale=sign * big), "scale")
+    accepted(lambda: ops.residual_rms_norm(x, eps=3e38))
+    accepted(lambda: ops.rotary_embedding(q, None, p, f, scale=-3e38))
+    accepted(lambda: ops.window_attention(q, q, q, 3, scale=3e38))
