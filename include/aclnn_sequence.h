@@ -115,7 +115,7 @@ ACLNN_API aclnnStatus aclnnRotaryFrequencies(void* workspace, uint64_t workspace
  * Causal attention over a sliding window with a few first tokens ("sinks") that stay visible, for prompts, chunks of new tokens
  * over a cache, single tokens and training.
  * q, out: [batch, queries, heads, dim]; k, v: [batch, keys, kvHeads, dim]; heads a multiple of kvHeads (head h reads key head
- * h / (heads / kvHeads)), 1 <= dim <= 256.
+ * h / (heads / kvHeads)), at most 2^24 to a key head; 1 <= dim <= 256; batch, queries, keys, heads and batch * heads at most 2^30.
  * kvLengths, qLengths: [batch], ACL_INT32 or ACL_INT64, contiguous, or null (all keys, all queries): how many keys and queries of
  * each sequence count; values outside [0, keys] and [0, queries] are cut to it. Query i of a sequence sits at position
  * p = kvLength - qLength + i, so that the last query sits at the last key; it sees the keys j <= p with j > p - window

@@ -459,6 +459,8 @@ aclnnStatus CheckAttention(const char* api, const aclTensor* q, const aclTensor*
     OPSCV_REQUIRE(q->dims[1] <= most && k->dims[1] <= most && q->dims[0] <= most && q->dims[2] <= most &&
                       q->dims[0] * q->dims[2] <= most && k->dims[2] <= most && k->dims[0] * k->dims[2] <= most,
                   "%s: extents above 2^30 are not supported", api);
+    // (query, head) pairs of a key head are counted in 32 bits where queries are few
+    OPSCV_REQUIRE(q->dims[2] / k->dims[2] <= (1 << 24), "%s: more than 2^24 heads to a key head are not supported", api);
     for (const aclTensor* n : {qLengths, kvLengths}) {
         OPSCV_REQUIRE(n == nullptr || n->dtype == ACL_INT32 || n->dtype == ACL_INT64, "%s: lengths must be INT32 or INT64, got %s",
                       api, DtypeName(n->dtype));

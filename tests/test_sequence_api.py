@@ -295,3 +295,24 @@ def test_scalars_beyond_fp32(ops):
     accepted(lambda: ops.residual_rms_norm(x, eps=3e38))
     accepted(lambda: ops.rotary_embedding(q, None, p, f, scale=-3e38))
     accepted(lambda: ops.window_attention(q, q, q, 3, scale=3e38))
+
+
+def test_attention_refuses_too_many_heads_to_a_key_head(ops):
+    """Their products with 8 queries would not fit 32 bits."""
+    L = ops.lib()
+
+    def tensor(*shape):
+        dims = (ctypes.c_int64 * len(shape))(*shape)
+        return ctypes.c_void_p(L.aclCreateTensor(dims, len(shape), ops.ACL_FLOAT, None, 0, ops.ACL_FORMAT_ND, dims, len(shape), ctypes.c_void_p(4096)))
+
+    n, e = ctypes.c_uint64(0), ctypes.c_void_p(None)
+    for heads, status in ((2 ** 24, 0), (2 ** 24 + 1, INVALID), (2 ** 28, INVALID)):
+        q, k, lse = tensor(1, 8, heads, 1), tensor(1, 8, 1, 1), tensor(1, heads, 8)
+        got = L.aclnnWindowAttentionGetWorkspaceSize(q, k, k, None, None, 3, 0, 1.0, q, lse, ctypes.byref(n), ctypes.byref(e))
+        assert got == status
+        if got == 0:
+            L.aclDestroyAclOpExecutor(e)
+        assert L.aclnnWindowAttentionBackwardGetWorkspaceSize(q, q, k, k, q, lse, None, None, 3, 0, 1.0, q, k, k, ctypes.byref(n),
+                                                              ctypes.byref(e)) == status
+        if status == 0:
+            L.aclDestroyAclOpExecutor(e)
