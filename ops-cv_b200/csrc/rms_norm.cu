@@ -408,16 +408,17 @@ struct Divisor {
     }
 };
 
-// LG: lanes of a group where a group lies within a warp (a power of two), 0 where groups go through shared memory, one word each, and
-// kRowScale where the row has one scale.
-constexpr int kRowScale = -1;
+// Where the largest magnitudes of a row's groups come together. LG > 0: within warps, LG lanes to a group (groups of a power of two of
+// columns); kShared: in one word of shared memory each; kRowScale: in the row's block, one scale for all. (With the lanes as an argument
+// of the kernel, groups of 128 of 8192 x 5120 take 65.6 us, not 63.8.)
+constexpr int kShared = 0, kRowScale = -1;
 
 // 48 registers where 16 values a thread allow it: blocks of 320 threads come four to an SM, not three (8192 x 5120 to int8 in groups of
 // 128, bf16: 69.6 us against 80.5; fp32 to either type 123 against 139).
 template <typename T, int V, int NV, Q8 Q, int LG>
-__global__ void __launch_bounds__(kMaxThreads) __maxnreg__(NV * V == 16 && LG != 0 ? 48 : 64) RmsNormQuantKernel(FwdArgs a)
+__global__ void __launch_bounds__(kMaxThreads) __maxnreg__(NV * V == 16 && LG != kShared ? 48 : 64) RmsNormQuantKernel(FwdArgs a)
 {
-    extern __shared__ uint32_t most[]; // [groups] (LG == 0)
+    extern __shared__ uint32_t most[]; // [groups] (kShared)
     __shared__ float part[32];
     using QT = Q8Type<Q>;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(kMaxThreads) __maxnreg__(NV * V == 16 && LG !=
     WeightOf<T, V, N> w;
     F2 sq = MakeF2(0.0f, 0.0f);
     float f[V];
-    if constexpr (LG == 0) { // one row a block (the launcher sees to it)
+    if constexpr (LG == kShared) { // one row a block (the launcher sees to it)
         for (int32_t g = threadIdx.x; g < a.groups; g += blockDim.x) {
             most[g] = 0;
         }
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(kMaxThreads) __maxnreg__(NV * V == 16 && LG !=
         }
         return;
     }
-    if constexpr (LG == 0) {
+    if constexpr (LG == kShared) {
         // two passes over the row's values: largest magnitudes, then the quantised values
         for (int pass = 0; pass < 2; ++pass) {
             float top = 0.0f; // of all of this thread's values
@@ -960,11 +961,12 @@ cudaError_t RmsNormQuant(Dt dt, const NormShape& n, const void* x, RowStride xs,
     while (v > 1 && !(n.width % v == 0 && Aligned(q, v))) {
         v >>= 1;
     }
-    const bool small = a.groups > 1 && a.group == 128 && v >= 4;
+    // Groups of a power of two of columns that one to 32 lanes hold lie within a warp: lanes hold consecutive chunks of a row, and a
+    // warp's first chunk starts a group. Others go through shared memory, with one row a block. 8192 x 5120 bf16 to e4m3: groups of 32, 64,
+    // 128 and 256 68 us a call, through shared memory 106 to 112.
+    const bool small = a.groups > 1 && (a.group & (a.group - 1)) == 0 && a.group <= 32 * v;
     // with groups in a warp, 512 threads a row are a little faster (8192 x 5120 bf16: 64 us against 68 with 256)
     RowShape shape = ShapeOfRow(n.width, v, 32, kMaxThreads, small ? 0 : n.rows);
-    // Groups of 128 columns read with at least four to a lane lie within a warp (lanes hold consecutive chunks of a row, and a
-    // warp's first chunk starts a group); others go through shared memory, with one row a block.
     const bool inWarp = small && shape.nv > 0, ofRow = a.groups == 1 && shape.nv > 0;
     if (!inWarp && !ofRow) {
         shape.rows = 1;
@@ -978,15 +980,23 @@ cudaError_t RmsNormQuant(Dt dt, const NormShape& n, const void* x, RowStride xs,
     const unsigned grid = static_cast<unsigned>(blocks);
     OPSCV_DISPATCH_DT(dt, T, OPSCV_DISPATCH_VEC(v, V, if constexpr (V * sizeof(T) <= 16) {
         OPSCV_DISPATCH_NV(shape.nv, NV, if constexpr (NV * V <= 32) {
-            constexpr int LG = NV > 0 && V >= 4 ? 128 / V : 0;
+            constexpr int Least = 32 / V; // lanes of a group of 32 columns
             auto launch = [&](auto tag) {
                 constexpr Q8 Q = decltype(tag)::value;
-                if (inWarp) {
-                    RmsNormQuantKernel<T, V, NV, Q, LG><<<grid, block, shared, s>>>(a);
-                } else if (ofRow) {
-                    RmsNormQuantKernel<T, V, NV, Q, (NV > 0 ? kRowScale : 0)><<<grid, block, shared, s>>>(a);
-                } else {
-                    RmsNormQuantKernel<T, V, NV, Q, 0><<<grid, block, shared, s>>>(a);
+                auto with = [&](auto lanes) {
+                    constexpr int LG = decltype(lanes)::value;
+                    if constexpr (LG <= 32 && (NV > 0 || LG == kShared)) {
+                        RmsNormQuantKernel<T, V, NV, Q, LG><<<grid, block, shared, s>>>(a);
+                    }
+                };
+                const int lanes = inWarp ? a.group / V : ofRow ? kRowScale : kShared;
+                switch (lanes) {
+                    case kShared: with(std::integral_constant<int, kShared>{}); break;
+                    case kRowScale: with(std::integral_constant<int, kRowScale>{}); break;
+                    case Least: with(std::integral_constant<int, Least>{}); break;
+                    case 2 * Least: with(std::integral_constant<int, 2 * Least>{}); break;
+                    case 4 * Least: with(std::integral_constant<int, 4 * Least>{}); break;
+                    default: with(std::integral_constant<int, 8 * Least>{}); break;
                 }
             };
             if (type == Q8::E4M3) {

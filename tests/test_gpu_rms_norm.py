@@ -340,3 +340,21 @@ def test_backward_of_rows_of_16_million_values(ops, dev):
     terms = rstd * (g.abs() + u.abs() * (g * u).abs().mean(-1, keepdim=True))
     chain = width // 1024 + CHAIN  # a thread adds up its share of the row in turn
     close(gx, want, half_step(t) * want.abs() + 2 * chain * STEP32 * terms + torch.finfo(t).tiny)
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,width", [(5, 64), (9, 500), (33, 1000), (6, 1153), (700, 2050), (3, 5120), (2, 8196), (2, 40000)])
+@pytest.mark.parametrize("group", [32, 64, 128, 256, 512])
+def test_quant_by_groups_of_a_power_of_two(ops, dev, t, rows, width, dtype, group):
+    """Groups that one to 32 lanes hold and wider ones, of rows that end inside one, read 8, 4, 2 and 1 values at a time."""
+    x = inputs((rows, width), t, 29, dev)[0]
+    w = weights(width, torch.float32, 30, dev)
+    q, scales, _ = ops.residual_rms_norm_quant(x, None, w, dtype=dtype, group=group)
+    y, _ = forward64(x, w, 1e-6)
+    g = min(group, width)
+    want = torch.stack([p.abs().amax(-1) for p in torch.split(y, g, -1)], -1) / (127.0 if dtype == torch.int8 else 448.0)
+    assert scales.shape == want.shape
+    close(scales, want, want * 2 * CHAIN * STEP32)
+    wide = torch.repeat_interleave(scales.double(), g, -1)[:, :width]
+    close(q.double() * wide, y, quant_bound(y, wide, dtype))
