@@ -481,3 +481,11 @@ def test_block_of_a_model(ops, dev):
     # a chain of fp32 steps with sums of at most 256 terms: 2^-12 of the largest value is 2^12 half steps of slack
     for got, want in ((out, o6.detach()), (gx, want_x), (gw, want_w)):
         assert (got.double() - want).abs().max() < 2.0 ** -12 * want.abs().max()
+
+
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("d", [8, 16, 24, 32, 48, 64, 80, 88, 96, 104, 112, 120, 128])
+def test_heads_of_every_number_of_steps(ops, dev, t, d):
+    q, g = normal((2, 140, 4, d), t, 151, dev), normal((2, 140, 4, d), t, 154, dev)
+    k, v = normal((2, 200, 2, d), t, 152, dev), normal((2, 200, 2, d), t, 153, dev)
+    check(ops, q, k, v, 70, 3, g=g)
