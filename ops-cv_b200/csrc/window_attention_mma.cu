@@ -52,6 +52,48 @@ __device__ __forceinline__ void RowBarrier()
     asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
 }
 
+// ---- what lies behind a sequence's lengths ---------------------------------------------------------------------------------
+// Its weights are 0, but 0 times a NaN would send every row of the tile to the warps that form rows again (4 x 4096 tokens, window 1024: 24 ms
+// in place of 0.13, backward 98 in place of 0.38). So a tile that reaches behind the end comes on a barrier of the loading thread's own
+// (`tail`), which then copies zeros over the last rows, on the barrier that the products wait for. Other tiles, and the warps that
+// multiply and form weights, have no part in it (zeros written by the product warp cost the backward 2 % where nothing is padded).
+__device__ uint4 g_zeroRows[kTile * 128 / sizeof(uint4)];
+
+// Bytes of rows [from, ROWS) of an operand of HALVES blocks of 64 values, and zeros for them on `bar`, which expects them.
+template <int ROWS, int HALVES>
+__device__ __forceinline__ uint32_t BytesFrom(int32_t from)
+{
+    return HALVES * (ROWS - max(from, 0)) * 128;
+}
+template <int ROWS, int HALVES>
+__device__ __forceinline__ void ZerosFrom(unsigned char* operand, int32_t from, uint64_t* bar)
+{
+#pragma unroll
+    for (int c = 0; c < HALVES; ++c) {
+        BulkLoad(operand + (c * ROWS + max(from, 0)) * 128, g_zeroRows, BytesFrom<ROWS, 1>(from), bar);
+    }
+}
+
+// A tile that reaches behind the end, at row `row` of a head, its rows from `from` on as zeros: on `tail` first, then on `bar`. false: a wait
+// ran out. Apart from the loops that call it, which keep their registers (in line, the forward took 1 to 2 % longer where nothing is padded).
+template <int ROWS, int HALVES>
+__device__ __noinline__ bool LoadTail(unsigned char* dst, const CUtensorMap* map, int32_t row, int32_t head, int32_t b, int32_t from,
+                                      uint64_t* tail, uint32_t phase, uint64_t* bar, volatile uint32_t* failed)
+{
+    BarExpect(tail, HALVES * ROWS * 128);
+#pragma unroll
+    for (int c = 0; c < HALVES; ++c) {
+        TmaLoad4(dst + c * ROWS * 128, map, tail, 64 * c, row, head, b);
+    }
+    BarWait(tail, phase, failed);
+    if (*failed != 0) {
+        return false;
+    }
+    BarExpect(bar, BytesFrom<ROWS, HALVES>(from));
+    ZerosFrom<ROWS, HALVES>(dst, from, bar);
+    return true;
+}
+
 // columns of an accumulator times a factor a row
 template <int N>
 __device__ __forceinline__ void TmemScale(uint32_t addr, float f)
@@ -130,7 +172,7 @@ constexpr int kKeys = 64;
 constexpr uint32_t kKeyHalf = kKeys * 128;
 
 struct ForwardShared {
-    uint64_t qFull, kFull[2], vFull[2], sFull[2], pFull[2], pvDone[2], allDone, drain;
+    uint64_t qFull, kFull[2], vFull[2], tail, sFull[2], pFull[2], pvDone[2], allDone, drain;
     uint32_t tmem, failed;
 };
 
@@ -167,6 +209,7 @@ __global__ void __launch_bounds__(192, 2)
             BarInit(&sh.pFull[e], kRowThreads);
             BarInit(&sh.pvDone[e], 1);
         }
+        BarInit(&sh.tail, 1);
         BarInit(&sh.allDone, 1);
         BarInit(&sh.drain, 1);
         BarInitDone();
@@ -195,7 +238,8 @@ __global__ void __launch_bounds__(192, 2)
                     TmaLoad4(dst + c * kKeyHalf, map, bar, 64 * c, row, u, b);
                 }
             };
-            int32_t ks = 0, vs = 0; // loads so far
+            const int32_t end = n.kv < s.lk ? n.kv : INT32_MAX; // tiles that reach behind it come with zeros there
+            int32_t ks = 0, vs = 0, tails = 0;                  // loads so far
             for (int32_t it = 0; it < count; ++it) {
                 const int32_t st = it & 1, j0 = steps.Key(it);
                 if (it >= 2) {
@@ -212,11 +256,21 @@ __global__ void __launch_bounds__(192, 2)
                 if (*failed != 0) {
                     break;
                 }
-                load(sv + st * kKeyBytes, &mapV, &sh.vFull[st], j0);
+                if (j0 + kKeys > end) { // the scores of its keys are replaced as they are
+                    if (!LoadTail<kKeys, HALVES>(sv + st * kKeyBytes, &mapV, j0, u, b, n.kv - j0, &sh.tail, tails++ & 1, &sh.vFull[st],
+                                                 failed)) {
+                        break;
+                    }
+                } else {
+                    load(sv + st * kKeyBytes, &mapV, &sh.vFull[st], j0);
+                }
                 ++vs;
             }
             // own copies end before the block does, whatever became of the others
             BarDrain(&sh.qFull, 0);
+            if (tails > 0) {
+                BarDrain(&sh.tail, (tails - 1) & 1);
+            }
             for (int32_t e = ks > 2 ? ks - 2 : 0; e < ks; ++e) {
                 BarDrain(&sh.kFull[e & 1], (e / 2) & 1);
             }
@@ -586,7 +640,7 @@ __device__ __forceinline__ uint32_t LargestOfRow(uint8_t (&most)[kSides][kTile],
 }
 
 struct GradQShared {
-    uint64_t qFull, kFull[3], kEmpty[3], vFull[2], vEmpty[2], sFull[2], dpFull, dsReady, dqDone, allDone, exchanged, drain;
+    uint64_t qFull, kFull[3], kEmpty[3], vFull[2], vEmpty[2], tail, sFull[2], dpFull, dsReady, dqDone, allDone, exchanged, drain;
     uint32_t tmem, failed, bad[4];
     uint8_t most[2][kSides][kTile]; // fp16: exponents of a row's largest ds, of even and odd steps, of its threads
 };
@@ -625,6 +679,7 @@ __device__ __forceinline__ void GradQBlock(const BackwardArgs& m, const CUtensor
             BarInit(&sh.vEmpty[e], 1);
             BarInit(&sh.sFull[e], 1);
         }
+        BarInit(&sh.tail, 1);
         BarInit(&sh.dpFull, 1);
         BarInit(&sh.dsReady, kGradThreads);
         BarInit(&sh.dqDone, 1);
@@ -657,7 +712,8 @@ __device__ __forceinline__ void GradQBlock(const BackwardArgs& m, const CUtensor
             BarExpect(&sh.qFull, 2 * kBytes);
             load(sq, &mapQ, &sh.qFull, i0, h);
             load(sg, &mapG, &sh.qFull, i0, h);
-            int32_t it = 0;
+            const int32_t end = n.kv < s.lk ? n.kv : INT32_MAX; // tiles that reach behind it come with zeros there
+            int32_t it = 0, tails = 0;
             for (; it < count; ++it) {
                 const int32_t j0 = steps.Key(it), ks = it % 3, vs = it & 1;
                 if (it >= 3) {
@@ -669,6 +725,17 @@ __device__ __forceinline__ void GradQBlock(const BackwardArgs& m, const CUtensor
                 if (*failed != 0) {
                     break;
                 }
+                if (j0 + kTile > end) { // of the products for dP and gradQ
+                    const int32_t from = n.kv - j0;
+                    if (!LoadTail<kTile, HALVES>(sk + ks * kBytes, &mapK, j0, u, b, from, &sh.tail, tails++ & 1, &sh.kFull[ks], failed)) {
+                        break;
+                    }
+                    if (!LoadTail<kTile, HALVES>(sv + vs * kBytes, &mapV, j0, u, b, from, &sh.tail, tails++ & 1, &sh.vFull[vs], failed)) {
+                        BarDrain(&sh.kFull[ks], (it / 3) & 1);
+                        break;
+                    }
+                    continue;
+                }
                 BarExpect(&sh.kFull[ks], kBytes);
                 load(sk + ks * kBytes, &mapK, &sh.kFull[ks], j0, u);
                 BarExpect(&sh.vFull[vs], kBytes);
@@ -676,6 +743,9 @@ __device__ __forceinline__ void GradQBlock(const BackwardArgs& m, const CUtensor
             }
             // own copies end before the block does, whatever became of the others
             BarDrain(&sh.qFull, 0);
+            if (tails > 0) {
+                BarDrain(&sh.tail, (tails - 1) & 1);
+            }
             for (int32_t e = it > 3 ? it - 3 : 0; e < it; ++e) {
                 BarDrain(&sh.kFull[e % 3], (e / 3) & 1);
             }
@@ -880,7 +950,7 @@ __device__ __forceinline__ void GradQBlock(const BackwardArgs& m, const CUtensor
 }
 
 struct GradKvShared {
-    uint64_t kvFull, full[2], empty[2], sFull, dpFull, pReady, dsReady, dvDone, dkDone, exchanged, drain;
+    uint64_t kvFull, full[2], empty[2], tail, sFull, dpFull, pReady, dsReady, dvDone, dkDone, exchanged, drain;
     uint32_t tmem, failed, bad[4];
     uint8_t most[2][kSides][kTile]; // fp16: exponents of a row's largest ds, of even and odd steps, of its threads
 };
@@ -944,6 +1014,7 @@ __device__ __forceinline__ void GradKvBlock(const BackwardArgs& m, const CUtenso
             BarInit(&sh.full[e], 1);
             BarInit(&sh.empty[e], 1);
         }
+        BarInit(&sh.tail, 1);
         BarInit(&sh.sFull, 1);
         BarInit(&sh.dpFull, 1);
         BarInit(&sh.pReady, kGradThreads);
@@ -977,7 +1048,8 @@ __device__ __forceinline__ void GradKvBlock(const BackwardArgs& m, const CUtenso
             BarExpect(&sh.kvFull, 2 * kBytes);
             load(sk, &mapK, &sh.kvFull, j0, u);
             load(sv, &mapV, &sh.kvFull, j0, u);
-            int32_t it = 0;
+            const int32_t last = n.q < s.lq ? n.q : INT32_MAX; // tiles that reach behind it come with zeros there
+            int32_t it = 0, tails = 0;
             for (; it < count; ++it) {
                 const int32_t st = it & 1, h = u * m.a.group + (begin + it) / perGroup;
                 const int32_t i0 = iBase + (begin + it) % perGroup * kTile;
@@ -987,14 +1059,31 @@ __device__ __forceinline__ void GradKvBlock(const BackwardArgs& m, const CUtenso
                 if (*failed != 0) {
                     break;
                 }
-                BarExpect(&sh.full[st], kStage);
-                load(sqg + st * 2 * kBytes, &mapQ, &sh.full[st], i0, h);
-                load(sqg + st * 2 * kBytes + kBytes, &mapG, &sh.full[st], i0, h);
+                unsigned char *q = sqg + st * 2 * kBytes, *g = q + kBytes;
+                if (i0 + kTile > last) { // of the products for dP and of both outer ones
+                    BarExpect(&sh.tail, 2 * kBytes);
+                    load(q, &mapQ, &sh.tail, i0, h);
+                    load(g, &mapG, &sh.tail, i0, h);
+                    BarWait(&sh.tail, tails++ & 1, failed);
+                    if (*failed != 0) {
+                        break;
+                    }
+                    BarExpect(&sh.full[st], 2 * BytesFrom<kTile, HALVES>(n.q - i0) + 2 * kTile * 4);
+                    ZerosFrom<kTile, HALVES>(q, n.q - i0, &sh.full[st]);
+                    ZerosFrom<kTile, HALVES>(g, n.q - i0, &sh.full[st]);
+                } else {
+                    BarExpect(&sh.full[st], kStage);
+                    load(q, &mapQ, &sh.full[st], i0, h);
+                    load(g, &mapG, &sh.full[st], i0, h);
+                }
                 const int64_t row = (static_cast<int64_t>(b) * s.heads + h) * m.stride + i0;
                 BulkLoad(stats + st * 2 * kTile, m.lse2 + row, kTile * 4, &sh.full[st]);
                 BulkLoad(stats + st * 2 * kTile + kTile, m.delta + row, kTile * 4, &sh.full[st]);
             }
             BarDrain(&sh.kvFull, 0);
+            if (tails > 0) {
+                BarDrain(&sh.tail, (tails - 1) & 1);
+            }
             for (int32_t e = it > 2 ? it - 2 : 0; e < it; ++e) {
                 BarDrain(&sh.full[e & 1], (e / 2) & 1);
             }

@@ -489,3 +489,34 @@ def test_heads_of_every_number_of_steps(ops, dev, t, d):
     q, g = normal((2, 140, 4, d), t, 151, dev), normal((2, 140, 4, d), t, 154, dev)
     k, v = normal((2, 200, 2, d), t, 152, dev), normal((2, 200, 2, d), t, 153, dev)
     check(ops, q, k, v, 70, 3, g=g)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("lq,lk,h,hk,d,window,sinks", [
+    (200, 300, 4, 2, 64, 150, 3), (300, 300, 4, 2, 128, 150, 3), (5, 300, 4, 2, 64, 150, 3), (130, 300, 4, 2, 80, 150, 0), (1, 700, 4, 1, 128, 600, 2),
+    (400, 400, 2, 1, 128, 1000, 0), (257, 257, 6, 2, 96, 20, 200), (700, 700, 2, 2, 64, 40, 140), (64, 64, 2, 1, 40, 10, 1), (150, 150, 2, 1, 200, 70, 3)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_padding_costs_nothing(ops, dev, t, lq, lk, h, hk, d, window, sinks, bad):
+    """What lies behind the sequences' lengths changes no bit of the results: no row is formed again on its account."""
+    b = 5
+    q, k, v, g = normal((b, lq, h, d), t, 161, dev), normal((b, lk, hk, d), t, 162, dev), normal((b, lk, hk, d), t, 163, dev), normal(
+        (b, lq, h, d), t, 164, dev)
+    kn = torch.tensor([lk, lk - 1, lk - lk // 3, max(1, lk - 129), 1], device=dev)
+    qn = torch.tensor([lq, max(1, lq - 1), lq - lq // 3, max(1, lq - 129), 1], device=dev)
+    same = torch.minimum(kn, qn)
+
+    def padded(x, n, value):
+        x = x.clone()
+        for i in range(b):
+            x[i, int(n[i]):] = value
+        return x
+
+    for qs, ks in ((qn, kn), (None, kn), (qn, None), (same, same)):
+        results = []
+        for value in (0.0, bad):
+            q1, g1 = (padded(x, qs, value) if qs is not None else x for x in (q, g))
+            k1, v1 = (padded(x, ks, value) if ks is not None else x for x in (k, v))
+            out, lse = ops.window_attention(q1, k1, v1, window, sinks, q_lengths=qs, kv_lengths=ks)
+            results.append((out, lse) + tuple(ops.window_attention_backward(g1, q1, k1, v1, out, lse, window, sinks, q_lengths=qs, kv_lengths=ks)))
+        for name, x, y in zip(("out", "lse", "gradQ", "gradK", "gradV"), *results):
+            assert torch.isfinite(y if name != "lse" else y.nan_to_num(neginf=0.0)).all() and torch.equal(x, y), name
