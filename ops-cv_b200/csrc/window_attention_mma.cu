@@ -13,8 +13,9 @@ __device__ unsigned int g_attentionTimeouts = 0;
 constexpr int kTile = 128;                        // rows of a tile
 constexpr uint32_t kHalfBytes = kTile * 128;      // 64 of the up to 128 values of 128 rows
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// The running maximum stays as it is while the scores outgrow it by no more than a factor of 2^8: weights up to 2^8 lose nothing in
-// a floating-point type, and most tiles then need no rescaling of the accumulators.
+// Softmax in one pass with a running maximum and sum (M. Milakov, N. Gimelshein, "Online normalizer calculation for softmax", 2018). The
+// maximum stays as it is while the scores outgrow it by no more than a factor of 2^8: any reference will do as long as the weights keep
+// their bits, which weights up to 2^8 do in a floating-point type, and most tiles then need no rescaling of the accumulators.
 constexpr float kGrowth = 8.0f;
 
 struct MmaArgs {
@@ -165,7 +166,10 @@ __device__ __forceinline__ void LiveColumns(uint32_t (&live)[N / 32], int32_t fr
 // of tensor memory, 97 KB of shared memory and 192 threads each), one's exponentials under the other's products.
 //
 // Bound by the chain of a row's thread: scores from tensor memory, their maximum, 64 exponentials, weights back. The running maximum moves
-// only where a row has outgrown it by 2^8 (at the start, mostly); O is rescaled then and not otherwise. 8192 tokens, 16 heads of 128 on 4:
+// only where a row has outgrown it by 2^8 (at the start, mostly); O is rescaled then and not otherwise. The weights are rounded to the
+// tensors' type, as the product takes both operands in one type: half a step each, as much as the rounding of the result itself; the sum
+// that they are divided by is of the weights before that. A second 16-bit part, as for few queries, would double the product. 8192
+// tokens, 16 heads of 128 on 4:
 // 301 us (906 TFLOP/s) without a window; 106 us (window 1024, 4 sinks; with the tensor pipe and the special-function units 37 % busy).
 constexpr int kRowThreads = 128;
 constexpr int kKeys = 64;
@@ -487,7 +491,8 @@ __global__ void __launch_bounds__(192, 2)
 // to itself: warps 0 to 15 have a row each four threads (32 columns each), warp 16 loads, warp 17 issues the products; with two threads
 // a row, the chain of one thread's exponentials was longer than the products. 8192 tokens, 16 heads of 128 on 4: 858 us (801 TFLOP/s of
 // the 5 products) without a window; 2 x 4096, window 1024, 4 sinks: 302 us, the tensor pipe 45 % busy. The weights are scaled by 2^8
-// (folded into the statistics), which keeps small ones out of fp16's subnormal range.
+// (folded into the statistics), which keeps small ones out of fp16's subnormal range. Weights and ds are rounded to the tensors' type for
+// their products, half a step each; delta is formed from `out` as it is stored, the only form of it that the call has.
 constexpr int kSides = 4;
 constexpr int kColumns = kTile / kSides;
 constexpr int kGradThreads = kTile * kSides;
