@@ -74,7 +74,7 @@ ACLNN_API aclnnStatus aclnnResidualRmsNormQuant(void* workspace, uint64_t worksp
  * 64 bits.
  * positions: q's leading dimensions, ACL_INT32 or ACL_INT64. Any of these may have stride 0, where one position serves several tokens;
  * the others have any strides, as long as they merge to at most two dimensions (neighbours merge where the outer one's stride is the
- * inner one's times its extent). With `sections` (at most 4 whole numbers >= 0 that add up to half): [axes, ...], axis a turning the
+ * inner one's times its extent), and to at most four with those of stride 0 between and behind them. With `sections` (at most 4 whole numbers >= 0 that add up to half): [axes, ...], axis a turning the
  * a-th section of the frequencies.
  * qOut may lie over q and kOut over k. */
 ACLNN_API aclnnStatus aclnnRotaryEmbeddingGetWorkspaceSize(const aclTensor* q, const aclTensor* k, const aclTensor* positions,

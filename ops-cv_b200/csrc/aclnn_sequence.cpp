@@ -1,6 +1,7 @@
 // First- and second-phase entry points of the token-sequence operators (include/aclnn_sequence.h).
 #include <cmath>
 #include <exception>
+#include <optional>
 
 #include "../../include/aclnn_sequence.h"
 #include "host_common.h"
@@ -295,22 +296,64 @@ NormShape ShapeOf(const aclTensor* x, const aclTensor* weight, double eps)
 }
 
 // ---- rotary ------------------------------------------------------------------------------------------------------------------
-// Positions that broadcast along a dimension between others do not merge with them; such go through a copy. Those that stand for
-// themselves in three dimensions or more do not: the kernel reads two.
-bool PositionsStageable(const aclTensor* positions, size_t axesDim)
-{
-    int levels = 0;
-    int64_t last = 0;
-    for (size_t i = axesDim; i < positions->dims.size(); ++i) {
-        const int64_t n = positions->dims[i], stride = positions->strides[i];
-        if (n == 1 || stride == 0) {
-            continue;
+// Positions that broadcast along a dimension between others do not merge with them; such go through a copy, axis by axis, in which the
+// dimensions that broadcast in front of all others stay as they are. Those that stand for themselves in three dimensions or more do not:
+// the kernel reads two.
+class PositionsCopy {
+public:
+    PositionsCopy(const aclTensor* positions, size_t axesDim) : given_(positions), axesDim_(axesDim), axis_(*positions), copied_(*positions)
+    {
+        const size_t rank = positions->dims.size();
+        from_ = axesDim;
+        while (from_ < rank && (positions->dims[from_] == 1 || positions->strides[from_] == 0)) {
+            ++from_;
         }
-        levels += levels == 0 || last != stride * n ? 1 : 0;
-        last = stride;
+        axis_.dims.assign(positions->dims.begin() + from_, positions->dims.end());
+        axis_.strides.assign(positions->strides.begin() + from_, positions->strides.end());
+        int64_t stride = 1;
+        for (size_t i = rank; i-- > from_;) {
+            copied_.strides[i] = stride;
+            stride *= positions->dims[i];
+        }
     }
-    return levels <= 2 && ViewStageable(positions);
-}
+    bool Possible() const
+    {
+        int levels = 0;
+        int64_t last = 0;
+        for (size_t i = 0; i < axis_.dims.size(); ++i) {
+            const int64_t n = axis_.dims[i], stride = axis_.strides[i];
+            if (n == 1 || stride == 0) {
+                continue;
+            }
+            levels += levels == 0 || last != stride * n ? 1 : 0;
+            last = stride;
+        }
+        return levels <= 2 && !IsContiguous(&axis_) && ViewStageable(&axis_);
+    }
+    const aclTensor& View() const { return copied_; } // strides of one axis; that between axes comes with Stage
+    // the copies, and the stride between their axes
+    BufRef Stage(WsPlan& ws, aclOpExecutor* ex, int64_t* axisStride)
+    {
+        const int64_t axes = axesDim_ != 0 ? given_->dims[0] : 1;
+        BufRef first;
+        for (int64_t a = 0; a < axes; ++a) {
+            aclTensor one = axis_;
+            one.offset += axesDim_ != 0 ? a * given_->strides[0] : 0;
+            const BufRef at = StageInput(&one, ws, ex);
+            if (a == 0) {
+                first = at;
+            } else if (a == 1) {
+                *axisStride = static_cast<int64_t>(at.wsOff - first.wsOff) / ElemSize(given_->dtype);
+            }
+        }
+        return first;
+    }
+
+private:
+    const aclTensor* given_;
+    size_t axesDim_, from_ = 0;
+    aclTensor axis_, copied_;
+};
 
 aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, const aclTensor* positions,
                        const aclTensor* frequencies, const aclIntArray* sections, bool interleaved, double scale, bool inverse,
@@ -382,30 +425,36 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
     const auto all = {&oq, &ok, &oqo, &oko};
     // the views as they are; with copied positions; with copies of the others; with copies of all
     bool merges = MergesAsGiven(all, lead, addAll, merged);
-    const aclTensor copied = ContiguousLike(positions);
-    const bool mayCopy = !merges && PositionsStageable(positions, axesDim);
+    std::optional<PositionsCopy> copy;
     bool copies = false;
-    if (mayCopy) {
-        pos = copied;
+    if (!merges) {
+        copy.emplace(positions, axesDim);
+        if (!copy->Possible()) {
+            copy.reset();
+        }
+    }
+    if (copy) {
+        pos = copy->View();
         merges = copies = MergesAsGiven(all, lead, addAll, merged);
-        pos = copies ? copied : *positions;
+        pos = copies ? pos : *positions;
     }
     OPSCV_TRY(Place(api, all, !merges, ex, ws));
     if (!merges) {
         LeadMerge asGiven(lead), withCopy(lead);
         addAll(asGiven);
         if (!asGiven.Run(merged)) {
-            OPSCV_REQUIRE(mayCopy, "%s: positions with more than two strided leading dimensions are not supported", api);
+            OPSCV_REQUIRE(copy, "%s: positions with more than two strided leading dimensions are not supported", api);
             copies = true;
-            pos = copied;
+            pos = copy->View();
             addAll(withCopy);
-            withCopy.Run(merged); // contiguous tensors merge to one
+            withCopy.Run(merged); // contiguous tensors merge to one dimension, the copy to two
         }
     }
+    r.posAxis = axesDim != 0 ? positions->strides[0] : 0;
     BufRef posBuf;
     posBuf.base = DataOf(positions, ElemSize(positions->dtype));
     if (copies) {
-        posBuf = StageInput(positions, ws, &ex);
+        posBuf = copy->Stage(ws, &ex, &r.posAxis);
     }
     r.tokens = merged.total;
     r.inner = merged.inner;
@@ -415,7 +464,6 @@ aclnnStatus PlanRotary(const char* api, const aclTensor* q, const aclTensor* k, 
     r.inverse = inverse;
     r.freq64 = frequencies->dtype == ACL_DOUBLE;
     r.pos64 = positions->dtype == ACL_INT64;
-    r.posAxis = axesDim != 0 ? pos.strides[0] : 0;
     r.scale = static_cast<float>(scale);
     tq.heads = static_cast<int32_t>(heads);
     tq.inHead = oq.view.strides[lead];

@@ -259,3 +259,22 @@ def test_ramp_without_frequencies_between(ops, dev, half):
         assert ((got - want).abs() <= 1e-14 * want).all()
     got = ops.rotary_frequencies(2 * half, 10000.0, "ramp", 8.0, 2 * math.pi * 1.5, 1.5, 1.5 + 1e-13, torch.float64, dev)
     assert ((got[1:] - plain[1:] / 8).abs() <= 1e-14 * plain[1:]).all()
+
+
+@pytest.mark.parametrize("axes", [1, 2, 4])
+def test_positions_of_many_dimensions_that_broadcast(ops, dev, axes):
+    """Strided dimensions with broadcast ones in front, between and behind, for each axis."""
+    lead, f = (2, 3, 2, 5, 3), frequencies(8, dev)
+    q, k = normal((*lead, 3, 20), torch.bfloat16, 31, dev), normal((*lead, 1, 20), torch.bfloat16, 32, dev)
+    sections = (8,) if axes == 1 else (5, 3) if axes == 2 else (1, 2, 0, 5)
+    for n, shape in enumerate(((2, 1, 2, 1, 3), (1, 3, 1, 5, 1), (2, 1, 2, 1, 1), (1, 1, 2, 1, 3), (2, 3, 1, 5, 3), (1, 3, 1, 1, 3), (2, 1, 1, 5, 1))):
+        p = torch.randint(0, 9000, (axes, *shape), generator=torch.Generator().manual_seed(33 + n)).to(dev)
+        full = p.expand(axes, *lead).contiguous()
+        want = ops.rotary_embedding(q, k, full, f, sections=sections)
+        if shape == (2, 1, 2, 1, 3):  # five that do not merge
+            with pytest.raises(ops.AclnnError, match="positions"):
+                ops.rotary_embedding(q, k, p, f, sections=sections)
+            continue
+        got = ops.rotary_embedding(q, k, p, f, sections=sections)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    check(want[0], q, full, f, False, sections, 1.0)

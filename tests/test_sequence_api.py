@@ -316,3 +316,10 @@ def test_attention_refuses_too_many_heads_to_a_key_head(ops):
                                                               ctypes.byref(e)) == status
         if status == 0:
             L.aclDestroyAclOpExecutor(e)
+
+
+def test_rotary_accepts_positions_by_axes_that_broadcast_between(ops):
+    q, f = torch.zeros(2, 3, 4, 5, 2, 8), torch.zeros(4)
+    for shape in ((1, 3, 1, 5), (2, 1, 4, 1), (1, 1, 4, 1), (1, 3, 4, 1), (2, 1, 1, 5)):
+        accepted(lambda: ops.rotary_embedding(q, None, torch.zeros((2, *shape), dtype=torch.int64), f, sections=(3, 1)))
+        accepted(lambda: ops.rotary_embedding(q, None, torch.zeros(shape, dtype=torch.int32), f))
