@@ -636,7 +636,7 @@ bool ReadsByFour(Dt dt, const AttnTensor& t)
 
 // Rows of the tiles that blocks own: 64 (32 of more than 128 values), or 32 where that leaves SMs with one block: a block's loads and waits
 // then hide behind another's products (2 x 777 tokens, 6 heads of 72: forward 94 us with 64 rows, 64 us with 32,
-// both before copies ran ahead; 56 us since).
+// both before copies ran ahead; 56 us since). The SMs are a constant here and in PlanKv because both phases of a call have to come to one plan.
 int OwnRows(const AttnShape& s, int64_t units, int64_t tokens)
 {
     return s.dim > 128 || units * CeilDiv(tokens, 64) < 2 * kNumSMsFallback ? 32 : 64;
